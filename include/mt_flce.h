@@ -588,6 +588,119 @@ int mt_ce_backward(const void* logits, int64_t T, int64_t V, int64_t ld, int dty
                    const float* grad_loss, int64_t grad_stride, void* dlogits, int64_t ldd,
                    mt_stream_t stream);
 
+/*
+ * Attention over a packed row of T tokens (no counterpart in the reference's
+ * own files; it stands where the reference runs flash attention over the
+ * boundaries of position_ids, setup_model_for_training.py:91).
+ *
+ * The plan: which rows each workgroup takes, from the documents' boundaries
+ * cu_seqlens int32 [S + 1] (0 = cu[0] <= ... <= cu[S] <= T; the rows behind
+ * cu[S] belong to no document), their prefix lengths (int32 [S] or null: key j
+ * of a document's first prefix tokens is seen by every query of the document)
+ * and the window (a query sees at most that many tokens up to itself;
+ * INT32_MAX: all).  Every key is seen by the queries of its own document alone.
+ *   plan    int32, mt_attn_plan_bytes(T, S) bytes, 16-byte aligned
+ *   status  int32 [1] out (device): 0; 1 if cu_seqlens is malformed (every row
+ *           then counts as lying behind the last document); 2 if some prefix
+ *           lies outside its document (it is then clamped)
+ * A plan serves any number of calls of the same T, S and window.
+ */
+size_t mt_attn_plan_bytes(int64_t T, int64_t S);
+int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t S, int64_t T,
+                 int64_t window, int32_t* plan, size_t plan_bytes, int32_t* status,
+                 mt_stream_t stream);
+
+/*
+ * out[t, h] = sum_j softmax_j(z_tj) v[j, h'] over the keys j that t sees, with
+ * z = scale q . k, capped as softcap tanh(z / softcap) if softcap > 0; query
+ * head h reads key head h' = h / (heads / kv_heads).  Rows behind the last
+ * document: zeros.
+ *   q [T, heads, head_dim], k, v [T, kv_heads, head_dim], dout as q: unit
+ *     stride along head_dim, the strides of rows (_t) and heads (_h) in
+ *     elements, whole 16-byte chunks, 0 allowed; head_dim whole 16-byte chunks,
+ *     at most 128
+ *   out, dq [T, heads, head_dim], dk, dv [T, kv_heads, head_dim]: contiguous
+ *   lse fp32 [heads, T]: log2 of the sum of 2^(z log2 e), from the forward to
+ *     the backward; 0 behind the last document
+ *   plan, window: as mt_attn_plan was given them
+ * The backward reads q, k, v, out, lse, dout and writes dq, dk, dv.  Sums in
+ * fp32; results do not depend on the order workgroups run in.
+ */
+typedef struct mt_attn_args {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv;
+  const int32_t* plan;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, dout_t, dout_h;
+  int64_t T, S, heads, kv_heads, head_dim, window;
+  float scale, softcap;
+  int dtype;
+} mt_attn_args;
+
+int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream);
+size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args);
+int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream);
+
+/*
+ * Residual and RMS norms between two blocks of a decoder (the norms that Liger
+ * replaces, setup_model_for_training.py:98-99, with the addition before them):
+ *   u = x, or x / rms(x) (weight_offset + post_weight)
+ *   new_residual = residual_scale residual + block_scale gate u
+ *   normed = new_residual / rms(new_residual) (weight_offset + weight)
+ * computed in fp32 and rounded once; rms(t) = sqrt(mean(t^2) + eps).
+ *   x, residual [T, H] with row pitches x_t, residual_t (elements); weight,
+ *     post_weight (null: none) [H]; gate by gate_mode: 0 none, 1 [H], 2 [T] with
+ *     element pitch gate_t, 3 [T, H] with row pitch gate_t
+ *   normed, new_residual [T, H] contiguous; rstd fp32 [2, T], from the forward to
+ *     the backward; H at most 32768; all tensors of one dtype
+ * The backward takes the upstream gradients dnormed and dresidual_out (null:
+ * zeros) with row pitches, reads x (with post_weight or a gate), new_residual,
+ * rstd and the weights, and writes what is not null of dx, dresidual [T, H]
+ * (contiguous), dweight, dpost_weight [H] and dgate (the gate's shape,
+ * contiguous).
+ */
+typedef struct mt_norm_args {
+  const void *x, *residual, *weight, *post_weight, *gate;
+  void *normed, *new_residual;
+  float* rstd;
+  const void *dnormed, *dresidual_out;
+  void *dx, *dresidual, *dweight, *dpost_weight, *dgate;
+  int64_t x_t, residual_t, gate_t, dnormed_t, dresidual_out_t;
+  int64_t T, H;
+  float eps, block_scale, residual_scale, weight_offset;
+  int gate_mode, dtype;
+} mt_norm_args;
+
+int mt_norm_forward(const mt_norm_args* args, mt_stream_t stream);
+size_t mt_norm_backward_workspace_bytes(int64_t T, int64_t H);
+int mt_norm_backward(const mt_norm_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream);
+
+/*
+ * The global norm of n gradients, and their scaling in place (the arithmetic of
+ * the clip_grad_norm_ at train.py:24).  Tensor i has numel[i] elements of type
+ * dtypes[i] at ptrs[i], in one run (cols[i] = 0) or in rows of cols[i] elements
+ * pitch[i] apart; the tensors must not overlap.  The five tables are host memory,
+ * read during the call.
+ *   mt_grad_norm   norm_and_coef fp32 [2] out (device): the 2-norm over all
+ *                  elements (inf_norm: the largest magnitude), and
+ *                  min(1, max_norm / (norm + 1e-6)).  Squares are summed in 64
+ *                  bits in a fixed order.
+ *   mt_grad_scale  multiplies every element by norm_and_coef[1]; touches nothing
+ *                  when that is 1.
+ */
+size_t mt_grad_norm_workspace_bytes(const int64_t* numel, int64_t n);
+int mt_grad_norm(void* const* ptrs, const int64_t* numel, const int64_t* cols,
+                 const int64_t* pitch, const int32_t* dtypes, int64_t n, int inf_norm,
+                 double max_norm, void* workspace, size_t workspace_bytes, float* norm_and_coef,
+                 mt_stream_t stream);
+int mt_grad_scale(void* const* ptrs, const int64_t* numel, const int64_t* cols,
+                  const int64_t* pitch, const int32_t* dtypes, int64_t n,
+                  const float* norm_and_coef, mt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

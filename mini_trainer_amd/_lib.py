@@ -27,6 +27,29 @@ STATUS_NAMES = {
     4: "MT_ERR_HIP",
 }
 
+
+
+class AttnArgs(ctypes.Structure):
+    """mt_attn_args of include/mt_flce.h."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv",
+                                         "plan")]
+                + [(n, c_int64) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h", "dout_t",
+                                          "dout_h", "T", "S", "heads", "kv_heads", "head_dim",
+                                          "window")]
+                + [("scale", c_float), ("softcap", c_float), ("dtype", c_int)])
+
+
+class NormArgs(ctypes.Structure):
+    """mt_norm_args of include/mt_flce.h."""
+    _fields_ = ([(n, c_void_p) for n in ("x", "residual", "weight", "post_weight", "gate", "normed",
+                                         "new_residual", "rstd", "dnormed", "dresidual_out", "dx",
+                                         "dresidual", "dweight", "dpost_weight", "dgate")]
+                + [(n, c_int64) for n in ("x_t", "residual_t", "gate_t", "dnormed_t",
+                                          "dresidual_out_t", "T", "H")]
+                + [(n, c_float) for n in ("eps", "block_scale", "residual_scale", "weight_offset")]
+                + [("gate_mode", c_int), ("dtype", c_int)])
+
+
 # name -> (restype, argtypes); mirrors include/mt_flce.h
 SIGNATURES = {
     "mt_flce_abi_version": (c_int, []),
@@ -113,6 +136,22 @@ SIGNATURES = {
     "mt_ce_check_targets": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
     "mt_ce_backward": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64,
                                c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
+    "mt_attn_plan_bytes": (c_size_t, [c_int64, c_int64]),
+    "mt_attn_plan": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t,
+                             c_void_p, c_void_p]),
+    "mt_attn_forward": (c_int, [POINTER(AttnArgs), c_void_p]),
+    "mt_attn_backward_workspace_bytes": (c_size_t, [POINTER(AttnArgs)]),
+    "mt_attn_backward": (c_int, [POINTER(AttnArgs), c_void_p, c_size_t, c_void_p]),
+    "mt_norm_forward": (c_int, [POINTER(NormArgs), c_void_p]),
+    "mt_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "mt_norm_backward": (c_int, [POINTER(NormArgs), c_void_p, c_size_t, c_void_p]),
+    "mt_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int64]),
+    "mt_grad_norm": (c_int, [POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64),
+                             POINTER(c_int64), POINTER(ctypes.c_int32), c_int64, c_int,
+                             ctypes.c_double, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "mt_grad_scale": (c_int, [POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64),
+                              POINTER(c_int64), POINTER(ctypes.c_int32), c_int64, c_void_p,
+                              c_void_p]),
 }
 
 _lib = None

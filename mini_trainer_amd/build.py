@@ -1,8 +1,9 @@
 """Build recipe for libmt_flce.so (gfx950 only).
 
-The library is one translation unit (csrc/flce_capi.hip, which includes the
-kernel headers) compiled with hipcc for gfx950 into the package directory, so
-it travels with the source tree.  `python -m mini_trainer_amd.build` rebuilds it.
+The library is two translation units (csrc/flce_capi.hip: the loss;
+csrc/step_capi.hip: attention, norms and clipping; each includes its kernels'
+headers) compiled side by side with hipcc for gfx950 and linked into the package
+directory, so it travels with the source tree.  `python -m mini_trainer_amd.build` rebuilds it.
 """
 from __future__ import annotations
 
@@ -15,7 +16,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libmt_flce.so"
-SOURCES = [CSRC / "flce_capi.hip"]
+SOURCES = [CSRC / "flce_capi.hip", CSRC / "step_capi.hip"]
 DEPENDS = sorted(CSRC.glob("*.h")) + SOURCES + [PKG_DIR.parent / "include" / "mt_flce.h"]
 
 ARCH = "gfx950"
@@ -24,7 +25,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # Packed fp32 VALU ops stay disabled in all device code of this library.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wno-unused-command-line-argument",
@@ -44,7 +44,7 @@ SAN_LIB_PATH = PKG_DIR / "_build" / "libmt_flce_san.so"
 # runs: the CPU tests exercise the argument checks, planners and error
 # paths, on a machine without a GPU).
 SAN_FLAGS = [
-    f"--offload-arch={ARCH}", "-O1", "-g", "-std=c++17", "-fPIC", "-shared",
+    f"--offload-arch={ARCH}", "-O1", "-g", "-std=c++17", "-fPIC",
     "-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
     "-Xarch_host", "-fno-sanitize-recover=all", "-Xarch_host", "-fno-omit-frame-pointer",
     "-Xarch_device", "-g0",
@@ -60,19 +60,37 @@ def san_is_stale() -> bool:
     return any(p.stat().st_mtime > t for p in DEPENDS if p.exists())
 
 
+def _compile(out: Path, flags: list, verbose: bool) -> str:
+    """Compile every source with `flags` at the same time, link them into `out`
+    and return what the compiler said."""
+    objects = PKG_DIR / "_build"
+    objects.mkdir(exist_ok=True)
+    steps = []
+    for src in SOURCES:
+        obj = objects / f"{out.stem}-{src.stem}.o"
+        cmd = [hipcc(), *flags, "-c", str(src), "-o", str(obj)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        steps.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                            text=True)))
+    said = [p.communicate()[0] for _, p in steps]  # all have ended before one may raise
+    for (_, p), text in zip(steps, said):
+        if p.returncode != 0:
+            raise RuntimeError(f"hipcc failed ({p.returncode}):\n{text}")
+    tmp = out.with_suffix(".so.tmp")
+    link = [hipcc(), *flags, "-shared", "-o", str(tmp), *(str(obj) for obj, _ in steps)]
+    proc = subprocess.run(link, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"hipcc (link) failed ({proc.returncode}):\n{proc.stderr}")
+    os.replace(tmp, out)
+    return "".join(said)
+
+
 def build_sanitized(verbose: bool = False) -> Path:
     """Compile the sanitized test build (_build/libmt_flce_san.so).  Always
     recompiles (about a minute).  Load it with the clang ASan runtime
     preloaded."""
-    SAN_LIB_PATH.parent.mkdir(exist_ok=True)
-    tmp = SAN_LIB_PATH.with_suffix(".so.tmp")
-    cmd = [hipcc(), *SAN_FLAGS, "-o", str(tmp), *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc (sanitized build) failed ({proc.returncode}):\n{proc.stderr}")
-    os.replace(tmp, SAN_LIB_PATH)
+    _compile(SAN_LIB_PATH, SAN_FLAGS, verbose)
     return SAN_LIB_PATH
 
 
@@ -88,19 +106,12 @@ def asan_runtime() -> Path:
 
 def build_library(verbose: bool = False) -> Path:
     """Compile libmt_flce.so for gfx950.  Always recompiles."""
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [hipcc(), *HIPCC_FLAGS, "-o", str(tmp), *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    said = _compile(LIB_PATH, HIPCC_FLAGS, verbose)
     # hipcc's host pass does not know the packed-fp32 feature; drop that noise.
     noise = "is not a recognized feature for this target"
-    err = "\n".join(l for l in proc.stderr.splitlines() if noise not in l)
-    if proc.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{err}")
+    err = "\n".join(l for l in said.splitlines() if noise not in l)
     if verbose and err.strip():
         print(err, file=sys.stderr)
-    os.replace(tmp, LIB_PATH)
     return LIB_PATH
 
 

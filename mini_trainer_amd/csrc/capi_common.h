@@ -1,0 +1,23 @@
+// What the translation units of libmt_flce.so share on the host side: the
+// thread's last error and the check of a launch.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace mtf {
+
+// Records the thread's last error (mt_flce_last_error) and returns `code`.
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// MT_OK, or MT_ERR_HIP if the launch just made failed (or is made to look so
+// by the test hook MT_FLCE_TEST_FAIL_LAUNCH).
+int check_launch(const char* what);
+
+}  // namespace mtf
+
+#define MT_TRY(expr)             \
+  do {                           \
+    int _rc = (expr);            \
+    if (_rc != MT_OK) return _rc; \
+  } while (0)

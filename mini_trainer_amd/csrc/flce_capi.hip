@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/mt_flce.h"
+#include "capi_common.h"
 #include "flce_kernels.h"
 #include "flce_kernels_bf16.h"
 #include "flce_kernels_f32.h"
@@ -22,8 +23,10 @@
 using namespace mtf;
 
 namespace {
-
 thread_local std::string g_last_error;
+}  // namespace
+
+namespace mtf {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -48,11 +51,9 @@ int check_launch(const char* what) {
   return MT_OK;
 }
 
-#define MT_TRY(expr)             \
-  do {                           \
-    int _rc = (expr);            \
-    if (_rc != MT_OK) return _rc; \
-  } while (0)
+}  // namespace mtf
+
+namespace {
 
 // Planning assumes the MI355X shape (256 CUs) so that the workspace queries
 // are pure functions of the problem size and can run without a device.

@@ -1,0 +1,784 @@
+// Attention over a packed row of documents (gfx950): forward, and the two
+// kernels of its backward.
+//
+// Rows are tokens; documents [ds, de) follow one another, each with a prefix
+// end pe in [ds, de].  Key j is seen by query i of the same document when
+// (j <= i or j < pe) and i - j < window.  For a fixed query these keys are one
+// range [lo, hi), for a fixed key these queries are one range, and both ends
+// grow with the row, so a tile's masks are two comparisons per element, needed
+// only in blocks that a range's end crosses.
+//
+//   z_ij = scale q_i . k_j, then cap tanh(z_ij / cap) with a softcap
+//   p_ij = exp(z_ij - lse_i),  o_i = sum_j p_ij v_j
+//   delta_i = sum_d do_id o_id,  ds_ij = p_ij (do_i . v_j - delta_i) z'_ij
+//   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+// where z' = scale, times 1 - (z / cap)^2 with a softcap.
+//
+// A workgroup owns kAttnRows rows of one document and one head (backward of
+// keys: one key head and its query heads one after the other), so that no value
+// of another document, and none behind the last one, enters its products.
+//
+// Every product is a 32 x 32 MFMA arranged so that its left operand comes from
+// an LDS tile and the softmax stays in registers: with the scores transposed
+// (keys down, the wave's 32 queries across) a lane holds 16 keys of one query,
+// which is the layout the next product wants its right operand in -- the order
+// of the summed index differs, and the left operand is read from LDS in the
+// same order.  Sums are fp32; P and dS are rounded to the inputs' type before
+// their products (bf16: at most 2^-8 of each term, as the inputs' own rounding), the row sums of P are taken before that rounding.
+#pragma once
+
+#include "flce_device.h"
+
+namespace mtf {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kAttnRows = 128;    // rows of a workgroup: 4 waves of 32
+constexpr int kAttnThreads = 256;
+constexpr int kPlanHeader = 16;   // int32 words before the plan's tiles
+constexpr int kPlanTile = 8;
+constexpr int kPlanBuckets = 1024;
+
+// One tile of the plan.  For a query tile [beg, end) are the keys its rows see,
+// for a key tile the queries that see its rows.  tail: rows behind the last
+// document, whose results are zeros.
+struct AttnTile {
+  int32_t row0, rows, ds, de, pe, beg, end, tail;
+};
+
+__device__ __forceinline__ int32_t attn_row_lo(int32_t i, int32_t ds, int32_t w) {
+  return max(ds, i - w + 1);
+}
+__device__ __forceinline__ int32_t attn_row_hi(int32_t i, int32_t pe) { return max(i + 1, pe); }
+__device__ __forceinline__ int32_t attn_col_lo(int32_t j, int32_t ds, int32_t pe) {
+  return j < pe ? ds : j;
+}
+__device__ __forceinline__ int32_t attn_col_hi(int32_t j, int32_t de, int32_t w) {
+  return j > de - w ? de : j + w;
+}
+
+// The plan: tiles of every document and of the rows behind the last one, the
+// costliest first (counting sort by the blocks a tile visits), so that the
+// workgroups dispatched last are the short ones.  One workgroup.
+//   plan: kPlanHeader words ([0] = tiles), tiles_max query tiles, tiles_max key
+//   tiles, S + 2 words of scratch.  status: 0, or 1 for cu_seqlens that are not
+//   0 = cu[0] <= ... <= cu[S] <= T, or 2 for a prefix outside its document; the
+//   plan of such a call is one tail over all T rows (status 1) or clamps the
+//   prefix (status 2), so that no kernel reads out of range.
+__global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, const int32_t* prefix,
+                                                         int32_t S, int32_t T, int32_t window,
+                                                         int32_t tiles_max, int32_t* plan,
+                                                         int32_t* status) {
+  __shared__ int32_t hist[2][kPlanBuckets];
+  __shared__ int32_t wave_sum[16];
+  __shared__ int32_t bad, bad_prefix;
+  const int32_t tid = threadIdx.x;
+  AttnTile* qt = reinterpret_cast<AttnTile*>(plan + kPlanHeader);
+  AttnTile* kt = qt + tiles_max;
+  int32_t* off = reinterpret_cast<int32_t*>(kt + tiles_max);
+  if (tid == 0) bad = cu[0] != 0 || cu[S] > T || cu[S] < 0, bad_prefix = 0;
+  hist[0][tid] = hist[1][tid] = 0;
+  __syncthreads();
+  for (int32_t s = tid; s < S; s += 1024) {
+    const int32_t a = cu[s], b = cu[s + 1];
+    if (b < a) atomicOr(&bad, 1);
+    if (prefix && (prefix[s] < 0 || prefix[s] > b - a)) atomicOr(&bad_prefix, 1);
+  }
+  __syncthreads();
+  const bool broken = bad != 0;
+  const int32_t end = broken ? 0 : cu[S];
+  if (tid == 0) *status = broken ? 1 : (bad_prefix ? 2 : 0);
+  // off[s] = first tile of document s (s == S: of the tail), off[S + 1] = tiles
+  int32_t base = 0;
+  for (int64_t s0 = 0; s0 <= S; s0 += 1024) {
+    const int64_t s = s0 + tid;
+    int32_t n = 0;
+    if (s < S && !broken) n = (cu[s + 1] - cu[s] + kAttnRows - 1) / kAttnRows;
+    if (s == S) n = (T - end + kAttnRows - 1) / kAttnRows;
+    int32_t x = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int32_t y = __shfl_up(x, d);
+      if ((tid & 63) >= d) x += y;
+    }
+    if ((tid & 63) == 63) wave_sum[tid >> 6] = x;
+    __syncthreads();
+    int32_t before = base, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < (tid >> 6)) before += wave_sum[w];
+      all += wave_sum[w];
+    }
+    if (s <= S) off[s] = before + x - n;
+    base += all;
+    __syncthreads();
+  }
+  const int32_t tiles = base;
+  if (tid == 0) plan[0] = tiles;
+  __threadfence_block();
+  __syncthreads();
+  // twice over the tiles: their costs' histogram, then their places
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int32_t t = tid; t < tiles; t += 1024) {
+      int32_t a = 0, b = S;  // the last document whose first tile is <= t
+      while (a < b) {
+        const int32_t m = a + (b - a + 1) / 2;
+        if (off[m] <= t) a = m; else b = m - 1;
+      }
+      AttnTile q;
+      q.tail = a == S;
+      q.ds = q.tail ? end : cu[a];
+      q.de = q.tail ? T : cu[a + 1];
+      q.row0 = q.ds + (t - off[a]) * kAttnRows;
+      q.rows = min(kAttnRows, q.de - q.row0);
+      q.pe = q.ds;
+      if (prefix && !q.tail) q.pe = q.ds + min(max(prefix[a], 0), q.de - q.ds);
+      AttnTile k = q;
+      const int32_t last = q.row0 + q.rows - 1;
+      q.beg = q.tail ? 0 : attn_row_lo(q.row0, q.ds, window);
+      q.end = q.tail ? 0 : attn_row_hi(last, q.pe);
+      k.beg = k.tail ? 0 : attn_col_lo(k.row0, k.ds, k.pe);
+      k.end = k.tail ? 0 : attn_col_hi(last, k.de, window);
+      const int32_t cq = min(kPlanBuckets - 1, (q.end - q.beg + 63) >> 6);
+      const int32_t ck = min(kPlanBuckets - 1, (k.end - k.beg + 63) >> 6);
+      if (pass == 0) {
+        atomicAdd(&hist[0][cq], 1);
+        atomicAdd(&hist[1][ck], 1);
+      } else {  // (the order within a bucket changes no result)
+        qt[atomicAdd(&hist[0][cq], 1)] = q;
+        kt[atomicAdd(&hist[1][ck], 1)] = k;
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {  // hist[b] -> tiles in the costlier buckets
+      for (int which = 0; which < 2; ++which) {
+        const int32_t bucket = kPlanBuckets - 1 - tid;
+        const int32_t n = hist[which][bucket];
+        int32_t x = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const int32_t y = __shfl_up(x, d);
+          if ((tid & 63) >= d) x += y;
+        }
+        if ((tid & 63) == 63) wave_sum[tid >> 6] = x;
+        __syncthreads();
+        for (int w = 0; w < (tid >> 6); ++w) x += wave_sum[w];
+        hist[which][bucket] = x - n;
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// --- tiles, fragments, products -------------------------------------------
+
+// An LDS tile of rows of DP elements in 16-byte chunks, the chunk index XORed
+// with a permutation of the row's low bits: 16 consecutive rows of one chunk
+// (the row fragments) lie in distinct 16-byte slots of a 256-byte window, and
+// so do the pieces that four consecutive rows (bf16: a transposing read of a
+// half wave) or rows four apart (fp32: a wave's column read) contribute.
+template <class T, int DP>
+struct AttnLds {
+  static constexpr uint32_t kRowB = DP * sizeof(T);
+  static constexpr uint32_t kCh = kRowB / 16;
+  __device__ __forceinline__ static uint32_t swz(uint32_t row) {
+    if constexpr (sizeof(T) == 4)
+      return (((row >> 2) & 1u) << 3) | (((row >> 3) & 1u) << 2) | (row & 3u);
+    else if constexpr (DP == 64)
+      return (((row >> 1) & 1u) << 2) | ((row >> 2) & 3u);
+    else
+      return ((row & 3u) << 2) | ((row >> 2) & 3u);
+  }
+  __device__ __forceinline__ static uint32_t off(uint32_t row, uint32_t chunk) {
+    return row * kRowB + ((chunk ^ swz(row)) << 4);
+  }
+};
+
+// The rows that a lane keeps in registers as the right operand of a product
+// over d: row (l & 31) of the wave, half of d by l >> 5.
+template <class T, int DP>
+struct AttnFrag {
+  static constexpr int kN = (int)(DP * sizeof(T) / 32);
+  u32x4_t v[kN];
+  __device__ __forceinline__ static uint32_t chunk(int t) {
+    const uint32_t h = lane_id() >> 5;
+    return sizeof(T) == 4 ? h * (uint32_t)kN + (uint32_t)t : 2u * (uint32_t)t + h;
+  }
+  // row: address of the row's first element; chunks at or beyond d_bytes are zeros.
+  __device__ __forceinline__ void load(const char* row, uint32_t d_bytes, bool valid) {
+#pragma unroll
+    for (int t = 0; t < kN; ++t) {
+      v[t] = u32x4_t{0u, 0u, 0u, 0u};
+      if (valid && chunk(t) * 16u < d_bytes)
+        v[t] = *reinterpret_cast<const u32x4_t*>(row + chunk(t) * 16u);
+    }
+  }
+};
+
+// acc[r] += sum_d tile[row0 + R(r)][d] * frag row (l & 31), R(r) = 8 (r / 4) +
+// 4 (l >> 5) + r % 4.
+template <class T, int DP>
+__device__ __forceinline__ void attn_row_product(f32x16_t& acc, const char* tile, uint32_t row0,
+                                                 const AttnFrag<T, DP>& frag) {
+  const uint32_t row = row0 + (lane_id() & 31u);
+#pragma unroll
+  for (int t = 0; t < AttnFrag<T, DP>::kN; ++t) {
+    const u32x4_t a = lds_read16(tile, AttnLds<T, DP>::off(row, AttnFrag<T, DP>::chunk(t)));
+    if constexpr (sizeof(T) == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                    __builtin_bit_cast(bf16x8_t, frag.v[t]), acc, 0,
+                                                    0, 0);
+    } else {
+      const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, frag.v[t]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], acc, 0, 0, 0);
+    }
+  }
+}
+
+typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
+
+// acc[db][r] += sum over the 32 rows of tile[row0 + row][32 db + R(r)] * w[row],
+// w held as attn_row_product leaves it (w[r] belongs to row R(r)).
+template <class T, int DP>
+__device__ __forceinline__ void attn_col_product(f32x16_t (&acc)[DP / 32], const char* tile,
+                                                 uint32_t row0, const f32x16_t& w) {
+  typedef AttnLds<T, DP> L;
+  const uint32_t l = lane_id(), h = l >> 5;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {  // rows 16 t .. + 15, slot j: row 16 t + 8 (j / 4) + 4 h + j % 4
+      u32x4_t b;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = pack_bf16x2(w[8 * t + 2 * e], w[8 * t + 2 * e + 1]);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        // a 16-lane group's lane g * 16 + i reads row (i >> 2), columns 4 (i & 3) .. + 3 of the
+        // group's 4 x 16 block and receives column i of its four rows
+        bf16x4_t a[2];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+          const uint32_t row = row0 + 16u * t + 8u * u + 4u * h + ((l & 15u) >> 2);
+          const uint32_t ch = 4u * db + 2u * ((l >> 4) & 1u) + ((l & 3u) >> 1);
+          a[u] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+              (lds_bf16x4_t*)(tile + L::off(row, ch) + (l & 1u) * 8u));
+        }
+        const bf16x8_t av = __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, __builtin_bit_cast(bf16x8_t, b),
+                                                          acc[db], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const uint32_t row = row0 + 8u * (r / 4) + 4u * h + r % 4;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        const uint32_t d = 32u * db + (l & 31u);
+        const float x = *reinterpret_cast<const float*>(tile + L::off(row, d / 4) + (d % 4) * 4u);
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, w[r], acc[db], 0, 0, 0);
+      }
+    }
+  }
+}
+
+typedef __amdgpu_buffer_rsrc_t attn_rsrc_t;
+
+// ROWS rows of a [rows, head, d] tensor on their way from memory to an LDS tile
+// through registers.  Rows at or beyond `rows` and chunks at or beyond d_bytes
+// arrive as zeros (an offset past the resource touches no memory).  The resource
+// starts at the tile's first row, so 32-bit offsets reach it wherever it lies.
+template <class T, int DP, int ROWS>
+struct AttnStage {
+  static constexpr int kN = (int)(ROWS * AttnLds<T, DP>::kCh / kAttnThreads);
+  u32x4_t v[kN];
+  __device__ __forceinline__ void load(const char* base, int32_t rows, uint32_t stride_b,
+                                       uint32_t d_bytes) {
+    const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * stride_b + d_bytes : 0u;
+    const attn_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t idx = threadIdx.x + (uint32_t)i * kAttnThreads;
+      const uint32_t row = idx / AttnLds<T, DP>::kCh, ch = idx % AttnLds<T, DP>::kCh;
+      const bool in = ch * 16u < d_bytes && (int32_t)row < rows;
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, in ? row * stride_b + ch * 16u : 0xfffffff0u, 0,
+                                                   0);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t idx = threadIdx.x + (uint32_t)i * kAttnThreads;
+      lds_write16(tile, AttnLds<T, DP>::off(idx / AttnLds<T, DP>::kCh, idx % AttnLds<T, DP>::kCh), v[i]);
+    }
+  }
+};
+
+// Sums of the two halves of the wave (a row's two lanes), in both.
+__device__ __forceinline__ float attn_pair_add(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                                  __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float attn_pair_max(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x),
+                                                  __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+
+// tanh: bf16 inputs take 1 - 2 / (exp(2x) + 1) (absolute error some 2^-23, far
+// below a score's own), fp32 the library's.
+template <class T>
+__device__ __forceinline__ float attn_tanh(float x) {
+  if constexpr (sizeof(T) == 4) return tanhf(x);
+  return fmaf(-2.0f, __builtin_amdgcn_rcpf(fast_exp2(x * (2.0f * kLog2e)) + 1.0f), 1.0f);
+}
+
+// acc^T [DP x 32 rows] * s to one row of D elements per lane.
+template <class T, int DP, class Out>
+__device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float s, Out* row,
+                                           int32_t D, bool valid) {
+  const uint32_t h = lane_id() >> 5;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int32_t d = 32 * db + 8 * g + 4 * (int32_t)h;
+      if (valid && d < D) {
+        const float x0 = acc[db][4 * g] * s, x1 = acc[db][4 * g + 1] * s;
+        const float x2 = acc[db][4 * g + 2] * s, x3 = acc[db][4 * g + 3] * s;
+        if constexpr (sizeof(Out) == 2)
+          *reinterpret_cast<u32x2_t*>(row + d) = u32x2_t{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
+        else
+          *reinterpret_cast<f32x4_t*>(row + d) = f32x4_t{x0, x1, x2, x3};
+      }
+    }
+}
+
+// rows x D zeros, rows `pitch` elements apart (D: whole 16-byte chunks).
+template <class Out>
+__device__ __forceinline__ void attn_zero_rows(Out* base, int32_t rows, int64_t pitch, int32_t D) {
+  const int32_t per = D * (int32_t)sizeof(Out) / 16;
+  for (int32_t i = threadIdx.x; i < rows * per; i += kAttnThreads)
+    *reinterpret_cast<u32x4_t*>(reinterpret_cast<char*>(base + (int64_t)(i / per) * pitch) +
+                                (i % per) * 16) = u32x4_t{0u, 0u, 0u, 0u};
+}
+
+__device__ __forceinline__ AttnTile attn_tile(const int32_t* at) {
+  AttnTile t;
+  t.row0 = __builtin_amdgcn_readfirstlane(at[0]);
+  t.rows = __builtin_amdgcn_readfirstlane(at[1]);
+  t.ds = __builtin_amdgcn_readfirstlane(at[2]);
+  t.de = __builtin_amdgcn_readfirstlane(at[3]);
+  t.pe = __builtin_amdgcn_readfirstlane(at[4]);
+  t.beg = __builtin_amdgcn_readfirstlane(at[5]);
+  t.end = __builtin_amdgcn_readfirstlane(at[6]);
+  t.tail = __builtin_amdgcn_readfirstlane(at[7]);
+  return t;
+}
+
+struct AttnArgs {
+  const char *q, *k, *v, *o, *dout;            // element (t, h, d) at t * *_t + h * *_h + d * size
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h;  // bytes
+  char *out, *dq, *dk, *dv;                    // [T, heads, D], contiguous
+  float *lse, *delta;                          // [Hq, T]; lse in units of log2
+  float* part;                                 // [hsplit][2][T][Hk][D] when hsplit > 1
+  const int32_t* plan;
+  int32_t T, Hq, Hk, G, D, tiles_max, window, hsplit;
+  float scale;     // of the scores
+  float z_mul;     // log2 units: scale log2(e), or cap log2(e) with a softcap
+  float cap_mul;   // scale / cap
+};
+
+// --- forward ----------------------------------------------------------------
+
+constexpr int kAttnKeys = 64;  // keys per block of the forward and of dQ
+
+template <class T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_fwd_kernel(AttnArgs a) {
+  typedef AttnLds<T, DP> L;
+  constexpr uint32_t kTile = kAttnKeys * L::kRowB;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];  // 2 x (K, V)
+  const uint32_t id = blockIdx.x;
+  // consecutive workgroups lie on different XCDs: with 8 key heads an XCD's L2 holds one of them
+  const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
+  const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
+  const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
+  if (ti >= a.plan[0]) return;
+  const AttnTile t = attn_tile(a.plan + kPlanHeader + (int64_t)ti * kPlanTile);
+  const int64_t o_t = (int64_t)a.Hq * a.D;
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)t.row0 * o_t + (int64_t)head * a.D;
+  float* lse = a.lse + (int64_t)head * a.T;
+  if (t.tail) {
+    attn_zero_rows(out, t.rows, o_t, a.D);
+    for (int32_t i = threadIdx.x; i < t.rows; i += kAttnThreads) lse[t.row0 + i] = 0.f;
+    return;
+  }
+  const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
+  const uint32_t d_bytes = (uint32_t)a.D * sizeof(T);
+  const int32_t r0 = t.row0 + 32 * (int32_t)w, row = r0 + (int32_t)(l & 31u);
+  const int32_t r_end = t.row0 + t.rows;
+  const bool active = r0 < r_end, valid = row < r_end;
+  const int32_t r_last = min(r0 + 31, r_end - 1);
+  // the wave's keys [w_lo, w_hi), of which every row sees [f_lo, f_hi)
+  const int32_t w_lo = attn_row_lo(r0, t.ds, a.window), w_hi = attn_row_hi(r_last, t.pe);
+  const int32_t f_lo = attn_row_lo(r_last, t.ds, a.window), f_hi = attn_row_hi(r0, t.pe);
+  const int32_t lo = attn_row_lo(row, t.ds, a.window), hi = valid ? attn_row_hi(row, t.pe) : lo;
+
+  AttnFrag<T, DP> qf;
+  qf.load(a.q + (int64_t)row * a.q_t + (int64_t)head * a.q_h, d_bytes, valid);
+  f32x16_t acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
+  float m = kNegBig, sum = 0.f;
+
+  const char* kbase = a.k + (int64_t)kvh * a.k_h;
+  const char* vbase = a.v + (int64_t)kvh * a.v_h;
+  AttnStage<T, DP, kAttnKeys> sk, sv;
+  auto fetch = [&](int32_t k0) {
+    const int32_t n = min(kAttnKeys, t.end - k0);
+    sk.load(kbase + (int64_t)k0 * a.k_t, n, (uint32_t)a.k_t, d_bytes);
+    sv.load(vbase + (int64_t)k0 * a.v_t, n, (uint32_t)a.v_t, d_bytes);
+  };
+  fetch(t.beg);
+  sk.store(smem);
+  sv.store(smem + kTile);
+  if (t.beg + kAttnKeys < t.end) fetch(t.beg + kAttnKeys);
+  uint32_t buf = 0;
+  for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
+    __syncthreads();
+    if (k0 + kAttnKeys < t.end) {  // into the buffer that every wave has left at the barrier
+      sk.store(smem + (buf ^ 1u) * 2 * kTile);
+      sv.store(smem + (buf ^ 1u) * 2 * kTile + kTile);
+      if (k0 + 2 * kAttnKeys < t.end) fetch(k0 + 2 * kAttnKeys);
+    }
+    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
+    const char* kt = smem + buf * 2 * kTile;
+    f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b) attn_row_product<T, DP>(s[b], kt, 32u * b, qf);
+    if constexpr (CAP) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[b][r] = attn_tanh<T>(s[b][r] * a.cap_mul);
+    }
+    if (k0 < f_lo || k0 + kAttnKeys > f_hi) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int32_t key = k0 + 32 * b + 8 * (r / 4) + 4 * (int32_t)h + r % 4;
+          if (key < lo || key >= hi) s[b][r] = -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    mx = attn_pair_max(mx) * a.z_mul;
+    // the running maximum moves when it has to: up to 2^8 of slack costs no
+    // precision in a floating format and saves rescaling the sums.  Each row goes
+    // by its own scores, so that no other row of the wave changes its rounding.
+    const bool grown = mx > m + 8.f;
+    if (__any(grown)) {
+      const float mn = grown ? mx : m, f = fast_exp2(m - mn);
+      m = mn;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][r] *= f;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = fast_exp2(fmaf(s[b][r], a.z_mul, -m));
+        sum += s[b][r];
+      }
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b) attn_col_product<T, DP>(acc, kt + kTile, 32u * b, s[b]);
+  }
+  sum = attn_pair_add(sum);
+  if (valid && h == 0) lse[row] = m + fast_log2(sum);
+  attn_store<T, DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + (int64_t)row * o_t + (int64_t)head * a.D,
+                    a.D, valid);
+}
+
+// --- backward: delta and dQ ---------------------------------------------------
+
+template <class T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dq_kernel(AttnArgs a) {
+  typedef AttnLds<T, DP> L;
+  constexpr uint32_t kTile = kAttnKeys * L::kRowB;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];  // 2 x (K, V)
+  const uint32_t id = blockIdx.x;
+  const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
+  const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
+  const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
+  if (ti >= a.plan[0]) return;
+  const AttnTile t = attn_tile(a.plan + kPlanHeader + (int64_t)ti * kPlanTile);
+  const int64_t o_t = (int64_t)a.Hq * a.D;
+  T* dq = reinterpret_cast<T*>(a.dq) + (int64_t)head * a.D;
+  if (t.tail) {
+    attn_zero_rows(dq + (int64_t)t.row0 * o_t, t.rows, o_t, a.D);
+    return;
+  }
+  const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
+  const uint32_t d_bytes = (uint32_t)a.D * sizeof(T);
+  const int32_t r0 = t.row0 + 32 * (int32_t)w, row = r0 + (int32_t)(l & 31u);
+  const int32_t r_end = t.row0 + t.rows;
+  const bool active = r0 < r_end, valid = row < r_end;
+  const int32_t r_last = min(r0 + 31, r_end - 1);
+  const int32_t w_lo = attn_row_lo(r0, t.ds, a.window), w_hi = attn_row_hi(r_last, t.pe);
+  const int32_t f_lo = attn_row_lo(r_last, t.ds, a.window), f_hi = attn_row_hi(r0, t.pe);
+  const int32_t lo = attn_row_lo(row, t.ds, a.window);
+  // a row that sees one key has p = 1 and ds = 0 exactly, which do . v - delta, two
+  // sums in different orders, would miss by their rounding: it counts as seeing none
+  const int32_t hi = valid && attn_row_hi(row, t.pe) - lo > 1 ? attn_row_hi(row, t.pe) : lo;
+
+  AttnFrag<T, DP> qf, dof;
+  float delta = 0.f, lse = 0.f;
+  dof.load(a.dout + (int64_t)row * a.do_t + (int64_t)head * a.do_h, d_bytes, valid);
+  {
+    AttnFrag<T, DP> of;
+    of.load(a.o + ((int64_t)row * o_t + (int64_t)head * a.D) * (int64_t)sizeof(T), d_bytes, valid);
+#pragma unroll
+    for (int i = 0; i < AttnFrag<T, DP>::kN; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = of.v[i][e], y = dof.v[i][e];
+        if constexpr (sizeof(T) == 2) {
+          delta = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), delta);
+          delta = fmaf(__uint_as_float(x & 0xffff0000u),
+                       __uint_as_float(y & 0xffff0000u), delta);
+        } else {
+          delta = fmaf(__uint_as_float(x), __uint_as_float(y), delta);
+        }
+      }
+    delta = attn_pair_add(delta);
+    if (valid) {
+      lse = a.lse[(int64_t)head * a.T + row];
+      if (h == 0) a.delta[(int64_t)head * a.T + row] = delta;
+    }
+  }
+  qf.load(a.q + (int64_t)row * a.q_t + (int64_t)head * a.q_h, d_bytes, valid);
+  f32x16_t acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
+
+  const char* kbase = a.k + (int64_t)kvh * a.k_h;
+  const char* vbase = a.v + (int64_t)kvh * a.v_h;
+  AttnStage<T, DP, kAttnKeys> sk, sv;
+  auto fetch = [&](int32_t k0) {
+    const int32_t n = min(kAttnKeys, t.end - k0);
+    sk.load(kbase + (int64_t)k0 * a.k_t, n, (uint32_t)a.k_t, d_bytes);
+    sv.load(vbase + (int64_t)k0 * a.v_t, n, (uint32_t)a.v_t, d_bytes);
+  };
+  fetch(t.beg);
+  sk.store(smem);
+  sv.store(smem + kTile);
+  if (t.beg + kAttnKeys < t.end) fetch(t.beg + kAttnKeys);
+  uint32_t buf = 0;
+  for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
+    __syncthreads();
+    if (k0 + kAttnKeys < t.end) {
+      sk.store(smem + (buf ^ 1u) * 2 * kTile);
+      sv.store(smem + (buf ^ 1u) * 2 * kTile + kTile);
+      if (k0 + 2 * kAttnKeys < t.end) fetch(k0 + 2 * kAttnKeys);
+    }
+    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
+    const char* kt = smem + buf * 2 * kTile;
+    const bool edge = k0 < f_lo || k0 + kAttnKeys > f_hi;
+#pragma unroll
+    for (uint32_t b = 0; b < 2; ++b) {
+      f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+      attn_row_product<T, DP>(s, kt, 32u * b, qf);
+      attn_row_product<T, DP>(dp, kt + kTile, 32u * b, dof);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = s[r];
+        if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
+        float d = fast_exp2(fmaf(x, a.z_mul, -lse)) * (dp[r] - delta);
+        if constexpr (CAP) d *= fmaf(-x, x, 1.0f);
+        if (edge) {
+          const int32_t key = k0 + 32 * (int32_t)b + 8 * (r / 4) + 4 * (int32_t)h + r % 4;
+          if (key < lo || key >= hi) d = 0.f;
+        }
+        s[r] = d;
+      }
+      attn_col_product<T, DP>(acc, kt, 32u * b, s);
+    }
+  }
+  attn_store<T, DP>(acc, a.scale, dq + (int64_t)row * o_t, a.D, valid);
+}
+
+// --- backward: dK and dV --------------------------------------------------------
+
+// Rows of Q and dO per block: 64, or 32 where a row takes 512 bytes of LDS.
+template <class T, int DP>
+constexpr int attn_q_rows() {
+  return sizeof(T) * DP > 256 ? 32 : 64;
+}
+
+template <class T, int DP, bool CAP>
+__global__ __launch_bounds__(kAttnThreads, 1) void attn_dkdv_kernel(AttnArgs a) {
+  typedef AttnLds<T, DP> L;
+  constexpr int kQ = attn_q_rows<T, DP>();
+  constexpr uint32_t kTile = kQ * L::kRowB;
+  constexpr uint32_t kBuf = 2 * kTile + 2 * kQ * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kBuf];  // 2 x (Q, dO, lse, delta)
+  const uint32_t id = blockIdx.x;
+  const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
+  const uint32_t hs = rest % (uint32_t)a.hsplit;
+  const int32_t ti = (int32_t)(rest / (uint32_t)a.hsplit);
+  if (ti >= a.plan[0]) return;
+  const AttnTile t = attn_tile(a.plan + kPlanHeader + ((int64_t)a.tiles_max + ti) * kPlanTile);
+  const int64_t o_t = (int64_t)a.Hk * a.D;
+  const int64_t o_at = (int64_t)t.row0 * o_t + (int64_t)kvh * a.D;
+  const int64_t part_n = (int64_t)a.T * o_t;
+  T* dk = reinterpret_cast<T*>(a.dk) + o_at;
+  T* dv = reinterpret_cast<T*>(a.dv) + o_at;
+  float* pk = a.part + (int64_t)hs * 2 * part_n + o_at;
+  float* pv = pk + part_n;
+  if (t.tail) {
+    if (a.hsplit > 1) {
+      attn_zero_rows(pk, t.rows, o_t, a.D);
+      attn_zero_rows(pv, t.rows, o_t, a.D);
+    } else {
+      attn_zero_rows(dk, t.rows, o_t, a.D);
+      attn_zero_rows(dv, t.rows, o_t, a.D);
+    }
+    return;
+  }
+  const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
+  const uint32_t d_bytes = (uint32_t)a.D * sizeof(T);
+  const int32_t j0 = t.row0 + 32 * (int32_t)w, key = j0 + (int32_t)(l & 31u);
+  const int32_t j_end = t.row0 + t.rows;
+  const bool active = j0 < j_end, valid = key < j_end;
+  const int32_t j_last = min(j0 + 31, j_end - 1);
+  // the queries [w_lo, w_hi) that see some key of the wave; [f_lo, f_hi) see all of them
+  const int32_t w_lo = attn_col_lo(j0, t.ds, t.pe), w_hi = attn_col_hi(j_last, t.de, a.window);
+  const int32_t f_lo = attn_col_lo(j_last, t.ds, t.pe), f_hi = attn_col_hi(j0, t.de, a.window);
+  const int32_t lo = attn_col_lo(key, t.ds, t.pe);
+  const int32_t hi = valid ? attn_col_hi(key, t.de, a.window) : lo;
+
+  // the queries [s_lo, s_hi) that see one key: ds = 0 exactly (attn_dq_kernel); no
+  // block with one of them is seen whole
+  int32_t s_lo = t.ds, s_hi = t.pe <= t.ds + 1 ? t.ds + 1 : t.ds;
+  if (a.window == 1) s_lo = max(t.ds, t.pe - 1), s_hi = t.de;
+
+  AttnFrag<T, DP> kf, vf;
+  kf.load(a.k + (int64_t)key * a.k_t + (int64_t)kvh * a.k_h, d_bytes, valid);
+  vf.load(a.v + (int64_t)key * a.v_t + (int64_t)kvh * a.v_h, d_bytes, valid);
+  f32x16_t ak[DP / 32], av[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) ak[i] = av[i] = f32x16_t{};
+
+  // the group's heads one after the other, each over the query blocks of [beg, end)
+  const int32_t per = (a.G + a.hsplit - 1) / a.hsplit;
+  const int32_t g0 = (int32_t)hs * per, g1 = min(a.G, g0 + per);
+  AttnStage<T, DP, kQ> sq, sdo;
+  float s_lse = 0.f, s_delta = 0.f;
+  int32_t fg = g0, fi = t.beg;  // the block to fetch next
+  auto fetch = [&]() {
+    const int64_t head = (int64_t)kvh * a.G + fg;
+    const int32_t n = min(kQ, t.end - fi);
+    sq.load(a.q + (int64_t)fi * a.q_t + head * a.q_h, n, (uint32_t)a.q_t, d_bytes);
+    sdo.load(a.dout + (int64_t)fi * a.do_t + head * a.do_h, n, (uint32_t)a.do_t, d_bytes);
+    if ((int32_t)threadIdx.x < kQ) {
+      const bool in = (int32_t)threadIdx.x < n;
+      s_lse = in ? a.lse[head * a.T + fi + threadIdx.x] : 0.f;
+      s_delta = in ? a.delta[head * a.T + fi + threadIdx.x] : 0.f;
+    }
+    fi += kQ;
+    if (fi >= t.end) fi = t.beg, ++fg;
+  };
+  auto put = [&](uint32_t buf) {
+    char* at = smem + buf * kBuf;
+    sq.store(at);
+    sdo.store(at + kTile);
+    if ((int32_t)threadIdx.x < kQ) {
+      reinterpret_cast<float*>(at + 2 * kTile)[threadIdx.x] = s_lse;
+      reinterpret_cast<float*>(at + 2 * kTile)[kQ + threadIdx.x] = s_delta;
+    }
+  };
+  const int32_t blocks = g1 > g0 ? (g1 - g0) * ((t.end - t.beg + kQ - 1) / kQ) : 0;
+  if (blocks > 0) {
+    fetch();
+    put(0);
+    if (blocks > 1) fetch();
+  }
+  uint32_t buf = 0;
+  int32_t i0 = t.beg;
+  for (int32_t n = 0; n < blocks; ++n, buf ^= 1u) {
+    __syncthreads();
+    if (n + 1 < blocks) {
+      put(buf ^ 1u);
+      if (n + 2 < blocks) fetch();
+    }
+    const char* qt = smem + buf * kBuf;
+    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
+#pragma unroll
+    for (int32_t b = 0; b < kQ / 32; ++b) {
+      const int32_t q0 = i0 + 32 * b;
+      if (!active || q0 >= w_hi || q0 + 32 <= w_lo) continue;
+      const bool edge = q0 < f_lo || q0 + 32 > f_hi;
+      f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+      attn_row_product<T, DP>(s, qt, 32u * b, kf);
+      attn_row_product<T, DP>(dp, qt + kTile, 32u * b, vf);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(rows + 32 * b + 8 * g + 4 * h);
+        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(rows + kQ + 32 * b + 8 * g + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          float x = s[r];
+          if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
+          float p = fast_exp2(fmaf(x, a.z_mul, -lse[e]));
+          float d = p * (dp[r] - delta[e]);
+          if constexpr (CAP) d *= fmaf(-x, x, 1.0f);
+          if (edge) {
+            const int32_t q = q0 + 8 * g + 4 * (int32_t)h + e;
+            if (q < lo || q >= hi) p = d = 0.f;
+            if (q >= s_lo && q < s_hi) d = 0.f;
+          }
+          s[r] = p;
+          dp[r] = d;
+        }
+      }
+      attn_col_product<T, DP>(av, qt + kTile, 32u * b, s);
+      attn_col_product<T, DP>(ak, qt, 32u * b, dp);
+    }
+    i0 += kQ;
+    if (i0 >= t.end) i0 = t.beg;
+  }
+  const int64_t at = (int64_t)(key - t.row0) * o_t;
+  if (a.hsplit > 1) {
+    attn_store<T, DP>(ak, a.scale, pk + at, a.D, valid);
+    attn_store<T, DP>(av, 1.0f, pv + at, a.D, valid);
+  } else {
+    attn_store<T, DP>(ak, a.scale, dk + at, a.D, valid);
+    attn_store<T, DP>(av, 1.0f, dv + at, a.D, valid);
+  }
+}
+
+// dK and dV as the sums of their parts over the head groups, in order; four
+// elements per thread.
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* part, int32_t hsplit, int64_t n,
+                                                        T* dk, T* dv) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= 2 * n) return;
+  f32x4_t x = *reinterpret_cast<const f32x4_t*>(part + i);
+  for (int32_t s = 1; s < hsplit; ++s)
+    x += *reinterpret_cast<const f32x4_t*>(part + (int64_t)s * 2 * n + i);
+  T* to = i < n ? dk + i : dv + (i - n);
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+  else
+    *reinterpret_cast<f32x4_t*>(to) = x;
+}
+
+}  // namespace mtf

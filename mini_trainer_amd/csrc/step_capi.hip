@@ -1,0 +1,495 @@
+// C ABI of libmt_flce.so, the operators of a packed training step around the
+// loss: attention, residual and norms, gradient norm and clipping.
+// Declarations and contracts: include/mt_flce.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+#include "../../include/mt_flce.h"
+#include "capi_common.h"
+#include "step_attention.h"
+#include "step_clip.h"
+#include "step_norm.h"
+
+using namespace mtf;
+
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int esize(int dtype) {
+  return dtype == MT_DTYPE_BF16 ? 2 : (dtype == MT_DTYPE_F32 ? 4 : 0);
+}
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// --- attention ---------------------------------------------------------------
+
+constexpr int64_t kMaxRows = INT32_MAX - 1024;  // row numbers, plus a block, in 32 bits
+
+// Tiles of a plan at most: every document and the tail end in a partial one.
+inline int64_t attn_tiles(int64_t T, int64_t S) { return cdiv(T, kAttnRows) + S + 1; }
+
+inline size_t plan_bytes(int64_t T, int64_t S) {
+  return 4 * ((size_t)kPlanHeader + 2 * (size_t)kPlanTile * attn_tiles(T, S) + (size_t)S + 2);
+}
+
+// Groups of query heads whose dK, dV are formed by workgroups of their own and
+// joined: as many as give each CU some three workgroups.
+int32_t attn_hsplit(const mt_attn_args& a) {
+  const int64_t groups = cdiv(a.T, kAttnRows) * a.kv_heads, G = a.heads / a.kv_heads;
+  if (groups <= 0) return 1;
+  const int64_t want = std::min<int64_t>(G, cdiv(768, groups));
+  return (int32_t)cdiv(G, cdiv(G, want));
+}
+
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t attn_part_bytes(const mt_attn_args& a) {
+  const int32_t hs = attn_hsplit(a);
+  return hs > 1 ? (size_t)hs * 2 * (size_t)a.T * (size_t)a.kv_heads * (size_t)a.head_dim * 4 : 0;
+}
+
+int attn_check(const mt_attn_args* p, bool backward) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_attn_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.T < 0 || a.T > kMaxRows || a.S < 0 || a.S > kMaxRows)
+    return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld or S=%lld out of range", (long long)a.T, (long long)a.S);
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads > 65536 || a.heads % a.kv_heads != 0)
+    return fail(MT_ERR_INVALID_ARGUMENT, "heads=%lld must be a positive multiple of kv_heads=%lld",
+                (long long)a.heads, (long long)a.kv_heads);
+  if (a.head_dim <= 0 || a.head_dim % (16 / es) != 0)
+    return fail(MT_ERR_UNSUPPORTED, "head_dim=%lld must be whole 16-byte chunks (pad the rows)",
+                (long long)a.head_dim);
+  if (a.head_dim > 128)
+    return fail(MT_ERR_UNSUPPORTED, "head_dim=%lld is above 128", (long long)a.head_dim);
+  if (a.window < 1 || a.window > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
+    return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
+  if (attn_tiles(a.T, a.S) * a.heads > INT32_MAX)
+    return fail(MT_ERR_UNSUPPORTED, "%lld tiles x %lld heads exceed one launch",
+                (long long)attn_tiles(a.T, a.S), (long long)a.heads);
+  const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
+                             backward ? a.dout_h : 0};
+  for (int64_t s : strides)
+    if (s < 0 || (s * es) % 16 != 0)
+      return fail(MT_ERR_INVALID_ARGUMENT, "strides must be whole 16-byte chunks, not negative");
+  for (int i = 0; i < 8; i += 2)
+    if (strides[i] > (int64_t)1 << 24)
+      return fail(MT_ERR_UNSUPPORTED, "rows %lld elements apart: at most 2^24", (long long)strides[i]);
+  if (a.T == 0) return MT_OK;
+  const void* need[] = {a.q, a.k, a.v, a.out, a.lse, a.plan};
+  for (const void* x : need)
+    if (!x || !aligned16(x))
+      return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned (16 bytes) tensor pointer");
+  if (backward) {
+    const void* more[] = {a.dout, a.dq, a.dk, a.dv};
+    for (const void* x : more)
+      if (!x || !aligned16(x))
+        return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned (16 bytes) gradient pointer");
+  }
+  return MT_OK;
+}
+
+AttnArgs attn_args(const mt_attn_args& a) {
+  const int64_t es = esize(a.dtype);
+  AttnArgs k{};
+  k.q = static_cast<const char*>(a.q);
+  k.k = static_cast<const char*>(a.k);
+  k.v = static_cast<const char*>(a.v);
+  k.o = static_cast<const char*>(a.out);
+  k.dout = static_cast<const char*>(a.dout);
+  k.q_t = a.q_t * es, k.q_h = a.q_h * es, k.k_t = a.k_t * es, k.k_h = a.k_h * es;
+  k.v_t = a.v_t * es, k.v_h = a.v_h * es, k.do_t = a.dout_t * es, k.do_h = a.dout_h * es;
+  k.out = static_cast<char*>(a.out);
+  k.dq = static_cast<char*>(a.dq);
+  k.dk = static_cast<char*>(a.dk);
+  k.dv = static_cast<char*>(a.dv);
+  k.lse = a.lse;
+  k.plan = a.plan;
+  k.T = (int32_t)a.T;
+  k.Hq = (int32_t)a.heads;
+  k.Hk = (int32_t)a.kv_heads;
+  k.G = k.Hq / k.Hk;
+  k.D = (int32_t)a.head_dim;
+  k.tiles_max = (int32_t)attn_tiles(a.T, a.S);
+  k.window = (int32_t)a.window;
+  k.hsplit = 1;
+  k.scale = a.scale;
+  k.z_mul = (a.softcap > 0.f ? a.softcap : a.scale) * kLog2e;
+  k.cap_mul = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  return k;
+}
+
+// kernel<T, DP, CAP> for a type, head width and softcap.
+#define MT_ATTN_PICK(kernel, dtype, D, cap)                                                       \
+  ((dtype) == MT_DTYPE_BF16                                                                       \
+       ? ((D) <= 64 ? ((cap) ? kernel<__bf16, 64, true> : kernel<__bf16, 64, false>)              \
+                    : ((cap) ? kernel<__bf16, 128, true> : kernel<__bf16, 128, false>))           \
+       : ((D) <= 64 ? ((cap) ? kernel<float, 64, true> : kernel<float, 64, false>)                \
+                    : ((cap) ? kernel<float, 128, true> : kernel<float, 128, false>)))
+
+// --- residual and norms --------------------------------------------------------
+
+struct NormShape {
+  int tpr, rows;
+};
+
+// Calls f with the kernels' template arguments for a row of H elements: the
+// fewest threads and registers that hold it (vec: rows of whole aligned 16-byte
+// vectors).
+template <class T, class F>
+int norm_pick(int64_t H, bool vec, F f) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (vec) {
+    if (H <= 64 * 2 * V) return f(std::integral_constant<int, V>(), std::integral_constant<int, 2>(),
+                                  std::integral_constant<int, 64>());
+    if (H <= 256 * 1 * V) return f(std::integral_constant<int, V>(), std::integral_constant<int, 1>(),
+                                   std::integral_constant<int, 256>());
+    if (H <= 256 * 2 * V) return f(std::integral_constant<int, V>(), std::integral_constant<int, 2>(),
+                                   std::integral_constant<int, 256>());
+    if (H <= 256 * 4 * V) return f(std::integral_constant<int, V>(), std::integral_constant<int, 4>(),
+                                   std::integral_constant<int, 256>());
+    if (H <= 1024 * 4 * V) return f(std::integral_constant<int, V>(), std::integral_constant<int, 4>(),
+                                    std::integral_constant<int, 1024>());
+  }
+  if (H <= 256 * 8) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 8>(),
+                             std::integral_constant<int, 256>());
+  if (H <= 256 * 32) return f(std::integral_constant<int, 1>(), std::integral_constant<int, 32>(),
+                              std::integral_constant<int, 256>());
+  return f(std::integral_constant<int, 1>(), std::integral_constant<int, 32>(),
+           std::integral_constant<int, 1024>());
+}
+
+constexpr int64_t kNormMaxH = 1024 * 32;
+constexpr int64_t kNormGroups = 512;  // workgroups that sum weight gradients
+
+// Rows at a time of the backward, and so partial rows of the weight gradients:
+// at most kNormGroups workgroups of up to four rows each.
+int64_t norm_parts(int64_t T) { return std::max<int64_t>(4, std::min<int64_t>(cdiv(T, 4), kNormGroups) * 4); }
+
+int norm_check(const mt_norm_args* p, bool backward) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_norm_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.T < 0 || a.T > kMaxRows) return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld out of range", (long long)a.T);
+  if (a.H <= 0) return fail(MT_ERR_INVALID_ARGUMENT, "H=%lld out of range", (long long)a.H);
+  if (a.H > kNormMaxH)
+    return fail(MT_ERR_UNSUPPORTED, "H=%lld is above %lld", (long long)a.H, (long long)kNormMaxH);
+  if (a.gate_mode < 0 || a.gate_mode > 3 || (a.gate_mode != 0) != (a.gate != nullptr))
+    return fail(MT_ERR_INVALID_ARGUMENT, "gate_mode=%d does not fit the gate pointer", a.gate_mode);
+  if (!(a.eps >= 0.f) || !std::isfinite(a.eps) || !std::isfinite(a.block_scale) ||
+      !std::isfinite(a.residual_scale) || !std::isfinite(a.weight_offset))
+    return fail(MT_ERR_INVALID_ARGUMENT, "eps must be >= 0 and the scales finite");
+  if (a.x_t < a.H || a.residual_t < a.H || (a.gate_mode == 3 && a.gate_t < a.H) ||
+      (a.gate_mode == 2 && a.gate_t < 1) ||
+      (backward && ((a.dnormed && a.dnormed_t < a.H) || (a.dresidual_out && a.dresidual_out_t < a.H))))
+    return fail(MT_ERR_INVALID_ARGUMENT, "row pitches must be >= H");
+  if (a.T == 0) return MT_OK;
+  if (!a.weight || !a.rstd || !a.new_residual || (!backward && (!a.x || !a.residual || !a.normed)) ||
+      (backward && (!a.dnormed || ((a.post_weight || a.gate) && !a.x))))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  const void* all[] = {a.x, a.residual, a.weight, a.post_weight, a.gate, a.normed, a.new_residual,
+                       a.dnormed, a.dresidual_out, a.dx, a.dresidual, a.dgate};
+  for (const void* x : all)
+    if (reinterpret_cast<uintptr_t>(x) % es != 0)
+      return fail(MT_ERR_INVALID_ARGUMENT, "tensors must be aligned to their element size");
+  return MT_OK;
+}
+
+// Whether every row of every tensor is whole aligned 16-byte vectors.
+bool norm_vectors(const mt_norm_args& a) {
+  const int64_t V = 16 / esize(a.dtype);
+  const void* all[] = {a.x, a.residual, a.weight, a.post_weight, a.gate_mode == 2 ? nullptr : a.gate,
+                       a.normed, a.new_residual, a.dnormed, a.dresidual_out, a.dx, a.dresidual,
+                       a.gate_mode == 2 ? nullptr : a.dgate};
+  for (const void* x : all)
+    if (!aligned16(x)) return false;
+  return a.H % V == 0 && a.x_t % V == 0 && a.residual_t % V == 0 &&
+         (a.gate_mode != 3 || a.gate_t % V == 0) && a.dnormed_t % V == 0 && a.dresidual_out_t % V == 0;
+}
+
+NormArgs norm_args(const mt_norm_args& a) {
+  NormArgs k{};
+  k.x = static_cast<const char*>(a.x);
+  k.residual = static_cast<const char*>(a.residual);
+  k.w = static_cast<const char*>(a.weight);
+  k.pw = static_cast<const char*>(a.post_weight);
+  k.gate = static_cast<const char*>(a.gate);
+  k.dy = static_cast<const char*>(a.dnormed);
+  k.dh = static_cast<const char*>(a.dresidual_out);
+  k.h = static_cast<const char*>(a.new_residual);
+  k.y = static_cast<char*>(a.normed);
+  k.h_out = static_cast<char*>(a.new_residual);
+  k.dx = static_cast<char*>(a.dx);
+  k.dresidual = static_cast<char*>(a.dresidual);
+  k.dgate = static_cast<char*>(a.dgate);
+  k.rstd = a.rstd;
+  k.x_t = a.x_t, k.r_t = a.residual_t, k.gate_t = a.gate_t;
+  k.dy_t = a.dnormed_t, k.dh_t = a.dresidual_out_t, k.h_t = a.H;
+  k.T = a.T;
+  k.H = (int32_t)a.H;
+  k.gate_mode = a.gate_mode;
+  k.eps = a.eps;
+  k.block_scale = a.block_scale;
+  k.residual_scale = a.residual_scale;
+  k.offset = a.weight_offset;
+  return k;
+}
+
+template <class T>
+int launch_norm_fwd(const NormArgs& k, bool vec, hipStream_t stream) {
+  return norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+    constexpr int threads = norm_threads(decltype(TPR)::value);
+    constexpr int rows = threads / decltype(TPR)::value;
+    hipLaunchKernelGGL((norm_fwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value>),
+                       dim3((uint32_t)cdiv(k.T, rows)), dim3(threads), 0, stream, k);
+    return check_launch("norm_fwd_kernel");
+  });
+}
+
+template <class T>
+int launch_norm_bwd(NormArgs k, const mt_norm_args& a, bool vec, hipStream_t stream) {
+  const int rc = norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+    constexpr int threads = norm_threads(decltype(TPR)::value);
+    constexpr int rows = threads / decltype(TPR)::value;
+    const int64_t groups = std::min<int64_t>(cdiv(k.T, rows), kNormGroups);
+    k.parts = (int32_t)(groups * rows);
+    auto kern = (k.pw || k.gate)
+                    ? norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, true>
+                    : norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, false>;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)groups), dim3(threads), 0, stream, k);
+    return check_launch("norm_bwd_kernel");
+  });
+  if (rc != MT_OK) return rc;
+  T* dgate = k.gate_mode == 1 ? static_cast<T*>(a.dgate) : nullptr;
+  T* dpw = k.pw ? static_cast<T*>(a.dpost_weight) : nullptr;
+  if (!a.dweight && !dpw && !dgate) return MT_OK;
+  hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((uint32_t)cdiv(k.H, 64), dgate ? 3 : dpw ? 2 : 1),
+                     dim3(1024), 0, stream, k.part, k.parts, k.H, static_cast<T*>(a.dweight), dpw, dgate);
+  return check_launch("norm_columns_kernel");
+}
+
+// --- gradient norm and clipping --------------------------------------------------
+
+// Elements per workgroup: the smallest chunk that keeps the sums of a call
+// within 16384.
+int64_t clip_chunk(const int64_t* numel, int64_t n) {
+  int64_t chunk = 16384;
+  for (;; chunk *= 2) {
+    int64_t chunks = 0;
+    for (int64_t i = 0; i < n; ++i) chunks += cdiv(numel[i], chunk);
+    if (chunks <= 16384 + n) return chunk;
+  }
+}
+
+int clip_check(void* const* ptrs, const int64_t* numel, const int64_t* cols, const int64_t* pitch,
+               const int32_t* dtypes, int64_t n) {
+  if (n < 0 || n > (1 << 24)) return fail(MT_ERR_INVALID_ARGUMENT, "n=%lld out of range", (long long)n);
+  if (n > 0 && (!ptrs || !numel || !cols || !pitch || !dtypes))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null table");
+  for (int64_t i = 0; i < n; ++i) {
+    const int es = esize(dtypes[i]);
+    if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "tensor %lld: dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16",
+                         (long long)i, dtypes[i]);
+    if (numel[i] < 0 || numel[i] > (int64_t)1 << 40 || (numel[i] > 0 && !ptrs[i]) ||
+        reinterpret_cast<uintptr_t>(ptrs[i]) % es != 0)
+      return fail(MT_ERR_INVALID_ARGUMENT, "tensor %lld: bad size or pointer", (long long)i);
+    if (cols[i] < 0 || (cols[i] > 0 && (pitch[i] < cols[i] || numel[i] % cols[i] != 0)))
+      return fail(MT_ERR_INVALID_ARGUMENT, "tensor %lld: rows of %lld elements, %lld apart", (long long)i,
+                  (long long)cols[i], (long long)pitch[i]);
+  }
+  return MT_OK;
+}
+
+// Calls launch(table, chunks, first chunk of the call) for the tensors in
+// groups of up to kClipTensors.
+template <class F>
+int clip_groups(void* const* ptrs, const int64_t* numel, const int64_t* cols, const int64_t* pitch,
+                const int32_t* dtypes, int64_t n, F launch) {
+  const int64_t chunk = clip_chunk(numel, n);
+  int64_t done = 0;
+  for (int64_t at = 0; at < n;) {
+    ClipTable t;
+    t.n = 0;
+    t.chunk = (int32_t)std::min<int64_t>(chunk, 1 << 30);
+    uint32_t chunks = 0;
+    while (at < n && t.n < kClipTensors) {
+      if (numel[at] > 0) {
+        t.ptr[t.n] = static_cast<char*>(ptrs[at]);
+        t.numel[t.n] = numel[at];
+        t.cols[t.n] = cols[at] == numel[at] ? 0 : cols[at];
+        t.pitch[t.n] = pitch[at];
+        t.bf16[t.n] = dtypes[at] == MT_DTYPE_BF16;
+        t.first[t.n] = chunks;
+        chunks += (uint32_t)cdiv(numel[at], t.chunk);
+        ++t.n;
+      }
+      ++at;
+    }
+    t.first[t.n] = chunks;
+    if (chunks) MT_TRY(launch(t, chunks, done));
+    done += chunks;
+  }
+  return MT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mt_attn_plan_bytes(int64_t T, int64_t S) {
+  return T < 0 || T > kMaxRows || S < 0 || S > kMaxRows ? 0 : plan_bytes(T, S);
+}
+
+int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t S, int64_t T,
+                 int64_t window, int32_t* plan, size_t plan_size, int32_t* status, mt_stream_t stream) {
+  if (T < 0 || T > kMaxRows || S < 0 || S > kMaxRows || attn_tiles(T, S) > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "bad sizes T=%lld S=%lld", (long long)T, (long long)S);
+  if (window < 1 || window > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)window);
+  if (!cu_seqlens || !plan || !status) return fail(MT_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!aligned16(plan)) return fail(MT_ERR_INVALID_ARGUMENT, "plan must be 16-byte aligned");
+  if (plan_size < plan_bytes(T, S))
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "plan: %zu bytes, %zu needed", plan_size, plan_bytes(T, S));
+  hipLaunchKernelGGL(attn_plan_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, cu_seqlens,
+                     prefix_lens, (int32_t)S, (int32_t)T, (int32_t)window, (int32_t)attn_tiles(T, S),
+                     plan, status);
+  return check_launch("attn_plan_kernel");
+}
+
+int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
+  MT_TRY(attn_check(args, false));
+  const mt_attn_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const AttnArgs k = attn_args(a);
+  auto kern = MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, a.softcap > 0.f);
+  hipLaunchKernelGGL(kern, dim3((uint32_t)(k.tiles_max * k.Hq)), dim3(kAttnThreads), 0,
+                     (hipStream_t)stream, k);
+  return check_launch("attn_fwd_kernel");
+}
+
+size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args) {
+  if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0) return 0;
+  return round256((size_t)args->heads * (size_t)args->T * 4) + attn_part_bytes(*args);
+}
+
+int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream) {
+  MT_TRY(attn_check(args, true));
+  const mt_attn_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const size_t need = mt_attn_backward_workspace_bytes(args);
+  if (!workspace || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
+  if (workspace_bytes < need)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
+  AttnArgs k = attn_args(a);
+  k.delta = static_cast<float*>(workspace);
+  k.part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                    round256((size_t)a.heads * (size_t)a.T * 4));
+  k.hsplit = attn_hsplit(a);
+  const bool cap = a.softcap > 0.f;
+  hipStream_t s = (hipStream_t)stream;
+  auto dq = MT_ATTN_PICK(attn_dq_kernel, a.dtype, a.head_dim, cap);
+  hipLaunchKernelGGL(dq, dim3((uint32_t)(k.tiles_max * k.Hq)), dim3(kAttnThreads), 0, s, k);
+  MT_TRY(check_launch("attn_dq_kernel"));
+  auto dkdv = MT_ATTN_PICK(attn_dkdv_kernel, a.dtype, a.head_dim, cap);
+  hipLaunchKernelGGL(dkdv, dim3((uint32_t)(k.tiles_max * k.Hk * k.hsplit)), dim3(kAttnThreads), 0, s, k);
+  MT_TRY(check_launch("attn_dkdv_kernel"));
+  if (k.hsplit == 1) return MT_OK;
+  const int64_t n = a.T * a.kv_heads * a.head_dim;
+  const dim3 grid((uint32_t)cdiv(2 * n, 1024));
+  if (a.dtype == MT_DTYPE_BF16)
+    hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
+                       reinterpret_cast<__bf16*>(k.dk), reinterpret_cast<__bf16*>(k.dv));
+  else
+    hipLaunchKernelGGL(attn_join_kernel<float>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
+                       reinterpret_cast<float*>(k.dk), reinterpret_cast<float*>(k.dv));
+  return check_launch("attn_join_kernel");
+}
+
+int mt_norm_forward(const mt_norm_args* args, mt_stream_t stream) {
+  MT_TRY(norm_check(args, false));
+  const mt_norm_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const NormArgs k = norm_args(a);
+  return a.dtype == MT_DTYPE_BF16 ? launch_norm_fwd<__bf16>(k, norm_vectors(a), (hipStream_t)stream)
+                                  : launch_norm_fwd<float>(k, norm_vectors(a), (hipStream_t)stream);
+}
+
+size_t mt_norm_backward_workspace_bytes(int64_t T, int64_t H) {
+  return T <= 0 || H <= 0 || H > kNormMaxH ? 0 : (size_t)3 * norm_parts(T) * (size_t)H * 4;
+}
+
+int mt_norm_backward(const mt_norm_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream) {
+  MT_TRY(norm_check(args, true));
+  const mt_norm_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const size_t need = mt_norm_backward_workspace_bytes(a.T, a.H);
+  if (!workspace || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
+  if (workspace_bytes < need)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
+  NormArgs k = norm_args(a);
+  k.part = static_cast<float*>(workspace);
+  return a.dtype == MT_DTYPE_BF16 ? launch_norm_bwd<__bf16>(k, a, norm_vectors(a), (hipStream_t)stream)
+                                  : launch_norm_bwd<float>(k, a, norm_vectors(a), (hipStream_t)stream);
+}
+
+size_t mt_grad_norm_workspace_bytes(const int64_t* numel, int64_t n) {
+  if (!numel || n <= 0) return 8;
+  const int64_t chunk = clip_chunk(numel, n);
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < n; ++i) chunks += cdiv(numel[i], chunk);
+  return 8 * (size_t)std::max<int64_t>(1, chunks);
+}
+
+int mt_grad_norm(void* const* ptrs, const int64_t* numel, const int64_t* cols, const int64_t* pitch,
+                 const int32_t* dtypes, int64_t n, int inf_norm, double max_norm, void* workspace,
+                 size_t workspace_bytes, float* out, mt_stream_t stream) {
+  MT_TRY(clip_check(ptrs, numel, cols, pitch, dtypes, n));
+  if (!(max_norm >= 0.0)) return fail(MT_ERR_INVALID_ARGUMENT, "max_norm must be >= 0");
+  if (!workspace || !out || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace or result");
+  const size_t need = mt_grad_norm_workspace_bytes(numel, n);
+  if (workspace_bytes < need)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
+  hipStream_t s = (hipStream_t)stream;
+  double* parts = static_cast<double*>(workspace);
+  int64_t total = 0;
+  MT_TRY(clip_groups(ptrs, numel, cols, pitch, dtypes, n, [&](const ClipTable& t, uint32_t chunks,
+                                                              int64_t first) {
+    if (inf_norm)
+      hipLaunchKernelGGL(clip_norm_kernel<true>, dim3(chunks), dim3(256), 0, s, t, parts + first);
+    else
+      hipLaunchKernelGGL(clip_norm_kernel<false>, dim3(chunks), dim3(256), 0, s, t, parts + first);
+    total = first + chunks;
+    return check_launch("clip_norm_kernel");
+  }));
+  if (inf_norm)
+    hipLaunchKernelGGL(clip_join_kernel<true>, dim3(1), dim3(1024), 0, s, parts, total, max_norm, out);
+  else
+    hipLaunchKernelGGL(clip_join_kernel<false>, dim3(1), dim3(1024), 0, s, parts, total, max_norm, out);
+  return check_launch("clip_join_kernel");
+}
+
+int mt_grad_scale(void* const* ptrs, const int64_t* numel, const int64_t* cols, const int64_t* pitch,
+                  const int32_t* dtypes, int64_t n, const float* norm_and_coef, mt_stream_t stream) {
+  MT_TRY(clip_check(ptrs, numel, cols, pitch, dtypes, n));
+  if (!norm_and_coef) return fail(MT_ERR_INVALID_ARGUMENT, "null pointer argument");
+  return clip_groups(ptrs, numel, cols, pitch, dtypes, n,
+                     [&](const ClipTable& t, uint32_t chunks, int64_t) {
+                       hipLaunchKernelGGL(clip_scale_kernel, dim3(chunks), dim3(256), 0,
+                                          (hipStream_t)stream, t, norm_and_coef);
+                       return check_launch("clip_scale_kernel");
+                     });
+}
+
+}  // extern "C"

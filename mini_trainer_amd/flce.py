@@ -8,6 +8,7 @@ tensors or a missing library raise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional, Tuple
@@ -45,7 +46,7 @@ def _dtype_code(dt: torch.dtype) -> int:
         return MT_DTYPE_BF16
     if dt == torch.float32:
         return MT_DTYPE_F32
-    raise TypeError(f"fused linear cross-entropy supports bfloat16 and float32, got {dt}")
+    raise TypeError(f"bfloat16 and float32 are supported, got {dt}")
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -58,10 +59,18 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _on_device(device: torch.device):
+    """Makes `device` the current one where it is not: a launch goes to the
+    stream's device only from there."""
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
 def _require_device(name: str, t: torch.Tensor) -> None:
     if not t.is_cuda:
         raise RuntimeError(
-            f"{name} must be a ROCm device tensor; the fused linear cross-entropy has no CPU path"
+            f"{name} must be a ROCm device tensor; mini_trainer_amd has no CPU path"
         )
 
 
