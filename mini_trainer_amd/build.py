@@ -1,8 +1,8 @@
 """Build recipe for libmt_flce.so (gfx950 only).
 
-The library is two translation units (csrc/flce_capi.hip: the loss;
-csrc/step_capi.hip: attention, norms and clipping; each includes its kernels'
-headers) compiled side by side with hipcc for gfx950 and linked into the package
+The library is three translation units (csrc/flce_capi.hip: the loss;
+csrc/attn_capi.hip: attention; csrc/step_capi.hip: norms and clipping; each
+includes its kernels' headers) compiled side by side with hipcc for gfx950 and linked into the package
 directory, so it travels with the source tree.  `python -m mini_trainer_amd.build` rebuilds it.
 """
 from __future__ import annotations
@@ -16,7 +16,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libmt_flce.so"
-SOURCES = [CSRC / "flce_capi.hip", CSRC / "step_capi.hip"]
+SOURCES = [CSRC / "flce_capi.hip", CSRC / "attn_capi.hip", CSRC / "step_capi.hip"]
 DEPENDS = sorted(CSRC.glob("*.h")) + SOURCES + [PKG_DIR.parent / "include" / "mt_flce.h"]
 
 ARCH = "gfx950"

@@ -1,0 +1,198 @@
+// C ABI of libmt_flce.so, attention over a packed row.  Declarations and
+// contracts: include/mt_flce.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mt_flce.h"
+#include "capi_common.h"
+#include "attn_kernels.h"
+
+using namespace mtf;
+
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles of a plan at most: every document and the tail end in a partial one.
+inline int64_t attn_tiles(int64_t T, int64_t S) { return cdiv(T, kAttnRows) + S + 1; }
+
+inline size_t plan_bytes(int64_t T, int64_t S) {
+  return 4 * ((size_t)kPlanHeader + 2 * (size_t)kPlanTile * attn_tiles(T, S) + (size_t)S + 2);
+}
+
+// Groups of query heads whose dK, dV are formed by workgroups of their own and
+// joined: as many as give each CU some three workgroups.
+int32_t attn_hsplit(const mt_attn_args& a) {
+  const int64_t groups = cdiv(a.T, kAttnRows) * a.kv_heads, G = a.heads / a.kv_heads;
+  if (groups <= 0) return 1;
+  const int64_t want = std::min<int64_t>(G, cdiv(2048, groups));
+  return (int32_t)cdiv(G, cdiv(G, want));
+}
+
+inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t attn_part_bytes(const mt_attn_args& a) {
+  const int32_t hs = attn_hsplit(a);
+  return hs > 1 ? (size_t)hs * 2 * (size_t)a.T * (size_t)a.kv_heads * (size_t)a.head_dim * 4 : 0;
+}
+
+int attn_check(const mt_attn_args* p, bool backward) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_attn_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.T < 0 || a.T > kMaxRows || a.S < 0 || a.S > kMaxRows)
+    return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld or S=%lld out of range", (long long)a.T, (long long)a.S);
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads > 65536 || a.heads % a.kv_heads != 0)
+    return fail(MT_ERR_INVALID_ARGUMENT, "heads=%lld must be a positive multiple of kv_heads=%lld",
+                (long long)a.heads, (long long)a.kv_heads);
+  if (a.head_dim <= 0 || a.head_dim % (16 / es) != 0)
+    return fail(MT_ERR_UNSUPPORTED, "head_dim=%lld must be whole 16-byte chunks (pad the rows)",
+                (long long)a.head_dim);
+  if (a.head_dim > 128)
+    return fail(MT_ERR_UNSUPPORTED, "head_dim=%lld is above 128", (long long)a.head_dim);
+  if (a.window < 1 || a.window > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
+  if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
+    return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
+  if (attn_tiles(a.T, a.S) * a.heads > INT32_MAX)
+    return fail(MT_ERR_UNSUPPORTED, "%lld tiles x %lld heads exceed one launch",
+                (long long)attn_tiles(a.T, a.S), (long long)a.heads);
+  const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
+                             backward ? a.dout_h : 0};
+  for (int64_t s : strides)
+    if (s < 0 || (s * es) % 16 != 0)
+      return fail(MT_ERR_INVALID_ARGUMENT, "strides must be whole 16-byte chunks, not negative");
+  for (int i = 0; i < 8; i += 2)
+    if (strides[i] > (int64_t)1 << 24)
+      return fail(MT_ERR_UNSUPPORTED, "rows %lld elements apart: at most 2^24", (long long)strides[i]);
+  if (a.T == 0) return MT_OK;
+  const void* need[] = {a.q, a.k, a.v, a.out, a.lse, a.plan};
+  for (const void* x : need)
+    if (!x || !aligned16(x))
+      return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned (16 bytes) tensor pointer");
+  if (backward) {
+    const void* more[] = {a.dout, a.dq, a.dk, a.dv};
+    for (const void* x : more)
+      if (!x || !aligned16(x))
+        return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned (16 bytes) gradient pointer");
+  }
+  return MT_OK;
+}
+
+AttnArgs attn_args(const mt_attn_args& a) {
+  const int64_t es = esize(a.dtype);
+  AttnArgs k{};
+  k.q = static_cast<const char*>(a.q);
+  k.k = static_cast<const char*>(a.k);
+  k.v = static_cast<const char*>(a.v);
+  k.o = static_cast<const char*>(a.out);
+  k.dout = static_cast<const char*>(a.dout);
+  k.q_t = a.q_t * es, k.q_h = a.q_h * es, k.k_t = a.k_t * es, k.k_h = a.k_h * es;
+  k.v_t = a.v_t * es, k.v_h = a.v_h * es, k.do_t = a.dout_t * es, k.do_h = a.dout_h * es;
+  k.out = static_cast<char*>(a.out);
+  k.dq = static_cast<char*>(a.dq);
+  k.dk = static_cast<char*>(a.dk);
+  k.dv = static_cast<char*>(a.dv);
+  k.lse = a.lse;
+  k.plan = a.plan;
+  k.T = (int32_t)a.T;
+  k.Hq = (int32_t)a.heads;
+  k.Hk = (int32_t)a.kv_heads;
+  k.G = k.Hq / k.Hk;
+  k.D = (int32_t)a.head_dim;
+  k.tiles_max = (int32_t)attn_tiles(a.T, a.S);
+  k.window = (int32_t)a.window;
+  k.hsplit = 1;
+  k.scale = a.scale;
+  k.z_mul = (a.softcap > 0.f ? a.softcap : a.scale) * kLog2e;
+  k.cap_mul = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  return k;
+}
+
+// kernel<T, DP, CAP> for a type, head width and softcap.
+#define MT_ATTN_PICK(kernel, dtype, D, cap)                                                       \
+  ((dtype) == MT_DTYPE_BF16                                                                       \
+       ? ((D) <= 64 ? ((cap) ? kernel<__bf16, 64, true> : kernel<__bf16, 64, false>)              \
+                    : ((cap) ? kernel<__bf16, 128, true> : kernel<__bf16, 128, false>))           \
+       : ((D) <= 64 ? ((cap) ? kernel<float, 64, true> : kernel<float, 64, false>)                \
+                    : ((cap) ? kernel<float, 128, true> : kernel<float, 128, false>)))
+
+}  // namespace
+
+extern "C" {
+
+size_t mt_attn_plan_bytes(int64_t T, int64_t S) {
+  return T < 0 || T > kMaxRows || S < 0 || S > kMaxRows ? 0 : plan_bytes(T, S);
+}
+
+int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t S, int64_t T,
+                 int64_t window, int32_t* plan, size_t plan_size, int32_t* status, mt_stream_t stream) {
+  if (T < 0 || T > kMaxRows || S < 0 || S > kMaxRows || attn_tiles(T, S) > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "bad sizes T=%lld S=%lld", (long long)T, (long long)S);
+  if (window < 1 || window > INT32_MAX)
+    return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)window);
+  if (!cu_seqlens || !plan || !status) return fail(MT_ERR_INVALID_ARGUMENT, "null pointer argument");
+  if (!aligned16(plan)) return fail(MT_ERR_INVALID_ARGUMENT, "plan must be 16-byte aligned");
+  if (plan_size < plan_bytes(T, S))
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "plan: %zu bytes, %zu needed", plan_size, plan_bytes(T, S));
+  hipLaunchKernelGGL(attn_plan_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, cu_seqlens,
+                     prefix_lens, (int32_t)S, (int32_t)T, (int32_t)window, (int32_t)attn_tiles(T, S),
+                     plan, status);
+  return check_launch("attn_plan_kernel");
+}
+
+int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
+  MT_TRY(attn_check(args, false));
+  const mt_attn_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const AttnArgs k = attn_args(a);
+  auto kern = MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, a.softcap > 0.f);
+  hipLaunchKernelGGL(kern, dim3((uint32_t)(k.tiles_max * k.Hq)), dim3(kAttnThreads), 0,
+                     (hipStream_t)stream, k);
+  return check_launch("attn_fwd_kernel");
+}
+
+size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args) {
+  if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0) return 0;
+  return round256((size_t)args->heads * (size_t)args->T * 4) + attn_part_bytes(*args);
+}
+
+int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream) {
+  MT_TRY(attn_check(args, true));
+  const mt_attn_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const size_t need = mt_attn_backward_workspace_bytes(args);
+  if (!workspace || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
+  if (workspace_bytes < need)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
+  AttnArgs k = attn_args(a);
+  k.delta = static_cast<float*>(workspace);
+  k.part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                    round256((size_t)a.heads * (size_t)a.T * 4));
+  k.hsplit = attn_hsplit(a);
+  const bool cap = a.softcap > 0.f;
+  hipStream_t s = (hipStream_t)stream;
+  auto dq = MT_ATTN_PICK(attn_dq_kernel, a.dtype, a.head_dim, cap);
+  hipLaunchKernelGGL(dq, dim3((uint32_t)(k.tiles_max * k.Hq)), dim3(kAttnThreads), 0, s, k);
+  MT_TRY(check_launch("attn_dq_kernel"));
+  auto dkdv = MT_ATTN_PICK(attn_dkdv_kernel, a.dtype, a.head_dim, cap);
+  hipLaunchKernelGGL(dkdv, dim3((uint32_t)(k.tiles_max * k.Hk * k.hsplit)), dim3(kAttnThreads), 0, s, k);
+  MT_TRY(check_launch("attn_dkdv_kernel"));
+  if (k.hsplit == 1) return MT_OK;
+  const int64_t n = a.T * a.kv_heads * a.head_dim;
+  const dim3 grid((uint32_t)cdiv(2 * n, 1024));
+  if (a.dtype == MT_DTYPE_BF16)
+    hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
+                       reinterpret_cast<__bf16*>(k.dk), reinterpret_cast<__bf16*>(k.dv));
+  else
+    hipLaunchKernelGGL(attn_join_kernel<float>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
+                       reinterpret_cast<float*>(k.dk), reinterpret_cast<float*>(k.dv));
+  return check_launch("attn_join_kernel");
+}
+
+}  // extern "C"

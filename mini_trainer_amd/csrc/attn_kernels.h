@@ -27,6 +27,8 @@
 // their products (bf16: at most 2^-8 of each term, as the inputs' own rounding), the row sums of P are taken before that rounding.
 #pragma once
 
+#include <type_traits>
+
 #include "flce_device.h"
 
 namespace mtf {
@@ -235,6 +237,26 @@ __device__ __forceinline__ void attn_row_product(f32x16_t& acc, const char* tile
   }
 }
 
+// The same with the right operand in an LDS tile too (row col0 + (l & 31)).
+template <class T, int DP>
+__device__ __forceinline__ void attn_row_product(f32x16_t& acc, const char* tile, uint32_t row0,
+                                                 const char* right, uint32_t col0) {
+  const uint32_t row = row0 + (lane_id() & 31u), col = col0 + (lane_id() & 31u);
+#pragma unroll
+  for (int t = 0; t < AttnFrag<T, DP>::kN; ++t) {
+    const u32x4_t a = lds_read16(tile, AttnLds<T, DP>::off(row, AttnFrag<T, DP>::chunk(t)));
+    const u32x4_t b = lds_read16(right, AttnLds<T, DP>::off(col, AttnFrag<T, DP>::chunk(t)));
+    if constexpr (sizeof(T) == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                    __builtin_bit_cast(bf16x8_t, b), acc, 0, 0, 0);
+    } else {
+      const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], acc, 0, 0, 0);
+    }
+  }
+}
+
 typedef __attribute__((address_space(3))) bf16x4_t lds_bf16x4_t;
 
 // acc[db][r] += sum over the 32 rows of tile[row0 + row][32 db + R(r)] * w[row],
@@ -283,36 +305,53 @@ __device__ __forceinline__ void attn_col_product(f32x16_t (&acc)[DP / 32], const
 
 typedef __amdgpu_buffer_rsrc_t attn_rsrc_t;
 
-// ROWS rows of a [rows, head, d] tensor on their way from memory to an LDS tile
-// through registers.  Rows at or beyond `rows` and chunks at or beyond d_bytes
-// arrive as zeros (an offset past the resource touches no memory).  The resource
-// starts at the tile's first row, so 32-bit offsets reach it wherever it lies.
+__device__ __forceinline__ attn_rsrc_t attn_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+// LDS DMA: LDS[dst + size lane] = mem[r + off], `size` bytes per lane.
+__device__ __forceinline__ void attn_dma16(attn_rsrc_t r, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)dst, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void attn_dma4(attn_rsrc_t r, char* dst, uint32_t off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)dst, 4, off, 0, 0, 0);
+}
+
+// ROWS rows of a [rows, head, d] tensor from memory to an LDS tile by LDS DMA: an
+// instruction writes 1 KiB of the tile in order, so the lane that writes a slot
+// loads the chunk that the swizzle puts there.  Rows at or beyond `rows` and
+// chunks at or beyond d_bytes arrive as zeros (an offset past the resource
+// touches no memory).  The resource starts at the tile's first row, so 32-bit
+// offsets reach it wherever it lies.
 template <class T, int DP, int ROWS>
-struct AttnStage {
+struct AttnDma {
   static constexpr int kN = (int)(ROWS * AttnLds<T, DP>::kCh / kAttnThreads);
-  u32x4_t v[kN];
-  __device__ __forceinline__ void load(const char* base, int32_t rows, uint32_t stride_b,
-                                       uint32_t d_bytes) {
-    const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * stride_b + d_bytes : 0u;
-    const attn_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), (short)0, (int)bytes, 0x00020000);
+  uint32_t off[kN];
+  uint32_t stride, d_bytes;
+  __device__ __forceinline__ void init(uint32_t stride_b, uint32_t d_bytes_) {
+    stride = stride_b;
+    d_bytes = d_bytes_;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const uint32_t idx = threadIdx.x + (uint32_t)i * kAttnThreads;
-      const uint32_t row = idx / AttnLds<T, DP>::kCh, ch = idx % AttnLds<T, DP>::kCh;
-      const bool in = ch * 16u < d_bytes && (int32_t)row < rows;
-      v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, in ? row * stride_b + ch * 16u : 0xfffffff0u, 0,
-                                                   0);
+      const uint32_t idx = (wave_id() * kN + (uint32_t)i) * 64u + lane_id();
+      const uint32_t row = idx / AttnLds<T, DP>::kCh;
+      const uint32_t ch = (idx % AttnLds<T, DP>::kCh) ^ AttnLds<T, DP>::swz(row);
+      off[i] = ch * 16u < d_bytes ? row * stride + ch * 16u : 0xfffffff0u;
     }
   }
-  __device__ __forceinline__ void store(char* tile) const {
+  __device__ __forceinline__ void issue(const char* base, int32_t rows, char* tile) const {
+    const uint32_t bytes = rows > 0 ? (uint32_t)(min(rows, ROWS) - 1) * stride + d_bytes : 0u;
+    const attn_rsrc_t r = attn_rsrc(base, bytes);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const uint32_t idx = threadIdx.x + (uint32_t)i * kAttnThreads;
-      lds_write16(tile, AttnLds<T, DP>::off(idx / AttnLds<T, DP>::kCh, idx % AttnLds<T, DP>::kCh), v[i]);
-    }
+    for (int i = 0; i < kN; ++i)
+      attn_dma16(r, tile + (wave_id() * kN + (uint32_t)i) * 1024u, off[i]);
   }
 };
+
+// This wave's LDS DMA has landed and every wave's LDS reads are done.
+__device__ __forceinline__ void attn_sync() {
+  __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
+  __syncthreads();
+}
 
 // Sums of the two halves of the wave (a row's two lanes), in both.
 __device__ __forceinline__ float attn_pair_add(float x) {
@@ -325,6 +364,26 @@ __device__ __forceinline__ float attn_pair_max(float x) {
                                                   __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
+
+// Order of a run of N matrix instructions and their LDS reads (READS for each):
+// the reads of AHEAD of them first, then one instruction and the reads of a later
+// one in turn.  Left to itself the compiler, short of registers, reads each
+// operand right before its use and every instruction waits for the LDS.
+template <int N, int READS, int AHEAD>
+__device__ __forceinline__ void attn_sched_reads() {
+  constexpr int kMfma = 0x8, kDsRead = 0x100;
+  __builtin_amdgcn_sched_group_barrier(kDsRead, READS * AHEAD, 0);
+#pragma unroll
+  for (int i = 0; i < N - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kDsRead, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(kMfma, AHEAD, 0);
+}
+
+// Keeps a rarely entered branch a branch: turned into selects, the masks of the
+// few blocks that a range's end crosses would be evaluated in all of them.
+__device__ __forceinline__ void attn_no_if_conversion() { asm volatile("" ::: "memory"); }
 
 // tanh: bf16 inputs take 1 - 2 / (exp(2x) + 1) (absolute error some 2^-23, far
 // below a score's own), fp32 the library's.
@@ -364,16 +423,15 @@ __device__ __forceinline__ void attn_zero_rows(Out* base, int32_t rows, int64_t 
                                 (i % per) * 16) = u32x4_t{0u, 0u, 0u, 0u};
 }
 
-__device__ __forceinline__ AttnTile attn_tile(const int32_t* at) {
-  AttnTile t;
-  t.row0 = __builtin_amdgcn_readfirstlane(at[0]);
-  t.rows = __builtin_amdgcn_readfirstlane(at[1]);
-  t.ds = __builtin_amdgcn_readfirstlane(at[2]);
-  t.de = __builtin_amdgcn_readfirstlane(at[3]);
-  t.pe = __builtin_amdgcn_readfirstlane(at[4]);
-  t.beg = __builtin_amdgcn_readfirstlane(at[5]);
-  t.end = __builtin_amdgcn_readfirstlane(at[6]);
-  t.tail = __builtin_amdgcn_readfirstlane(at[7]);
+// Tile `at` of a plan, or tail < 0 where the plan has fewer.  Read through the
+// scalar cache (the plan was written by an earlier launch), the count beside it.
+__device__ __forceinline__ AttnTile attn_tile(const int32_t* plan, int64_t at, int32_t ti) {
+  typedef const __attribute__((address_space(4))) int32_t* scalar_t;
+  const scalar_t c = (scalar_t)(uintptr_t)(plan);
+  const scalar_t p = (scalar_t)(uintptr_t)(plan + kPlanHeader + at * kPlanTile);
+  const int32_t tiles = c[0];
+  AttnTile t = {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
+  if (ti >= tiles) t.tail = -1;
   return t;
 }
 
@@ -404,8 +462,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
   const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
-  if (ti >= a.plan[0]) return;
-  const AttnTile t = attn_tile(a.plan + kPlanHeader + (int64_t)ti * kPlanTile);
+  const AttnTile t = attn_tile(a.plan, ti, ti);
+  if (t.tail < 0) return;
   const int64_t o_t = (int64_t)a.Hq * a.D;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)t.row0 * o_t + (int64_t)head * a.D;
   float* lse = a.lse + (int64_t)head * a.T;
@@ -434,29 +492,25 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 
   const char* kbase = a.k + (int64_t)kvh * a.k_h;
   const char* vbase = a.v + (int64_t)kvh * a.v_h;
-  AttnStage<T, DP, kAttnKeys> sk, sv;
-  auto fetch = [&](int32_t k0) {
-    const int32_t n = min(kAttnKeys, t.end - k0);
-    sk.load(kbase + (int64_t)k0 * a.k_t, n, (uint32_t)a.k_t, d_bytes);
-    sv.load(vbase + (int64_t)k0 * a.v_t, n, (uint32_t)a.v_t, d_bytes);
+  AttnDma<T, DP, kAttnKeys> sk, sv;
+  sk.init((uint32_t)a.k_t, d_bytes);
+  sv.init((uint32_t)a.v_t, d_bytes);
+  auto fetch = [&](int32_t k0, uint32_t buf) {
+    sk.issue(kbase + (int64_t)k0 * a.k_t, t.end - k0, smem + buf * 2 * kTile);
+    sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
-  fetch(t.beg);
-  sk.store(smem);
-  sv.store(smem + kTile);
-  if (t.beg + kAttnKeys < t.end) fetch(t.beg + kAttnKeys);
+  fetch(t.beg, 0);
   uint32_t buf = 0;
   for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
-    __syncthreads();
-    if (k0 + kAttnKeys < t.end) {  // into the buffer that every wave has left at the barrier
-      sk.store(smem + (buf ^ 1u) * 2 * kTile);
-      sv.store(smem + (buf ^ 1u) * 2 * kTile + kTile);
-      if (k0 + 2 * kAttnKeys < t.end) fetch(k0 + 2 * kAttnKeys);
-    }
+    attn_sync();
+    // into the buffer that every wave has left at the barrier
+    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf ^ 1u);
     if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
     const char* kt = smem + buf * 2 * kTile;
     f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
 #pragma unroll
     for (uint32_t b = 0; b < 2; ++b) attn_row_product<T, DP>(s[b], kt, 32u * b, qf);
+    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 1, 4>();
     if constexpr (CAP) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -464,13 +518,13 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
         for (int r = 0; r < 16; ++r) s[b][r] = attn_tanh<T>(s[b][r] * a.cap_mul);
     }
     if (k0 < f_lo || k0 + kAttnKeys > f_hi) {
+      attn_no_if_conversion();
+      const uint32_t from = (uint32_t)(k0 + 4 * (int32_t)h - lo), n = (uint32_t)(hi - lo);
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int32_t key = k0 + 32 * b + 8 * (r / 4) + 4 * (int32_t)h + r % 4;
-          if (key < lo || key >= hi) s[b][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r)
+          if (from + (uint32_t)(32 * b + 8 * (r / 4) + r % 4) >= n) s[b][r] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
@@ -498,6 +552,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
       }
 #pragma unroll
     for (uint32_t b = 0; b < 2; ++b) attn_col_product<T, DP>(acc, kt + kTile, 32u * b, s[b]);
+    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 2, 4>();
   }
   sum = attn_pair_add(sum);
   if (valid && h == 0) lse[row] = m + fast_log2(sum);
@@ -516,8 +571,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
   const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
-  if (ti >= a.plan[0]) return;
-  const AttnTile t = attn_tile(a.plan + kPlanHeader + (int64_t)ti * kPlanTile);
+  const AttnTile t = attn_tile(a.plan, ti, ti);
+  if (t.tail < 0) return;
   const int64_t o_t = (int64_t)a.Hq * a.D;
   T* dq = reinterpret_cast<T*>(a.dq) + (int64_t)head * a.D;
   if (t.tail) {
@@ -569,24 +624,18 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
 
   const char* kbase = a.k + (int64_t)kvh * a.k_h;
   const char* vbase = a.v + (int64_t)kvh * a.v_h;
-  AttnStage<T, DP, kAttnKeys> sk, sv;
-  auto fetch = [&](int32_t k0) {
-    const int32_t n = min(kAttnKeys, t.end - k0);
-    sk.load(kbase + (int64_t)k0 * a.k_t, n, (uint32_t)a.k_t, d_bytes);
-    sv.load(vbase + (int64_t)k0 * a.v_t, n, (uint32_t)a.v_t, d_bytes);
+  AttnDma<T, DP, kAttnKeys> sk, sv;
+  sk.init((uint32_t)a.k_t, d_bytes);
+  sv.init((uint32_t)a.v_t, d_bytes);
+  auto fetch = [&](int32_t k0, uint32_t buf) {
+    sk.issue(kbase + (int64_t)k0 * a.k_t, t.end - k0, smem + buf * 2 * kTile);
+    sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
-  fetch(t.beg);
-  sk.store(smem);
-  sv.store(smem + kTile);
-  if (t.beg + kAttnKeys < t.end) fetch(t.beg + kAttnKeys);
+  fetch(t.beg, 0);
   uint32_t buf = 0;
   for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
-    __syncthreads();
-    if (k0 + kAttnKeys < t.end) {
-      sk.store(smem + (buf ^ 1u) * 2 * kTile);
-      sv.store(smem + (buf ^ 1u) * 2 * kTile + kTile);
-      if (k0 + 2 * kAttnKeys < t.end) fetch(k0 + 2 * kAttnKeys);
-    }
+    attn_sync();
+    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf ^ 1u);
     if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
     const char* kt = smem + buf * 2 * kTile;
     const bool edge = k0 < f_lo || k0 + kAttnKeys > f_hi;
@@ -595,19 +644,24 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
       f32x16_t s = f32x16_t{}, dp = f32x16_t{};
       attn_row_product<T, DP>(s, kt, 32u * b, qf);
       attn_row_product<T, DP>(dp, kt + kTile, 32u * b, dof);
+      if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 1, 4>();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float x = s[r];
         if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
-        float d = fast_exp2(fmaf(x, a.z_mul, -lse)) * (dp[r] - delta);
-        if constexpr (CAP) d *= fmaf(-x, x, 1.0f);
-        if (edge) {
-          const int32_t key = k0 + 32 * (int32_t)b + 8 * (r / 4) + 4 * (int32_t)h + r % 4;
-          if (key < lo || key >= hi) d = 0.f;
-        }
-        s[r] = d;
+        s[r] = fast_exp2(fmaf(x, a.z_mul, -lse)) * (dp[r] - delta);
+        if constexpr (CAP) s[r] *= fmaf(-x, x, 1.0f);
+      }
+      if (edge) {
+        attn_no_if_conversion();
+        const uint32_t from = (uint32_t)(k0 + 32 * (int32_t)b + 4 * (int32_t)h - lo);
+        const uint32_t n = (uint32_t)(hi - lo);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (from + (uint32_t)(8 * (r / 4) + r % 4) >= n) s[r] = 0.f;
       }
       attn_col_product<T, DP>(acc, kt, 32u * b, s);
+      if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 16, 2, 4>();
     }
   }
   attn_store<T, DP>(acc, a.scale, dq + (int64_t)row * o_t, a.D, valid);
@@ -615,25 +669,34 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
 
 // --- backward: dK and dV --------------------------------------------------------
 
-// Rows of Q and dO per block: 64, or 32 where a row takes 512 bytes of LDS.
+// Rows of Q and dO per block: 32 where a row of an LDS tile takes 256 bytes or
+// more (two workgroups per CU then fit its LDS), 64 else.
 template <class T, int DP>
 constexpr int attn_q_rows() {
-  return sizeof(T) * DP > 256 ? 32 : 64;
+  return sizeof(T) * DP >= 256 ? 32 : 64;
 }
 
+// Both accumulators of a wave's 32 keys take 128 registers at DP = 128 and the
+// keys' K rows 32; their V rows stay in LDS, because with them in registers too a
+// wave needs more than the 256 that let two share a SIMD, and a wave alone hides
+// neither the LDS reads nor the softmax.  One document of 16384 tokens, 32 heads
+// of 128 (8 key heads): 4.5 ms, 970 TFLOP/s; with V in registers 7.4 ms; as two
+// kinds of workgroup, dK and dV each with their own scores, 5.5 ms.
 template <class T, int DP, bool CAP>
-__global__ __launch_bounds__(kAttnThreads, 1) void attn_dkdv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dkdv_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr int kQ = attn_q_rows<T, DP>();
+  constexpr bool kVLds = sizeof(T) == 2 && DP == 128;
   constexpr uint32_t kTile = kQ * L::kRowB;
-  constexpr uint32_t kBuf = 2 * kTile + 2 * kQ * 4;
+  constexpr uint32_t kBuf = 2 * kTile + 2 * 256;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kBuf];  // 2 x (Q, dO, lse, delta)
+  __shared__ __attribute__((aligned(1024))) char vt[kVLds ? kAttnRows * L::kRowB : 16];
   const uint32_t id = blockIdx.x;
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t hs = rest % (uint32_t)a.hsplit;
   const int32_t ti = (int32_t)(rest / (uint32_t)a.hsplit);
-  if (ti >= a.plan[0]) return;
-  const AttnTile t = attn_tile(a.plan + kPlanHeader + ((int64_t)a.tiles_max + ti) * kPlanTile);
+  const AttnTile t = attn_tile(a.plan, (int64_t)a.tiles_max + ti, ti);
+  if (t.tail < 0) return;
   const int64_t o_t = (int64_t)a.Hk * a.D;
   const int64_t o_at = (int64_t)t.row0 * o_t + (int64_t)kvh * a.D;
   const int64_t part_n = (int64_t)a.T * o_t;
@@ -662,15 +725,20 @@ __global__ __launch_bounds__(kAttnThreads, 1) void attn_dkdv_kernel(AttnArgs a) 
   const int32_t f_lo = attn_col_lo(j_last, t.ds, t.pe), f_hi = attn_col_hi(j0, t.de, a.window);
   const int32_t lo = attn_col_lo(key, t.ds, t.pe);
   const int32_t hi = valid ? attn_col_hi(key, t.de, a.window) : lo;
-
   // the queries [s_lo, s_hi) that see one key: ds = 0 exactly (attn_dq_kernel); no
   // block with one of them is seen whole
   int32_t s_lo = t.ds, s_hi = t.pe <= t.ds + 1 ? t.ds + 1 : t.ds;
-  if (a.window == 1) s_lo = max(t.ds, t.pe - 1), s_hi = t.de;
+  if (a.window == 1) s_lo = max(t.ds, t.pe - 1), s_hi = t.de;  // (s_lo <= s_hi)
 
   AttnFrag<T, DP> kf, vf;
   kf.load(a.k + (int64_t)key * a.k_t + (int64_t)kvh * a.k_h, d_bytes, valid);
-  vf.load(a.v + (int64_t)key * a.v_t + (int64_t)kvh * a.v_h, d_bytes, valid);
+  if constexpr (kVLds) {
+    AttnDma<T, DP, kAttnRows> sv;
+    sv.init((uint32_t)a.v_t, d_bytes);
+    sv.issue(a.v + (int64_t)t.row0 * a.v_t + (int64_t)kvh * a.v_h, t.rows, vt);
+  } else {
+    vf.load(a.v + (int64_t)key * a.v_t + (int64_t)kvh * a.v_h, d_bytes, valid);
+  }
   f32x16_t ak[DP / 32], av[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) ak[i] = av[i] = f32x16_t{};
@@ -678,81 +746,79 @@ __global__ __launch_bounds__(kAttnThreads, 1) void attn_dkdv_kernel(AttnArgs a) 
   // the group's heads one after the other, each over the query blocks of [beg, end)
   const int32_t per = (a.G + a.hsplit - 1) / a.hsplit;
   const int32_t g0 = (int32_t)hs * per, g1 = min(a.G, g0 + per);
-  AttnStage<T, DP, kQ> sq, sdo;
-  float s_lse = 0.f, s_delta = 0.f;
-  int32_t fg = g0, fi = t.beg;  // the block to fetch next
-  auto fetch = [&]() {
+  AttnDma<T, DP, kQ> sq, sdo;
+  sq.init((uint32_t)a.q_t, d_bytes);
+  sdo.init((uint32_t)a.do_t, d_bytes);
+  // from the last block to the first: workgroups of one document then pass the
+  // same blocks at the same time, whichever keys they own, and find them in L2
+  const int32_t i_last = t.beg + (t.end - t.beg - 1) / kQ * kQ;
+  int32_t fg = g0, fi = i_last;  // the block to fetch next
+  auto fetch = [&](uint32_t buf) {
     const int64_t head = (int64_t)kvh * a.G + fg;
     const int32_t n = min(kQ, t.end - fi);
-    sq.load(a.q + (int64_t)fi * a.q_t + head * a.q_h, n, (uint32_t)a.q_t, d_bytes);
-    sdo.load(a.dout + (int64_t)fi * a.do_t + head * a.do_h, n, (uint32_t)a.do_t, d_bytes);
-    if ((int32_t)threadIdx.x < kQ) {
-      const bool in = (int32_t)threadIdx.x < n;
-      s_lse = in ? a.lse[head * a.T + fi + threadIdx.x] : 0.f;
-      s_delta = in ? a.delta[head * a.T + fi + threadIdx.x] : 0.f;
-    }
-    fi += kQ;
-    if (fi >= t.end) fi = t.beg, ++fg;
-  };
-  auto put = [&](uint32_t buf) {
     char* at = smem + buf * kBuf;
-    sq.store(at);
-    sdo.store(at + kTile);
-    if ((int32_t)threadIdx.x < kQ) {
-      reinterpret_cast<float*>(at + 2 * kTile)[threadIdx.x] = s_lse;
-      reinterpret_cast<float*>(at + 2 * kTile)[kQ + threadIdx.x] = s_delta;
+    sq.issue(a.q + (int64_t)fi * a.q_t + head * a.q_h, n, at);
+    sdo.issue(a.dout + (int64_t)fi * a.do_t + head * a.do_h, n, at + kTile);
+    if (w < 2) {  // the rows' lse by the first wave, their delta by the second
+      const float* from = (w == 0 ? a.lse : a.delta) + head * a.T + fi;
+      attn_dma4(attn_rsrc(from, 4u * (uint32_t)n), at + 2 * kTile + w * 256u, l * 4u);
     }
+    fi -= kQ;
+    if (fi < t.beg) fi = i_last, ++fg;
   };
   const int32_t blocks = g1 > g0 ? (g1 - g0) * ((t.end - t.beg + kQ - 1) / kQ) : 0;
-  if (blocks > 0) {
-    fetch();
-    put(0);
-    if (blocks > 1) fetch();
-  }
+  if (blocks > 0) fetch(0);
+  const uint32_t range = (uint32_t)(hi - lo), ones = (uint32_t)(s_hi - s_lo);
   uint32_t buf = 0;
-  int32_t i0 = t.beg;
+  int32_t i0 = i_last;
   for (int32_t n = 0; n < blocks; ++n, buf ^= 1u) {
-    __syncthreads();
-    if (n + 1 < blocks) {
-      put(buf ^ 1u);
-      if (n + 2 < blocks) fetch();
-    }
-    const char* qt = smem + buf * kBuf;
-    const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
+    attn_sync();
+    if (n + 1 < blocks) fetch(buf ^ 1u);
+    if (active && i0 < w_hi && i0 + kQ > w_lo) {
+      const char* qt = smem + buf * kBuf;
+      const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
+      const bool edge = i0 < f_lo || i0 + kQ > f_hi;
 #pragma unroll
-    for (int32_t b = 0; b < kQ / 32; ++b) {
-      const int32_t q0 = i0 + 32 * b;
-      if (!active || q0 >= w_hi || q0 + 32 <= w_lo) continue;
-      const bool edge = q0 < f_lo || q0 + 32 > f_hi;
-      f32x16_t s = f32x16_t{}, dp = f32x16_t{};
-      attn_row_product<T, DP>(s, qt, 32u * b, kf);
-      attn_row_product<T, DP>(dp, qt + kTile, 32u * b, vf);
+      for (int b = 0; b < kQ / 32; ++b) {
+        f32x16_t s = f32x16_t{}, dp = f32x16_t{};
+        attn_row_product<T, DP>(s, qt, 32u * b, kf);
+        if constexpr (kVLds)
+          attn_row_product<T, DP>(dp, qt + kTile, 32u * b, vt, 32u * w);
+        else
+          attn_row_product<T, DP>(dp, qt + kTile, 32u * b, vf);
+        if constexpr (sizeof(T) == 2 && !kVLds) attn_sched_reads<DP / 8, 1, 4>();
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(rows + 32 * b + 8 * g + 4 * h);
-        const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(rows + kQ + 32 * b + 8 * g + 4 * h);
+        for (int g = 0; g < 4; ++g) {
+          const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(rows + 32 * b + 8 * g + 4 * h);
+          const f32x4_t delta = *reinterpret_cast<const f32x4_t*>(rows + 64 + 32 * b + 8 * g + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          float x = s[r];
-          if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
-          float p = fast_exp2(fmaf(x, a.z_mul, -lse[e]));
-          float d = p * (dp[r] - delta[e]);
-          if constexpr (CAP) d *= fmaf(-x, x, 1.0f);
-          if (edge) {
-            const int32_t q = q0 + 8 * g + 4 * (int32_t)h + e;
-            if (q < lo || q >= hi) p = d = 0.f;
-            if (q >= s_lo && q < s_hi) d = 0.f;
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float x = s[r];
+            if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
+            s[r] = fast_exp2(fmaf(x, a.z_mul, -lse[e]));
+            dp[r] = s[r] * (dp[r] - delta[e]);
+            if constexpr (CAP) dp[r] *= fmaf(-x, x, 1.0f);
           }
-          s[r] = p;
-          dp[r] = d;
         }
+        if (edge) {
+          attn_no_if_conversion();
+          const uint32_t from = (uint32_t)(i0 + 32 * b + 4 * (int32_t)h - lo);
+          const uint32_t one = (uint32_t)(i0 + 32 * b + 4 * (int32_t)h - s_lo);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const uint32_t at = (uint32_t)(8 * (r / 4) + r % 4);
+            if (from + at >= range) s[r] = dp[r] = 0.f;
+            if (one + at < ones) dp[r] = 0.f;
+          }
+        }
+        attn_col_product<T, DP>(av, qt + kTile, 32u * b, s);
+        attn_col_product<T, DP>(ak, qt, 32u * b, dp);
+        if constexpr (sizeof(T) == 2 && !kVLds) attn_sched_reads<DP / 8, 2, 4>();
       }
-      attn_col_product<T, DP>(av, qt + kTile, 32u * b, s);
-      attn_col_product<T, DP>(ak, qt, 32u * b, dp);
     }
-    i0 += kQ;
-    if (i0 >= t.end) i0 = t.beg;
+    i0 -= kQ;
+    if (i0 < t.beg) i0 = i_last;
   }
   const int64_t at = (int64_t)(key - t.row0) * o_t;
   if (a.hsplit > 1) {
