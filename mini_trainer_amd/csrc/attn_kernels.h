@@ -59,10 +59,14 @@ __device__ __forceinline__ int32_t attn_col_hi(int32_t j, int32_t de, int32_t w)
   return j > de - w ? de : j + w;
 }
 
+// Blocks of 64 rows that a tile visits.
+__device__ __forceinline__ int32_t attn_cost(const AttnTile& t) { return (t.end - t.beg + 63) >> 6; }
+
 // The plan: tiles of every document and of the rows behind the last one, the
 // costliest first (counting sort by the blocks a tile visits), so that the
 // workgroups dispatched last are the short ones.  One workgroup.
-//   plan: kPlanHeader words ([0] = tiles), tiles_max query tiles, tiles_max key
+//   plan: kPlanHeader words ([0] = tiles, [1] = the key tiles'
+//   cost, [2] = the costliest one's), tiles_max query tiles, tiles_max key
 //   tiles, S + 2 words of scratch.  status: 0, or 1 for cu_seqlens that are not
 //   0 = cu[0] <= ... <= cu[S] <= T, or 2 for a prefix outside its document; the
 //   plan of such a call is one tail over all T rows (status 1) or clamps the
@@ -73,12 +77,12 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
                                                          int32_t* status) {
   __shared__ int32_t hist[2][kPlanBuckets];
   __shared__ int32_t wave_sum[16];
-  __shared__ int32_t bad, bad_prefix;
+  __shared__ int32_t bad, bad_prefix, total, most;
   const int32_t tid = threadIdx.x;
   AttnTile* qt = reinterpret_cast<AttnTile*>(plan + kPlanHeader);
   AttnTile* kt = qt + tiles_max;
   int32_t* off = reinterpret_cast<int32_t*>(kt + tiles_max);
-  if (tid == 0) bad = cu[0] != 0 || cu[S] > T || cu[S] < 0, bad_prefix = 0;
+  if (tid == 0) bad = cu[0] != 0 || cu[S] > T || cu[S] < 0, bad_prefix = total = most = 0;
   hist[0][tid] = hist[1][tid] = 0;
   __syncthreads();
   for (int32_t s = tid; s < S; s += 1024) {
@@ -140,9 +144,11 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
       q.end = q.tail ? 0 : attn_row_hi(last, q.pe);
       k.beg = k.tail ? 0 : attn_col_lo(k.row0, k.ds, k.pe);
       k.end = k.tail ? 0 : attn_col_hi(last, k.de, window);
-      const int32_t cq = min(kPlanBuckets - 1, (q.end - q.beg + 63) >> 6);
-      const int32_t ck = min(kPlanBuckets - 1, (k.end - k.beg + 63) >> 6);
+      const int32_t cq = min(kPlanBuckets - 1, attn_cost(q));
+      const int32_t ck = min(kPlanBuckets - 1, attn_cost(k));
       if (pass == 0) {
+        atomicAdd(&total, attn_cost(k));
+        atomicMax(&most, attn_cost(k));
         atomicAdd(&hist[0][cq], 1);
         atomicAdd(&hist[1][ck], 1);
       } else {  // (the order within a bucket changes no result)
@@ -152,6 +158,7 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
     }
     __syncthreads();
     if (pass == 0) {  // hist[b] -> tiles in the costlier buckets
+      if (tid == 0) plan[1] = total, plan[2] = most;
       for (int which = 0; which < 2; ++which) {
         const int32_t bucket = kPlanBuckets - 1 - tid;
         const int32_t n = hist[which][bucket];
@@ -347,6 +354,11 @@ struct AttnDma {
   }
 };
 
+// Which of two LDS buffers a block uses, known to the compiler: the buffer's
+// place then is part of an LDS instruction's own offset.
+template <uint32_t N>
+using AttnBuf = std::integral_constant<uint32_t, N>;
+
 // This wave's LDS DMA has landed and every wave's LDS reads are done.
 __device__ __forceinline__ void attn_sync() {
   __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0)
@@ -435,18 +447,91 @@ __device__ __forceinline__ AttnTile attn_tile(const int32_t* plan, int64_t at, i
   return t;
 }
 
+// Workgroups among which the query heads of a key tile's group are divided, each
+// writing fp32 parts of dK and dV for attn_join_kernel: as many as keep a
+// workgroup below three quarters of what each of 512 resident ones gets of all the
+// work (`cost` of this tile, `most` of the costliest and `total` of all, each for
+// one head), and one, writing the results themselves, for the tiles below that.
+// Where even the costliest tile is within 1.25 shares none is divided: the order
+// of the tiles balances those, and workgroups that walk the same heads share them
+// in L2.  64 documents in 32768 tokens, 6 heads a group, dK/dV and join: 320 us;
+// every tile in 6 parts 422, in 3 479 us.  One document of 16384 tokens: 4.5 ms
+// undivided, 5.1 with its longer half in two parts.
+__device__ __forceinline__ int32_t attn_parts(int32_t cost, int32_t most, int32_t total, int32_t Hq,
+                                              int32_t G, int32_t parts_max) {
+  const int64_t work = (int64_t)total * Hq;
+  int32_t n = 1;
+  if ((int64_t)most * G * 410 > work)
+    while (n < parts_max && (int64_t)cost * G * 700 > n * work) ++n;
+  const int32_t per = (G + n - 1) / n;
+  return (G + per - 1) / per;
+}
+
 struct AttnArgs {
   const char *q, *k, *v, *o, *dout;            // element (t, h, d) at t * *_t + h * *_h + d * size
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h;  // bytes
   char *out, *dq, *dk, *dv;                    // [T, heads, D], contiguous
   float *lse, *delta;                          // [Hq, T]; lse in units of log2
-  float* part;                                 // [hsplit][2][T][Hk][D] when hsplit > 1
+  int32_t* items;                              // attn_items: count, 3 unused, then (tile, part) pairs
+  float* part;                                 // [parts_max][2][T][Hk][D] when parts_max > 1
   const int32_t* plan;
-  int32_t T, Hq, Hk, G, D, tiles_max, window, hsplit;
+  int32_t T, Hq, Hk, G, D, tiles_max, window, parts_max;
   float scale;     // of the scores
   float z_mul;     // log2 units: scale log2(e), or cap log2(e) with a softcap
   float cap_mul;   // scale / cap
 };
+
+__device__ __forceinline__ int32_t attn_parts(const AttnTile& t, const AttnArgs& a) {
+  const auto* head = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)a.plan;
+  return attn_parts(attn_cost(t), head[2], head[1], a.Hq, a.G, a.parts_max);
+}
+
+// What attn_dkdv_kernel's workgroups of one key head take: (tile, part) pairs, the
+// costliest first (counting sort), and none without work among them: those would
+// be dealt out in turn with the others and leave the shader engines that get them
+// idle.  One workgroup.
+__device__ __forceinline__ void attn_items(const AttnArgs& a, int32_t* scratch) {
+  int32_t* hist = scratch;                  // kPlanBuckets
+  int32_t* sums = scratch + kPlanBuckets;   // one per thread
+  const int32_t tid = (int32_t)threadIdx.x, tiles = a.plan[0];
+  constexpr int32_t kPer = kPlanBuckets / kAttnThreads;
+  const AttnTile* kt = reinterpret_cast<const AttnTile*>(a.plan + kPlanHeader) + a.tiles_max;
+  // costs of an item are at most G times that of the first tile (the costliest)
+  const int64_t most = tiles > 0 ? max((int64_t)1, (int64_t)attn_cost(kt[0]) * a.G) : 1;
+  for (int32_t i = tid; i < kPlanBuckets; i += kAttnThreads) hist[i] = 0;
+  __syncthreads();
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int32_t t = tid; t < tiles; t += kAttnThreads) {
+      const int32_t cost = attn_cost(kt[t]), parts = attn_parts(kt[t], a);
+      const int32_t per = (a.G + parts - 1) / parts;
+      for (int32_t p = 0; p < parts; ++p) {
+        const int64_t c = (int64_t)cost * min(per, a.G - p * per);
+        const int32_t b = (int32_t)(min(c, most) * (kPlanBuckets - 1) / most);
+        const int32_t at = atomicAdd(&hist[kPlanBuckets - 1 - b], 1);
+        if (pass == 1) {
+          a.items[4 + 2 * at] = t;
+          a.items[5 + 2 * at] = p;
+        }
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {  // counts -> first places
+      int32_t n = 0;
+      for (int32_t i = 0; i < kPer; ++i) n += hist[tid * kPer + i];
+      sums[tid] = n;
+      __syncthreads();
+      int32_t at = 0;
+      for (int32_t i = 0; i < tid; ++i) at += sums[i];
+      if (tid == kAttnThreads - 1) a.items[0] = at + n;
+      for (int32_t i = 0; i < kPer; ++i) {
+        const int32_t m = hist[tid * kPer + i];
+        hist[tid * kPer + i] = at;
+        at += m;
+      }
+      __syncthreads();
+    }
+  }
+}
 
 // --- forward ----------------------------------------------------------------
 
@@ -500,13 +585,12 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
   fetch(t.beg, 0);
-  uint32_t buf = 0;
-  for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
+  auto block = [&](int32_t k0, auto buf) {
     attn_sync();
     // into the buffer that every wave has left at the barrier
-    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf ^ 1u);
-    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
-    const char* kt = smem + buf * 2 * kTile;
+    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf.value ^ 1u);
+    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) return;
+    const char* kt = smem + buf.value * 2 * kTile;
     f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
 #pragma unroll
     for (uint32_t b = 0; b < 2; ++b) attn_row_product<T, DP>(s[b], kt, 32u * b, qf);
@@ -553,6 +637,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 #pragma unroll
     for (uint32_t b = 0; b < 2; ++b) attn_col_product<T, DP>(acc, kt + kTile, 32u * b, s[b]);
     if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 2, 4>();
+  };
+  for (int32_t k0 = t.beg; k0 < t.end; k0 += 2 * kAttnKeys) {
+    block(k0, AttnBuf<0>());
+    if (k0 + kAttnKeys < t.end) block(k0 + kAttnKeys, AttnBuf<1>());
   }
   sum = attn_pair_add(sum);
   if (valid && h == 0) lse[row] = m + fast_log2(sum);
@@ -567,7 +655,11 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
   __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];  // 2 x (K, V)
-  const uint32_t id = blockIdx.x;
+  if (blockIdx.x == 0) {  // beside the others, for the launch that follows
+    attn_items(a, reinterpret_cast<int32_t*>(smem));
+    return;
+  }
+  const uint32_t id = blockIdx.x - 1;
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
   const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
@@ -632,12 +724,11 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
   fetch(t.beg, 0);
-  uint32_t buf = 0;
-  for (int32_t k0 = t.beg; k0 < t.end; k0 += kAttnKeys, buf ^= 1u) {
+  auto block = [&](int32_t k0, auto buf) {
     attn_sync();
-    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf ^ 1u);
-    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) continue;
-    const char* kt = smem + buf * 2 * kTile;
+    if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf.value ^ 1u);
+    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) return;
+    const char* kt = smem + buf.value * 2 * kTile;
     const bool edge = k0 < f_lo || k0 + kAttnKeys > f_hi;
 #pragma unroll
     for (uint32_t b = 0; b < 2; ++b) {
@@ -663,6 +754,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
       attn_col_product<T, DP>(acc, kt, 32u * b, s);
       if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 16, 2, 4>();
     }
+  };
+  for (int32_t k0 = t.beg; k0 < t.end; k0 += 2 * kAttnKeys) {
+    block(k0, AttnBuf<0>());
+    if (k0 + kAttnKeys < t.end) block(k0 + kAttnKeys, AttnBuf<1>());
   }
   attn_store<T, DP>(acc, a.scale, dq + (int64_t)row * o_t, a.D, valid);
 }
@@ -691,12 +786,15 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   constexpr uint32_t kBuf = 2 * kTile + 2 * 256;
   __shared__ __attribute__((aligned(1024))) char smem[2 * kBuf];  // 2 x (Q, dO, lse, delta)
   __shared__ __attribute__((aligned(1024))) char vt[kVLds ? kAttnRows * L::kRowB : 16];
-  const uint32_t id = blockIdx.x;
-  const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
-  const uint32_t hs = rest % (uint32_t)a.hsplit;
-  const int32_t ti = (int32_t)(rest / (uint32_t)a.hsplit);
+  typedef const __attribute__((address_space(4))) int32_t* scalar_t;
+  const scalar_t items = (scalar_t)(uintptr_t)a.items;
+  const uint32_t kvh = blockIdx.x % (uint32_t)a.Hk;
+  const int32_t item = (int32_t)(blockIdx.x / (uint32_t)a.Hk);
+  if (item >= items[0]) return;
+  const int32_t ti = items[4 + 2 * item], hs = items[5 + 2 * item];
   const AttnTile t = attn_tile(a.plan, (int64_t)a.tiles_max + ti, ti);
-  if (t.tail < 0) return;
+  // (uniform: see grouped_tile of flce_device.h)
+  const int32_t parts = __builtin_amdgcn_readfirstlane(attn_parts(t, a));
   const int64_t o_t = (int64_t)a.Hk * a.D;
   const int64_t o_at = (int64_t)t.row0 * o_t + (int64_t)kvh * a.D;
   const int64_t part_n = (int64_t)a.T * o_t;
@@ -705,13 +803,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   float* pk = a.part + (int64_t)hs * 2 * part_n + o_at;
   float* pv = pk + part_n;
   if (t.tail) {
-    if (a.hsplit > 1) {
-      attn_zero_rows(pk, t.rows, o_t, a.D);
-      attn_zero_rows(pv, t.rows, o_t, a.D);
-    } else {
-      attn_zero_rows(dk, t.rows, o_t, a.D);
-      attn_zero_rows(dv, t.rows, o_t, a.D);
-    }
+    attn_zero_rows(dk, t.rows, o_t, a.D);
+    attn_zero_rows(dv, t.rows, o_t, a.D);
     return;
   }
   const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
@@ -744,8 +837,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   for (int i = 0; i < DP / 32; ++i) ak[i] = av[i] = f32x16_t{};
 
   // the group's heads one after the other, each over the query blocks of [beg, end)
-  const int32_t per = (a.G + a.hsplit - 1) / a.hsplit;
-  const int32_t g0 = (int32_t)hs * per, g1 = min(a.G, g0 + per);
+  const int32_t per = (a.G + parts - 1) / parts;
+  const int32_t g0 = hs * per, g1 = min(a.G, g0 + per);
   AttnDma<T, DP, kQ> sq, sdo;
   sq.init((uint32_t)a.q_t, d_bytes);
   sdo.init((uint32_t)a.do_t, d_bytes);
@@ -769,13 +862,12 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   const int32_t blocks = g1 > g0 ? (g1 - g0) * ((t.end - t.beg + kQ - 1) / kQ) : 0;
   if (blocks > 0) fetch(0);
   const uint32_t range = (uint32_t)(hi - lo), ones = (uint32_t)(s_hi - s_lo);
-  uint32_t buf = 0;
   int32_t i0 = i_last;
-  for (int32_t n = 0; n < blocks; ++n, buf ^= 1u) {
+  auto block = [&](int32_t n, auto buf) {
     attn_sync();
-    if (n + 1 < blocks) fetch(buf ^ 1u);
+    if (n + 1 < blocks) fetch(buf.value ^ 1u);
     if (active && i0 < w_hi && i0 + kQ > w_lo) {
-      const char* qt = smem + buf * kBuf;
+      const char* qt = smem + buf.value * kBuf;
       const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
       const bool edge = i0 < f_lo || i0 + kQ > f_hi;
 #pragma unroll
@@ -819,9 +911,13 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     }
     i0 -= kQ;
     if (i0 < t.beg) i0 = i_last;
+  };
+  for (int32_t n = 0; n < blocks; n += 2) {
+    block(n, AttnBuf<0>());
+    if (n + 1 < blocks) block(n + 1, AttnBuf<1>());
   }
   const int64_t at = (int64_t)(key - t.row0) * o_t;
-  if (a.hsplit > 1) {
+  if (parts > 1) {
     attn_store<T, DP>(ak, a.scale, pk + at, a.D, valid);
     attn_store<T, DP>(av, 1.0f, pv + at, a.D, valid);
   } else {
@@ -830,21 +926,40 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   }
 }
 
-// dK and dV as the sums of their parts over the head groups, in order; four
-// elements per thread.
+// dK and dV of the tiles whose heads were divided, as the sums of their parts in
+// order; four workgroups per tile and key head.
 template <class T>
-__global__ __launch_bounds__(256) void attn_join_kernel(const float* part, int32_t hsplit, int64_t n,
-                                                        T* dk, T* dv) {
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= 2 * n) return;
-  f32x4_t x = *reinterpret_cast<const f32x4_t*>(part + i);
-  for (int32_t s = 1; s < hsplit; ++s)
-    x += *reinterpret_cast<const f32x4_t*>(part + (int64_t)s * 2 * n + i);
-  T* to = i < n ? dk + i : dv + (i - n);
-  if constexpr (sizeof(T) == 2)
-    *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-  else
-    *reinterpret_cast<f32x4_t*>(to) = x;
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
+  const int32_t rest = (int32_t)(blockIdx.x >> 2);
+  const int32_t kvh = rest % a.Hk, ti = rest / a.Hk;
+  const AttnTile t = attn_tile(a.plan, (int64_t)a.tiles_max + ti, ti);
+  if (t.tail != 0) return;
+  const int32_t parts = attn_parts(t, a);
+  if (parts == 1) return;
+  const int64_t o_t = (int64_t)a.Hk * a.D, part_n = (int64_t)a.T * o_t;
+  const int32_t per = a.D / 4;
+  for (int32_t i = (int32_t)((blockIdx.x & 3u) * kAttnThreads + threadIdx.x); i < 2 * t.rows * per;
+       i += 4 * kAttnThreads) {
+    const int32_t which = i >= t.rows * per, j = i - which * t.rows * per;
+    const int64_t at = (int64_t)(t.row0 + j / per) * o_t + (int64_t)kvh * a.D + (j % per) * 4;
+    const float* from = a.part + which * part_n + at;
+    f32x4_t x = f32x4_t{};
+    for (int32_t s0 = 0; s0 < parts; s0 += 4) {  // four loads in flight, added in order
+      f32x4_t y[4];
+#pragma unroll
+      for (int32_t s = 0; s < 4; ++s)
+        y[s] = s0 + s < parts
+                   ? *reinterpret_cast<const f32x4_t*>(from + (int64_t)(s0 + s) * 2 * part_n)
+                   : f32x4_t{};
+#pragma unroll
+      for (int32_t s = 0; s < 4; ++s) x += y[s];
+    }
+    T* to = reinterpret_cast<T*>(which ? a.dv : a.dk) + at;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    else
+      *reinterpret_cast<f32x4_t*>(to) = x;
+  }
 }
 
 }  // namespace mtf

@@ -62,9 +62,12 @@ def _stream(device: torch.device) -> int:
 def _on_device(device: torch.device):
     """Makes `device` the current one where it is not: a launch goes to the
     stream's device only from there."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index == torch._C._cuda_getDevice():
+        return _HERE
     return torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _require_device(name: str, t: torch.Tensor) -> None:

@@ -14,8 +14,8 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._lib import check, load
-from .flce import _dtype_code, _on_device, _p, _require_device, _stream
+from ._lib import MT_DTYPE_BF16, MT_DTYPE_F32, check, load
+from .flce import _on_device, _require_device, _stream
 
 __all__ = ["clip_grad_norm_", "clip_gradients_"]
 
@@ -49,46 +49,58 @@ def _disjoint(a: tuple, b: tuple) -> bool:
     return off >= cols and off + cols2 <= pitch
 
 
+# type -> (code of the C ABI, bytes)
+_TYPES = {torch.bfloat16: (MT_DTYPE_BF16, 2), torch.float32: (MT_DTYPE_F32, 4)}
+
+
 def _table(gradients: Sequence[torch.Tensor]):
     """(ctypes tables, count, device) of the distinct gradients."""
-    seen, rows, dev = set(), [], None
+    rows = []
+    first = None
     for g in gradients:
-        if id(g) in seen:
-            continue
-        seen.add(id(g))
-        if hasattr(g, "to_local"):
+        if type(g) is not torch.Tensor and hasattr(g, "to_local"):
             raise TypeError("gradients that are shards of a distributed tensor are not supported")
-        _require_device("gradient", g)
-        if g.is_sparse or g.layout != torch.strided:
+        if g.layout is not torch.strided:
             raise TypeError("sparse gradients are not supported")
-        if dev is None:
-            dev = g.device
-        elif g.device != dev:
-            raise ValueError(f"gradients lie on {dev} and {g.device}: one device is supported")
-        code, n = _dtype_code(g.dtype), g.numel()
-        if n == 0:
-            continue
-        cols, pitch = (0, 0) if g.is_contiguous() else _layout(g)
-        es = g.element_size()
-        span = n if not cols else (n // cols - 1) * pitch + cols
-        rows.append((g.data_ptr(), es, cols, pitch, span * es, n, code))
+        where = g.get_device()
+        if where != first:
+            _require_device("gradient", g)
+            if first is not None:
+                raise ValueError(f"gradients lie on devices {first} and {where}: one is supported")
+            first = where
+        n = g.numel()
+        try:
+            code, es = _TYPES[g.dtype]
+        except KeyError:
+            raise TypeError(f"bfloat16 and float32 are supported, got {g.dtype}") from None
+        if g.is_contiguous():
+            if n:
+                rows.append((g.data_ptr(), es, 0, 0, n * es, n, code))
+        else:
+            cols, pitch = _layout(g)
+            span = n if not cols else (n // cols - 1) * pitch + cols
+            rows.append((g.data_ptr(), es, cols, pitch, span * es, n, code))
     rows.sort()
     kept: List[tuple] = []
     open_: List[tuple] = []  # gradients whose range may still reach the next one
+    end = 0
     for r in rows:
-        if open_ or kept:
-            if kept and r == kept[-1]:
-                continue  # the same memory twice: one gradient
+        if kept and r == kept[-1]:
+            continue  # the same memory twice: one gradient
+        if r[0] < end:
             open_ = [o for o in open_ if o[0] + o[4] > r[0]]
             for o in open_:
                 if not _disjoint(o[:5], r[:5]):
                     raise ValueError("two gradients share part of their memory")
+        else:
+            open_ = []
         open_.append(r)
         kept.append(r)
+        end = max(end, r[0] + r[4])
     n = len(kept)
     ptr, _, cols, pitch, _, numel, code = zip(*kept) if n else ((),) * 7
     return ((ctypes.c_void_p * n)(*ptr), (ctypes.c_int64 * n)(*numel), (ctypes.c_int64 * n)(*cols),
-            (ctypes.c_int64 * n)(*pitch), (ctypes.c_int32 * n)(*code)), n, dev
+            (ctypes.c_int64 * n)(*pitch), (ctypes.c_int32 * n)(*code)), n, gradients[0].device
 
 
 @torch.no_grad()
@@ -119,13 +131,13 @@ def clip_gradients_(gradients: Iterable[torch.Tensor], max_norm: float, norm_typ
     out = torch.empty(2, dtype=torch.float32, device=dev)
     ws = torch.empty(lib.mt_grad_norm_workspace_bytes(tables[1], n), dtype=torch.uint8, device=dev)
     with _on_device(dev):
-        check(lib.mt_grad_norm(*tables, n, int(norm_type == math.inf), max_norm, _p(ws), ws.numel(),
-                               _p(out), _stream(dev)), "mt_grad_norm")
+        check(lib.mt_grad_norm(*tables, n, int(norm_type == math.inf), max_norm,
+                               ws.data_ptr(), ws.numel(), out.data_ptr(), _stream(dev)), "mt_grad_norm")
         if error_if_nonfinite and not bool(torch.isfinite(out[0])):
             raise RuntimeError(f"The total norm of order {norm_type} for gradients is non-finite, so "
                                "it cannot be clipped. To disable this error and scale the gradients by "
                                "the non-finite norm anyway, set `error_if_nonfinite=False`")
-        check(lib.mt_grad_scale(*tables, n, _p(out), _stream(dev)), "mt_grad_scale")
+        check(lib.mt_grad_scale(*tables, n, out.data_ptr(), _stream(dev)), "mt_grad_scale")
     torch.autograd.graph.increment_version(gradients)
     return out[0]
 
