@@ -426,6 +426,34 @@ __device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float
     }
 }
 
+// The two waves of a pair (SPLIT = 2): the odd one leaves its accumulators, m and
+// sum in LDS and is done (false); the even one gets the other's m and sum, and its
+// accumulators from attn_add_pair.
+template <int DP>
+__device__ __forceinline__ bool attn_join_pair(const f32x16_t (&acc)[DP / 32], float& m, float& sum,
+                                               char* lds) {
+  float* at = reinterpret_cast<float*>(lds) + (wave_id() >> 1) * (64 * (DP / 2 + 2)) + lane_id();
+  __syncthreads();  // the tiles have been read
+  if (wave_id() & 1u) {
+#pragma unroll
+    for (int i = 0; i < DP / 2; ++i) at[64 * i] = acc[i / 16][i % 16];
+    at[64 * (DP / 2)] = m;
+    at[64 * (DP / 2 + 1)] = sum;
+  }
+  __syncthreads();
+  if (wave_id() & 1u) return false;
+  m = at[64 * (DP / 2)];
+  sum = at[64 * (DP / 2 + 1)];
+  return true;
+}
+template <int DP>
+__device__ __forceinline__ void attn_add_pair(f32x16_t (&acc)[DP / 32], float f, float f2, const char* lds) {
+  const float* at = reinterpret_cast<const float*>(lds) + (wave_id() >> 1) * (64 * (DP / 2 + 2)) + lane_id();
+#pragma unroll
+  for (int i = 0; i < DP / 2; ++i)
+    acc[i / 16][i % 16] = fmaf(at[64 * i], f2, acc[i / 16][i % 16] * f);
+}
+
 // rows x D zeros, rows `pitch` elements apart (D: whole 16-byte chunks).
 template <class Out>
 __device__ __forceinline__ void attn_zero_rows(Out* base, int32_t rows, int64_t pitch, int32_t D) {
@@ -465,6 +493,23 @@ __device__ __forceinline__ int32_t attn_parts(int32_t cost, int32_t most, int32_
     while (n < parts_max && (int64_t)cost * G * 700 > n * work) ++n;
   const int32_t per = (G + n - 1) / n;
   return (G + per - 1) / per;
+}
+
+// Half `which` of a query tile, the later rows first; false if it has none.
+__device__ __forceinline__ bool attn_half(AttnTile& t, int32_t which, int32_t window) {
+  constexpr int32_t kHalf = kAttnRows / 2;
+  if (which == 1) {
+    t.rows = min(t.rows, kHalf);
+  } else {
+    t.row0 += kHalf;
+    t.rows -= kHalf;
+    if (t.rows <= 0) return false;
+  }
+  if (!t.tail) {
+    t.beg = attn_row_lo(t.row0, t.ds, window);
+    t.end = attn_row_hi(t.row0 + t.rows - 1, t.pe);
+  }
+  return true;
 }
 
 struct AttnArgs {
@@ -537,7 +582,10 @@ __device__ __forceinline__ void attn_items(const AttnArgs& a, int32_t* scratch) 
 
 constexpr int kAttnKeys = 64;  // keys per block of the forward and of dQ
 
-template <class T, int DP, bool CAP>
+// SPLIT = 2: a workgroup takes half a tile, its waves in pairs that share 32 rows,
+// each over half of every block's keys, and join at the end: twice the workgroups,
+// each with half the way, where there are few of them (attn_split of the host).
+template <class T, int DP, bool CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_fwd_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
@@ -546,9 +594,11 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
   // consecutive workgroups lie on different XCDs: with 8 key heads an XCD's L2 holds one of them
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
-  const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
-  const AttnTile t = attn_tile(a.plan, ti, ti);
+  const int32_t ti = (int32_t)(rest / (uint32_t)a.G) / SPLIT;
+  AttnTile t = attn_tile(a.plan, ti, ti);
   if (t.tail < 0) return;
+  if constexpr (SPLIT == 2)
+    if (!attn_half(t, (int32_t)(rest / (uint32_t)a.G) & 1, a.window)) return;
   const int64_t o_t = (int64_t)a.Hq * a.D;
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)t.row0 * o_t + (int64_t)head * a.D;
   float* lse = a.lse + (int64_t)head * a.T;
@@ -559,7 +609,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
   }
   const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
   const uint32_t d_bytes = (uint32_t)a.D * sizeof(T);
-  const int32_t r0 = t.row0 + 32 * (int32_t)w, row = r0 + (int32_t)(l & 31u);
+  const int32_t r0 = t.row0 + 32 * (int32_t)(w / SPLIT), row = r0 + (int32_t)(l & 31u);
+  // the wave's keys of a block: kOwn from `first` on
+  constexpr int32_t kOwn = kAttnKeys / SPLIT;
+  const int32_t first = SPLIT == 2 ? 32 * (int32_t)(w & 1u) : 0;
   const int32_t r_end = t.row0 + t.rows;
   const bool active = r0 < r_end, valid = row < r_end;
   const int32_t r_last = min(r0 + 31, r_end - 1);
@@ -589,30 +642,34 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     attn_sync();
     // into the buffer that every wave has left at the barrier
     if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf.value ^ 1u);
-    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) return;
+    k0 += first;
+    if (!active || k0 >= w_hi || k0 + kOwn <= w_lo) return;
     const char* kt = smem + buf.value * 2 * kTile;
-    f32x16_t s[2] = {f32x16_t{}, f32x16_t{}};
+    f32x16_t s[2 / SPLIT];
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b) attn_row_product<T, DP>(s[b], kt, 32u * b, qf);
-    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 1, 4>();
+    for (uint32_t b = 0; b < 2 / SPLIT; ++b) {
+      s[b] = f32x16_t{};
+      attn_row_product<T, DP>(s[b], kt, (uint32_t)first + 32u * b, qf);
+    }
+    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8 / SPLIT, 1, 4>();
     if constexpr (CAP) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2 / SPLIT; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[b][r] = attn_tanh<T>(s[b][r] * a.cap_mul);
     }
-    if (k0 < f_lo || k0 + kAttnKeys > f_hi) {
+    if (k0 < f_lo || k0 + kOwn > f_hi) {
       attn_no_if_conversion();
       const uint32_t from = (uint32_t)(k0 + 4 * (int32_t)h - lo), n = (uint32_t)(hi - lo);
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2 / SPLIT; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (from + (uint32_t)(32 * b + 8 * (r / 4) + r % 4) >= n) s[b][r] = -INFINITY;
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < 32; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
+    for (int i = 1; i < 32 / SPLIT; ++i) mx = fmaxf(mx, s[i / 16][i % 16]);
     mx = attn_pair_max(mx) * a.z_mul;
     // the running maximum moves when it has to: up to 2^8 of slack costs no
     // precision in a floating format and saves rescaling the sums.  Each row goes
@@ -628,21 +685,30 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
         for (int r = 0; r < 16; ++r) acc[i][r] *= f;
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2 / SPLIT; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[b][r] = fast_exp2(fmaf(s[b][r], a.z_mul, -m));
         sum += s[b][r];
       }
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b) attn_col_product<T, DP>(acc, kt + kTile, 32u * b, s[b]);
-    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 2, 4>();
+    for (uint32_t b = 0; b < 2 / SPLIT; ++b)
+      attn_col_product<T, DP>(acc, kt + kTile, (uint32_t)first + 32u * b, s[b]);
+    if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8 / SPLIT, 2, 4>();
   };
   for (int32_t k0 = t.beg; k0 < t.end; k0 += 2 * kAttnKeys) {
     block(k0, AttnBuf<0>());
     if (k0 + kAttnKeys < t.end) block(k0 + kAttnKeys, AttnBuf<1>());
   }
   sum = attn_pair_add(sum);
+  if constexpr (SPLIT == 2) {
+    float m2 = m, sum2 = sum;
+    if (!attn_join_pair<DP>(acc, m2, sum2, smem)) return;
+    const float mn = fmaxf(m, m2), f = fast_exp2(m - mn), f2 = fast_exp2(m2 - mn);
+    m = mn;
+    sum = sum * f + sum2 * f2;
+    attn_add_pair<DP>(acc, f, f2, smem);
+  }
   if (valid && h == 0) lse[row] = m + fast_log2(sum);
   attn_store<T, DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + (int64_t)row * o_t + (int64_t)head * a.D,
                     a.D, valid);
@@ -650,7 +716,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 
 // --- backward: delta and dQ ---------------------------------------------------
 
-template <class T, int DP, bool CAP>
+template <class T, int DP, bool CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dq_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
@@ -662,9 +728,11 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   const uint32_t id = blockIdx.x - 1;
   const uint32_t kvh = id % (uint32_t)a.Hk, rest = id / (uint32_t)a.Hk;
   const uint32_t head = kvh * (uint32_t)a.G + rest % (uint32_t)a.G;
-  const int32_t ti = (int32_t)(rest / (uint32_t)a.G);
-  const AttnTile t = attn_tile(a.plan, ti, ti);
+  const int32_t ti = (int32_t)(rest / (uint32_t)a.G) / SPLIT;
+  AttnTile t = attn_tile(a.plan, ti, ti);
   if (t.tail < 0) return;
+  if constexpr (SPLIT == 2)
+    if (!attn_half(t, (int32_t)(rest / (uint32_t)a.G) & 1, a.window)) return;
   const int64_t o_t = (int64_t)a.Hq * a.D;
   T* dq = reinterpret_cast<T*>(a.dq) + (int64_t)head * a.D;
   if (t.tail) {
@@ -673,7 +741,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   }
   const uint32_t w = wave_id(), l = lane_id(), h = l >> 5;
   const uint32_t d_bytes = (uint32_t)a.D * sizeof(T);
-  const int32_t r0 = t.row0 + 32 * (int32_t)w, row = r0 + (int32_t)(l & 31u);
+  const int32_t r0 = t.row0 + 32 * (int32_t)(w / SPLIT), row = r0 + (int32_t)(l & 31u);
+  // the wave's keys of a block: kOwn from `first` on
+  constexpr int32_t kOwn = kAttnKeys / SPLIT;
+  const int32_t first = SPLIT == 2 ? 32 * (int32_t)(w & 1u) : 0;
   const int32_t r_end = t.row0 + t.rows;
   const bool active = r0 < r_end, valid = row < r_end;
   const int32_t r_last = min(r0 + 31, r_end - 1);
@@ -727,14 +798,15 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   auto block = [&](int32_t k0, auto buf) {
     attn_sync();
     if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf.value ^ 1u);
-    if (!active || k0 >= w_hi || k0 + kAttnKeys <= w_lo) return;
+    k0 += first;
+    if (!active || k0 >= w_hi || k0 + kOwn <= w_lo) return;
     const char* kt = smem + buf.value * 2 * kTile;
-    const bool edge = k0 < f_lo || k0 + kAttnKeys > f_hi;
+    const bool edge = k0 < f_lo || k0 + kOwn > f_hi;
 #pragma unroll
-    for (uint32_t b = 0; b < 2; ++b) {
+    for (uint32_t b = 0; b < 2 / SPLIT; ++b) {
       f32x16_t s = f32x16_t{}, dp = f32x16_t{};
-      attn_row_product<T, DP>(s, kt, 32u * b, qf);
-      attn_row_product<T, DP>(dp, kt + kTile, 32u * b, dof);
+      attn_row_product<T, DP>(s, kt, (uint32_t)first + 32u * b, qf);
+      attn_row_product<T, DP>(dp, kt + kTile, (uint32_t)first + 32u * b, dof);
       if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 1, 4>();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -751,13 +823,18 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
         for (int r = 0; r < 16; ++r)
           if (from + (uint32_t)(8 * (r / 4) + r % 4) >= n) s[r] = 0.f;
       }
-      attn_col_product<T, DP>(acc, kt, 32u * b, s);
+      attn_col_product<T, DP>(acc, kt, (uint32_t)first + 32u * b, s);
       if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 16, 2, 4>();
     }
   };
   for (int32_t k0 = t.beg; k0 < t.end; k0 += 2 * kAttnKeys) {
     block(k0, AttnBuf<0>());
     if (k0 + kAttnKeys < t.end) block(k0 + kAttnKeys, AttnBuf<1>());
+  }
+  if constexpr (SPLIT == 2) {
+    float none = 0.f, none2 = 0.f;
+    if (!attn_join_pair<DP>(acc, none, none2, smem)) return;
+    attn_add_pair<DP>(acc, 1.0f, 1.0f, smem);
   }
   attn_store<T, DP>(acc, a.scale, dq + (int64_t)row * o_t, a.D, valid);
 }
