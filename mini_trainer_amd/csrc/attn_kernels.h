@@ -202,6 +202,20 @@ struct AttnLds {
   }
 };
 
+typedef __amdgpu_buffer_rsrc_t attn_rsrc_t;
+
+__device__ __forceinline__ attn_rsrc_t attn_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4_t attn_load16(attn_rsrc_t r, uint32_t off) {
+  return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+}
+__device__ __forceinline__ void attn_store16(u32x4_t v, attn_rsrc_t r, uint32_t off) {
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, off, 0, 0);
+}
+
+constexpr uint32_t kAttnOut = 0xfffffff0u;  // an offset past every resource: loads give 0, stores are dropped
+
 // The rows that a lane keeps in registers as the right operand of a product
 // over d: row (l & 31) of the wave, half of d by l >> 5.
 template <class T, int DP>
@@ -212,14 +226,15 @@ struct AttnFrag {
     const uint32_t h = lane_id() >> 5;
     return sizeof(T) == 4 ? h * (uint32_t)kN + (uint32_t)t : 2u * (uint32_t)t + h;
   }
-  // row: address of the row's first element; chunks at or beyond d_bytes are zeros.
-  __device__ __forceinline__ void load(const char* row, uint32_t d_bytes, bool valid) {
+  // base (uniform): the first of the wave's rows, `stride` bytes apart; rows at or
+  // beyond `rows` and chunks at or beyond d_bytes are zeros.
+  __device__ __forceinline__ void load(const char* base, uint32_t stride, int32_t rows, uint32_t d_bytes) {
+    const uint32_t row = lane_id() & 31u;
+    const attn_rsrc_t r = attn_rsrc(base, rows > 0 ? (uint32_t)(min(rows, 32) - 1) * stride + d_bytes : 0u);
 #pragma unroll
-    for (int t = 0; t < kN; ++t) {
-      v[t] = u32x4_t{0u, 0u, 0u, 0u};
-      if (valid && chunk(t) * 16u < d_bytes)
-        v[t] = *reinterpret_cast<const u32x4_t*>(row + chunk(t) * 16u);
-    }
+    for (int t = 0; t < kN; ++t)
+      v[t] = attn_load16(r, (int32_t)row < rows && chunk(t) * 16u < d_bytes ? row * stride + chunk(t) * 16u
+                                                                           : kAttnOut);
   }
 };
 
@@ -310,11 +325,6 @@ __device__ __forceinline__ void attn_col_product(f32x16_t (&acc)[DP / 32], const
   }
 }
 
-typedef __amdgpu_buffer_rsrc_t attn_rsrc_t;
-
-__device__ __forceinline__ attn_rsrc_t attn_rsrc(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)bytes, 0x00020000);
-}
 // LDS DMA: LDS[dst + size lane] = mem[r + off], `size` bytes per lane.
 __device__ __forceinline__ void attn_dma16(attn_rsrc_t r, char* dst, uint32_t off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)dst, 16, off, 0, 0, 0);
@@ -342,7 +352,7 @@ struct AttnDma {
       const uint32_t idx = (wave_id() * kN + (uint32_t)i) * 64u + lane_id();
       const uint32_t row = idx / AttnLds<T, DP>::kCh;
       const uint32_t ch = (idx % AttnLds<T, DP>::kCh) ^ AttnLds<T, DP>::swz(row);
-      off[i] = ch * 16u < d_bytes ? row * stride + ch * 16u : 0xfffffff0u;
+      off[i] = ch * 16u < d_bytes ? row * stride + ch * 16u : kAttnOut;
     }
   }
   __device__ __forceinline__ void issue(const char* base, int32_t rows, char* tile) const {
@@ -405,25 +415,46 @@ __device__ __forceinline__ float attn_tanh(float x) {
   return fmaf(-2.0f, __builtin_amdgcn_rcpf(fast_exp2(x * (2.0f * kLog2e)) + 1.0f), 1.0f);
 }
 
-// acc^T [DP x 32 rows] * s to one row of D elements per lane.
-template <class T, int DP, class Out>
-__device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float s, Out* row,
-                                           int32_t D, bool valid) {
-  const uint32_t h = lane_id() >> 5;
+// acc^T [DP x 32 rows] * s (one per row) to the wave's rows of D elements, `pitch`
+// elements apart from base (uniform) on; rows at or beyond `rows` are not written.
+// The two lanes of a row hold four elements in turn; bf16 pairs of fours are
+// exchanged so that each lane writes 16 bytes.
+template <int DP, class Out>
+__device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float s, Out* base, int64_t pitch,
+                                           int32_t rows, int32_t D) {
+  const uint32_t h = lane_id() >> 5, row = lane_id() & 31u;
+  const uint32_t stride = (uint32_t)(pitch * (int64_t)sizeof(Out));
+  const attn_rsrc_t r =
+      attn_rsrc(base, rows > 0 ? (uint32_t)(min(rows, 32) - 1) * stride + (uint32_t)D * sizeof(Out) : 0u);
+  const uint32_t at = (int32_t)row < rows ? row * stride : kAttnOut;
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db)
+  for (int db = 0; db < DP / 32; ++db) {
+    if constexpr (sizeof(Out) == 2) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int32_t d = 32 * db + 8 * g + 4 * (int32_t)h;
-      if (valid && d < D) {
-        const float x0 = acc[db][4 * g] * s, x1 = acc[db][4 * g + 1] * s;
-        const float x2 = acc[db][4 * g + 2] * s, x3 = acc[db][4 * g + 3] * s;
-        if constexpr (sizeof(Out) == 2)
-          *reinterpret_cast<u32x2_t*>(row + d) = u32x2_t{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
-        else
-          *reinterpret_cast<f32x4_t*>(row + d) = f32x4_t{x0, x1, x2, x3};
+      for (int g = 0; g < 2; ++g) {
+        u32x4_t v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = pack_bf16x2(acc[db][8 * g + 2 * e] * s, acc[db][8 * g + 2 * e + 1] * s);
+          const uint32_t y = pack_bf16x2(acc[db][8 * g + 4 + 2 * e] * s, acc[db][8 * g + 5 + 2 * e] * s);
+          const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+          v[e] = z[0];
+          v[2 + e] = z[1];
+        }
+        const uint32_t d = 32u * db + 16u * g + 8u * h;
+        attn_store16(v, r, (int32_t)d < D && at != kAttnOut ? at + d * 2u : kAttnOut);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t d = 32u * db + 8u * g + 4u * h;
+        const f32x4_t v = {acc[db][4 * g] * s, acc[db][4 * g + 1] * s, acc[db][4 * g + 2] * s,
+                           acc[db][4 * g + 3] * s};
+        attn_store16(__builtin_bit_cast(u32x4_t, v), r,
+                     (int32_t)d < D && at != kAttnOut ? at + d * 4u : kAttnOut);
       }
     }
+  }
 }
 
 // The two waves of a pair (SPLIT = 2): the odd one leaves its accumulators, m and
@@ -476,21 +507,25 @@ __device__ __forceinline__ AttnTile attn_tile(const int32_t* plan, int64_t at, i
 }
 
 // Workgroups among which the query heads of a key tile's group are divided, each
-// writing fp32 parts of dK and dV for attn_join_kernel: as many as keep a
-// workgroup below three quarters of what each of 512 resident ones gets of all the
-// work (`cost` of this tile, `most` of the costliest and `total` of all, each for
-// one head), and one, writing the results themselves, for the tiles below that.
-// Where even the costliest tile is within 1.25 shares none is divided: the order
-// of the tiles balances those, and workgroups that walk the same heads share them
-// in L2.  64 documents in 32768 tokens, 6 heads a group, dK/dV and join: 320 us;
-// every tile in 6 parts 422, in 3 479 us.  One document of 16384 tokens: 4.5 ms
-// undivided, 5.1 with its longer half in two parts.
-__device__ __forceinline__ int32_t attn_parts(int32_t cost, int32_t most, int32_t total, int32_t Hq,
-                                              int32_t G, int32_t parts_max) {
+// writing fp32 parts of dK and dV for attn_join_kernel; with one, a workgroup
+// writes the results themselves.  (cost of this tile, most of the costliest, total
+// of all `tiles`, in blocks of 64 queries of one head.)
+//   The costliest tile more than 1.25 times what each of 512 resident workgroups
+//   gets of all the work, few long documents among short ones: as many as keep a
+//   workgroup below three quarters of that.  64 documents in 32768 tokens, 6 heads
+//   a group, dK/dV and join: 295 us; every tile in 6 parts 422, in 3 479 us.
+//   Otherwise, where a tile has 128 blocks on average: 2048 workgroups, so that
+//   they end together; one document of 16384 tokens 4.15 ms, undivided 4.4.
+//   Otherwise one: 256 documents of 128 tokens take 76 us so, 148 divided, since
+//   the parts are most of the bytes.
+__device__ __forceinline__ int32_t attn_parts(int32_t cost, int32_t most, int32_t total, int32_t tiles,
+                                              int32_t Hq, int32_t G, int32_t parts_max) {
   const int64_t work = (int64_t)total * Hq;
   int32_t n = 1;
   if ((int64_t)most * G * 410 > work)
     while (n < parts_max && (int64_t)cost * G * 700 > n * work) ++n;
+  else if ((int64_t)total * G >= (int64_t)tiles * 128)
+    while (n < parts_max && (int64_t)n * tiles * (Hq / G) < 2048) ++n;
   const int32_t per = (G + n - 1) / n;
   return (G + per - 1) / per;
 }
@@ -528,7 +563,7 @@ struct AttnArgs {
 
 __device__ __forceinline__ int32_t attn_parts(const AttnTile& t, const AttnArgs& a) {
   const auto* head = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)a.plan;
-  return attn_parts(attn_cost(t), head[2], head[1], a.Hq, a.G, a.parts_max);
+  return attn_parts(attn_cost(t), head[2], head[1], head[0], a.Hq, a.G, a.parts_max);
 }
 
 // What attn_dkdv_kernel's workgroups of one key head take: (tile, part) pairs, the
@@ -621,8 +656,6 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
   const int32_t f_lo = attn_row_lo(r_last, t.ds, a.window), f_hi = attn_row_hi(r0, t.pe);
   const int32_t lo = attn_row_lo(row, t.ds, a.window), hi = valid ? attn_row_hi(row, t.pe) : lo;
 
-  AttnFrag<T, DP> qf;
-  qf.load(a.q + (int64_t)row * a.q_t + (int64_t)head * a.q_h, d_bytes, valid);
   f32x16_t acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
@@ -638,6 +671,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
   fetch(t.beg, 0);
+  AttnFrag<T, DP> qf;
+  qf.load(a.q + (int64_t)r0 * a.q_t + (int64_t)head * a.q_h, (uint32_t)a.q_t, r_end - r0, d_bytes);
   auto block = [&](int32_t k0, auto buf) {
     attn_sync();
     // into the buffer that every wave has left at the barrier
@@ -710,8 +745,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     attn_add_pair<DP>(acc, f, f2, smem);
   }
   if (valid && h == 0) lse[row] = m + fast_log2(sum);
-  attn_store<T, DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + (int64_t)row * o_t + (int64_t)head * a.D,
-                    a.D, valid);
+  attn_store<DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + (int64_t)r0 * o_t + (int64_t)head * a.D, o_t,
+                 r_end - r0, a.D);
 }
 
 // --- backward: delta and dQ ---------------------------------------------------
@@ -755,36 +790,6 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   // sums in different orders, would miss by their rounding: it counts as seeing none
   const int32_t hi = valid && attn_row_hi(row, t.pe) - lo > 1 ? attn_row_hi(row, t.pe) : lo;
 
-  AttnFrag<T, DP> qf, dof;
-  float delta = 0.f, lse = 0.f;
-  dof.load(a.dout + (int64_t)row * a.do_t + (int64_t)head * a.do_h, d_bytes, valid);
-  {
-    AttnFrag<T, DP> of;
-    of.load(a.o + ((int64_t)row * o_t + (int64_t)head * a.D) * (int64_t)sizeof(T), d_bytes, valid);
-#pragma unroll
-    for (int i = 0; i < AttnFrag<T, DP>::kN; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t x = of.v[i][e], y = dof.v[i][e];
-        if constexpr (sizeof(T) == 2) {
-          delta = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), delta);
-          delta = fmaf(__uint_as_float(x & 0xffff0000u),
-                       __uint_as_float(y & 0xffff0000u), delta);
-        } else {
-          delta = fmaf(__uint_as_float(x), __uint_as_float(y), delta);
-        }
-      }
-    delta = attn_pair_add(delta);
-    if (valid) {
-      lse = a.lse[(int64_t)head * a.T + row];
-      if (h == 0) a.delta[(int64_t)head * a.T + row] = delta;
-    }
-  }
-  qf.load(a.q + (int64_t)row * a.q_t + (int64_t)head * a.q_h, d_bytes, valid);
-  f32x16_t acc[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
-
   const char* kbase = a.k + (int64_t)kvh * a.k_h;
   const char* vbase = a.v + (int64_t)kvh * a.v_h;
   AttnDma<T, DP, kAttnKeys> sk, sv;
@@ -795,6 +800,30 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     sv.issue(vbase + (int64_t)k0 * a.v_t, t.end - k0, smem + buf * 2 * kTile + kTile);
   };
   fetch(t.beg, 0);
+  AttnFrag<T, DP> qf, dof, of;
+  dof.load(a.dout + (int64_t)r0 * a.do_t + (int64_t)head * a.do_h, (uint32_t)a.do_t, r_end - r0, d_bytes);
+  of.load(a.o + ((int64_t)r0 * o_t + (int64_t)head * a.D) * (int64_t)sizeof(T), (uint32_t)o_t * sizeof(T),
+          r_end - r0, d_bytes);
+  qf.load(a.q + (int64_t)r0 * a.q_t + (int64_t)head * a.q_h, (uint32_t)a.q_t, r_end - r0, d_bytes);
+  const float lse = valid ? a.lse[(int64_t)head * a.T + row] : 0.f;
+  float delta = 0.f;
+#pragma unroll
+  for (int i = 0; i < AttnFrag<T, DP>::kN; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = of.v[i][e], y = dof.v[i][e];
+      if constexpr (sizeof(T) == 2) {
+        delta = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), delta);
+        delta = fmaf(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u), delta);
+      } else {
+        delta = fmaf(__uint_as_float(x), __uint_as_float(y), delta);
+      }
+    }
+  delta = attn_pair_add(delta);
+  if (valid && h == 0) a.delta[(int64_t)head * a.T + row] = delta;
+  f32x16_t acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
   auto block = [&](int32_t k0, auto buf) {
     attn_sync();
     if (k0 + kAttnKeys < t.end) fetch(k0 + kAttnKeys, buf.value ^ 1u);
@@ -836,7 +865,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     if (!attn_join_pair<DP>(acc, none, none2, smem)) return;
     attn_add_pair<DP>(acc, 1.0f, 1.0f, smem);
   }
-  attn_store<T, DP>(acc, a.scale, dq + (int64_t)row * o_t, a.D, valid);
+  attn_store<DP>(acc, a.scale, dq + (int64_t)r0 * o_t, o_t, r_end - r0, a.D);
 }
 
 // --- backward: dK and dV --------------------------------------------------------
@@ -852,7 +881,7 @@ constexpr int attn_q_rows() {
 // keys' K rows 32; their V rows stay in LDS, because with them in registers too a
 // wave needs more than the 256 that let two share a SIMD, and a wave alone hides
 // neither the LDS reads nor the softmax.  One document of 16384 tokens, 32 heads
-// of 128 (8 key heads): 4.5 ms, 970 TFLOP/s; with V in registers 7.4 ms; as two
+// of 128 (8 key heads): 4.1 ms, 1075 TFLOP/s; with V in registers 7.4 ms; as two
 // kinds of workgroup, dK and dV each with their own scores, 5.5 ms.
 template <class T, int DP, bool CAP>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dkdv_kernel(AttnArgs a) {
@@ -901,13 +930,13 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   if (a.window == 1) s_lo = max(t.ds, t.pe - 1), s_hi = t.de;  // (s_lo <= s_hi)
 
   AttnFrag<T, DP> kf, vf;
-  kf.load(a.k + (int64_t)key * a.k_t + (int64_t)kvh * a.k_h, d_bytes, valid);
+  kf.load(a.k + (int64_t)j0 * a.k_t + (int64_t)kvh * a.k_h, (uint32_t)a.k_t, j_end - j0, d_bytes);
   if constexpr (kVLds) {
     AttnDma<T, DP, kAttnRows> sv;
     sv.init((uint32_t)a.v_t, d_bytes);
     sv.issue(a.v + (int64_t)t.row0 * a.v_t + (int64_t)kvh * a.v_h, t.rows, vt);
   } else {
-    vf.load(a.v + (int64_t)key * a.v_t + (int64_t)kvh * a.v_h, d_bytes, valid);
+    vf.load(a.v + (int64_t)j0 * a.v_t + (int64_t)kvh * a.v_h, (uint32_t)a.v_t, j_end - j0, d_bytes);
   }
   f32x16_t ak[DP / 32], av[DP / 32];
 #pragma unroll
@@ -956,6 +985,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
         else
           attn_row_product<T, DP>(dp, qt + kTile, 32u * b, vf);
         if constexpr (sizeof(T) == 2 && !kVLds) attn_sched_reads<DP / 8, 1, 4>();
+        if constexpr (kVLds) {
+          attn_sched_reads<DP / 16, 1, 3>();
+          attn_sched_reads<DP / 16, 2, 2>();
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4_t lse = *reinterpret_cast<const f32x4_t*>(rows + 32 * b + 8 * g + 4 * h);
@@ -983,7 +1016,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
         }
         attn_col_product<T, DP>(av, qt + kTile, 32u * b, s);
         attn_col_product<T, DP>(ak, qt, 32u * b, dp);
-        if constexpr (sizeof(T) == 2 && !kVLds) attn_sched_reads<DP / 8, 2, 4>();
+        if constexpr (sizeof(T) == 2) attn_sched_reads<DP / 8, 2, (kVLds ? 3 : 4)>();
       }
     }
     i0 -= kQ;
@@ -993,13 +1026,13 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     block(n, AttnBuf<0>());
     if (n + 1 < blocks) block(n + 1, AttnBuf<1>());
   }
-  const int64_t at = (int64_t)(key - t.row0) * o_t;
+  const int64_t at = (int64_t)(j0 - t.row0) * o_t;
   if (parts > 1) {
-    attn_store<T, DP>(ak, a.scale, pk + at, a.D, valid);
-    attn_store<T, DP>(av, 1.0f, pv + at, a.D, valid);
+    attn_store<DP>(ak, a.scale, pk + at, o_t, j_end - j0, a.D);
+    attn_store<DP>(av, 1.0f, pv + at, o_t, j_end - j0, a.D);
   } else {
-    attn_store<T, DP>(ak, a.scale, dk + at, a.D, valid);
-    attn_store<T, DP>(av, 1.0f, dv + at, a.D, valid);
+    attn_store<DP>(ak, a.scale, dk + at, o_t, j_end - j0, a.D);
+    attn_store<DP>(av, 1.0f, dv + at, o_t, j_end - j0, a.D);
   }
 }
 
