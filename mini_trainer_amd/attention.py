@@ -12,10 +12,9 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, load, pack_attn_args
-from .flce import _dtype_code, _on_device, _p, _require_device, _stream
+from ._lib import load, pack_attn_args
+from .flce import _backward_once, _dtype_code, _launch, _require_device
 
 __all__ = ["AttentionPlan", "packed_attention", "packed_attention_plan"]
 
@@ -82,17 +81,18 @@ def packed_attention_plan(cu_seqlens: torch.Tensor, tokens: int, window: Optiona
                                "CPU path")
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
-    cu = cu_seqlens.reshape(-1).to(device=dev, dtype=torch.int32).contiguous()
+    cu = cu_seqlens
+    if cu.device != dev or cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous():
+        cu = cu.reshape(-1).to(device=dev, dtype=torch.int32).contiguous()
     pre = None
     if prefix_lens is not None:
         pre = prefix_lens.reshape(-1).to(device=dev, dtype=torch.int32).contiguous()
     nbytes = lib.mt_attn_plan_bytes(T, S)
-    buf = torch.empty(max(1, nbytes // 4), dtype=torch.int32, device=dev)
-    status = torch.empty(1, dtype=torch.int32, device=dev)
+    buf = cu.new_empty(nbytes // 4)
+    status = cu.new_empty(1)
     w = NO_WINDOW if window is None else min(int(window), NO_WINDOW)
-    with _on_device(dev):
-        check(lib.mt_attn_plan(_p(cu), _p(pre), S, T, w, _p(buf), buf.numel() * 4, _p(status),
-                               _stream(dev)), "mt_attn_plan")
+    _launch(dev, "mt_attn_plan", lib.mt_attn_plan, cu.data_ptr(), 0 if pre is None else pre.data_ptr(),
+            S, T, w, buf.data_ptr(), nbytes, status.data_ptr())
     plan = AttentionPlan(T, S, None if window is None else int(window), buf, status)
     if validate:
         plan.validate()
@@ -133,14 +133,12 @@ class _PackedAttention(torch.autograd.Function):
         tail = (T, plan.documents, heads, key.shape[1], D, w, scale, softcap, _dtype_code(query.dtype))
         args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, plan_at,
                               q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
-        with _on_device(dev):
-            check(load().mt_attn_forward(args, _stream(dev)), "mt_attn_forward")
+        _launch(dev, "mt_attn_forward", load().mt_attn_forward, args)
         ctx.save_for_backward(q, k, v, out, lse, plan.buffer)
         ctx.tail = tail
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_backward_once
     def backward(ctx, dout):
         query, key, value, out, lse, plan = ctx.saved_tensors
         dev = query.device
@@ -155,8 +153,7 @@ class _PackedAttention(torch.autograd.Function):
         lib = load()
         nbytes = lib.mt_attn_backward_workspace_bytes(args)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _on_device(dev):
-            check(lib.mt_attn_backward(args, ws.data_ptr(), nbytes, _stream(dev)), "mt_attn_backward")
+        _launch(dev, "mt_attn_backward", lib.mt_attn_backward, args, ws.data_ptr(), nbytes)
         return dq, dk, dv, None, None, None
 
 

@@ -8,12 +8,12 @@ tensors or a missing library raise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import MT_DTYPE_BF16, MT_DTYPE_F32, check, load
@@ -59,15 +59,26 @@ def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _on_device(device: torch.device):
-    """Makes `device` the current one where it is not: a launch goes to the
-    stream's device only from there."""
+def _launch(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, the current stream of `device`), with `device` current."""
     if device.index == torch._C._cuda_getDevice():
-        return _HERE
-    return torch.cuda.device(device)
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream(device))
+    if status:
+        check(status, what)
 
 
-_HERE = contextlib.nullcontext()
+def _backward_once(backward):
+    """A Function's backward that cannot itself be differentiated, with
+    once_differentiable's bookkeeping only where a graph of it is asked for."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
 
 
 def _require_device(name: str, t: torch.Tensor) -> None:

@@ -14,8 +14,8 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
-from ._lib import MT_DTYPE_BF16, MT_DTYPE_F32, check, load
-from .flce import _on_device, _require_device, _stream
+from ._lib import MT_DTYPE_BF16, MT_DTYPE_F32, load
+from .flce import _launch, _require_device
 
 __all__ = ["clip_grad_norm_", "clip_gradients_"]
 
@@ -130,14 +130,13 @@ def clip_gradients_(gradients: Iterable[torch.Tensor], max_norm: float, norm_typ
     lib = load()
     out = torch.empty(2, dtype=torch.float32, device=dev)
     ws = torch.empty(lib.mt_grad_norm_workspace_bytes(tables[1], n), dtype=torch.uint8, device=dev)
-    with _on_device(dev):
-        check(lib.mt_grad_norm(*tables, n, int(norm_type == math.inf), max_norm,
-                               ws.data_ptr(), ws.numel(), out.data_ptr(), _stream(dev)), "mt_grad_norm")
-        if error_if_nonfinite and not bool(torch.isfinite(out[0])):
-            raise RuntimeError(f"The total norm of order {norm_type} for gradients is non-finite, so "
-                               "it cannot be clipped. To disable this error and scale the gradients by "
-                               "the non-finite norm anyway, set `error_if_nonfinite=False`")
-        check(lib.mt_grad_scale(*tables, n, out.data_ptr(), _stream(dev)), "mt_grad_scale")
+    _launch(dev, "mt_grad_norm", lib.mt_grad_norm, *tables, n, int(norm_type == math.inf), max_norm,
+            ws.data_ptr(), ws.numel(), out.data_ptr())
+    if error_if_nonfinite and not bool(torch.isfinite(out[0])):
+        raise RuntimeError(f"The total norm of order {norm_type} for gradients is non-finite, so it "
+                           "cannot be clipped. To disable this error and scale the gradients by the "
+                           "non-finite norm anyway, set `error_if_nonfinite=False`")
+    _launch(dev, "mt_grad_scale", lib.mt_grad_scale, *tables, n, out.data_ptr())
     torch.autograd.graph.increment_version(gradients)
     return out[0]
 

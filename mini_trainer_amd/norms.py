@@ -12,10 +12,9 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ._lib import check, load, pack_norm_args
-from .flce import _dtype_code, _on_device, _require_device, _stream
+from ._lib import load, pack_norm_args
+from .flce import _backward_once, _dtype_code, _launch, _require_device
 
 __all__ = ["residual_rms_norm"]
 
@@ -65,16 +64,14 @@ class _ResidualRmsNorm(torch.autograd.Function):
         args = pack_norm_args(x2.data_ptr(), r2.data_ptr(), w.data_ptr(), _at(pw), _at(g),
                               normed.data_ptr(), new_residual.data_ptr(), rstd.data_ptr(),
                               0, 0, 0, 0, 0, 0, 0, x_t, _pitch(r2), gate_t, 0, 0, T, H, *tail)
-        with _on_device(dev):
-            check(load().mt_norm_forward(args, _stream(dev)), "mt_norm_forward")
+        _launch(dev, "mt_norm_forward", load().mt_norm_forward, args)
         # x is read again only for the gradients of a gate or of a norm on it
         extra = pw is not None or g is not None
         ctx.save_for_backward(x2 if extra else None, w, pw, g, new_residual, rstd)
         ctx.meta = (T, H, x_t, gate_t, tail, None if gate is None else gate.shape)
         return normed, new_residual
 
-    @staticmethod
-    @once_differentiable
+    @_backward_once
     def backward(ctx, dnormed, dnew):
         if dnormed is None and dnew is None:
             return (None,) * 10
@@ -101,8 +98,7 @@ class _ResidualRmsNorm(torch.autograd.Function):
         lib = load()
         nbytes = lib.mt_norm_backward_workspace_bytes(T, H)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        with _on_device(dev):
-            check(lib.mt_norm_backward(args, ws.data_ptr(), nbytes, _stream(dev)), "mt_norm_backward")
+        _launch(dev, "mt_norm_backward", lib.mt_norm_backward, args, ws.data_ptr(), nbytes)
         if T == 0:
             for t in (dw, dpw, dg):
                 if t is not None:
