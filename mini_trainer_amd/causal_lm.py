@@ -18,6 +18,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn.functional as F
 
+from .decoder import ATTENTION_NAME, PLANS_KWARG, minibatch_plans, patch_decoder_layers
 from .flce import fused_linear_cross_entropy, per_sample_loss_sums
 
 __all__ = ["causal_lm_loss", "patch_causal_lm", "sample_loss_sums", "cu_seqlens_from_position_ids",
@@ -76,8 +77,8 @@ def _output_cls():
     return _OUTPUT_CLS
 
 
-def patch_causal_lm(model: torch.nn.Module,
-                    dw_accumulator: Optional[torch.Tensor] = None) -> torch.nn.Module:
+def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tensor] = None,
+                    packed_layers: bool = False) -> torch.nn.Module:
     """Give a transformers *ForCausalLM model a forward that, when labels (or
     shift_labels) are passed, runs the decoder, hands its last hidden states
     and the output-embedding weight to causal_lm_loss and returns a
@@ -95,6 +96,15 @@ def patch_causal_lm(model: torch.nn.Module,
     ignored, as by the reference's loss (none_reduction_losses.py:9).  With
     dw_accumulator (fp32 [V, H]) the lm_head gradient is added there in fp32
     instead of reaching autograd.
+
+    With packed_layers the labelled forward also runs the decoder's attention
+    as packed_attention over the samples of the packed row (bounded by
+    `cu_seqlens`, else by position_ids that restart, which costs a sync, else
+    each row a sample; with each layer's window and softcap), and the addition
+    after attention with the norm behind it as residual_rms_norm in layers of
+    the plain form (decoder.PLAIN_LAYERS).  It takes no attention_mask, cache
+    or attention dropout then, and dense attention weights are not formed.
+    Without labels the model's own attention runs as before.
     """
     decoder = model.get_decoder()
     head = model.get_output_embeddings()
@@ -102,6 +112,7 @@ def patch_causal_lm(model: torch.nn.Module,
         raise ValueError("patch_causal_lm needs an output embedding without bias")
     original = model.forward
     softcap = getattr(model.config, "final_logit_softcapping", None)
+    own_attention = patch_decoder_layers(decoder) if packed_layers else None
 
     def forward(input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
                 inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,
@@ -109,10 +120,23 @@ def patch_causal_lm(model: torch.nn.Module,
                 ignore_index: int = -100, **kwargs):
         kwargs.pop("num_items_in_batch", None)
         if labels is None and shift_labels is None:
-            return original(input_ids=input_ids, attention_mask=attention_mask,
-                            position_ids=position_ids, past_key_values=past_key_values,
-                            inputs_embeds=inputs_embeds, use_cache=use_cache,
-                            logits_to_keep=logits_to_keep, **kwargs)
+            if packed_layers:
+                decoder.config._attn_implementation = own_attention
+            try:
+                return original(input_ids=input_ids, attention_mask=attention_mask,
+                                position_ids=position_ids, past_key_values=past_key_values,
+                                inputs_embeds=inputs_embeds, use_cache=use_cache,
+                                logits_to_keep=logits_to_keep, **kwargs)
+            finally:
+                if packed_layers:
+                    decoder.config._attn_implementation = ATTENTION_NAME
+        if packed_layers:
+            if attention_mask is not None or past_key_values is not None or use_cache:
+                raise ValueError("packed layers take cu_seqlens or position_ids, no attention_mask "
+                                 "and no cache")
+            use_cache = False
+            kwargs[PLANS_KWARG] = minibatch_plans(
+                input_ids if input_ids is not None else inputs_embeds, position_ids, cu_seqlens)
         out = decoder(input_ids=input_ids, attention_mask=attention_mask,
                       position_ids=position_ids, past_key_values=past_key_values,
                       inputs_embeds=inputs_embeds, use_cache=use_cache, **kwargs)

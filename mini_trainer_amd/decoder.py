@@ -1,0 +1,107 @@
+"""A transformers decoder's layers on this package's operators: attention over
+the packed row, and the residual addition with the norm behind it in one pass.
+
+The reference hands attention to a library (setup_model_for_training.py:91) and
+the norms to another (:98-99); patch_causal_lm(packed_layers=True) puts these
+here in their place for the labelled forward, which train.py:97 runs.
+"""
+from __future__ import annotations
+
+import types
+from typing import Optional
+
+import torch
+
+from .attention import AttentionPlan, packed_attention, packed_attention_plan
+from .norms import residual_rms_norm
+
+__all__ = ["AttentionPlans", "patch_decoder_layers"]
+
+ATTENTION_NAME = "mt_packed"
+PLANS_KWARG = "mt_attention_plans"
+# Layers whose forward is norm, attention, addition, norm, MLP, addition.
+PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
+
+
+class AttentionPlans:
+    """The plans of one packed minibatch, one for each window its layers use."""
+
+    def __init__(self, cu_seqlens: torch.Tensor, tokens: int, device: torch.device):
+        self._args = (cu_seqlens, tokens, device)
+        self._plans: dict = {}
+
+    def get(self, window: Optional[int]) -> AttentionPlan:
+        if window not in self._plans:
+            cu, tokens, device = self._args
+            self._plans[window] = packed_attention_plan(
+                cu, tokens, window=window, validate=False, device=None if cu.is_cuda else device)
+        return self._plans[window]
+
+
+def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
+               softcap=None, sliding_window=None, **kwargs):
+    """The attention function of a layer: query [B, heads, T, D], key and value
+    [B, kv_heads, T, D] -> ([B, T, heads, D], None)."""
+    plans = kwargs.get(PLANS_KWARG)
+    if plans is None:
+        raise RuntimeError("packed attention runs in the labelled forward of a model patched with "
+                           "patch_causal_lm(packed_layers=True) only")
+    if dropout:
+        raise ValueError("packed attention has no dropout")
+    if key.shape[2] != query.shape[2]:
+        raise ValueError("packed attention takes no cache of earlier keys")
+    B, heads, T, D = query.shape
+    q, k, v = (t.transpose(1, 2).reshape(B * T, t.shape[1], D) for t in (query, key, value))
+    out = packed_attention(q, k, v, plans.get(sliding_window), scale=scaling, softcap=softcap)
+    return out.view(B, T, heads, D), None
+
+
+def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
+                   past_key_values=None, use_cache=False, position_embeddings=None, **kwargs):
+    """A PLAIN_LAYERS forward with the addition after attention and the norm
+    behind it in one pass."""
+    residual = hidden_states
+    hidden_states, _ = self.self_attn(
+        hidden_states=self.input_layernorm(hidden_states), attention_mask=attention_mask,
+        position_ids=position_ids, past_key_values=past_key_values, use_cache=use_cache,
+        position_embeddings=position_embeddings, **kwargs)
+    norm = self.post_attention_layernorm
+    if PLANS_KWARG in kwargs and hidden_states.dtype == residual.dtype == norm.weight.dtype:
+        hidden_states, residual = residual_rms_norm(hidden_states, residual, norm.weight,
+                                                    eps=norm.variance_epsilon)
+    else:
+        residual = residual + hidden_states
+        hidden_states = norm(residual)
+    return residual + self.mlp(hidden_states)
+
+
+def patch_decoder_layers(decoder: torch.nn.Module) -> str:
+    """Give the decoder's attention modules the packed attention and its plain
+    layers the fused forward; returns the name of the attention it had."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    ALL_ATTENTION_FUNCTIONS.register(ATTENTION_NAME, _attention)
+    had = decoder.config._attn_implementation
+    decoder.config._attn_implementation = ATTENTION_NAME
+    for layer in decoder.modules():
+        if type(layer).__name__ in PLAIN_LAYERS:
+            layer.forward = types.MethodType(_layer_forward, layer)
+    return had
+
+
+def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],
+                    cu_seqlens: Optional[torch.Tensor]) -> AttentionPlans:
+    """The plans of a minibatch of `tokens` [B, T, ...]: documents by cu_seqlens, or
+    where position_ids restart (one sync), or one for each row."""
+    from .causal_lm import cu_seqlens_from_lengths, cu_seqlens_from_position_ids
+
+    B, T = tokens.shape[:2]
+    if B > 1:
+        if cu_seqlens is not None:
+            raise ValueError("cu_seqlens bounds the samples of one packed row; got "
+                             f"{B} rows")
+        cu_seqlens = cu_seqlens_from_lengths([T] * B)
+    elif cu_seqlens is None:
+        cu_seqlens = cu_seqlens_from_lengths([T]) if position_ids is None else \
+            cu_seqlens_from_position_ids(position_ids)
+    return AttentionPlans(cu_seqlens, B * T, tokens.device)
