@@ -32,13 +32,26 @@ int32_t attn_parts_max(const mt_attn_args& a) {
 
 inline size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Places for the parts of one key head.  Where attn_parts goes by the costliest
+// tile, a tile of cost c gets fewer than 700 c / (total kv_heads) + 1 parts and more
+// than one only if that quotient is above 1: below 1400 / kv_heads together.  Where
+// it goes by the number of tiles, n tiles kv_heads < 2048 + tiles kv_heads, and it
+// divides below 2048 tiles x kv_heads: below 4096 / kv_heads.  (A whole copy of dK
+// and dV for each of four heads of a group takes 4.3 GB at 131072 tokens with 8
+// heads of 128; this 0.2 GB, in the same time.)
+int64_t attn_slots(const mt_attn_args& a) {
+  const int64_t parts = attn_parts_max(a);
+  if (parts == 1) return 0;
+  const int64_t most = cdiv(a.T, kAttnRows) * a.kv_heads < 2048 ? 4096 : 1400;
+  return std::min(parts * attn_tiles(a.T, a.S), cdiv(most, a.kv_heads) + parts);
+}
+
 size_t attn_part_bytes(const mt_attn_args& a) {
-  const int32_t parts = attn_parts_max(a);
-  return parts > 1 ? (size_t)parts * 2 * (size_t)a.T * (size_t)a.kv_heads * (size_t)a.head_dim * 4 : 0;
+  return (size_t)attn_slots(a) * (size_t)a.kv_heads * 2 * kAttnRows * (size_t)a.head_dim * 4;
 }
 
 size_t attn_item_bytes(const mt_attn_args& a) {
-  return round256(16 + 8 * (size_t)attn_tiles(a.T, a.S) * (size_t)attn_parts_max(a));
+  return round256(16 + 8 * (size_t)attn_tiles(a.T, a.S) * ((size_t)attn_parts_max(a) + 1));
 }
 
 int attn_check(const mt_attn_args* p, bool backward) {
@@ -60,7 +73,7 @@ int attn_check(const mt_attn_args* p, bool backward) {
     return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
   if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
     return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
-  if (attn_tiles(a.T, a.S) * 4 * a.heads > INT32_MAX)
+  if ((attn_tiles(a.T, a.S) + 1) * 4 * (a.heads + 1) > INT32_MAX)
     return fail(MT_ERR_UNSUPPORTED, "%lld tiles x %lld heads exceed one launch",
                 (long long)attn_tiles(a.T, a.S), (long long)a.heads);
   const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
@@ -190,6 +203,7 @@ int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace
   k.items = reinterpret_cast<int32_t*>(items);
   k.part = reinterpret_cast<float*>(items + attn_item_bytes(a));
   k.parts_max = attn_parts_max(a);
+  k.slots = (int32_t)attn_slots(a);
   const bool cap = a.softcap > 0.f;
   hipStream_t s = (hipStream_t)stream;
   const int split = attn_split(a);

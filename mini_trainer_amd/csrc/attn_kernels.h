@@ -77,12 +77,13 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
                                                          int32_t* status) {
   __shared__ int32_t hist[2][kPlanBuckets];
   __shared__ int32_t wave_sum[16];
-  __shared__ int32_t bad, bad_prefix, total, most;
+  __shared__ int32_t bad, bad_prefix, most;
+  __shared__ unsigned long long total;
   const int32_t tid = threadIdx.x;
   AttnTile* qt = reinterpret_cast<AttnTile*>(plan + kPlanHeader);
   AttnTile* kt = qt + tiles_max;
   int32_t* off = reinterpret_cast<int32_t*>(kt + tiles_max);
-  if (tid == 0) bad = cu[0] != 0 || cu[S] > T || cu[S] < 0, bad_prefix = total = most = 0;
+  if (tid == 0) bad = cu[0] != 0 || cu[S] > T || cu[S] < 0, bad_prefix = most = 0, total = 0;
   hist[0][tid] = hist[1][tid] = 0;
   __syncthreads();
   for (int32_t s = tid; s < S; s += 1024) {
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
       const int32_t cq = min(kPlanBuckets - 1, attn_cost(q));
       const int32_t ck = min(kPlanBuckets - 1, attn_cost(k));
       if (pass == 0) {
-        atomicAdd(&total, attn_cost(k));
+        atomicAdd(&total, (unsigned long long)attn_cost(k));
         atomicMax(&most, attn_cost(k));
         atomicAdd(&hist[0][cq], 1);
         atomicAdd(&hist[1][ck], 1);
@@ -158,7 +159,7 @@ __global__ __launch_bounds__(1024) void attn_plan_kernel(const int32_t* cu, cons
     }
     __syncthreads();
     if (pass == 0) {  // hist[b] -> tiles in the costlier buckets
-      if (tid == 0) plan[1] = total, plan[2] = most;
+      if (tid == 0) plan[1] = (int32_t)min(total, 0x7fffffffull), plan[2] = most;
       for (int which = 0; which < 2; ++which) {
         const int32_t bucket = kPlanBuckets - 1 - tid;
         const int32_t n = hist[which][bucket];
@@ -552,10 +553,10 @@ struct AttnArgs {
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h;  // bytes
   char *out, *dq, *dk, *dv;                    // [T, heads, D], contiguous
   float *lse, *delta;                          // [Hq, T]; lse in units of log2
-  int32_t* items;                              // attn_items: count, 3 unused, then (tile, part) pairs
-  float* part;                                 // [parts_max][2][T][Hk][D] when parts_max > 1
+  int32_t* items;                              // attn_items
+  float* part;                                 // [Hk][slots][2][kAttnRows][D]: dK, dV of one part
   const int32_t* plan;
-  int32_t T, Hq, Hk, G, D, tiles_max, window, parts_max;
+  int32_t T, Hq, Hk, G, D, tiles_max, window, parts_max, slots;
   float scale;     // of the scores
   float z_mul;     // log2 units: scale log2(e), or cap log2(e) with a softcap
   float cap_mul;   // scale / cap
@@ -569,20 +570,40 @@ __device__ __forceinline__ int32_t attn_parts(const AttnTile& t, const AttnArgs&
 // What attn_dkdv_kernel's workgroups of one key head take: (tile, part) pairs, the
 // costliest first (counting sort), and none without work among them: those would
 // be dealt out in turn with the others and leave the shader engines that get them
-// idle.  One workgroup.
+// idle (9.4 instead of 4.4 ms).  Tiles with several parts get places for them in
+// a.part, as long as there are any (attn_slots of the host has enough for what
+// attn_parts divides).  One workgroup.
+//   a.items: [0] pairs; from 4 on the pairs; from 4 + 2 tiles_max parts_max on for
+//   each tile its parts and the first one's place
+__device__ __forceinline__ int32_t attn_tile_info(const AttnArgs& a, int32_t ti) {
+  return 4 + 2 * a.tiles_max * a.parts_max + 2 * ti;
+}
 __device__ __forceinline__ void attn_items(const AttnArgs& a, int32_t* scratch) {
   int32_t* hist = scratch;                  // kPlanBuckets
   int32_t* sums = scratch + kPlanBuckets;   // one per thread
+  int32_t* used = sums + kAttnThreads;      // places given out
   const int32_t tid = (int32_t)threadIdx.x, tiles = a.plan[0];
   constexpr int32_t kPer = kPlanBuckets / kAttnThreads;
   const AttnTile* kt = reinterpret_cast<const AttnTile*>(a.plan + kPlanHeader) + a.tiles_max;
   // costs of an item are at most G times that of the first tile (the costliest)
   const int64_t most = tiles > 0 ? max((int64_t)1, (int64_t)attn_cost(kt[0]) * a.G) : 1;
   for (int32_t i = tid; i < kPlanBuckets; i += kAttnThreads) hist[i] = 0;
+  if (tid == 0) *used = 0;
   __syncthreads();
   for (int pass = 0; pass < 2; ++pass) {
     for (int32_t t = tid; t < tiles; t += kAttnThreads) {
-      const int32_t cost = attn_cost(kt[t]), parts = attn_parts(kt[t], a);
+      const int32_t cost = attn_cost(kt[t]);
+      int32_t* info = a.items + attn_tile_info(a, t);
+      if (pass == 0) {
+        int32_t n = attn_parts(kt[t], a), slot = 0;
+        if (n > 1) {
+          slot = atomicAdd(used, n);
+          if (slot + n > a.slots) n = 1;
+        }
+        info[0] = n;
+        info[1] = slot;
+      }
+      const int32_t parts = info[0];  // (this thread's own of the first pass)
       const int32_t per = (a.G + parts - 1) / parts;
       for (int32_t p = 0; p < parts; ++p) {
         const int64_t c = (int64_t)cost * min(per, a.G - p * per);
@@ -756,6 +777,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
   __shared__ __attribute__((aligned(1024))) char smem[4 * kTile];  // 2 x (K, V)
+  static_assert(sizeof(smem) >= 4 * (kPlanBuckets + kAttnThreads + 1), "attn_items");
   if (blockIdx.x == 0) {  // beside the others, for the launch that follows
     attn_items(a, reinterpret_cast<int32_t*>(smem));
     return;
@@ -899,15 +921,11 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   if (item >= items[0]) return;
   const int32_t ti = items[4 + 2 * item], hs = items[5 + 2 * item];
   const AttnTile t = attn_tile(a.plan, (int64_t)a.tiles_max + ti, ti);
-  // (uniform: see grouped_tile of flce_device.h)
-  const int32_t parts = __builtin_amdgcn_readfirstlane(attn_parts(t, a));
+  const int32_t info = attn_tile_info(a, ti), parts = items[info], slot = items[info + 1] + hs;
   const int64_t o_t = (int64_t)a.Hk * a.D;
   const int64_t o_at = (int64_t)t.row0 * o_t + (int64_t)kvh * a.D;
-  const int64_t part_n = (int64_t)a.T * o_t;
   T* dk = reinterpret_cast<T*>(a.dk) + o_at;
   T* dv = reinterpret_cast<T*>(a.dv) + o_at;
-  float* pk = a.part + (int64_t)hs * 2 * part_n + o_at;
-  float* pv = pk + part_n;
   if (t.tail) {
     attn_zero_rows(dk, t.rows, o_t, a.D);
     attn_zero_rows(dv, t.rows, o_t, a.D);
@@ -1026,11 +1044,12 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     block(n, AttnBuf<0>());
     if (n + 1 < blocks) block(n + 1, AttnBuf<1>());
   }
-  const int64_t at = (int64_t)(j0 - t.row0) * o_t;
   if (parts > 1) {
-    attn_store<DP>(ak, a.scale, pk + at, o_t, j_end - j0, a.D);
-    attn_store<DP>(av, 1.0f, pv + at, o_t, j_end - j0, a.D);
+    float* part = a.part + (((int64_t)kvh * a.slots + slot) * 2 * kAttnRows + (j0 - t.row0)) * a.D;
+    attn_store<DP>(ak, a.scale, part, a.D, j_end - j0, a.D);
+    attn_store<DP>(av, 1.0f, part + (int64_t)kAttnRows * a.D, a.D, j_end - j0, a.D);
   } else {
+    const int64_t at = (int64_t)(j0 - t.row0) * o_t;
     attn_store<DP>(ak, a.scale, dk + at, o_t, j_end - j0, a.D);
     attn_store<DP>(av, 1.0f, dv + at, o_t, j_end - j0, a.D);
   }
@@ -1044,22 +1063,23 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnArgs a) {
   const int32_t kvh = rest % a.Hk, ti = rest / a.Hk;
   const AttnTile t = attn_tile(a.plan, (int64_t)a.tiles_max + ti, ti);
   if (t.tail != 0) return;
-  const int32_t parts = attn_parts(t, a);
+  const int32_t* info = a.items + attn_tile_info(a, ti);
+  const int32_t parts = info[0], n = kAttnRows * a.D;
   if (parts == 1) return;
-  const int64_t o_t = (int64_t)a.Hk * a.D, part_n = (int64_t)a.T * o_t;
+  const float* slot = a.part + ((int64_t)kvh * a.slots + info[1]) * 2 * n;
   const int32_t per = a.D / 4;
   for (int32_t i = (int32_t)((blockIdx.x & 3u) * kAttnThreads + threadIdx.x); i < 2 * t.rows * per;
        i += 4 * kAttnThreads) {
     const int32_t which = i >= t.rows * per, j = i - which * t.rows * per;
-    const int64_t at = (int64_t)(t.row0 + j / per) * o_t + (int64_t)kvh * a.D + (j % per) * 4;
-    const float* from = a.part + which * part_n + at;
+    const int64_t at = ((int64_t)(t.row0 + j / per) * a.Hk + kvh) * a.D + (j % per) * 4;
+    const float* from = slot + which * n + (j / per) * a.D + (j % per) * 4;
     f32x4_t x = f32x4_t{};
     for (int32_t s0 = 0; s0 < parts; s0 += 4) {  // four loads in flight, added in order
       f32x4_t y[4];
 #pragma unroll
       for (int32_t s = 0; s < 4; ++s)
         y[s] = s0 + s < parts
-                   ? *reinterpret_cast<const f32x4_t*>(from + (int64_t)(s0 + s) * 2 * part_n)
+                   ? *reinterpret_cast<const f32x4_t*>(from + (int64_t)(s0 + s) * 2 * n)
                    : f32x4_t{};
 #pragma unroll
       for (int32_t s = 0; s < 4; ++s) x += y[s];
