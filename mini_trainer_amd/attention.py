@@ -81,12 +81,18 @@ def packed_attention_plan(cu_seqlens: torch.Tensor, tokens: int, window: Optiona
                                "CPU path")
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
+    def words(t):  # int64 values that no int32 holds stay malformed
+        t = t.reshape(-1)
+        if t.dtype == torch.int64:
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
+        return t.to(device=dev, dtype=torch.int32).contiguous()
+
     cu = cu_seqlens
     if cu.device != dev or cu.dtype != torch.int32 or cu.dim() != 1 or not cu.is_contiguous():
-        cu = cu.reshape(-1).to(device=dev, dtype=torch.int32).contiguous()
+        cu = words(cu)
     pre = None
     if prefix_lens is not None:
-        pre = prefix_lens.reshape(-1).to(device=dev, dtype=torch.int32).contiguous()
+        pre = words(prefix_lens)
     nbytes = lib.mt_attn_plan_bytes(T, S)
     buf = cu.new_empty(nbytes // 4)
     status = cu.new_empty(1)

@@ -73,9 +73,12 @@ int attn_check(const mt_attn_args* p, bool backward) {
     return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
   if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
     return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
-  if ((attn_tiles(a.T, a.S) + 1) * 4 * (a.heads + 1) > INT32_MAX)
-    return fail(MT_ERR_UNSUPPORTED, "%lld tiles x %lld heads exceed one launch",
-                (long long)attn_tiles(a.T, a.S), (long long)a.heads);
+  if (a.softcap > 0.f && !std::isfinite(a.scale / a.softcap))
+    return fail(MT_ERR_INVALID_ARGUMENT, "scale / softcap is not finite");
+  // workgroups of kAttnThreads, of which a launch takes fewer than 2^32 threads
+  if ((attn_tiles(a.T, a.S) + 1) * std::max(a.heads, 4 * a.kv_heads) >= ((int64_t)1 << 32) / kAttnThreads)
+    return fail(MT_ERR_UNSUPPORTED, "%lld tiles (of %d rows, and one for each document) x %lld heads "
+                "exceed one launch", (long long)attn_tiles(a.T, a.S), kAttnRows, (long long)a.heads);
   const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
                              backward ? a.dout_h : 0};
   for (int64_t s : strides)

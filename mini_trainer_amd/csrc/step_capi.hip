@@ -133,6 +133,8 @@ int launch_norm_fwd(const NormArgs& k, bool vec, hipStream_t stream) {
   return norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
     constexpr int threads = norm_threads(decltype(TPR)::value);
     constexpr int rows = threads / decltype(TPR)::value;
+    if (cdiv(k.T, rows) * threads >= (int64_t)1 << 32)  // threads of a launch
+      return fail(MT_ERR_UNSUPPORTED, "%lld rows of %d exceed one launch", (long long)k.T, k.H);
     hipLaunchKernelGGL((norm_fwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value>),
                        dim3((uint32_t)cdiv(k.T, rows)), dim3(threads), 0, stream, k);
     return check_launch("norm_fwd_kernel");

@@ -19,8 +19,10 @@ __all__ = ["AttentionPlans", "patch_decoder_layers"]
 
 ATTENTION_NAME = "mt_packed"
 PLANS_KWARG = "mt_attention_plans"
-# Layers whose forward is norm, attention, addition, norm, MLP, addition.
+# Layers whose forward is norm, attention, addition, norm, MLP, addition, and the
+# norms that are rms_norm(x) * weight.
 PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
+PLAIN_NORMS = ("LlamaRMSNorm", "Qwen2RMSNorm")
 
 
 class AttentionPlans:
@@ -66,7 +68,8 @@ def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
         position_ids=position_ids, past_key_values=past_key_values, use_cache=use_cache,
         position_embeddings=position_embeddings, **kwargs)
     norm = self.post_attention_layernorm
-    if PLANS_KWARG in kwargs and hidden_states.dtype == residual.dtype == norm.weight.dtype:
+    if PLANS_KWARG in kwargs and type(norm).__name__ in PLAIN_NORMS and \
+            hidden_states.dtype == residual.dtype == norm.weight.dtype:
         hidden_states, residual = residual_rms_norm(hidden_states, residual, norm.weight,
                                                     eps=norm.variance_epsilon)
     else:
@@ -92,16 +95,17 @@ def patch_decoder_layers(decoder: torch.nn.Module) -> str:
 def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],
                     cu_seqlens: Optional[torch.Tensor]) -> AttentionPlans:
     """The plans of a minibatch of `tokens` [B, T, ...]: documents by cu_seqlens, or
-    where position_ids restart (one sync), or one for each row."""
+    where position_ids restart (one sync) and with each row."""
     from .causal_lm import cu_seqlens_from_lengths, cu_seqlens_from_position_ids
 
     B, T = tokens.shape[:2]
-    if B > 1:
-        if cu_seqlens is not None:
-            raise ValueError("cu_seqlens bounds the samples of one packed row; got "
-                             f"{B} rows")
-        cu_seqlens = cu_seqlens_from_lengths([T] * B)
-    elif cu_seqlens is None:
-        cu_seqlens = cu_seqlens_from_lengths([T]) if position_ids is None else \
-            cu_seqlens_from_position_ids(position_ids)
+    if B > 1 and cu_seqlens is not None:
+        raise ValueError(f"cu_seqlens bounds the samples of one packed row; got {B} rows")
+    if cu_seqlens is None:
+        if position_ids is None:
+            cu_seqlens = cu_seqlens_from_lengths([T] * B)
+        else:
+            starts = position_ids.reshape(-1, T).expand(B, T).clone()
+            starts[:, :1] = 0  # a row is no continuation of the one before
+            cu_seqlens = cu_seqlens_from_position_ids(starts)
     return AttentionPlans(cu_seqlens, B * T, tokens.device)

@@ -240,6 +240,15 @@ def test_malformed_boundaries(gpu):
         assert all(torch.equal(got[n], want[n]) for n in got)
 
 
+def test_boundaries_that_no_int32_holds(gpu):
+    wrapped = torch.tensor([0, 2 ** 32 + 300])
+    for where in (wrapped, wrapped.to(gpu)):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            packed_attention_plan(where, 300)
+    with pytest.raises(ValueError, match="prefix"):
+        packed_attention_plan(cu_of([300], gpu), 300, prefix_lens=torch.tensor([2 ** 32 + 5]))
+
+
 def test_plans(gpu):
     """Boundaries as int64, on the CPU, as the call's own argument; one plan for
     several layers with their own heads."""
@@ -356,6 +365,43 @@ def test_captured_and_replayed(gpu):
         want = run(*new, packed_attention_plan(cu_of(bounds, gpu), T), softcap=20.0)
         for g, w in zip(got, want.values()):
             assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_as_far_apart_as_they_may_be(gpu, dtype):
+    """2^24 elements: the last row of a tile lies just below 4 GiB from its first."""
+    T, pitch = 140, 1 << 24
+    big = torch.empty(T * pitch, dtype=dtype, device=gpu)
+    q, k, v, do = inputs(T, 1, 1, 128, dtype, seed=19)
+    plan = packed_attention_plan(cu_of([T], gpu), T)
+    want = run(q, k, v, do, plan)
+    views = [big.as_strided((T, 1, 128), (pitch, 128, 1), 128 * i) for i in range(4)]
+    for view, t in zip(views, (q, k, v, do)):
+        view.copy_(t)
+    got = run(*views, plan)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+
+
+@pytest.mark.parametrize("lengths,heads", [
+    ([2000], 32),                              # divided by cost, 256 tiles x key heads
+    ([3] * 20 + [2000] + [128] * 120, 32),     # by cost, the heavy document's tiles of 2500 only
+    ([2000] * 4, 128)], ids=["one", "heavy", "number"])  # by the number of tiles
+def test_parts_of_divided_heads_find_their_places(gpu, lengths, heads):
+    """Every document's results against those it has alone, in two of 16 key heads."""
+    kv, G, T = 16, heads // 16, sum(lengths)
+    q, k, v, do = inputs(T, heads, kv, 32, torch.float32, seed=21)
+    got = run(q, k, v, do, packed_attention_plan(cu_of(lengths, gpu), T))
+    at = 0
+    for n in lengths:
+        rows = slice(at, at + n)
+        at += n
+        if n < 2000 and at < T:
+            continue  # (the heavy ones and the last)
+        mask = ref.seen_mask([n], n)
+        for h in (0, 15):
+            kh, qh = slice(h, h + 1), slice(G * h, G * h + G)
+            want = ref.attention(q[rows, qh], k[rows, kh], v[rows, kh], do[rows, qh], mask)
+            check({name: t[rows, qh if name in ("out", "dq") else kh] for name, t in got.items()}, want)
 
 
 def test_rows_beyond_32_bit_offsets(gpu):

@@ -140,6 +140,19 @@ def test_rows_window_and_unlabelled_calls(gpu):
         model(input_ids=ids.to(gpu), labels=ids.to(gpu), cu_seqlens=torch.tensor([0, 120]))
 
 
+@pytest.mark.gpu
+def test_another_norm_keeps_its_own_forward(gpu):
+    """A layer whose norm was replaced does not go through residual_rms_norm."""
+    model = tiny(seed=7)
+    for layer in model.model.layers:
+        layer.post_attention_layernorm = torch.nn.LayerNorm(128)
+    ids, labels, pos = packed()
+    loss_ref, _, _ = reference(model, ids, labels)
+    model = patch_causal_lm(model.to(gpu), packed_layers=True)
+    out = model(input_ids=ids.to(gpu), labels=labels.to(gpu), position_ids=pos.to(gpu))
+    assert rel(out.loss.detach(), loss_ref) <= TOL
+
+
 def test_patched_layers_without_a_gpu():
     model = tiny(seed=5)
     ids, labels, pos = packed()

@@ -93,6 +93,9 @@ def attn(**kw):
     (dict(softcap=-1.0), 1), (dict(softcap=math.nan), 1), (dict(q_t=4), 1), (dict(k_h=-8), 1),
     (dict(v_t=(1 << 24) + 8), 3), (dict(q=None), 1), (dict(k=P + 8), 1), (dict(lse=None), 1),
     (dict(plan=None), 1), (dict(T=1 << 28, heads=4096, kv_heads=2), 3),
+    (dict(scale=10.0, softcap=1e-38), 1),                     # their quotient is infinite
+    (dict(T=1 << 24, S=1 << 19, heads=32, kv_heads=8), 3),    # 2^32 threads and more
+    (dict(T=1 << 24, S=1 << 22, heads=4, kv_heads=4), 3),
 ])
 def test_attention_host_checks(kw, code):
     lib = _lib.load()
@@ -147,6 +150,24 @@ def test_norm_host_checks(kw, code):
     lib = _lib.load()
     assert lib.mt_norm_forward(ctypes.byref(norm(**kw)), None) == code
     assert lib.mt_norm_backward(ctypes.byref(norm(**kw)), P, 1 << 40, None) == code
+
+
+def test_rows_beyond_one_launch():
+    lib = _lib.load()
+    assert lib.mt_norm_forward(ctypes.byref(norm(T=1 << 26)), None) == 3
+
+
+def test_plans_of_several_rows():
+    """Rows are documents of their own, and so are the parts of a row whose
+    position_ids restart."""
+    from mini_trainer_amd.decoder import minibatch_plans
+
+    tokens = torch.zeros(2, 6, dtype=torch.int64)
+    for pos, want in ((None, [0, 6, 12]), (torch.arange(6)[None], [0, 6, 12]),
+                      (torch.tensor([[0, 1, 2, 0, 1, 2], [3, 4, 0, 1, 2, 3]]), [0, 3, 6, 8, 12])):
+        assert minibatch_plans(tokens, pos, None)._args[0].tolist() == want
+    assert minibatch_plans(tokens[:1], torch.tensor([[0, 1, 0, 1, 2, 3]]), None)._args[0].tolist() == [0, 2, 6]
+    assert minibatch_plans(tokens[:1], None, None)._args[0].tolist() == [0, 6]
 
 
 def test_norm_backward_workspace():
