@@ -623,6 +623,9 @@ int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t 
  *   lse fp32 [heads, T]: log2 of the sum of 2^(z log2 e), from the forward to
  *     the backward; 0 behind the last document
  *   plan, window: as mt_attn_plan was given them
+ *   out_lo: T x heads x (head_dim rounded up to 32) bytes (bf16; fp32 ignores it)
+ *     for what out's rounding took from it, from the forward to the backward, which
+ *     without it (null) forms the rows' dout . out from the rounded values
  * The backward reads q, k, v, out, lse, dout and writes dq, dk, dv.  Sums in
  * fp32; results do not depend on the order workgroups run in.
  */
@@ -633,6 +636,7 @@ typedef struct mt_attn_args {
   const void* dout;
   void *dq, *dk, *dv;
   const int32_t* plan;
+  void* out_lo;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, dout_t, dout_h;
   int64_t T, S, heads, kv_heads, head_dim, window;
   float scale, softcap;

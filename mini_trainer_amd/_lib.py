@@ -33,7 +33,7 @@ STATUS_NAMES = {
 class AttnArgs(ctypes.Structure):
     """mt_attn_args of include/mt_flce.h."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv",
-                                         "plan")]
+                                         "plan", "out_lo")]
                 + [(n, c_int64) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h", "dout_t",
                                           "dout_h", "T", "S", "heads", "kv_heads", "head_dim",
                                           "window")]

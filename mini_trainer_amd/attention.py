@@ -133,15 +133,21 @@ class _PackedAttention(torch.autograd.Function):
         k, kp, k_t, k_h = _heads(key)
         v, vp, v_t, v_h = _heads(value)
         out = query.new_empty((T, heads, D))
-        lse = torch.empty((heads, T), dtype=torch.float32, device=dev)
+        # lse [heads, T] and, for a backward in bf16, what the rounding of out took from
+        # it, a byte for each element (rows of whole 32) from `low` fp32 words on (a
+        # 16-byte boundary)
+        low = -(-heads * T // 4) * 4 if out.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else 0
+        words = low + T * heads * (-(-D // 32) * 8) if low else heads * T
+        lse = torch.empty(words, dtype=torch.float32, device=dev)
+        lse_at = lse.data_ptr()
         plan_at = plan.buffer.data_ptr()
         w = NO_WINDOW if plan.window is None else min(plan.window, NO_WINDOW)
         tail = (T, plan.documents, heads, key.shape[1], D, w, scale, softcap, _dtype_code(query.dtype))
-        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse.data_ptr(), 0, 0, 0, 0, plan_at,
-                              q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
+        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse_at, 0, 0, 0, 0, plan_at,
+                              lse_at + 4 * low if low else 0, q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
         _launch(dev, "mt_attn_forward", load().mt_attn_forward, args)
         ctx.save_for_backward(q, k, v, out, lse, plan.buffer)
-        ctx.tail = tail
+        ctx.tail, ctx.low = tail, low
         return out
 
     @_backward_once
@@ -153,9 +159,10 @@ class _PackedAttention(torch.autograd.Function):
         value, vp, v_t, v_h = _heads(value)
         dout, dop, do_t, do_h = _heads(dout)
         dq, dk, dv = (t.new_empty(t.shape) for t in (query, key, value))
-        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse.data_ptr(), dop, dq.data_ptr(),
-                              dk.data_ptr(), dv.data_ptr(), plan.data_ptr(), q_t, q_h, k_t, k_h, v_t,
-                              v_h, do_t, do_h, *ctx.tail)
+        lse_at = lse.data_ptr()
+        args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse_at, dop, dq.data_ptr(), dk.data_ptr(),
+                              dv.data_ptr(), plan.data_ptr(), lse_at + 4 * ctx.low if ctx.low else 0,
+                              q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h, *ctx.tail)
         lib = load()
         nbytes = lib.mt_attn_backward_workspace_bytes(args)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -92,6 +92,7 @@ int attn_check(const mt_attn_args* p, bool backward) {
   for (const void* x : need)
     if (!x || !aligned16(x))
       return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned (16 bytes) tensor pointer");
+  if (!aligned16(a.out_lo)) return fail(MT_ERR_INVALID_ARGUMENT, "misaligned (16 bytes) out_lo");
   if (backward) {
     const void* more[] = {a.dout, a.dq, a.dk, a.dv};
     for (const void* x : more)
@@ -116,6 +117,7 @@ AttnArgs attn_args(const mt_attn_args& a) {
   k.dk = static_cast<char*>(a.dk);
   k.dv = static_cast<char*>(a.dv);
   k.lse = a.lse;
+  k.out_lo = a.dtype == MT_DTYPE_BF16 ? static_cast<char*>(a.out_lo) : nullptr;
   k.plan = a.plan;
   k.T = (int32_t)a.T;
   k.Hq = (int32_t)a.heads;

@@ -26,9 +26,7 @@
 // same order.  Sums are fp32.  P and dS are rounded to the inputs' type before
 // their products, since only then these run on the bf16 matrix instructions (at
 // most 2^-8 of each term; the fp32 ones have a sixteenth of their rate); the row sums of P
-// are taken before that rounding.  Against 64 bits the outputs are off by
-// 0.0022 to 0.0030 of their norm, of which 0.0017 is their own rounding to bf16;
-// in fp32 by 5.5e-7.
+// are taken before that rounding, and delta from O before its own (attn_store_out).
 #pragma once
 
 #include <type_traits>
@@ -462,6 +460,67 @@ __device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float
   }
 }
 
+// acc * s as attn_store writes it in bf16, rounded to nearest with ties away from
+// zero, and, if `low` is not null, the byte beneath each value's two: with it the
+// backward has the value to 16 bits (attn_unround), for delta.  Where a few keys hold
+// all of a row's probability, dO . V - delta cancels, and delta from the rounded
+// rows alone leaves dQ and dK off by 0.0057 of their norm (rows of two keys; with
+// these bytes 0.0025, of which 0.0017 is the outputs' own rounding), in long documents
+// by 0.0027 against 0.0024.  The bytes lie as a wave's lanes hold and want them,
+// attn_low_bytes(D) for each row and head: chunks of 8 elements, the even ones, then
+// the odd ones.  low_pitch: bytes from row to row.
+__device__ __host__ __forceinline__ int32_t attn_low_bytes(int32_t D) { return (D + 31) & ~31; }
+
+template <int DP>
+__device__ __forceinline__ void attn_store_out(const f32x16_t (&acc)[DP / 32], float s, __bf16* base,
+                                               int64_t pitch, int32_t rows, int32_t D, char* low,
+                                               int64_t low_pitch) {
+  const uint32_t h = lane_id() >> 5, row = lane_id() & 31u;
+  const uint32_t stride = (uint32_t)pitch * 2u, low_stride = (uint32_t)low_pitch;
+  const uint32_t n = (uint32_t)attn_low_bytes(D) / 2, last = (uint32_t)(min(rows, 32) - 1);
+  const attn_rsrc_t r = attn_rsrc(base, rows > 0 ? last * stride + (uint32_t)D * 2u : 0u);
+  const attn_rsrc_t r_low = attn_rsrc(low, rows > 0 && low ? last * low_stride + 2 * n : 0u);
+  const bool mine = (int32_t)row < rows;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) {
+    uint32_t bytes[4];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t top[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // pairs of the eight elements that a half wave holds
+        const uint32_t x = __float_as_uint(acc[db][8 * g + 2 * e] * s);
+        const uint32_t y = __float_as_uint(acc[db][8 * g + 2 * e + 1] * s);
+        top[e] = __builtin_amdgcn_perm(y + 0x8000u, x + 0x8000u, 0x07060302u);
+        const uint32_t b = __builtin_amdgcn_perm(y, x, 0x0c0c0501u);
+        bytes[2 * g + e / 2] = e & 1 ? __builtin_amdgcn_perm(b, bytes[2 * g + e / 2], 0x05040100u) : b;
+      }
+      u32x4_t v;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const auto z = __builtin_amdgcn_permlane32_swap(top[e], top[2 + e], false, false);
+        v[e] = z[0];
+        v[2 + e] = z[1];
+      }
+      const uint32_t d = 32u * db + 16u * g + 8u * h;
+      attn_store16(v, r, mine && (int32_t)d < D ? row * stride + d * 2u : kAttnOut);
+    }
+    if (low) {
+      const auto x = __builtin_amdgcn_permlane32_swap(bytes[0], bytes[1], false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(bytes[2], bytes[3], false, false);
+      attn_store16(u32x4_t{x[0], x[1], y[0], y[1]}, r_low,
+                   mine && 16u * db < n ? row * low_stride + h * n + 16u * db : kAttnOut);
+    }
+  }
+}
+
+// The value that attn_store_out rounded to `top` (its bits, the lower half zero), from
+// byte `i` of `low`: rounded up where that byte is 128 or more, so that it counts
+// from -128 on; the middle of what lies beneath it.
+__device__ __forceinline__ float attn_unround(uint32_t top, uint32_t low, int i) {
+  return __uint_as_float((top | 0x80u) + ((uint32_t)__builtin_amdgcn_sbfe((int32_t)low, 8 * i, 8) << 8));
+}
+
 // The two waves of a pair (SPLIT = 2): the odd one leaves its accumulators, m and
 // sum in LDS and is done (false); the even one gets the other's m and sum, and its
 // accumulators from attn_add_pair.
@@ -556,6 +615,7 @@ struct AttnArgs {
   const char *q, *k, *v, *o, *dout;            // element (t, h, d) at t * *_t + h * *_h + d * size
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h;  // bytes
   char *out, *dq, *dk, *dv;                    // [T, heads, D], contiguous
+  char* out_lo;                                // attn_store_out's bytes, rows [T, Hq]; or null
   float *lse, *delta;                          // [Hq, T]; lse in units of log2
   int32_t* items;                              // attn_items
   float* part;                                 // [Hk][slots][2][kAttnRows][D]: dK, dV of one part
@@ -780,8 +840,14 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     attn_add_pair<DP>(acc, f, f2, smem);
   }
   if (valid && h == 0) lse[row] = m + fast_log2(sum);
-  attn_store<DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + (int64_t)r0 * o_t + (int64_t)head * a.D, o_t,
-                 r_end - r0, a.D);
+  const int64_t at = (int64_t)r0 * o_t + (int64_t)head * a.D;
+  if constexpr (sizeof(T) == 2) {
+    const int64_t n = attn_low_bytes(a.D);
+    attn_store_out<DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + at, o_t, r_end - r0, a.D,
+                       a.out_lo ? a.out_lo + ((int64_t)r0 * a.Hq + head) * n : nullptr, a.Hq * n);
+  } else {
+    attn_store<DP>(acc, 1.0f / sum, reinterpret_cast<T*>(a.out) + at, o_t, r_end - r0, a.D);
+  }
 }
 
 // --- backward: delta and dQ ---------------------------------------------------
@@ -845,6 +911,17 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   dof.load(a.dout + (int64_t)r0 * a.do_t + (int64_t)head * a.do_h, (uint32_t)a.do_t, r_end - r0, d_bytes);
   of.load(a.o + ((int64_t)r0 * o_t + (int64_t)head * a.D) * (int64_t)sizeof(T), (uint32_t)o_t * sizeof(T),
           r_end - r0, d_bytes);
+  u32x4_t low[sizeof(T) == 2 ? DP / 32 : 1];
+  if constexpr (sizeof(T) == 2) {  // (without out_lo: zeros)
+    const uint32_t n = (uint32_t)attn_low_bytes(a.D) / 2, stride = 2 * n * (uint32_t)a.Hq;
+    const int32_t rows = a.out_lo ? min(r_end - r0, 32) : 0;
+    const attn_rsrc_t r = attn_rsrc(a.out_lo + ((int64_t)r0 * a.Hq + head) * (2 * n),
+                                    rows > 0 ? (uint32_t)(rows - 1) * stride + 2 * n : 0u);
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+      low[i] = attn_load16(r, (int32_t)(l & 31u) < rows && 16u * i < n ? (l & 31u) * stride + h * n + 16u * i
+                                                                       : kAttnOut);
+  }
   qf.load(a.q + (int64_t)r0 * a.q_t + (int64_t)head * a.q_h, (uint32_t)a.q_t, r_end - r0, d_bytes);
   const float lse = valid ? a.lse[(int64_t)head * a.T + row] : 0.f;
   float delta = 0.f;
@@ -854,8 +931,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     for (int e = 0; e < 4; ++e) {
       const uint32_t x = of.v[i][e], y = dof.v[i][e];
       if constexpr (sizeof(T) == 2) {
-        delta = fmaf(__uint_as_float(x << 16), __uint_as_float(y << 16), delta);
-        delta = fmaf(__uint_as_float(x & 0xffff0000u), __uint_as_float(y & 0xffff0000u), delta);
+        const uint32_t lw = low[i / 2][2 * (i % 2) + e / 2];
+        delta = fmaf(attn_unround(x << 16, lw, 2 * (e % 2)), __uint_as_float(y << 16), delta);
+        delta = fmaf(attn_unround(x & 0xffff0000u, lw, 2 * (e % 2) + 1), __uint_as_float(y & 0xffff0000u),
+                     delta);
       } else {
         delta = fmaf(__uint_as_float(x), __uint_as_float(y), delta);
       }

@@ -128,6 +128,50 @@ def test_gradient_is_the_difference_quotient(gpu, dtype):
         assert abs(quotient - (got[name].double().cpu() * d).sum()) <= tol, name
 
 
+def peaked_gradients(q, k, v, do, mask, rounded_out=False):
+    """((dq, tolerance), (dk, tolerance)) of one head in 64 bits where all keys of a row
+    lie in one block.  There its largest probability is 2^0 to fp32's rounding and
+    enters the product with V unrounded, so delta is off by at most
+        e = 2^-8 sum over the other keys of p_j |dP_j| + 2^-16 |dO| . |O|
+    (the second: O kept to 16 bits; its halves' rounding and the fp32 sums), and
+        |error of dS_j| <= 2^-8 |dS_j| + p_j (e + fp32's (D + C) 2^-24 terms).
+    rounded_out: the gradients themselves with delta from bf16(O)."""
+    D = q.shape[-1]
+    scale, F = D ** -0.5, (D + ref.C) * ref.F32
+    q, k, v, do = (t.double().cpu() for t in (q, k, v, do))
+    p = torch.softmax((scale * q @ k.T).masked_fill(~mask, -math.inf), -1)
+    o, dp = p @ v, do @ v.T
+    delta = (do * (o.to(torch.bfloat16).double() if rounded_out else o)).sum(1, keepdim=True)
+    alone = (mask.sum(1, keepdim=True) > 1).double()  # (one key: dS is exactly 0)
+    ds = alone * p * (dp - delta)
+    others = torch.where(p == p.amax(1, keepdim=True), torch.zeros(()).double(), p)
+    size = do.abs() @ v.abs().T                       # of dP's sum, and of delta's
+    e = 2.0 ** -8 * (others * dp.abs()).sum(1, keepdim=True) \
+        + 2.0 ** -16 * (do.abs() * o.abs()).sum(1, keepdim=True) + F * (p * size).sum(1, keepdim=True)
+    worst = (F * scale * (q.abs() @ k.abs().T)).masked_fill(~mask, 0.0).amax(1, keepdim=True)
+    tol = 2.0 ** -8 * ds.abs() + alone * p * (e + F * size + (2 * worst + F) * (dp.abs() + delta.abs()))
+    tol = 1.01 * tol + ref.FLOOR * mask  # (products of two errors)
+    made = ((scale * ds @ k, scale * tol @ k.abs()), (scale * ds.T @ q, scale * tol.T @ q.abs()))
+    return tuple((g, t + 2.0 ** -8 * (g.abs() + t) + ref.F32 * 64 * t) for g, t in made)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_with_one_large_probability(gpu, D):
+    lengths = [2] * 20 + [5] * 8 + [40, 64, 1, 33]
+    # queries so wide that most rows put nearly all of their probability on one key
+    q, k, v, do = inputs(sum(lengths), 4, 4, D, torch.bfloat16, seed=22, spread=6.0)
+    mask = ref.seen_mask(lengths, sum(lengths))
+    noticed = 0
+    got = run(q, k, v, do, packed_attention_plan(cu_of(lengths, gpu), sum(lengths)))
+    for h in range(4):
+        (dq, dq_tol), (dk, dk_tol) = peaked_gradients(*(t[:, h] for t in (q, k, v, do)), mask)
+        ref.assert_within(got["dq"][:, h], (dq, dq_tol), "dq")
+        ref.assert_within(got["dk"][:, h], (dk, dk_tol), "dk")
+        rounded = peaked_gradients(*(t[:, h] for t in (q, k, v, do)), mask, rounded_out=True)
+        noticed += int(((rounded[0][0] - dq).abs() > dq_tol).sum())
+    assert noticed > 100  # delta from bf16(O) is beyond the tolerance
+
+
 def test_strides(gpu):
     """Views of a fused projection, heads first, expanded key heads, odd addresses."""
     T, H, Hk, D = 150, 4, 2, 64

@@ -93,6 +93,7 @@ def attn(**kw):
     (dict(softcap=-1.0), 1), (dict(softcap=math.nan), 1), (dict(q_t=4), 1), (dict(k_h=-8), 1),
     (dict(v_t=(1 << 24) + 8), 3), (dict(q=None), 1), (dict(k=P + 8), 1), (dict(lse=None), 1),
     (dict(plan=None), 1), (dict(T=1 << 28, heads=4096, kv_heads=2), 3),
+    (dict(out_lo=P + 8), 1),
     (dict(scale=10.0, softcap=1e-38), 1),                     # their quotient is infinite
     (dict(T=1 << 24, S=1 << 19, heads=32, kv_heads=8), 3),    # 2^32 threads and more
     (dict(T=1 << 24, S=1 << 22, heads=4, kv_heads=4), 3),
