@@ -466,7 +466,9 @@ __device__ __forceinline__ void attn_store(const f32x16_t (&acc)[DP / 32], float
 // all of a row's probability, dO . V - delta cancels, and delta from the rounded
 // rows alone leaves dQ and dK off by 0.0057 of their norm (rows of two keys; with
 // these bytes 0.0025, of which 0.0017 is the outputs' own rounding), in long documents
-// by 0.0027 against 0.0024.  The bytes lie as a wave's lanes hold and want them,
+// by 0.0027 against 0.0024.  It costs a byte per element, written and read: nothing in
+// long documents, 41 -> 43 us of the forward and 59 -> 61 of dQ for 4096 tokens in
+// 12.  The bytes lie as a wave's lanes hold and want them,
 // attn_low_bytes(D) for each row and head: chunks of 8 elements, the even ones, then
 // the odd ones.  low_pitch: bytes from row to row.
 __device__ __host__ __forceinline__ int32_t attn_low_bytes(int32_t D) { return (D + 31) & ~31; }
@@ -709,11 +711,11 @@ constexpr int kAttnKeys = 64;  // keys per block of the forward and of dQ
 // Long rows are bound by the matrix instructions at the clock that the power limit
 // leaves, and by the LDS behind them (an instruction's left operand is 1 KiB, four
 // SIMDs ask for 128 bytes a cycle, all the LDS has): one document of 32768 tokens,
-// 32 heads of 128, 7.7 ms, 1150 TFLOP/s, where a large matrix product reaches
+// 32 heads of 128, 7.7 ms, 1140 TFLOP/s, where a large matrix product reaches
 // 1254.  A softcap adds two transcendentals per score to the exponential (16384
 // tokens: 2.0 -> 2.5 ms, MFMA busy 63% -> 43%).  Short documents are bound by each
 // workgroup's first tile, masks and last partial tile: 4096 tokens of 12 documents
-// 41 us.  Row tiles of 128 with two workgroups on a CU: a wave alone on its SIMD
+// 43 us.  Row tiles of 128 with two workgroups on a CU: a wave alone on its SIMD
 // with twice the rows hides neither the LDS nor the softmax (dK and dV below).
 template <class T, int DP, bool CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_fwd_kernel(AttnArgs a) {
