@@ -15,6 +15,10 @@
 // us, 5.6 TB/s; 16384 x 3584 with both: 86 us, 5.5 TB/s, and 147 us, 4.8 TB/s; a
 // large copy reaches 5.2).  The backward fetches the next row while it reduces the
 // present one: without that 506 and 233 us.
+// The backward takes h as it was stored, rounded to the type, which saves an fp32
+// copy of it (4 T H bytes written and read, against 8 T H of all else in bf16): its
+// bf16 gradients are off by 0.0022 to 0.0025 of their norm, their own rounding alone
+// by 0.0017.
 // A row lives in the registers of its TPR threads (K vectors of V elements
 // each) between its loads and its stores; everything is computed in fp32 and
 // rounded once.  The weight gradients are summed in registers over the rows a
