@@ -99,11 +99,14 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
 
     With packed_layers the labelled forward also runs the decoder's attention
     as packed_attention over the samples of the packed row (bounded by
-    `cu_seqlens`, else by position_ids that restart, which costs a sync, else
-    each row a sample; with each layer's window and softcap), and the addition
-    after attention with the norm behind it as residual_rms_norm in layers of
-    the plain form (decoder.PLAIN_LAYERS).  It takes no attention_mask, cache
-    or attention dropout then, and dense attention weights are not formed.
+    `cu_seqlens`, else by `cu_seq_lens_q`, else by position_ids that restart,
+    which costs a sync, else each row a sample; with each layer's window and
+    softcap), and the addition after attention with the norm behind it as
+    residual_rms_norm in layers of the plain form (decoder.PLAIN_LAYERS).  It
+    takes no attention_mask, cache or attention dropout then, and dense
+    attention weights are not formed.  A layer that asks its attention for more
+    than packed_attention computes (sinks, a mask of its own, attention that is
+    not causal, a keyword unknown here) raises ValueError.
     Without labels the model's own attention runs as before.
     """
     decoder = model.get_decoder()
@@ -135,8 +138,13 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
                 raise ValueError("packed layers take cu_seqlens or position_ids, no attention_mask "
                                  "and no cache")
             use_cache = False
+            # the boundaries as transformers' flash attention takes them
+            bounds = kwargs.pop("cu_seq_lens_q", None)
+            for name in ("cu_seq_lens_k", "max_length_q", "max_length_k"):
+                kwargs.pop(name, None)
             kwargs[PLANS_KWARG] = minibatch_plans(
-                input_ids if input_ids is not None else inputs_embeds, position_ids, cu_seqlens)
+                input_ids if input_ids is not None else inputs_embeds, position_ids,
+                bounds if cu_seqlens is None else cu_seqlens)
         out = decoder(input_ids=input_ids, attention_mask=attention_mask,
                       position_ids=position_ids, past_key_values=past_key_values,
                       inputs_embeds=inputs_embeds, use_cache=use_cache, **kwargs)

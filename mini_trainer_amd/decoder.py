@@ -23,6 +23,10 @@ PLANS_KWARG = "mt_attention_plans"
 # norms that are rms_norm(x) * weight.
 PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
 PLAIN_NORMS = ("LlamaRMSNorm", "Qwen2RMSNorm")
+# What a layer may hand to its attention beside what _attention reads: none of it
+# changes the result (positions are in query and key by then).
+HARMLESS = ("position_ids", "cache_position", "use_cache", "position_embeddings", "output_hidden_states",
+            "output_router_logits")
 
 
 class AttentionPlans:
@@ -41,15 +45,27 @@ class AttentionPlans:
 
 
 def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
-               softcap=None, sliding_window=None, **kwargs):
+               softcap=None, sliding_window=None, is_causal=None, **kwargs):
     """The attention function of a layer: query [B, heads, T, D], key and value
-    [B, kv_heads, T, D] -> ([B, T, heads, D], None)."""
-    plans = kwargs.get(PLANS_KWARG)
+    [B, kv_heads, T, D] -> ([B, T, heads, D], None).  What packed_attention does not
+    compute (a mask of the layer's own, sinks, attention that is not causal, any
+    keyword that is not known to change nothing) is refused."""
+    plans = kwargs.pop(PLANS_KWARG, None)
     if plans is None:
         raise RuntimeError("packed attention runs in the labelled forward of a model patched with "
                            "patch_causal_lm(packed_layers=True) only")
     if dropout:
         raise ValueError("packed attention has no dropout")
+    where = type(module).__name__
+    if attention_mask is not None:
+        raise ValueError(f"packed attention takes no attention mask; {where} passes its own")
+    if is_causal is False or not getattr(module, "is_causal", True):
+        raise ValueError(f"packed attention is causal; {where} is not")
+    if kwargs.get("output_attentions") is False:
+        del kwargs["output_attentions"]
+    unknown = sorted(n for n, x in kwargs.items() if x is not None and n not in HARMLESS)
+    if unknown:
+        raise ValueError(f"packed attention does not compute {', '.join(unknown)} of {where}")
     if key.shape[2] != query.shape[2]:
         raise ValueError("packed attention takes no cache of earlier keys")
     B, heads, T, D = query.shape

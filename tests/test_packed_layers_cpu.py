@@ -1,0 +1,153 @@
+"""patch_causal_lm(packed_layers=True) on the CPU: the host side of the patched
+forward, with the operators replaced by their definitions and the loss by the
+decoder's last hidden states.  Every model either agrees with each document run
+alone through the unpatched model, or is refused."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from mini_trainer_amd import causal_lm, cu_seqlens_from_lengths, decoder, patch_causal_lm
+
+tf = pytest.importorskip("transformers")
+
+LENGTHS = [25, 15]
+T = sum(LENGTHS)
+# fp32 through two small layers, each sum of at most 96 terms: some ten products of
+# relative error sqrt(96) 2^-24 = 6e-7 each
+TOL = 1e-5
+
+WIDE = dict(vocab_size=100, hidden_size=64, num_hidden_layers=2, num_attention_heads=4,
+            max_position_embeddings=128)
+BASE = dict(WIDE, intermediate_size=96, num_key_value_heads=2)
+
+
+def build(name, **more):
+    torch.manual_seed(0)
+    cls, config, kw = MODELS[name]
+    if not hasattr(tf, cls):
+        pytest.skip(f"this transformers has no {cls}")
+    return getattr(tf, cls)(getattr(tf, config)(**{**kw, **more})).float().eval()
+
+
+MODELS = {
+    "llama": ("LlamaForCausalLM", "LlamaConfig", BASE),
+    "qwen2": ("Qwen2ForCausalLM", "Qwen2Config", BASE),
+    "mistral": ("MistralForCausalLM", "MistralConfig", dict(BASE, sliding_window=8)),
+    "gemma2": ("Gemma2ForCausalLM", "Gemma2Config", dict(BASE, head_dim=16, sliding_window=8)),
+    "gpt2": ("GPT2LMHeadModel", "GPT2Config",
+             dict(vocab_size=100, n_embd=64, n_layer=2, n_head=4, n_positions=128, attn_pdrop=0.0,
+                  resid_pdrop=0.0, embd_pdrop=0.0)),
+    "gpt_oss": ("GptOssForCausalLM", "GptOssConfig",
+                dict(BASE, head_dim=16, num_local_experts=2, num_experts_per_tok=1)),
+    "doge": ("DogeForCausalLM", "DogeConfig", BASE),
+}
+
+
+@pytest.fixture
+def operators(monkeypatch):
+    """The operators' definitions in their places; the number of attention calls."""
+    calls = []
+
+    class Plan:
+        def __init__(self, cu, tokens, window=None, **_):
+            self.cu, self.tokens, self.window = cu.tolist(), tokens, window
+
+    def attention(q, k, v, plan, scale=None, softcap=None):
+        calls.append(plan)
+        out = torch.zeros_like(q)
+        G = q.shape[1] // k.shape[1]
+        for a, b in zip(plan.cu, plan.cu[1:]):
+            i, j = torch.arange(b - a)[:, None], torch.arange(b - a)[None, :]
+            seen = (j <= i) & (i - j < (plan.window or T))
+            z = torch.einsum("ihd,jhd->hij", q[a:b], k[a:b].repeat_interleave(G, 1)) * scale
+            if softcap:
+                z = softcap * torch.tanh(z / softcap)
+            p = torch.softmax(z.masked_fill(~seen, -math.inf), -1)
+            out[a:b] = torch.einsum("hij,jhd->ihd", p, v[a:b].repeat_interleave(G, 1))
+        return out
+
+    def norm(x, residual, weight, eps):
+        h = x + residual
+        return h * torch.rsqrt(h.pow(2).mean(-1, keepdim=True) + eps) * weight, h
+
+    monkeypatch.setattr(decoder, "packed_attention", attention)
+    monkeypatch.setattr(decoder, "packed_attention_plan", Plan)
+    monkeypatch.setattr(decoder, "residual_rms_norm", norm)
+    monkeypatch.setattr(causal_lm, "causal_lm_loss", lambda hidden, *_, **__: hidden[0])
+    monkeypatch.setattr(causal_lm, "sample_loss_sums", lambda *_, **__: (None, None))
+    return calls
+
+
+def batch(seed=1):
+    ids = torch.randint(1, 100, (1, T), generator=torch.Generator().manual_seed(seed))
+    pos = torch.cat([torch.arange(n) for n in LENGTHS])[None]
+    return dict(input_ids=ids, labels=ids, position_ids=pos,
+                cu_seqlens=cu_seqlens_from_lengths(LENGTHS))
+
+
+def alone(model, ids):
+    """Last hidden states of each document by itself."""
+    cu = cu_seqlens_from_lengths(LENGTHS).tolist()
+    return torch.cat([model.get_decoder()(input_ids=ids[:, a:b]).last_hidden_state[0]
+                      for a, b in zip(cu, cu[1:])])
+
+
+def rel(a, b):
+    return float((a - b).norm() / b.norm())
+
+
+def patched(name, **more):
+    return patch_causal_lm(build(name, **more), packed_layers=True)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("name", ["llama", "qwen2", "mistral", "gemma2", "gpt2"])
+def test_documents_are_as_alone(operators, name):
+    model, kw = build(name), batch()
+    want = alone(model, kw["input_ids"])
+    got = patch_causal_lm(model, packed_layers=True)(**kw).loss
+    assert rel(got, want) <= TOL and len(operators) == 2
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("name,what", [("gpt_oss", "s_aux"), ("doge", "attention mask")])
+def test_more_than_packed_attention_computes_is_refused(operators, name, what):
+    with pytest.raises(ValueError, match=what):
+        patched(name)(**batch())
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("kw", [dict(some_bias=torch.zeros(1)), dict(output_attentions=True),
+                                dict(is_causal=False), dict(head_mask=torch.ones(2, 4))])
+def test_unknown_keywords_are_refused(operators, kw):
+    model = patched("llama")
+    with pytest.raises(ValueError):
+        model(**batch(), **kw)
+    # not given, or changing nothing
+    assert len(operators) == 0
+    model(**batch(), some_bias=None, output_attentions=False, output_router_logits=False)
+    assert len(operators) == 2
+
+
+@torch.no_grad()
+def test_a_layer_that_is_not_causal_is_refused(operators):
+    model = patched("llama")
+    model.model.layers[1].self_attn.is_causal = False
+    with pytest.raises(ValueError, match="causal"):
+        model(**batch())
+
+
+@torch.no_grad()
+def test_flash_attention_boundaries(operators):
+    """cu_seq_lens_q bounds the documents where cu_seqlens does not; position_ids that
+    say otherwise do not."""
+    model, kw = patched("llama"), batch()
+    want = model(**kw).loss
+    cu, row = kw.pop("cu_seqlens"), torch.arange(T)[None]
+    kw["position_ids"] = row
+    got = model(**kw, cu_seq_lens_q=cu, cu_seq_lens_k=cu, max_length_q=25, max_length_k=25).loss
+    assert operators[-1].cu == [0, 25, 40]
+    assert rel(got, want) <= TOL  # (rotary positions are relative)
