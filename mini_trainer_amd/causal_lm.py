@@ -106,7 +106,9 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
     takes no attention_mask, cache or attention dropout then, and dense
     attention weights are not formed.  A layer that asks its attention for more
     than packed_attention computes (sinks, a mask of its own, attention that is
-    not causal, a keyword unknown here) raises ValueError.
+    not causal, a keyword unknown here) raises ValueError, and so does a decoder
+    that mixes tokens in another way in any layer (state spaces, convolutions,
+    attention of its own) or takes no position_ids.
     Without labels the model's own attention runs as before.
     """
     decoder = model.get_decoder()
@@ -148,6 +150,8 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
         out = decoder(input_ids=input_ids, attention_mask=attention_mask,
                       position_ids=position_ids, past_key_values=past_key_values,
                       inputs_embeds=inputs_embeds, use_cache=use_cache, **kwargs)
+        if packed_layers:
+            kwargs[PLANS_KWARG].check_layers(decoder)
         hidden = out.last_hidden_state
         if hidden.dtype != head.weight.dtype:
             # a decoder kept in another precision than its output embedding:

@@ -7,6 +7,7 @@ here in their place for the labelled forward, which train.py:97 runs.
 """
 from __future__ import annotations
 
+import inspect
 import types
 from typing import Optional
 
@@ -23,6 +24,8 @@ PLANS_KWARG = "mt_attention_plans"
 # norms that are rms_norm(x) * weight.
 PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
 PLAIN_NORMS = ("LlamaRMSNorm", "Qwen2RMSNorm")
+# Layer types whose mask is packed_attention's, without and with a window.
+FULL, SLIDING = "full_attention", "sliding_attention"
 # What a layer may hand to its attention beside what _attention reads: none of it
 # changes the result (positions are in query and key by then).
 HARMLESS = ("position_ids", "cache_position", "use_cache", "position_embeddings", "output_hidden_states",
@@ -35,6 +38,8 @@ class AttentionPlans:
     def __init__(self, cu_seqlens: torch.Tensor, tokens: int, device: torch.device):
         self._args = (cu_seqlens, tokens, device)
         self._plans: dict = {}
+        self._attended: set = set()
+        self._calls = 0
 
     def get(self, window: Optional[int]) -> AttentionPlan:
         if window not in self._plans:
@@ -42,6 +47,21 @@ class AttentionPlans:
             self._plans[window] = packed_attention_plan(
                 cu, tokens, window=window, validate=False, device=None if cu.is_cuda else device)
         return self._plans[window]
+
+    def attended(self, module: torch.nn.Module) -> None:
+        """Note that this attention module has run as packed attention."""
+        self._attended.add(id(module))
+        self._calls += 1
+
+    def check_layers(self, decoder: torch.nn.Module) -> None:
+        """Raise ValueError unless every layer of the decoder went through packed
+        attention: one that mixes tokens in another way has mixed the documents."""
+        layers, ran = decoder.config.num_hidden_layers, len(self._attended)
+        dropped = decoder.training and getattr(decoder.config, "layerdrop", 0.0)
+        # (two calls in a layer count once; a module that several layers share, for each)
+        if layers not in (ran, self._calls) and not (dropped and 0 < ran < layers):
+            raise ValueError(f"packed layers: {ran} of {type(decoder).__name__}'s {layers} layers run "
+                             "their attention as packed attention; the others would mix the documents")
 
 
 def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
@@ -68,6 +88,7 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
         raise ValueError(f"packed attention does not compute {', '.join(unknown)} of {where}")
     if key.shape[2] != query.shape[2]:
         raise ValueError("packed attention takes no cache of earlier keys")
+    plans.attended(module)
     B, heads, T, D = query.shape
     q, k, v = (t.transpose(1, 2).reshape(B * T, t.shape[1], D) for t in (query, key, value))
     out = packed_attention(q, k, v, plans.get(sliding_window), scale=scaling, softcap=softcap)
@@ -94,11 +115,30 @@ def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
     return residual + self.mlp(hidden_states)
 
 
+def _refuse_other_mixers(decoder: torch.nn.Module) -> None:
+    """Raise ValueError for a decoder that mixes tokens, or places them, in a way that
+    packed attention does not bound by the documents.  (Attention modules that never
+    ask for the configured attention show in AttentionPlans.check_layers.)"""
+    name = type(decoder).__name__
+    if "position_ids" not in inspect.signature(decoder.forward).parameters:
+        raise ValueError(f"packed layers: {name} takes no position_ids, so that no document but the "
+                         "first would start at position 0")
+    other = set(getattr(decoder.config, "layer_types", None) or ()) - {FULL, SLIDING}
+    if other:
+        raise ValueError(f"packed layers: {name} has layers of {', '.join(sorted(other))}")
+    for path, module in decoder.named_modules():
+        conv = isinstance(module, torch.nn.modules.conv._ConvNd) and max(module.kernel_size) > 1
+        if conv or isinstance(module, torch.nn.RNNBase):
+            raise ValueError(f"packed layers: {name}.{path} ({type(module).__name__}) mixes tokens "
+                             "across documents")
+
+
 def patch_decoder_layers(decoder: torch.nn.Module) -> str:
     """Give the decoder's attention modules the packed attention and its plain
     layers the fused forward; returns the name of the attention it had."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
+    _refuse_other_mixers(decoder)
     ALL_ATTENTION_FUNCTIONS.register(ATTENTION_NAME, _attention)
     had = decoder.config._attn_implementation
     decoder.config._attn_implementation = ATTENTION_NAME

@@ -43,6 +43,34 @@ MODELS = {
     "gpt_oss": ("GptOssForCausalLM", "GptOssConfig",
                 dict(BASE, head_dim=16, num_local_experts=2, num_experts_per_tok=1)),
     "doge": ("DogeForCausalLM", "DogeConfig", BASE),
+    "diffllama": ("DiffLlamaForCausalLM", "DiffLlamaConfig", BASE),
+    "bloom": ("BloomForCausalLM", "BloomConfig", dict(vocab_size=100, hidden_size=64, n_layer=2, n_head=4)),
+    "xglm": ("XGLMForCausalLM", "XGLMConfig",
+             dict(vocab_size=100, d_model=64, ffn_dim=96, num_layers=2, attention_heads=4, dropout=0.0,
+                  attention_dropout=0.0)),
+    "gpt_neo": ("GPTNeoForCausalLM", "GPTNeoConfig",
+                dict(vocab_size=100, hidden_size=64, num_layers=2, num_heads=4,
+                     attention_types=[[["global", "local"], 1]], max_position_embeddings=128,
+                     attention_dropout=0.0, resid_dropout=0.0, embed_dropout=0.0)),
+    "jamba": ("JambaForCausalLM", "JambaConfig",
+              dict(BASE, attn_layer_period=2, attn_layer_offset=1, num_experts=2, num_experts_per_tok=1,
+                   use_mamba_kernels=False, mamba_d_state=4, mamba_dt_rank=4, pad_token_id=0)),
+    "falcon_h1": ("FalconH1ForCausalLM", "FalconH1Config",
+                  dict(BASE, mamba_d_ssm=64, mamba_n_heads=4, mamba_d_head=16, mamba_d_state=8,
+                       mamba_n_groups=1)),
+    "recurrent_gemma": ("RecurrentGemmaForCausalLM", "RecurrentGemmaConfig",
+                        dict(BASE, lru_width=64, attention_window_size=8,
+                             block_types=["recurrent", "attention"])),
+    "minimax": ("MiniMaxForCausalLM", "MiniMaxConfig",
+                dict(BASE, head_dim=16, num_local_experts=2, num_experts_per_tok=1, block_size=8,
+                     layer_types=["linear_attention", "full_attention"])),
+    "llama4": ("Llama4ForCausalLM", "Llama4TextConfig",
+               dict(BASE, head_dim=16, num_local_experts=2, intermediate_size_mlp=96,
+                    attention_chunk_size=8)),
+    "bart": ("BartForCausalLM", "BartConfig",
+             dict(vocab_size=100, d_model=64, decoder_layers=2, decoder_attention_heads=4,
+                  decoder_ffn_dim=96, max_position_embeddings=128, is_decoder=True,
+                  is_encoder_decoder=False)),
 }
 
 
@@ -151,3 +179,31 @@ def test_flash_attention_boundaries(operators):
     got = model(**kw, cu_seq_lens_q=cu, cu_seq_lens_k=cu, max_length_q=25, max_length_k=25).loss
     assert operators[-1].cu == [0, 25, 40]
     assert rel(got, want) <= TOL  # (rotary positions are relative)
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("name", ["bloom", "xglm", "gpt_neo", "jamba", "falcon_h1", "recurrent_gemma",
+                                  "minimax", "llama4", "bart"])
+def test_decoders_that_mix_documents_elsewhere_are_refused(operators, name):
+    """Attention of their own, state spaces, recurrences, convolutions, chunks, positions
+    that cannot restart: when the model is patched, or in its first labelled forward."""
+    model = build(name)
+    with pytest.raises(ValueError, match="packed layers: "):
+        patch_causal_lm(model, packed_layers=True)(**batch())
+
+
+@torch.no_grad()
+def test_every_attention_layer_is_counted(operators):
+    model, kw = patched("llama"), batch()
+    first, second = (layer.self_attn for layer in model.model.layers)
+    own, second.forward = second.forward, lambda hidden_states, **_: (hidden_states, None)
+    with pytest.raises(ValueError, match="1 of LlamaModel's 2 layers"):
+        model(**kw)
+    second.forward = own
+    model(**kw)  # (each forward is counted afresh)
+    # two calls in each layer are two layers' calls
+    model = build("diffllama")
+    want = alone(model, kw["input_ids"])
+    del operators[:]
+    got = patch_causal_lm(model, packed_layers=True)(**kw).loss
+    assert rel(got, want) <= TOL and len(operators) == 4
