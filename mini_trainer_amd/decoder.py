@@ -64,6 +64,16 @@ class AttentionPlans:
                              "their attention as packed attention; the others would mix the documents")
 
 
+def _has_window(module) -> bool:
+    """Whether the model's configuration gives an attention module's layer a window."""
+    config = getattr(module, "config", None)
+    kinds, layer = getattr(config, "layer_types", None), getattr(module, "layer_idx", None)
+    if kinds and layer is not None and layer < len(kinds):
+        return kinds[layer] == SLIDING
+    return getattr(config, "sliding_window", None) is not None and \
+        getattr(config, "use_sliding_window", True)
+
+
 def _attention(module, query, key, value, attention_mask=None, scaling=None, dropout=0.0,
                softcap=None, sliding_window=None, is_causal=None, **kwargs):
     """The attention function of a layer: query [B, heads, T, D], key and value
@@ -88,6 +98,8 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
         raise ValueError(f"packed attention does not compute {', '.join(unknown)} of {where}")
     if key.shape[2] != query.shape[2]:
         raise ValueError("packed attention takes no cache of earlier keys")
+    if sliding_window is None and _has_window(module):
+        raise ValueError(f"{where} has a sliding window that it does not pass to its attention")
     plans.attended(module)
     B, heads, T, D = query.shape
     q, k, v = (t.transpose(1, 2).reshape(B * T, t.shape[1], D) for t in (query, key, value))

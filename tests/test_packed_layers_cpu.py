@@ -71,6 +71,8 @@ MODELS = {
              dict(vocab_size=100, d_model=64, decoder_layers=2, decoder_attention_heads=4,
                   decoder_ffn_dim=96, max_position_embeddings=128, is_decoder=True,
                   is_encoder_decoder=False)),
+    "phimoe": ("PhimoeForCausalLM", "PhimoeConfig",
+               dict(BASE, num_local_experts=4, num_experts_per_tok=2, sliding_window=8)),
 }
 
 
@@ -190,6 +192,12 @@ def test_decoders_that_mix_documents_elsewhere_are_refused(operators, name):
     model = build(name)
     with pytest.raises(ValueError, match="packed layers: "):
         patch_causal_lm(model, packed_layers=True)(**batch())
+
+
+@torch.no_grad()
+def test_a_window_that_reaches_only_the_mask_is_refused(operators):
+    with pytest.raises(ValueError, match="sliding window"):
+        patched("phimoe")(**batch())
 
 
 @torch.no_grad()
