@@ -18,7 +18,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn.functional as F
 
-from .decoder import ATTENTION_NAME, PLANS_KWARG, minibatch_plans, patch_decoder_layers
+from .decoder import PLANS_KWARG, minibatch_plans, patch_decoder_layers, unlabelled_forward
 from .flce import fused_linear_cross_entropy, per_sample_loss_sums
 
 __all__ = ["causal_lm_loss", "patch_causal_lm", "sample_loss_sums", "cu_seqlens_from_position_ids",
@@ -117,7 +117,8 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
         raise ValueError("patch_causal_lm needs an output embedding without bias")
     original = model.forward
     softcap = getattr(model.config, "final_logit_softcapping", None)
-    own_attention = patch_decoder_layers(decoder) if packed_layers else None
+    if packed_layers:
+        patch_decoder_layers(decoder)
 
     def forward(input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
                 inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,
@@ -125,16 +126,11 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
                 ignore_index: int = -100, **kwargs):
         kwargs.pop("num_items_in_batch", None)
         if labels is None and shift_labels is None:
-            if packed_layers:
-                decoder.config._attn_implementation = own_attention
-            try:
+            with unlabelled_forward():
                 return original(input_ids=input_ids, attention_mask=attention_mask,
                                 position_ids=position_ids, past_key_values=past_key_values,
                                 inputs_embeds=inputs_embeds, use_cache=use_cache,
                                 logits_to_keep=logits_to_keep, **kwargs)
-            finally:
-                if packed_layers:
-                    decoder.config._attn_implementation = ATTENTION_NAME
         if packed_layers:
             if attention_mask is not None or past_key_values is not None or use_cache:
                 raise ValueError("packed layers take cu_seqlens or position_ids, no attention_mask "

@@ -7,6 +7,9 @@ here in their place for the labelled forward, which train.py:97 runs.
 """
 from __future__ import annotations
 
+import contextlib
+import contextvars
+import functools
 import inspect
 import types
 from typing import Optional
@@ -16,7 +19,7 @@ import torch
 from .attention import AttentionPlan, packed_attention, packed_attention_plan
 from .norms import residual_rms_norm
 
-__all__ = ["AttentionPlans", "patch_decoder_layers"]
+__all__ = ["AttentionPlans", "patch_decoder_layers", "unlabelled_forward"]
 
 ATTENTION_NAME = "mt_packed"
 PLANS_KWARG = "mt_attention_plans"
@@ -30,6 +33,26 @@ FULL, SLIDING = "full_attention", "sliding_attention"
 # changes the result (positions are in query and key by then).
 HARMLESS = ("position_ids", "cache_position", "use_cache", "position_embeddings", "output_hidden_states",
             "output_router_logits")
+
+
+# Per thread: whether the modules that run now ask their configuration for packed
+# attention, and whether the unlabelled forward of a patched model is running.
+_packed = contextvars.ContextVar("mt_packed", default=False)
+_unlabelled = contextvars.ContextVar("mt_unlabelled", default=False)
+
+
+@contextlib.contextmanager
+def _set(var):
+    token = var.set(True)
+    try:
+        yield
+    finally:
+        var.reset(token)
+
+
+def unlabelled_forward():
+    """A context in which a patched decoder runs as it was."""
+    return _set(_unlabelled)
 
 
 class AttentionPlans:
@@ -81,12 +104,11 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
     compute (a mask of the layer's own, sinks, attention that is not causal, any
     keyword that is not known to change nothing) is refused."""
     plans = kwargs.pop(PLANS_KWARG, None)
+    where = type(module).__name__
     if plans is None:
-        raise RuntimeError("packed attention runs in the labelled forward of a model patched with "
-                           "patch_causal_lm(packed_layers=True) only")
+        raise ValueError(f"packed layers: {where} is not handed the keywords of the decoder's forward")
     if dropout:
         raise ValueError("packed attention has no dropout")
-    where = type(module).__name__
     if attention_mask is not None:
         raise ValueError(f"packed attention takes no attention mask; {where} passes its own")
     if is_causal is False or not getattr(module, "is_causal", True):
@@ -145,19 +167,74 @@ def _refuse_other_mixers(decoder: torch.nn.Module) -> None:
                              "across documents")
 
 
-def patch_decoder_layers(decoder: torch.nn.Module) -> str:
-    """Give the decoder's attention modules the packed attention and its plain
-    layers the fused forward; returns the name of the attention it had."""
+@functools.lru_cache(maxsize=None)
+def _config_view_cls(cls: type) -> type:
+    def get(self):
+        return ATTENTION_NAME if _packed.get() else super(view, self)._attn_implementation
+
+    def put(self, value):
+        cls._attn_implementation.fset(self, value)
+
+    view = type(cls.__name__, (cls,), {"__module__": cls.__module__, "mt_view": True,
+                                       "_attn_implementation": property(get, put)})
+    return view
+
+
+def _config_view(config):
+    """The same configuration (one dictionary), which names packed attention to the
+    modules of a labelled forward and what it names to all others: nothing that
+    another thread, or a checkpoint's recomputation, reads is changed for a call."""
+    if getattr(type(config), "mt_view", False):
+        return config
+    view = object.__new__(_config_view_cls(type(config)))
+    object.__setattr__(view, "__dict__", config.__dict__)
+    return view
+
+
+OWN_FORWARD = "_mt_own_forward"  # a module's attribute: the forward it had of its own
+
+
+@functools.lru_cache(maxsize=None)
+def _packed_forward(own, is_decoder: bool):
+    @functools.wraps(own)
+    def forward(self, *args, **kwargs):
+        run = self.__dict__.get(OWN_FORWARD) or functools.partial(own, self)
+        if kwargs.get(PLANS_KWARG) is not None:
+            with _set(_packed):
+                return run(*args, **kwargs)
+        if is_decoder and not _unlabelled.get():
+            raise RuntimeError("the decoder of a model patched with patch_causal_lm(packed_layers=True) "
+                               "runs in the model's own forward only: the labelled forward for packed "
+                               "attention")
+        return run(*args, **kwargs)
+
+    return forward
+
+
+def patch_decoder_layers(decoder: torch.nn.Module) -> None:
+    """Give the decoder's modules, where they run with plans among their keywords, a
+    configuration that names packed attention, and its plain layers the fused
+    forward.  Without plans the modules run as before."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
     _refuse_other_mixers(decoder)
     ALL_ATTENTION_FUNCTIONS.register(ATTENTION_NAME, _attention)
-    had = decoder.config._attn_implementation
-    decoder.config._attn_implementation = ATTENTION_NAME
-    for layer in decoder.modules():
-        if type(layer).__name__ in PLAIN_LAYERS:
-            layer.forward = types.MethodType(_layer_forward, layer)
-    return had
+    for module in decoder.modules():
+        if type(module).__name__ in PLAIN_LAYERS:
+            module.forward = types.MethodType(_layer_forward, module)
+        config = module.__dict__.get("config")
+        if config is None or getattr(type(config), "mt_view", False) or \
+                not hasattr(type(config), "_attn_implementation"):
+            continue
+        parameters = inspect.signature(module.forward).parameters.values()
+        if module is not decoder and all(p.kind is not p.VAR_KEYWORD for p in parameters):
+            continue  # (no plans reach it)
+        module.config = _config_view(config)
+        if type(module).__name__ in PLAIN_LAYERS:
+            continue
+        if "forward" in module.__dict__:
+            module.__dict__[OWN_FORWARD] = module.forward
+        module.forward = types.MethodType(_packed_forward(type(module).forward, module is decoder), module)
 
 
 def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],

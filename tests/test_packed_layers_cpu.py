@@ -4,7 +4,9 @@ decoder's last hidden states.  Every model either agrees with each document run
 alone through the unpatched model, or is refused."""
 from __future__ import annotations
 
+import copy
 import math
+import threading
 
 import pytest
 import torch
@@ -215,3 +217,105 @@ def test_every_attention_layer_is_counted(operators):
     del operators[:]
     got = patch_causal_lm(model, packed_layers=True)(**kw).loss
     assert rel(got, want) <= TOL and len(operators) == 4
+
+
+def gradients(model, loss):
+    model.zero_grad()
+    loss.backward()
+    return {n: p.grad.clone() for n, p in model.named_parameters() if p.grad is not None}
+
+
+@pytest.mark.parametrize("own", ["eager", "sdpa"])
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_unlabelled_checkpointed_step_is_the_unpatched_models(operators, own, reentrant):
+    """The layers are recomputed in the backward, after the unlabelled forward has ended."""
+    model = build("llama", attn_implementation=own).train()
+    model.gradient_checkpointing_enable({"use_reentrant": reentrant})
+    ids = batch()["input_ids"]
+
+    def step(m):
+        logits = m(input_ids=ids).logits
+        return logits.detach(), gradients(m, logits.float().pow(2).sum())
+
+    want, wants = step(copy.deepcopy(model))
+    patch_causal_lm(model, packed_layers=True)
+    for _ in range(2):
+        got, grads = step(model)
+        assert torch.equal(got, want) and grads.keys() == wants.keys()
+        assert all(torch.equal(grads[n], wants[n]) for n in wants)
+        assert model.config._attn_implementation == model.model.config._attn_implementation == own
+        with torch.no_grad():
+            model(**batch())  # a labelled forward between them
+    assert len(operators) == 4
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_labelled_checkpointed_step(operators, reentrant):
+    model = patched("llama").train()
+    kw = batch()
+    want = gradients(model, model(**kw).loss.pow(2).sum())
+    model.gradient_checkpointing_enable({"use_reentrant": reentrant})
+    del operators[:]
+    got = gradients(model, model(**kw).loss.pow(2).sum())
+    assert len(operators) == 4  # each layer's attention again in the backward
+    # the embedding's gradient comes from the whole first layer either way
+    assert got.keys() == want.keys() and all(rel(got[n], want[n]) <= TOL for n in want)
+
+
+@torch.no_grad()
+def test_labelled_and_unlabelled_forwards_in_two_threads(operators):
+    """Each goes by its own attention, whichever runs within the other's time."""
+    model, kw = build("llama"), batch()
+    docs, logits = alone(model, kw["input_ids"]), model(input_ids=kw["input_ids"]).logits
+    patch_causal_lm(model, packed_layers=True)
+    calls = {"labelled": lambda: model(**kw).loss, "unlabelled": lambda: model(input_ids=kw["input_ids"]).logits}
+    for outer, inner in (("labelled", "unlabelled"), ("unlabelled", "labelled")):
+        got, entered = {}, []
+
+        def other(*_):
+            if not entered:
+                entered.append(True)
+
+                def run():
+                    with torch.no_grad():
+                        got[inner] = calls[inner]()
+                thread = threading.Thread(target=run)
+                thread.start()
+                thread.join()
+
+        hook = model.model.layers[0].self_attn.register_forward_pre_hook(other)
+        got[outer] = calls[outer]()
+        hook.remove()
+        assert rel(got["labelled"], docs) <= TOL
+        assert torch.equal(got["unlabelled"], logits)
+
+
+@torch.no_grad()
+def test_forwards_of_the_modules_own_stay(operators):
+    """A forward that something else has put in an attention module's place is run."""
+    model, kw = build("llama"), batch()
+    want, ran = alone(model, kw["input_ids"]), []
+    module = model.model.layers[1].self_attn
+    own = module.forward
+
+    def forward(*args, **kwargs):
+        ran.append(True)
+        return own(*args, **kwargs)
+
+    module.forward = forward
+    patch_causal_lm(model, packed_layers=True)
+    assert rel(model(**kw).loss, want) <= TOL and ran == [True]
+    patch_causal_lm(model, packed_layers=True)  # again: as once
+    assert rel(model(**kw).loss, want) <= TOL and ran == [True] * 2
+
+
+@torch.no_grad()
+def test_configuration_stays_one(operators):
+    model = patched("llama", attn_implementation="sdpa")
+    model.config.rms_norm_eps, model.model.config.some_number = 1e-3, 5
+    assert model.model.config.rms_norm_eps == 1e-3 and model.config.some_number == 5
+    assert isinstance(model.model.config, tf.LlamaConfig)
+    model.set_attn_implementation("eager")
+    assert model.model.layers[0].self_attn.config._attn_implementation == "eager"
+    model(**batch())
+    assert len(operators) == 2
