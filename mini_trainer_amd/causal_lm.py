@@ -69,9 +69,12 @@ def _output_cls():
         @dataclass
         class CausalLMOutputWithSampleSums(CausalLMOutputWithPast):
             """seg_loss fp32 [S]: per-sample sum of the per-token loss over
-            cu_seqlens; seg_cnt int32 [S]: its counted (non-ignored) tokens."""
+            cu_seqlens; seg_cnt int32 [S]: its counted (non-ignored) tokens.
+            attention_status int32 [1], with packed layers: 1 if cu_seqlens was
+            malformed, so that all attention was zero; 0 otherwise."""
             seg_loss: Optional[torch.FloatTensor] = None
             seg_cnt: Optional[torch.IntTensor] = None
+            attention_status: Optional[torch.IntTensor] = None
 
         _OUTPUT_CLS = CausalLMOutputWithSampleSums
     return _OUTPUT_CLS
@@ -108,7 +111,12 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
     than packed_attention computes (sinks, a mask of its own, attention that is
     not causal, a keyword unknown here) raises ValueError, and so does a decoder
     that mixes tokens in another way in any layer (state spaces, convolutions,
-    attention of its own) or takes no position_ids.
+    attention of its own) or takes no position_ids.  A malformed cu_seqlens
+    raises ValueError as well, before anything runs where it lies on the CPU (the
+    collator's); one on the device is checked with a sync, which
+    `validate_cu_seqlens=False` goes without: all attention of a malformed
+    minibatch is then zero, and `attention_status` of the output (int32 [1] on
+    the device) is 1.
     Without labels the model's own attention runs as before.
     """
     decoder = model.get_decoder()
@@ -123,7 +131,7 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
     def forward(input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
                 inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,
                 shift_labels=None, mt_grad_scale=None, cu_seqlens=None,
-                ignore_index: int = -100, **kwargs):
+                ignore_index: int = -100, validate_cu_seqlens: bool = True, **kwargs):
         kwargs.pop("num_items_in_batch", None)
         if labels is None and shift_labels is None:
             with unlabelled_forward():
@@ -142,12 +150,14 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
                 kwargs.pop(name, None)
             kwargs[PLANS_KWARG] = minibatch_plans(
                 input_ids if input_ids is not None else inputs_embeds, position_ids,
-                bounds if cu_seqlens is None else cu_seqlens)
+                bounds if cu_seqlens is None else cu_seqlens, validate_cu_seqlens)
         out = decoder(input_ids=input_ids, attention_mask=attention_mask,
                       position_ids=position_ids, past_key_values=past_key_values,
                       inputs_embeds=inputs_embeds, use_cache=use_cache, **kwargs)
+        status = None
         if packed_layers:
             kwargs[PLANS_KWARG].check_layers(decoder)
+            status = kwargs[PLANS_KWARG].status
         hidden = out.last_hidden_state
         if hidden.dtype != head.weight.dtype:
             # a decoder kept in another precision than its output embedding:
@@ -164,7 +174,7 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
                                                  ignore_index=ignore_index)
         return _output_cls()(loss=loss, logits=None, past_key_values=out.past_key_values,
                              hidden_states=out.hidden_states, attentions=out.attentions,
-                             seg_loss=seg_loss, seg_cnt=seg_cnt)
+                             seg_loss=seg_loss, seg_cnt=seg_cnt, attention_status=status)
 
     model.forward = forward
     return model

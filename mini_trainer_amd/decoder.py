@@ -56,9 +56,21 @@ def unlabelled_forward():
 
 
 class AttentionPlans:
-    """The plans of one packed minibatch, one for each window its layers use."""
+    """The plans of one packed minibatch, one for each window its layers use.  With
+    `validate`, malformed boundaries raise ValueError: here where they lie on the CPU;
+    on the device with the first plan, which then synchronises once.  Without it every
+    attention of a minibatch malformed there gives zeros, and status (int32 [1], 0 or
+    1) says so."""
 
-    def __init__(self, cu_seqlens: torch.Tensor, tokens: int, device: torch.device):
+    def __init__(self, cu_seqlens: torch.Tensor, tokens: int, device: torch.device,
+                 validate: bool = True):
+        if not cu_seqlens.is_cuda:
+            cu = cu_seqlens.reshape(-1).to(torch.int64)
+            if cu.numel() == 0 or cu[0] != 0 or cu[-1] > tokens or bool((cu.diff() < 0).any()):
+                raise ValueError("cu_seqlens must start at 0, be non-decreasing and end at or below "
+                                 f"{tokens}, the row's tokens")
+        self._validate = validate and cu_seqlens.is_cuda
+        self.status: Optional[torch.Tensor] = None
         self._args = (cu_seqlens, tokens, device)
         self._plans: dict = {}
         self._attended: set = set()
@@ -67,8 +79,12 @@ class AttentionPlans:
     def get(self, window: Optional[int]) -> AttentionPlan:
         if window not in self._plans:
             cu, tokens, device = self._args
-            self._plans[window] = packed_attention_plan(
+            plan = self._plans[window] = packed_attention_plan(
                 cu, tokens, window=window, validate=False, device=None if cu.is_cuda else device)
+            if self.status is None:
+                self.status = plan.status
+                if self._validate:
+                    plan.validate()
         return self._plans[window]
 
     def attended(self, module: torch.nn.Module) -> None:
@@ -238,7 +254,7 @@ def patch_decoder_layers(decoder: torch.nn.Module) -> None:
 
 
 def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],
-                    cu_seqlens: Optional[torch.Tensor]) -> AttentionPlans:
+                    cu_seqlens: Optional[torch.Tensor], validate: bool = True) -> AttentionPlans:
     """The plans of a minibatch of `tokens` [B, T, ...]: documents by cu_seqlens, or
     where position_ids restart (one sync) and with each row."""
     from .causal_lm import cu_seqlens_from_lengths, cu_seqlens_from_position_ids
@@ -247,10 +263,11 @@ def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],
     if B > 1 and cu_seqlens is not None:
         raise ValueError(f"cu_seqlens bounds the samples of one packed row; got {B} rows")
     if cu_seqlens is None:
+        validate = False  # (made here)
         if position_ids is None:
             cu_seqlens = cu_seqlens_from_lengths([T] * B)
         else:
             starts = position_ids.reshape(-1, T).expand(B, T).clone()
             starts[:, :1] = 0  # a row is no continuation of the one before
             cu_seqlens = cu_seqlens_from_position_ids(starts)
-    return AttentionPlans(cu_seqlens, B * T, tokens.device)
+    return AttentionPlans(cu_seqlens, B * T, tokens.device, validate)

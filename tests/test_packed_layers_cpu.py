@@ -86,6 +86,7 @@ def operators(monkeypatch):
     class Plan:
         def __init__(self, cu, tokens, window=None, **_):
             self.cu, self.tokens, self.window = cu.tolist(), tokens, window
+            self.status = torch.zeros(1, dtype=torch.int32)
 
     def attention(q, k, v, plan, scale=None, softcap=None):
         calls.append(plan)
@@ -319,3 +320,17 @@ def test_configuration_stays_one(operators):
     assert model.model.layers[0].self_attn.config._attn_implementation == "eager"
     model(**batch())
     assert len(operators) == 2
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("bad", [[0, 25, T + 1], [1, 25, T], [0, 30, 25, T], [0, -5], [], [0, 2 ** 32 + 40]])
+def test_malformed_boundaries_are_refused(operators, bad):
+    """Boundaries on the CPU, before anything runs."""
+    model, kw = patched("llama"), batch()
+    kw["cu_seqlens"] = torch.tensor(bad, dtype=torch.int64)
+    for how in ({}, {"validate_cu_seqlens": False}):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            model(**kw, **how)
+    assert not operators
+    kw["cu_seqlens"] = torch.tensor([0, 25, 25, 30])  # an empty document, rows behind the last
+    assert model(**kw).attention_status.tolist() == [0]
