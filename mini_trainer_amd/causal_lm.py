@@ -18,7 +18,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn.functional as F
 
-from .decoder import PLANS_KWARG, minibatch_plans, patch_decoder_layers, unlabelled_forward
+from .decoder import PLANS_KWARG, minibatch_plans, patch_decoder_layers, positions_within, unlabelled_forward
 from .flce import fused_linear_cross_entropy, per_sample_loss_sums
 
 __all__ = ["causal_lm_loss", "patch_causal_lm", "sample_loss_sums", "cu_seqlens_from_position_ids",
@@ -148,9 +148,12 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
             bounds = kwargs.pop("cu_seq_lens_q", None)
             for name in ("cu_seq_lens_k", "max_length_q", "max_length_k"):
                 kwargs.pop(name, None)
-            kwargs[PLANS_KWARG] = minibatch_plans(
-                input_ids if input_ids is not None else inputs_embeds, position_ids,
-                bounds if cu_seqlens is None else cu_seqlens, validate_cu_seqlens)
+            if cu_seqlens is not None:
+                bounds = cu_seqlens
+            tokens = input_ids if input_ids is not None else inputs_embeds
+            kwargs[PLANS_KWARG] = minibatch_plans(tokens, position_ids, bounds, validate_cu_seqlens)
+            if position_ids is None and bounds is not None:
+                position_ids = positions_within(bounds, tokens.shape[1], tokens.device)
         out = decoder(input_ids=input_ids, attention_mask=attention_mask,
                       position_ids=position_ids, past_key_values=past_key_values,
                       inputs_embeds=inputs_embeds, use_cache=use_cache, **kwargs)

@@ -271,3 +271,13 @@ def minibatch_plans(tokens: torch.Tensor, position_ids: Optional[torch.Tensor],
             starts[:, :1] = 0  # a row is no continuation of the one before
             cu_seqlens = cu_seqlens_from_position_ids(starts)
     return AttentionPlans(cu_seqlens, B * T, tokens.device, validate)
+
+
+def positions_within(cu_seqlens: torch.Tensor, tokens: int, device: torch.device) -> torch.Tensor:
+    """[1, tokens] int64 on `device`: each token's place in its document, the rows behind
+    the last one counted as one.  No sync; within the row for malformed boundaries too,
+    so that no embedding is read out of range before they are checked."""
+    rows = torch.arange(tokens, device=cu_seqlens.device)
+    cu = cu_seqlens.reshape(-1).to(torch.int64)
+    document = torch.searchsorted(cu, rows, right=True) - 1
+    return (rows - cu[document]).clamp(0, max(tokens - 1, 0)).to(device, non_blocking=True)[None]

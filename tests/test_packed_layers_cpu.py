@@ -334,3 +334,26 @@ def test_malformed_boundaries_are_refused(operators, bad):
     assert not operators
     kw["cu_seqlens"] = torch.tensor([0, 25, 25, 30])  # an empty document, rows behind the last
     assert model(**kw).attention_status.tolist() == [0]
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("name", ["gpt2", "llama"])
+@pytest.mark.parametrize("bounds", ["cu_seqlens", "cu_seq_lens_q"])
+def test_positions_count_within_each_document(operators, name, bounds):
+    """cu_seqlens alone: positions that are learned start at 0 in every document."""
+    model, kw = build(name), batch()
+    want = alone(model, kw["input_ids"])
+    cu = kw.pop("cu_seqlens")
+    del kw["position_ids"]
+    got = patch_causal_lm(model, packed_layers=True)(**kw, **{bounds: cu}).loss
+    assert rel(got, want) <= TOL
+
+
+def test_positions():
+    for cu, want in (([0, 3, 3, 5], [0, 1, 2, 0, 1, 0, 1]), ([0], list(range(7))), ([0, 7], list(range(7))),
+                     ([0, 0, 1], [0, 0, 1, 2, 3, 4, 5])):
+        got = decoder.positions_within(torch.tensor(cu, dtype=torch.int32), 7, torch.device("cpu"))
+        assert got.tolist() == [want]
+    for bad in ([5, 7], [0, 9], [0, -3, 7], [-2 ** 31, 2 ** 31 - 1], [3, 1, 9]):
+        got = decoder.positions_within(torch.tensor(bad), 7, torch.device("cpu"))
+        assert got.min() >= 0 and got.max() < 7
