@@ -23,8 +23,8 @@ __all__ = ["AttentionPlans", "patch_decoder_layers", "unlabelled_forward"]
 
 ATTENTION_NAME = "mt_packed"
 PLANS_KWARG = "mt_attention_plans"
-# Layers whose forward is norm, attention, addition, norm, MLP, addition, and the
-# norms that are rms_norm(x) * weight.
+# transformers' layers whose forward is norm, attention, addition, norm, MLP, addition,
+# and the norms that are rms_norm(x) * weight.
 PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
 PLAIN_NORMS = ("LlamaRMSNorm", "Qwen2RMSNorm")
 # Layer types whose mask is packed_attention's, without and with a window.
@@ -145,6 +145,26 @@ def _attention(module, query, key, value, attention_mask=None, scaling=None, dro
     return out.view(B, T, heads, D), None
 
 
+def _is_plain(module: torch.nn.Module, names) -> bool:
+    """Whether the module is transformers' own of that name and its forward the class's:
+    not another class that is called so, nor one whose forward has been replaced, in
+    the class or in this module."""
+    cls = type(module)
+    forward = inspect.unwrap(cls.forward)
+    return (cls.__name__ in names and cls.__module__.startswith("transformers.models.")
+            and "forward" not in module.__dict__
+            and (forward.__module__, forward.__qualname__) == (cls.__module__, cls.__name__ + ".forward"))
+
+
+def _has_hooks(module: torch.nn.Module) -> bool:
+    """Whether something wants to see the module called."""
+    every = torch.nn.modules.module
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or every._global_forward_hooks
+                or every._global_forward_pre_hooks or every._global_backward_hooks
+                or every._global_backward_pre_hooks)
+
+
 def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
                    past_key_values=None, use_cache=False, position_embeddings=None, **kwargs):
     """A PLAIN_LAYERS forward with the addition after attention and the norm
@@ -155,7 +175,7 @@ def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
         position_ids=position_ids, past_key_values=past_key_values, use_cache=use_cache,
         position_embeddings=position_embeddings, **kwargs)
     norm = self.post_attention_layernorm
-    if PLANS_KWARG in kwargs and type(norm).__name__ in PLAIN_NORMS and \
+    if PLANS_KWARG in kwargs and _is_plain(norm, PLAIN_NORMS) and not _has_hooks(norm) and \
             hidden_states.dtype == residual.dtype == norm.weight.dtype:
         hidden_states, residual = residual_rms_norm(hidden_states, residual, norm.weight,
                                                     eps=norm.variance_epsilon)
@@ -236,8 +256,9 @@ def patch_decoder_layers(decoder: torch.nn.Module) -> None:
     _refuse_other_mixers(decoder)
     ALL_ATTENTION_FUNCTIONS.register(ATTENTION_NAME, _attention)
     for module in decoder.modules():
-        if type(module).__name__ in PLAIN_LAYERS:
+        if _is_plain(module, PLAIN_LAYERS):
             module.forward = types.MethodType(_layer_forward, module)
+            continue
         config = module.__dict__.get("config")
         if config is None or getattr(type(config), "mt_view", False) or \
                 not hasattr(type(config), "_attn_implementation"):
@@ -246,8 +267,6 @@ def patch_decoder_layers(decoder: torch.nn.Module) -> None:
         if module is not decoder and all(p.kind is not p.VAR_KEYWORD for p in parameters):
             continue  # (no plans reach it)
         module.config = _config_view(config)
-        if type(module).__name__ in PLAIN_LAYERS:
-            continue
         if "forward" in module.__dict__:
             module.__dict__[OWN_FORWARD] = module.forward
         module.forward = types.MethodType(_packed_forward(type(module).forward, module is decoder), module)

@@ -357,3 +357,66 @@ def test_positions():
     for bad in ([5, 7], [0, 9], [0, -3, 7], [-2 ** 31, 2 ** 31 - 1], [3, 1, 9]):
         got = decoder.positions_within(torch.tensor(bad), 7, torch.device("cpu"))
         assert got.min() >= 0 and got.max() < 7
+
+
+@pytest.mark.parametrize("where", ["hook", "pre_hook", "backward_hook", "global", "forward", "class", "name"])
+def test_the_norms_module_is_called_where_someone_looks(operators, monkeypatch, where):
+    """Hooks of the norm behind the attention run, and a norm whose forward is not
+    transformers' own keeps it."""
+    model, kw, fused, seen = patched("llama"), batch(), [], []
+    norm = model.model.layers[1].post_attention_layernorm
+    plain = decoder.residual_rms_norm
+    monkeypatch.setattr(decoder, "residual_rms_norm", lambda *a, **k: fused.append(True) or plain(*a, **k))
+    want = model(**kw).loss.detach()
+    assert fused == [True] * 2
+
+    def look(module, *_):
+        if module is norm:
+            seen.append(True)
+
+    def twice(self, x):
+        seen.append(True)
+        return 2 * x
+
+    handle = None
+    if where == "hook":
+        handle = norm.register_forward_hook(look)
+    elif where == "pre_hook":
+        handle = norm.register_forward_pre_hook(look)
+    elif where == "backward_hook":
+        handle = norm.register_full_backward_hook(look)
+    elif where == "global":
+        handle = torch.nn.modules.module.register_module_forward_hook(look)
+    elif where == "forward":
+        norm.forward = twice.__get__(norm)
+    elif where == "class":
+        monkeypatch.setattr(type(norm), "forward", twice)
+    else:
+        norm.__class__ = type("LlamaRMSNorm", (type(norm),), {"forward": twice})
+    try:
+        loss = model(**kw).loss
+        loss.sum().backward()
+    finally:
+        if handle is not None:
+            handle.remove()
+    assert seen
+    assert len(fused) == 2 + (0 if where in ("global", "class") else 1)
+    if handle is not None:
+        assert rel(loss.detach(), want) <= TOL
+
+
+@torch.no_grad()
+def test_layers_of_another_forward_keep_it(operators):
+    """A plain layer's forward that something else has put there is run."""
+    model, kw, ran = build("llama"), batch(), []
+    want = alone(model, kw["input_ids"])
+    layer = model.model.layers[0]
+    own = layer.forward
+
+    def forward(*args, **kwargs):
+        ran.append(True)
+        return own(*args, **kwargs)
+
+    layer.forward = forward
+    patch_causal_lm(model, packed_layers=True)
+    assert rel(model(**kw).loss, want) <= TOL and ran == [True] and len(operators) == 2
