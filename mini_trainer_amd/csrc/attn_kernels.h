@@ -39,6 +39,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kAttnRows = 128;    // rows of a workgroup: 4 waves of 32
 constexpr int kAttnThreads = 256;
+constexpr float kAttnLowest = -3.402823466e38f;  // a maximum before any score: no finite one lies below
 constexpr int kPlanHeader = 16;   // int32 words before the plan's tiles
 constexpr int kPlanTile = 8;
 constexpr int kPlanBuckets = 1024;
@@ -771,7 +772,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
   f32x16_t acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
-  float m = kNegBig, sum = 0.f;
+  float m = kAttnLowest, sum = 0.f;
 
   const char* kbase = a.k + (int64_t)kvh * a.k_h;
   const char* vbase = a.v + (int64_t)kvh * a.v_h;
