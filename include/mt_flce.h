@@ -56,7 +56,7 @@
 extern "C" {
 #endif
 
-#define MT_FLCE_ABI_VERSION 9
+#define MT_FLCE_ABI_VERSION 10
 
 typedef struct ihipStream_t* mt_stream_t; /* == hipStream_t */
 
@@ -626,6 +626,9 @@ int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t 
  *   out_lo: T x heads x (head_dim rounded up to 32) bytes (bf16; fp32 ignores it)
  *     for what out's rounding took from it, from the forward to the backward, which
  *     without it (null) forms the rows' dout . out from the rounded values
+ *   lse_lo fp32 [heads, T]: what lse's rounding took from it, from the forward to
+ *     the backward, which without it (null) is off by 2^-24 |lse| of each
+ *     probability
  * The backward reads q, k, v, out, lse, dout and writes dq, dk, dv.  Sums in
  * fp32; results do not depend on the order workgroups run in.
  */
@@ -637,6 +640,7 @@ typedef struct mt_attn_args {
   void *dq, *dk, *dv;
   const int32_t* plan;
   void* out_lo;
+  float* lse_lo;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, dout_t, dout_h;
   int64_t T, S, heads, kv_heads, head_dim, window;
   float scale, softcap;

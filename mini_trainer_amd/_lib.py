@@ -15,7 +15,7 @@ import os
 # MT_FLCE_LIB: another build of the same library (the sanitized host-only
 # build of the CPU tests); unset in production.
 LIB_PATH = Path(os.environ.get("MT_FLCE_LIB") or Path(__file__).resolve().parent / "libmt_flce.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 MT_DTYPE_F32 = 0
 MT_DTYPE_BF16 = 1
@@ -33,7 +33,7 @@ STATUS_NAMES = {
 class AttnArgs(ctypes.Structure):
     """mt_attn_args of include/mt_flce.h."""
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv",
-                                         "plan", "out_lo")]
+                                         "plan", "out_lo", "lse_lo")]
                 + [(n, c_int64) for n in ("q_t", "q_h", "k_t", "k_h", "v_t", "v_h", "dout_t",
                                           "dout_h", "T", "S", "heads", "kv_heads", "head_dim",
                                           "window")]

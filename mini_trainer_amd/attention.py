@@ -133,21 +133,27 @@ class _PackedAttention(torch.autograd.Function):
         k, kp, k_t, k_h = _heads(key)
         v, vp, v_t, v_h = _heads(value)
         out = query.new_empty((T, heads, D))
-        # lse [heads, T] and, for a backward in bf16, what the rounding of out took from
-        # it, a byte for each element (rows of whole 32) from `low` fp32 words on (a
-        # 16-byte boundary)
-        low = -(-heads * T // 4) * 4 if out.dtype == torch.bfloat16 and any(ctx.needs_input_grad) else 0
-        words = low + T * heads * (-(-D // 32) * 8) if low else heads * T
+        # lse [heads, T] and, for a backward, what its rounding took from it and, in bf16,
+        # what the rounding of out took from that, a byte for each element (rows of whole
+        # 32); `rest` and `low`: the fp32 words that they begin at (16-byte boundaries)
+        words, rest, low = heads * T, 0, 0
+        if any(ctx.needs_input_grad):
+            rest = -(-words // 4) * 4
+            words += rest
+            if out.dtype == torch.bfloat16:
+                low = -(-words // 4) * 4
+                words = low + T * heads * (-(-D // 32) * 8)
         lse = torch.empty(words, dtype=torch.float32, device=dev)
         lse_at = lse.data_ptr()
         plan_at = plan.buffer.data_ptr()
         w = NO_WINDOW if plan.window is None else min(plan.window, NO_WINDOW)
         tail = (T, plan.documents, heads, key.shape[1], D, w, scale, softcap, _dtype_code(query.dtype))
         args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse_at, 0, 0, 0, 0, plan_at,
-                              lse_at + 4 * low if low else 0, q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
+                              lse_at + 4 * low if low else 0, lse_at + 4 * rest if rest else 0,
+                              q_t, q_h, k_t, k_h, v_t, v_h, 0, 0, *tail)
         _launch(dev, "mt_attn_forward", load().mt_attn_forward, args)
         ctx.save_for_backward(q, k, v, out, lse, plan.buffer)
-        ctx.tail, ctx.low = tail, low
+        ctx.tail, ctx.rest, ctx.low = tail, rest, low
         return out
 
     @_backward_once
@@ -162,7 +168,7 @@ class _PackedAttention(torch.autograd.Function):
         lse_at = lse.data_ptr()
         args = pack_attn_args(qp, kp, vp, out.data_ptr(), lse_at, dop, dq.data_ptr(), dk.data_ptr(),
                               dv.data_ptr(), plan.data_ptr(), lse_at + 4 * ctx.low if ctx.low else 0,
-                              q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h, *ctx.tail)
+                              lse_at + 4 * ctx.rest if ctx.rest else 0, q_t, q_h, k_t, k_h, v_t, v_h, do_t, do_h, *ctx.tail)
         lib = load()
         nbytes = lib.mt_attn_backward_workspace_bytes(args)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

@@ -46,6 +46,10 @@ int64_t attn_slots(const mt_attn_args& a) {
   return std::min(parts * attn_tiles(a.T, a.S), cdiv(most, a.kv_heads) + parts);
 }
 
+// One fp32 number for each row and query head: delta, and the factor of its
+// probabilities.
+size_t attn_row_bytes(const mt_attn_args& a) { return round256((size_t)a.heads * (size_t)a.T * 4); }
+
 size_t attn_part_bytes(const mt_attn_args& a) {
   return (size_t)attn_slots(a) * (size_t)a.kv_heads * 2 * kAttnRows * (size_t)a.head_dim * 4;
 }
@@ -117,6 +121,7 @@ AttnArgs attn_args(const mt_attn_args& a) {
   k.dk = static_cast<char*>(a.dk);
   k.dv = static_cast<char*>(a.dv);
   k.lse = a.lse;
+  k.lse_lo = a.lse_lo;
   k.out_lo = a.dtype == MT_DTYPE_BF16 ? static_cast<char*>(a.out_lo) : nullptr;
   k.plan = a.plan;
   k.T = (int32_t)a.T;
@@ -188,8 +193,7 @@ int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
 size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args) {
   if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0 || args->S < 0)
     return 0;
-  return round256((size_t)args->heads * (size_t)args->T * 4) + attn_item_bytes(*args) +
-         attn_part_bytes(*args);
+  return 2 * attn_row_bytes(*args) + attn_item_bytes(*args) + attn_part_bytes(*args);
 }
 
 int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace_bytes,
@@ -204,7 +208,8 @@ int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace
     return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
   AttnArgs k = attn_args(a);
   k.delta = static_cast<float*>(workspace);
-  char* items = static_cast<char*>(workspace) + round256((size_t)a.heads * (size_t)a.T * 4);
+  k.factor = reinterpret_cast<float*>(static_cast<char*>(workspace) + attn_row_bytes(a));
+  char* items = static_cast<char*>(workspace) + 2 * attn_row_bytes(a);
   k.items = reinterpret_cast<int32_t*>(items);
   k.part = reinterpret_cast<float*>(items + attn_item_bytes(a));
   k.parts_max = attn_parts_max(a);

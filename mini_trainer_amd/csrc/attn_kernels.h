@@ -635,6 +635,7 @@ struct AttnArgs {
   char *out, *dq, *dk, *dv;                    // [T, heads, D], contiguous
   char* out_lo;                                // attn_store_out's bytes, rows [T, Hq]; or null
   float *lse, *delta;                          // [Hq, T]; lse in units of log2
+  float *lse_lo, *factor;                      // [Hq, T]: what its rounding took from lse (or null); kAttnFar
   int32_t* items;                              // attn_items
   float* part;                                 // [Hk][slots][2][kAttnRows][D]: dK, dV of one part
   const int32_t* plan;
@@ -715,6 +716,13 @@ __device__ __forceinline__ void attn_items(const AttnArgs& a, int32_t* scratch) 
     }
   }
 }
+
+// A row's probabilities are 2^(z - lse) times a factor 2^-lse_lo, which is far from 1
+// where the scores are so large that lse has no room for the logarithm of the sum
+// beside the maximum (beyond some 2^20: of two equal scores of 1e9 each would count
+// whole).  Below kAttnFar it is within 2^-12 ln 2 of 1, and so are the probabilities
+// by the rounding of scores of that size; dK and dV leave it out there.
+constexpr float kAttnFar = 8192.0f;
 
 // --- forward ----------------------------------------------------------------
 
@@ -857,7 +865,14 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
     sum = sum * f + sum2 * f2;
     attn_add_pair<DP>(acc, f, f2, smem);
   }
-  if (valid && h == 0) lse[row] = m + fast_log2(sum);
+  if (valid && h == 0) {
+    const float rest = fast_log2(sum), both = m + rest;
+    lse[row] = both;
+    if (a.lse_lo) {  // (the error of a sum, exactly)
+      const float part = both - m;
+      a.lse_lo[(int64_t)head * a.T + row] = (m - (both - part)) + (rest - part);
+    }
+  }
   const int64_t at = (int64_t)r0 * o_t + (int64_t)head * a.D;
   if constexpr (sizeof(T) == 2) {
     const int64_t n = attn_low_bytes(a.D);
@@ -942,6 +957,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   }
   qf.load(a.q + (int64_t)r0 * a.q_t + (int64_t)head * a.q_h, (uint32_t)a.q_t, r_end - r0, d_bytes);
   const float lse = valid ? a.lse[(int64_t)head * a.T + row] : 0.f;
+  const float factor = valid && a.lse_lo ? fast_exp2(-a.lse_lo[(int64_t)head * a.T + row]) : 1.0f;
   float delta = 0.f;
 #pragma unroll
   for (int i = 0; i < AttnFrag<T, DP>::kN; ++i)
@@ -958,7 +974,10 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
       }
     }
   delta = attn_pair_add(delta);
-  if (valid && h == 0) a.delta[(int64_t)head * a.T + row] = delta;
+  if (valid && h == 0) {
+    a.delta[(int64_t)head * a.T + row] = delta;
+    a.factor[(int64_t)head * a.T + row] = factor;
+  }
   f32x16_t acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = f32x16_t{};
@@ -1003,7 +1022,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     if (!attn_join_pair<DP>(acc, none, none2, smem)) return;
     attn_add_pair<DP>(acc, 1.0f, 1.0f, smem);
   }
-  attn_store<DP>(acc, a.scale, dq + (int64_t)r0 * o_t, o_t, r_end - r0, a.D);
+  // (linear in the row's probabilities)
+  attn_store<DP>(acc, a.scale * factor, dq + (int64_t)r0 * o_t, o_t, r_end - r0, a.D);
 }
 
 // --- backward: dK and dV --------------------------------------------------------
@@ -1027,8 +1047,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
   constexpr int kQ = attn_q_rows<T, DP>();
   constexpr bool kVLds = sizeof(T) == 2 && DP == 128;
   constexpr uint32_t kTile = kQ * L::kRowB;
-  constexpr uint32_t kBuf = 2 * kTile + 2 * 256;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * kBuf];  // 2 x (Q, dO, lse, delta)
+  constexpr uint32_t kBuf = 2 * kTile + 3 * 256;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kBuf];  // 2 x (Q, dO, lse, delta, factor)
   __shared__ __attribute__((aligned(1024))) char vt[kVLds ? kAttnRows * L::kRowB : 16];
   typedef const __attribute__((address_space(4))) int32_t* scalar_t;
   const scalar_t items = (scalar_t)(uintptr_t)a.items;
@@ -1092,8 +1112,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     char* at = smem + buf * kBuf;
     sq.issue(a.q + (int64_t)fi * a.q_t + head * a.q_h, n, at);
     sdo.issue(a.dout + (int64_t)fi * a.do_t + head * a.do_h, n, at + kTile);
-    if (w < 2) {  // the rows' lse by the first wave, their delta by the second
-      const float* from = (w == 0 ? a.lse : a.delta) + head * a.T + fi;
+    if (w < 3) {  // the rows' lse by the first wave, their delta and factor by the next two
+      const float* from = (w == 0 ? a.lse : w == 1 ? a.delta : a.factor) + head * a.T + fi;
       attn_dma4(attn_rsrc(from, 4u * (uint32_t)n), at + 2 * kTile + w * 256u, l * 4u);
     }
     fi -= kQ;
@@ -1109,7 +1129,9 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
     if (active && i0 < w_hi && i0 + kQ > w_lo) {
       const char* qt = smem + buf.value * kBuf;
       const float* rows = reinterpret_cast<const float*>(qt + 2 * kTile);
-      const bool edge = i0 < f_lo || i0 + kQ > f_hi;
+      // (in one branch with the masks: with a branch of its own the registers spill)
+      const bool far = __any(fabsf(rows[l & (uint32_t)(kQ - 1)]) >= kAttnFar);
+      const bool edge = i0 < f_lo || i0 + kQ > f_hi || far;
 #pragma unroll
       for (int b = 0; b < kQ / 32; ++b) {
         f32x16_t s = f32x16_t{}, dp = f32x16_t{};
@@ -1146,6 +1168,17 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
             const uint32_t at = (uint32_t)(8 * (r / 4) + r % 4);
             if (from + at >= range) s[r] = dp[r] = 0.f;
             if (one + at < ones) dp[r] = 0.f;
+          }
+          if (far) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const f32x4_t f = *reinterpret_cast<const f32x4_t*>(rows + 128 + 32 * b + 8 * g + 4 * h);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                s[4 * g + e] *= f[e];
+                dp[4 * g + e] *= f[e];
+              }
+            }
           }
         }
         attn_col_product<T, DP>(av, qt + kTile, 32u * b, s);

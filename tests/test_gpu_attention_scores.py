@@ -48,3 +48,56 @@ def test_scores_of_the_types_whole_range(gpu, dtype, heads):
         assert not dq[row].any() and not dk[row].any()
         assert torch.equal(dv[row], do[row])
 
+
+
+@pytest.mark.parametrize("heads", [HALF, WHOLE])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("half", [0, 3, 8, 12, 25, 50])
+def test_equal_scores_of_any_size(gpu, dtype, half, heads):
+    """All scores of a row the same, -2^(2 half + 6): its n probabilities are 1 / n each in
+    the forward and in the gradients, however little room the size of the scores leaves
+    for the logarithm of n in an fp32 log-sum.  Scores are exact here, so that the errors
+    are, with u = eps / 2 of the type and F = 2^-24:
+      probabilities  up (u for bf16's products) + (n + C) F, and where |lse| < 8192,
+                     F |lse| from the log-sum alone;
+      out            u |out| + theirs times mean |v|;
+      delta          theirs and 2^-16 (what is kept of bf16's out) of |dO| |out|, summed;
+      dS             up + the probabilities' of itself, plus p times those of delta and dP."""
+    D, lengths = 64, [1, 2, 3, 57, 7]
+    T = sum(lengths)
+    g = torch.Generator().manual_seed(3)
+    v, do = (torch.randn(T, heads, D, generator=g).to(dtype).to(gpu) for _ in range(2))
+    q = torch.full((T, heads, D), -2.0 ** half, dtype=dtype, device=gpu)
+    k = torch.full((T, heads, D), 2.0 ** half, dtype=dtype, device=gpu)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    out = packed_attention(*leaves, plan_of(lengths, gpu), scale=1.0)
+    got = {"out": out, **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)))}
+    u, F, C = ref.unit(dtype), ref.F32, ref.C
+    up = u if dtype == torch.bfloat16 else 0.0
+    mask = ref.seen_mask(lengths, T).double()
+    n = mask.sum(1, keepdim=True)
+    p = mask / n
+    lse = 2.0 ** (2 * half + 6) * 1.4427
+    rel_o = up + (n + C) * F
+    rel_p = rel_o + (F * lse if lse < 8192 else 0.0)
+    for h in (0, heads - 1):
+        vh, doh = v[:, h].double().cpu(), do[:, h].double().cpu()
+        o = p @ vh
+        o_err = rel_o * (p @ vh.abs())
+        dp = doh @ vh.T
+        delta = (doh * o).sum(1, keepdim=True)
+        delta_err = (doh.abs() * (o_err + (2.0 ** -16 + (D + C) * F) * o.abs())).sum(1, keepdim=True)
+        alone = (n == 1)
+        ds = torch.where(alone, torch.zeros(()).double(), p * (dp - delta))
+        ds_err = (rel_p + up) * ds.abs() + p * ((D + C) * F * (doh.abs() @ vh.abs().T) + delta_err)
+        ds_err = torch.where(alone, torch.zeros(()).double(), 1.01 * ds_err)
+        size = 2.0 ** half
+        dq, dk = ds.sum(1, keepdim=True) * size, -ds.sum(0)[:, None] * size
+        dq_err = (ds_err + (T + C) * F * ds.abs()).sum(1, keepdim=True) * size
+        dk_err = (ds_err + (T + C) * F * ds.abs()).sum(0)[:, None] * size
+        dv = p.T @ doh
+        dv_err = ((rel_p + (T + C) * F) * p).T @ doh.abs()
+        one = torch.ones(1, D, dtype=torch.float64)
+        for name, value, err in (("out", o, o_err), ("dq", dq * one, dq_err * one),
+                                 ("dk", dk * one, dk_err * one), ("dv", dv, dv_err)):
+            ref.assert_within(got[name][:, h], (value, err + u * (value.abs() + err)), f"{name} {h}")
