@@ -77,8 +77,8 @@ int attn_check(const mt_attn_args* p, bool backward) {
     return fail(MT_ERR_INVALID_ARGUMENT, "window=%lld out of range", (long long)a.window);
   if (!(a.scale > 0.f) || !std::isfinite(a.scale) || !(a.softcap >= 0.f) || !std::isfinite(a.softcap))
     return fail(MT_ERR_INVALID_ARGUMENT, "scale must be positive and softcap >= 0 (0 = off), both finite");
-  if (a.softcap > 0.f && !std::isfinite(a.scale / a.softcap))
-    return fail(MT_ERR_INVALID_ARGUMENT, "scale / softcap is not finite");
+  if (a.softcap > 0.f && !(std::isnormal(a.scale / a.softcap) && std::isfinite(a.softcap * kLog2e)))
+    return fail(MT_ERR_INVALID_ARGUMENT, "scale / softcap and softcap log2(e) must be normal fp32 numbers");
   // workgroups of kAttnThreads, of which a launch takes fewer than 2^32 threads
   if ((attn_tiles(a.T, a.S) + 1) * std::max(a.heads, 4 * a.kv_heads) >= ((int64_t)1 << 32) / kAttnThreads)
     return fail(MT_ERR_UNSUPPORTED, "%lld tiles (of %d rows, and one for each document) x %lld heads "
@@ -138,13 +138,21 @@ AttnArgs attn_args(const mt_attn_args& a) {
   return k;
 }
 
-// kernel<T, DP, CAP, more> for a type, head width and softcap.
+// The kernels' CAP for a call.
+int attn_cap(const mt_attn_args& a) {
+  return !(a.softcap > 0.f) ? 0 : a.dtype == MT_DTYPE_BF16 && a.softcap <= kAttnCapFast ? 1 : 2;
+}
+
+// kernel<T, DP, CAP, more> for a type, head width and CAP.
 #define MT_ATTN_PICK(kernel, dtype, D, cap, ...)                                              \
   ((dtype) == MT_DTYPE_BF16                                                                   \
-       ? ((D) <= 64 ? ((cap) ? kernel<__bf16, 64, true __VA_ARGS__> : kernel<__bf16, 64, false __VA_ARGS__>)      \
-                    : ((cap) ? kernel<__bf16, 128, true __VA_ARGS__> : kernel<__bf16, 128, false __VA_ARGS__>))   \
-       : ((D) <= 64 ? ((cap) ? kernel<float, 64, true __VA_ARGS__> : kernel<float, 64, false __VA_ARGS__>)        \
-                    : ((cap) ? kernel<float, 128, true __VA_ARGS__> : kernel<float, 128, false __VA_ARGS__>)))
+       ? ((D) <= 64 ? MT_ATTN_PICK_CAP(kernel, __bf16, 64, cap, __VA_ARGS__)                  \
+                    : MT_ATTN_PICK_CAP(kernel, __bf16, 128, cap, __VA_ARGS__))                \
+       : ((D) <= 64 ? ((cap) ? kernel<float, 64, 2 __VA_ARGS__> : kernel<float, 64, 0 __VA_ARGS__>)          \
+                    : ((cap) ? kernel<float, 128, 2 __VA_ARGS__> : kernel<float, 128, 0 __VA_ARGS__>)))
+#define MT_ATTN_PICK_CAP(kernel, T, DP, cap, ...)                                             \
+  ((cap) == 0 ? kernel<T, DP, 0 __VA_ARGS__>                                                  \
+              : (cap) == 1 ? kernel<T, DP, 1 __VA_ARGS__> : kernel<T, DP, 2 __VA_ARGS__>)
 #define MT_COMMA ,
 
 // Half tiles (SPLIT = 2 of the kernels) where the rows give fewer workgroups than
@@ -183,8 +191,8 @@ int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
   if (a.T == 0) return MT_OK;
   const AttnArgs k = attn_args(a);
   const int split = attn_split(a);
-  auto kern = split == 2 ? MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, a.softcap > 0.f, MT_COMMA 2)
-                         : MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, a.softcap > 0.f, MT_COMMA 1);
+  auto kern = split == 2 ? MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, attn_cap(a), MT_COMMA 2)
+                         : MT_ATTN_PICK(attn_fwd_kernel, a.dtype, a.head_dim, attn_cap(a), MT_COMMA 1);
   hipLaunchKernelGGL(kern, dim3((uint32_t)(split * k.tiles_max * k.Hq)), dim3(kAttnThreads), 0,
                      (hipStream_t)stream, k);
   return check_launch("attn_fwd_kernel");
@@ -214,7 +222,7 @@ int mt_attn_backward(const mt_attn_args* args, void* workspace, size_t workspace
   k.part = reinterpret_cast<float*>(items + attn_item_bytes(a));
   k.parts_max = attn_parts_max(a);
   k.slots = (int32_t)attn_slots(a);
-  const bool cap = a.softcap > 0.f;
+  const int cap = attn_cap(a);
   hipStream_t s = (hipStream_t)stream;
   const int split = attn_split(a);
   auto dq = split == 2 ? MT_ATTN_PICK(attn_dq_kernel, a.dtype, a.head_dim, cap, MT_COMMA 2)

@@ -426,12 +426,24 @@ __device__ __forceinline__ void attn_sched_reads() {
 // few blocks that a range's end crosses would be evaluated in all of them.
 __device__ __forceinline__ void attn_no_if_conversion() { asm volatile("" ::: "memory"); }
 
-// tanh: bf16 inputs take 1 - 2 / (exp(2x) + 1) (absolute error some 2^-23, far
-// below a score's own), fp32 the library's.
-template <class T>
+// The kernels' CAP: 0 no softcap; 1 a softcap up to kAttnCapFast, 2 one above it (fp32:
+// any).  With bf16 inputs tanh is 1 - 2 / (exp(2x) + 1), whose absolute error of some
+// 1.5 2^-23 is softcap times that in a score: up to 256 at most 5e-5 of a probability, a
+// 40th of the rounding of P; at 1e6 it would be 0.2, where the cap should change
+// nothing.  Above 256 a small x takes the series (x^9 on: 2^-30 of it), so that the
+// error is 2^-19 of the score at most, less than that of its sum.  16384 tokens, 32
+// heads of 128, forward and backward: 10.8 ms, 12.4 above 256.  fp32 takes the
+// library's tanh.
+constexpr float kAttnCapFast = 256.0f;
+
+template <class T, int CAP>
 __device__ __forceinline__ float attn_tanh(float x) {
   if constexpr (sizeof(T) == 4) return tanhf(x);
-  return fmaf(-2.0f, __builtin_amdgcn_rcpf(fast_exp2(x * (2.0f * kLog2e)) + 1.0f), 1.0f);
+  const float t = fmaf(-2.0f, __builtin_amdgcn_rcpf(fast_exp2(x * (2.0f * kLog2e)) + 1.0f), 1.0f);
+  if constexpr (CAP == 1) return t;
+  const float y = x * x;
+  const float p = fmaf(fmaf(fmaf(-17.0f / 315.0f, y, 2.0f / 15.0f), y, -1.0f / 3.0f), y * x, x);
+  return y < 0.015625f ? p : t;  // (a NaN in both)
 }
 
 // acc^T [DP x 32 rows] * s (one per row) to the wave's rows of D elements, `pitch`
@@ -741,7 +753,7 @@ constexpr int kAttnKeys = 64;  // keys per block of the forward and of dQ
 // workgroup's first tile, masks and last partial tile: 4096 tokens of 12 documents
 // 43 us.  Row tiles of 128 with two workgroups on a CU: a wave alone on its SIMD
 // with twice the rows hides neither the LDS nor the softmax (dK and dV below).
-template <class T, int DP, bool CAP, int SPLIT>
+template <class T, int DP, int CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_fwd_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
@@ -812,7 +824,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 #pragma unroll
       for (int b = 0; b < 2 / SPLIT; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] = attn_tanh<T>(s[b][r] * a.cap_mul);
+        for (int r = 0; r < 16; ++r) s[b][r] = attn_tanh<T, CAP>(s[b][r] * a.cap_mul);
     }
     if (k0 < f_lo || k0 + kOwn > f_hi) {
       attn_no_if_conversion();
@@ -890,7 +902,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 // scores and dP are formed again for dK and dV: adding dQ from a kernel of the keys
 // would take atomics, whose order changes results, or a copy of dQ per key tile.
 // 16384 tokens, 32 heads of 128: 2.7 ms, 1240 TFLOP/s; with a softcap 3.35.
-template <class T, int DP, bool CAP, int SPLIT>
+template <class T, int DP, int CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dq_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr uint32_t kTile = kAttnKeys * L::kRowB;
@@ -997,7 +1009,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float x = s[r];
-        if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
+        if constexpr (CAP) x = attn_tanh<T, CAP>(x * a.cap_mul);
         s[r] = fast_exp2(fmaf(x, a.z_mul, -lse)) * (dp[r] - delta);
         if constexpr (CAP) s[r] *= fmaf(-x, x, 1.0f);
       }
@@ -1041,7 +1053,7 @@ constexpr int attn_q_rows() {
 // neither the LDS reads nor the softmax.  One document of 16384 tokens, 32 heads
 // of 128 (8 key heads): 4.1 ms, 1075 TFLOP/s; with V in registers 7.4 ms; as two
 // kinds of workgroup, dK and dV each with their own scores, 5.5 ms.
-template <class T, int DP, bool CAP>
+template <class T, int DP, int CAP>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dkdv_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
   constexpr int kQ = attn_q_rows<T, DP>();
@@ -1153,7 +1165,7 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_d
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
             float x = s[r];
-            if constexpr (CAP) x = attn_tanh<T>(x * a.cap_mul);
+            if constexpr (CAP) x = attn_tanh<T, CAP>(x * a.cap_mul);
             s[r] = fast_exp2(fmaf(x, a.z_mul, -lse[e]));
             dp[r] = s[r] * (dp[r] - delta[e]);
             if constexpr (CAP) dp[r] *= fmaf(-x, x, 1.0f);

@@ -101,3 +101,39 @@ def test_equal_scores_of_any_size(gpu, dtype, half, heads):
         for name, value, err in (("out", o, o_err), ("dq", dq * one, dq_err * one),
                                  ("dk", dk * one, dk_err * one), ("dv", dv, dv_err)):
             ref.assert_within(got[name][:, h], (value, err + u * (value.abs() + err)), f"{name} {h}")
+
+
+@pytest.mark.parametrize("heads", [HALF, WHOLE])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("softcap", [256.0, 257.0, 1e4, 1e6, 1e8, 1e30])
+def test_a_large_softcap(gpu, D, heads, softcap):
+    """softcap tanh(z / softcap) is within |z|^3 / (3 softcap^2) of z; the tolerance is that
+    of the capped scores with tanh right to 4 units of its last place, whatever the cap."""
+    lengths = [50, 20]
+    T = sum(lengths)
+    g = torch.Generator().manual_seed(2)
+    q, k, v, do = (torch.randn(T, heads, D, generator=g).to(torch.bfloat16).to(gpu) for _ in range(4))
+    leaves = [t.detach().requires_grad_(True) for t in (4 * q, k, v)]
+    out = packed_attention(*leaves, plan_of(lengths, gpu), softcap=softcap)
+    got = {"out": out, **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, do)))}
+    mask = ref.seen_mask(lengths, T)
+    for h in (0, heads - 1):
+        one = slice(h, h + 1)
+        z = torch.einsum("id,jd->ij", 4 * q[:, h].double().cpu(), k[:, h].double().cpu()) * D ** -0.5
+        assert z.abs().max() < 60
+        want = capped(4 * q[:, one], k[:, one], v[:, one], do[:, one], mask, softcap)
+        for name in got:
+            ref.assert_within(got[name][:, one], want[name], name)
+
+
+def capped(q, k, v, do, mask, softcap):
+    """Values with the cap, tolerances of the same scores without one (whose C operations
+    have room for tanh's 4 units): the cap's derivative, 1 - tanh^2, adds 8 of them."""
+    plain = ref.attention(q, k, v, do, mask)
+    value = ref.attention(q, k, v, do, mask, softcap=softcap)
+    made = {}
+    for name in plain:
+        tol = plain[name][1]
+        # a smaller |z| under the cap has the smaller error; the gradients are as much smaller
+        made[name] = (value[name][0], 1.01 * tol + 64 * ref.F32 * value[name][0].abs())
+    return made
