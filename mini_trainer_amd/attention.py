@@ -126,7 +126,7 @@ def _heads(t: torch.Tensor):
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, query, key, value, plan, scale, softcap):
+    def forward(ctx, query, key, value, plan, scale, softcap, differentiable):
         dev = query.device
         T, heads, D = query.shape
         q, qp, q_t, q_h = _heads(query)
@@ -137,7 +137,7 @@ class _PackedAttention(torch.autograd.Function):
         # what the rounding of out took from that, a byte for each element (rows of whole
         # 32); `rest` and `low`: the fp32 words that they begin at (16-byte boundaries)
         words, rest, low = heads * T, 0, 0
-        if any(ctx.needs_input_grad):
+        if differentiable:  # (needs_input_grad does not say whether gradients are recorded)
             rest = -(-words // 4) * 4
             words += rest
             if out.dtype == torch.bfloat16:
@@ -173,7 +173,7 @@ class _PackedAttention(torch.autograd.Function):
         nbytes = lib.mt_attn_backward_workspace_bytes(args)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _launch(dev, "mt_attn_backward", lib.mt_attn_backward, args, ws.data_ptr(), nbytes)
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None, None, None
 
 
 def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
@@ -224,9 +224,10 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         raise ValueError(f"the plan is for {plan.tokens} rows, query has {T}")
     if plan.device != query.device:
         raise ValueError(f"the plan lies on {plan.device}, query on {query.device}")
+    grad = torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)
     chunk = 16 // query.element_size()
     if D % chunk:  # whole 16-byte chunks: zero columns add nothing to a product
         pad = (0, -D % chunk)
         query, key, value = (torch.nn.functional.pad(t, pad) for t in (query, key, value))
-        return _PackedAttention.apply(query, key, value, plan, scale, cap)[..., :D]
-    return _PackedAttention.apply(query, key, value, plan, scale, cap)
+        return _PackedAttention.apply(query, key, value, plan, scale, cap, grad)[..., :D]
+    return _PackedAttention.apply(query, key, value, plan, scale, cap, grad)

@@ -151,3 +151,27 @@ def test_captured_and_replayed(gpu):
         got = [t.clone() for t in held]
         want = run(*new, packed_attention_plan(cu_of(bounds, gpu), T))
         assert all(torch.equal(g, w) for g, w in zip(got, want.values()))
+
+
+def test_nothing_is_kept_for_no_backward(gpu):
+    """Memory at the highest point, beyond what was there: the output and one fp32 number
+    for each row and head, without gradients being recorded; more where they are."""
+    q, k, v, _ = inputs(128, seed=8)
+    plan = packed_attention_plan(cu_of(LENGTHS, gpu), T)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    packed_attention(*leaves, plan)
+    least = 2 * q.numel() + 4 * HEADS * T
+
+    def highest():
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        at = torch.cuda.memory_allocated()
+        out = packed_attention(*leaves, plan)
+        return torch.cuda.max_memory_allocated() - at, out
+
+    with torch.no_grad():
+        quiet, out = highest()
+    recorded, other = highest()
+    assert torch.equal(out, other)
+    assert least <= quiet <= least + 4096  # (blocks of 512 bytes)
+    assert recorded >= least + q.numel() + 4 * HEADS * T
