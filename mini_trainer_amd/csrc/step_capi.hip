@@ -54,9 +54,13 @@ constexpr int64_t kNormMaxH = 1024 * 32;
 // the plain form, 65536 x 4096: 382, 387, 453 us.
 constexpr int64_t kNormGroups = 512;
 
-// Rows at a time of the backward, and so partial rows of the weight gradients:
-// at most kNormGroups workgroups of up to four rows each.
-int64_t norm_parts(int64_t T) { return std::max<int64_t>(4, std::min<int64_t>(cdiv(T, 4), kNormGroups) * 4); }
+// Rows at a time of the backward, and so partial rows of the weight gradients, at
+// most: kNormGroups workgroups, of four rows up to the width that a wave holds
+// (norm_pick, bf16) and of one above it.
+int64_t norm_parts(int64_t T, int64_t H) {
+  return H <= 64 * 2 * 8 ? std::max<int64_t>(4, std::min<int64_t>(cdiv(T, 4), kNormGroups) * 4)
+                         : std::min<int64_t>(T, kNormGroups);
+}
 
 int norm_check(const mt_norm_args* p, bool backward) {
   if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
@@ -148,6 +152,8 @@ int launch_norm_bwd(NormArgs k, const mt_norm_args& a, bool vec, hipStream_t str
     constexpr int rows = threads / decltype(TPR)::value;
     const int64_t groups = std::min<int64_t>(cdiv(k.T, rows), kNormGroups);
     k.parts = (int32_t)(groups * rows);
+    if (k.parts > norm_parts(k.T, k.H))  // (the workspace's partial rows)
+      return fail(MT_ERR_UNSUPPORTED, "%d partial rows", (int)k.parts);
     auto kern = (k.pw || k.gate)
                     ? norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, true>
                     : norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, false>;
@@ -248,7 +254,7 @@ int mt_norm_forward(const mt_norm_args* args, mt_stream_t stream) {
 }
 
 size_t mt_norm_backward_workspace_bytes(int64_t T, int64_t H) {
-  return T <= 0 || H <= 0 || H > kNormMaxH ? 0 : (size_t)3 * norm_parts(T) * (size_t)H * 4;
+  return T <= 0 || H <= 0 || H > kNormMaxH ? 0 : (size_t)3 * norm_parts(T, H) * (size_t)H * 4;
 }
 
 int mt_norm_backward(const mt_norm_args* args, void* workspace, size_t workspace_bytes,
