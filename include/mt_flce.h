@@ -616,9 +616,9 @@ int mt_attn_plan(const int32_t* cu_seqlens, const int32_t* prefix_lens, int64_t 
  * head h reads key head h' = h / (heads / kv_heads).  Rows behind the last
  * document: zeros.
  *   q [T, heads, head_dim], k, v [T, kv_heads, head_dim], dout as q: unit
- *     stride along head_dim, the strides of rows (_t) and heads (_h) in
- *     elements, whole 16-byte chunks, 0 allowed; head_dim whole 16-byte chunks,
- *     at most 128
+ *     stride along head_dim, the strides of rows (_t, at most 2^24) and heads (_h,
+ *     at most 2^40) in elements, whole 16-byte chunks, 0 allowed; head_dim whole
+ *     16-byte chunks, at most 128
  *   out, dq [T, heads, head_dim], dk, dv [T, kv_heads, head_dim]: contiguous
  *   lse fp32 [heads, T]: log2 of the sum of 2^(z log2 e), from the forward to
  *     the backward; 0 behind the last document

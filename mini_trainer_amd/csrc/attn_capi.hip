@@ -58,6 +58,8 @@ size_t attn_item_bytes(const mt_attn_args& a) {
   return round256(16 + 8 * (size_t)attn_tiles(a.T, a.S) * ((size_t)attn_parts_max(a) + 1));
 }
 
+constexpr int64_t kMaxHeads = 65536;
+
 int attn_check(const mt_attn_args* p, bool backward) {
   if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
   const mt_attn_args& a = *p;
@@ -65,7 +67,7 @@ int attn_check(const mt_attn_args* p, bool backward) {
   if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
   if (a.T < 0 || a.T > kMaxRows || a.S < 0 || a.S > kMaxRows)
     return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld or S=%lld out of range", (long long)a.T, (long long)a.S);
-  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads > 65536 || a.heads % a.kv_heads != 0)
+  if (a.heads <= 0 || a.kv_heads <= 0 || a.heads > kMaxHeads || a.heads % a.kv_heads != 0)
     return fail(MT_ERR_INVALID_ARGUMENT, "heads=%lld must be a positive multiple of kv_heads=%lld",
                 (long long)a.heads, (long long)a.kv_heads);
   if (a.head_dim <= 0 || a.head_dim % (16 / es) != 0)
@@ -86,11 +88,14 @@ int attn_check(const mt_attn_args* p, bool backward) {
   const int64_t strides[] = {a.q_t, a.q_h, a.k_t, a.k_h, a.v_t, a.v_h, backward ? a.dout_t : 0,
                              backward ? a.dout_h : 0};
   for (int64_t s : strides)
-    if (s < 0 || (s * es) % 16 != 0)
+    if (s < 0 || s % (16 / es) != 0)
       return fail(MT_ERR_INVALID_ARGUMENT, "strides must be whole 16-byte chunks, not negative");
   for (int i = 0; i < 8; i += 2)
     if (strides[i] > (int64_t)1 << 24)
       return fail(MT_ERR_UNSUPPORTED, "rows %lld elements apart: at most 2^24", (long long)strides[i]);
+  for (int i = 1; i < 8; i += 2)  // (all heads' addresses in 64 bits)
+    if (strides[i] > (int64_t)1 << 40)
+      return fail(MT_ERR_UNSUPPORTED, "heads %lld elements apart: at most 2^40", (long long)strides[i]);
   if (a.T == 0) return MT_OK;
   const void* need[] = {a.q, a.k, a.v, a.out, a.lse, a.plan};
   for (const void* x : need)
@@ -199,8 +204,10 @@ int mt_attn_forward(const mt_attn_args* args, mt_stream_t stream) {
 }
 
 size_t mt_attn_backward_workspace_bytes(const mt_attn_args* args) {
-  if (!args || args->T <= 0 || args->kv_heads <= 0 || args->heads <= 0 || args->head_dim <= 0 || args->S < 0)
-    return 0;
+  if (!args || args->T <= 0 || args->T > kMaxRows || args->S < 0 || args->S > kMaxRows ||
+      args->kv_heads <= 0 || args->heads < args->kv_heads || args->heads > kMaxHeads ||
+      args->head_dim <= 0 || args->head_dim > 128)
+    return 0;  // (attn_check refuses these)
   return 2 * attn_row_bytes(*args) + attn_item_bytes(*args) + attn_part_bytes(*args);
 }
 

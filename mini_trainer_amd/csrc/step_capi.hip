@@ -186,6 +186,8 @@ int64_t clip_chunk(const int64_t* numel, int64_t n) {
   return chunk;
 }
 
+constexpr int64_t kClipMost = (int64_t)1 << 40;  // elements of one tensor
+
 int clip_check(void* const* ptrs, const int64_t* numel, const int64_t* cols, const int64_t* pitch,
                const int32_t* dtypes, int64_t n) {
   if (n < 0 || n > (1 << 24)) return fail(MT_ERR_INVALID_ARGUMENT, "n=%lld out of range", (long long)n);
@@ -195,7 +197,7 @@ int clip_check(void* const* ptrs, const int64_t* numel, const int64_t* cols, con
     const int es = esize(dtypes[i]);
     if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "tensor %lld: dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16",
                          (long long)i, dtypes[i]);
-    if (numel[i] < 0 || numel[i] > (int64_t)1 << 40 || (numel[i] > 0 && !ptrs[i]) ||
+    if (numel[i] < 0 || numel[i] > kClipMost || (numel[i] > 0 && !ptrs[i]) ||
         reinterpret_cast<uintptr_t>(ptrs[i]) % es != 0)
       return fail(MT_ERR_INVALID_ARGUMENT, "tensor %lld: bad size or pointer", (long long)i);
     if (cols[i] < 0 || (cols[i] > 0 && (pitch[i] < cols[i] || numel[i] % cols[i] != 0)))
@@ -254,7 +256,7 @@ int mt_norm_forward(const mt_norm_args* args, mt_stream_t stream) {
 }
 
 size_t mt_norm_backward_workspace_bytes(int64_t T, int64_t H) {
-  return T <= 0 || H <= 0 || H > kNormMaxH ? 0 : (size_t)3 * norm_parts(T, H) * (size_t)H * 4;
+  return T <= 0 || T > kMaxRows || H <= 0 || H > kNormMaxH ? 0 : (size_t)3 * norm_parts(T, H) * (size_t)H * 4;
 }
 
 int mt_norm_backward(const mt_norm_args* args, void* workspace, size_t workspace_bytes,
@@ -275,6 +277,9 @@ int mt_norm_backward(const mt_norm_args* args, void* workspace, size_t workspace
 
 size_t mt_grad_norm_workspace_bytes(const int64_t* numel, int64_t n) {
   if (!numel || n <= 0) return 8;
+  if (n > (1 << 24)) return 0;  // (clip_check refuses these)
+  for (int64_t i = 0; i < n; ++i)
+    if (numel[i] < 0 || numel[i] > kClipMost) return 0;
   const int64_t chunks = clip_chunks(numel, n, clip_chunk(numel, n));
   return 8 * (size_t)std::max<int64_t>(1, std::min(chunks, cdiv(n, kClipTensors) * kClipGroups));
 }

@@ -95,10 +95,10 @@ class AttentionPlans:
     def check_layers(self, decoder: torch.nn.Module) -> None:
         """Raise ValueError unless every layer of the decoder went through packed
         attention: one that mixes tokens in another way has mixed the documents."""
-        layers, ran = decoder.config.num_hidden_layers, len(self._attended)
+        layers, ran = getattr(decoder.config, "num_hidden_layers", None), len(self._attended)
         dropped = decoder.training and getattr(decoder.config, "layerdrop", 0.0)
         # (two calls in a layer count once; a module that several layers share, for each)
-        if layers not in (ran, self._calls) and not (dropped and 0 < ran < layers):
+        if layers not in (ran, self._calls) and not (dropped and layers and 0 < ran < layers):
             raise ValueError(f"packed layers: {ran} of {type(decoder).__name__}'s {layers} layers run "
                              "their attention as packed attention; the others would mix the documents")
 

@@ -47,3 +47,22 @@ def test_norm_workspace_holds_what_every_variant_writes(dtype, V):
             for T in (1, 3, 4, 5, 600, 2044, 2045, 5000):
                 parts = min(-(-T // per), 512) * per
                 assert 3 * parts * H * 4 <= lib.mt_norm_backward_workspace_bytes(T, H)
+
+
+BIG = 2 ** 63 - 1
+
+
+def test_queries_of_what_no_call_takes():
+    """No arithmetic on sizes that the calls refuse: 0 bytes."""
+    lib = _lib.load()
+    for kw in (dict(heads=BIG), dict(heads=2 ** 40, kv_heads=1), dict(T=BIG), dict(S=BIG), dict(head_dim=BIG),
+               dict(kv_heads=BIG), dict(kv_heads=8), dict(T=-BIG), dict(heads=-4)):
+        assert lib.mt_attn_backward_workspace_bytes(ctypes.byref(attn(**kw))) == 0
+        assert lib.mt_attn_backward(ctypes.byref(attn(**kw)), P, 1 << 40, None) in (1, 3)
+    for stride in ("q_h", "k_h", "v_h"):  # addresses in 64 bits
+        assert lib.mt_attn_forward(ctypes.byref(attn(**{stride: 2 ** 41})), None) == 3
+    assert lib.mt_norm_backward_workspace_bytes(BIG, 64) == 0
+    for bad in ([BIG, BIG], [8, -BIG], [2 ** 40 + 1]):
+        table = (ctypes.c_int64 * len(bad))(*bad)
+        assert lib.mt_grad_norm_workspace_bytes(table, len(bad)) == 0
+    assert lib.mt_grad_norm_workspace_bytes((ctypes.c_int64 * 2)(2 ** 40, 2 ** 40), 2) > 0
