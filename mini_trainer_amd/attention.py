@@ -187,7 +187,8 @@ def packed_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     prefixes is then built and validated, which synchronises once).  Scores are
     scale * q . k (default 1 / sqrt(D)), and softcap * tanh(score / softcap) with
     a softcap.  bf16 or fp32; scores, softmax and sums are computed in fp32, the
-    probabilities rounded to the inputs' type for the product with value.  No
+    probabilities, and in the gradients the scores' gradients, rounded to the
+    inputs' type for their products.  No
     value of another document, nor of a row behind the last one, enters a
     result; within a document NaN or infinite values reach, as 0 * NaN does, the
     rows whose mask hides them.  D is at most 128; strides are free as long as

@@ -747,11 +747,11 @@ constexpr int kAttnKeys = 64;  // keys per block of the forward and of dQ
 // Long rows are bound by the matrix instructions at the clock that the power limit
 // leaves, and by the LDS behind them (an instruction's left operand is 1 KiB, four
 // SIMDs ask for 128 bytes a cycle, all the LDS has): one document of 32768 tokens,
-// 32 heads of 128, 7.7 ms, 1140 TFLOP/s, where a large matrix product reaches
-// 1254.  A softcap adds two transcendentals per score to the exponential (16384
-// tokens: 2.0 -> 2.5 ms, MFMA busy 63% -> 43%).  Short documents are bound by each
-// workgroup's first tile, masks and last partial tile: 4096 tokens of 12 documents
-// 43 us.  Row tiles of 128 with two workgroups on a CU: a wave alone on its SIMD
+// 32 heads of 128, 7.5 to 8.4 ms from box to box, 1050 to 1170 TFLOP/s, 0.88 of what a
+// large matrix product reaches there.  A softcap adds two transcendentals per score to
+// the exponential (16384 tokens: 2.1 -> 2.7 ms, MFMA busy 43%).  Short documents are
+// bound by each workgroup's first tile, masks and last partial tile: 4096 tokens of 12
+// documents 45 us.  Row tiles of 128 with two workgroups on a CU: a wave alone on its SIMD
 // with twice the rows hides neither the LDS nor the softmax (dK and dV below).
 template <class T, int DP, int CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_fwd_kernel(AttnArgs a) {
@@ -901,7 +901,8 @@ __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_f
 // comes from the rows' own dO and O, once.  dQ has a kernel of its own, and the
 // scores and dP are formed again for dK and dV: adding dQ from a kernel of the keys
 // would take atomics, whose order changes results, or a copy of dQ per key tile.
-// 16384 tokens, 32 heads of 128: 2.7 ms, 1240 TFLOP/s; with a softcap 3.35.
+// 16384 tokens, 32 heads of 128: 2.8 to 2.9 ms from box to box, 1140 to 1190 TFLOP/s;
+// with a softcap 3.6.
 template <class T, int DP, int CAP, int SPLIT>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dq_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;
@@ -1051,8 +1052,9 @@ constexpr int attn_q_rows() {
 // keys' K rows 32; their V rows stay in LDS, because with them in registers too a
 // wave needs more than the 256 that let two share a SIMD, and a wave alone hides
 // neither the LDS reads nor the softmax.  One document of 16384 tokens, 32 heads
-// of 128 (8 key heads): 4.1 ms, 1075 TFLOP/s; with V in registers 7.4 ms; as two
-// kinds of workgroup, dK and dV each with their own scores, 5.5 ms.
+// of 128 (8 key heads): 4.2 to 4.3 ms from box to box, 1020 to 1050 TFLOP/s; where it
+// took 4.1, 7.4 with V in registers and 5.5 as two kinds of workgroup, dK and dV each
+// with their own scores.
 template <class T, int DP, int CAP>
 __global__ __launch_bounds__(kAttnThreads, (sizeof(T) == 2 ? 2 : 1)) void attn_dkdv_kernel(AttnArgs a) {
   typedef AttnLds<T, DP> L;

@@ -122,8 +122,9 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     (weight_offset = 1 for weights stored as differences from 1); gate is [H], or
     x's shape with a last dimension of 1 (one number per token), or x's shape.
     All tensors are bf16, or all fp32; everything is computed in fp32 and rounded
-    once (normed comes from the unrounded sum), weight gradients are summed in
-    fp32 in a fixed order.  H is at most 32768.
+    once (normed comes from the unrounded sum, the gradients from new_residual as
+    it was rounded), weight gradients are summed in fp32 in a fixed order.  H is at
+    most 32768.
     """
     dtype, dev = x.dtype, x.device
     for name, t in (("x", x), ("residual", residual), ("weight", weight),
