@@ -42,17 +42,20 @@ _unlabelled = contextvars.ContextVar("mt_unlabelled", default=False)
 
 
 @contextlib.contextmanager
-def _set(var):
-    token = var.set(True)
+def _set(var, value=True):
+    token = var.set(value)
     try:
         yield
     finally:
         var.reset(token)
 
 
+@contextlib.contextmanager
 def unlabelled_forward():
-    """A context in which a patched decoder runs as it was."""
-    return _set(_unlabelled)
+    """A context in which a patched decoder runs as it was, within another's labelled
+    forward too."""
+    with _set(_packed, False), _set(_unlabelled):
+        yield
 
 
 class AttentionPlans:

@@ -265,7 +265,7 @@ def test_labelled_checkpointed_step(operators, reentrant):
 
 @torch.no_grad()
 def test_labelled_and_unlabelled_forwards_in_two_threads(operators):
-    """Each goes by its own attention, whichever runs within the other's time."""
+    """Each goes by its own attention, whichever runs within the other."""
     model, kw = build("llama"), batch()
     docs, logits = alone(model, kw["input_ids"]), model(input_ids=kw["input_ids"]).logits
     patch_causal_lm(model, packed_layers=True)
@@ -284,11 +284,18 @@ def test_labelled_and_unlabelled_forwards_in_two_threads(operators):
                 thread.start()
                 thread.join()
 
-        hook = model.model.layers[0].self_attn.register_forward_pre_hook(other)
-        got[outer] = calls[outer]()
-        hook.remove()
-        assert rel(got["labelled"], docs) <= TOL
-        assert torch.equal(got["unlabelled"], logits)
+        def here(*_):
+            if not entered:
+                entered.append(True)
+                got[inner] = calls[inner]()
+
+        for hook in (other, here):  # in another thread, and within the same one
+            del entered[:]
+            handle = model.model.layers[0].self_attn.register_forward_pre_hook(hook)
+            got[outer] = calls[outer]()
+            handle.remove()
+            assert rel(got["labelled"], docs) <= TOL
+            assert torch.equal(got["unlabelled"], logits)
 
 
 @torch.no_grad()
