@@ -53,8 +53,9 @@ def test_scores_of_the_types_whole_range(gpu, dtype, heads):
 @pytest.mark.parametrize("heads", [HALF, WHOLE])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("half", [0, 3, 8, 12, 25, 50])
-def test_equal_scores_of_any_size(gpu, dtype, half, heads):
-    """All scores of a row the same, -2^(2 half + 6): its n probabilities are 1 / n each in
+@pytest.mark.parametrize("D", [64, 128])
+def test_equal_scores_of_any_size(gpu, D, dtype, half, heads):
+    """All scores of a row the same, -D 2^(2 half): its n probabilities are 1 / n each in
     the forward and in the gradients, however little room the size of the scores leaves
     for the logarithm of n in an fp32 log-sum.  Scores are exact here, so that the errors
     are, with u = eps / 2 of the type and F = 2^-24:
@@ -63,7 +64,7 @@ def test_equal_scores_of_any_size(gpu, dtype, half, heads):
       out            u |out| + theirs times mean |v|;
       delta          theirs and 2^-16 (what is kept of bf16's out) of |dO| |out|, summed;
       dS             up + the probabilities' of itself, plus p times those of delta and dP."""
-    D, lengths = 64, [1, 2, 3, 57, 7]
+    lengths = [1, 2, 3, 57, 7]
     T = sum(lengths)
     g = torch.Generator().manual_seed(3)
     v, do = (torch.randn(T, heads, D, generator=g).to(dtype).to(gpu) for _ in range(2))
@@ -77,7 +78,7 @@ def test_equal_scores_of_any_size(gpu, dtype, half, heads):
     mask = ref.seen_mask(lengths, T).double()
     n = mask.sum(1, keepdim=True)
     p = mask / n
-    lse = 2.0 ** (2 * half + 6) * 1.4427
+    lse = D * 2.0 ** (2 * half) * 1.4427
     rel_o = up + (n + C) * F
     rel_p = rel_o + (F * lse if lse < 8192 else 0.0)
     for h in (0, heads - 1):
