@@ -56,7 +56,7 @@
 extern "C" {
 #endif
 
-#define MT_FLCE_ABI_VERSION 10
+#define MT_FLCE_ABI_VERSION 11
 
 typedef struct ihipStream_t* mt_stream_t; /* == hipStream_t */
 
@@ -708,6 +708,71 @@ int mt_grad_norm(void* const* ptrs, const int64_t* numel, const int64_t* cols,
 int mt_grad_scale(void* const* ptrs, const int64_t* numel, const int64_t* cols,
                   const int64_t* pitch, const int32_t* dtypes, int64_t n,
                   const float* norm_and_coef, mt_stream_t stream);
+
+/*
+ * The token embedding (what a decoder begins with; the reference leaves it to the
+ * model library):
+ *   out[t] = scale weight[ids[t]], computed in fp32 and rounded once
+ *   ids     int32 or int64 [T] (ids_bytes 4 or 8)
+ *   weight  [V, H] with row pitch weight_t (elements);  out [T, H] contiguous
+ *   status  int32 [1] (device, set to 0 by the caller; null: not wanted): set to 1
+ *           if some id lies outside [0, V).  Such a token's row is NaN, and it adds
+ *           nothing to the gradient.
+ * The backward writes every row of dweight [V, H] (dtype; row pitch dweight_t), the sum
+ * of scale dout[t] (row pitch dout_t) over the tokens of that id, rounded once, or with
+ * accumulate != 0 adds these sums to an fp32 dweight, whose rows of ids that do not
+ * occur it leaves as they are.  The row padding_idx (-1: none) gets no gradient.  Sums in
+ * fp32 in a fixed order.  It reads ids and dout; H at most 2^24.
+ */
+typedef struct mt_embed_args {
+  const void *ids, *weight;
+  void* out;
+  const void* dout;
+  void* dweight;
+  int32_t* status;
+  int64_t weight_t, dout_t, dweight_t, T, V, H, padding_idx;
+  float scale;
+  int dtype, ids_bytes, accumulate;
+} mt_embed_args;
+
+int mt_embed_forward(const mt_embed_args* args, mt_stream_t stream);
+size_t mt_embed_backward_workspace_bytes(int64_t T, int64_t V, int64_t H);
+int mt_embed_backward(const mt_embed_args* args, void* workspace, size_t workspace_bytes,
+                      mt_stream_t stream);
+
+/*
+ * Layer norm, of x or of a block's output added to the residual (what decoders without
+ * RMS norms have in the place of mt_norm_*):
+ *   new_residual = residual_scale residual + block_scale x   (h; with has_residual)
+ *   normed = (h - mean(h)) / sqrt(var(h) + eps) weight + bias  (h = x without)
+ * computed in fp32 and rounded once; var is the mean square of the centred row.
+ *   x, residual [T, H] with row pitches x_t, residual_t (elements); weight (null:
+ *     ones), bias (null: zeros) [H]; normed, new_residual [T, H] contiguous
+ *   residual_lo  [T, H] bytes (bf16 with a residual; 8-byte aligned for the fastest
+ *     kernels): what new_residual's rounding took from it, from the forward to the
+ *     backward (null in a forward without a backward)
+ *   stat fp32 [2, T]: 1 / sqrt(var + eps) and the mean, from the forward to the
+ *     backward (null as above);  H at most 32768;  all tensors of one dtype
+ * The backward takes dnormed and (null: zeros) dresidual_out with row pitches, reads
+ * new_residual, or x without a residual, stat and weight, and writes what is not null of
+ * dx, dresidual [T, H] (contiguous), dweight, dbias [H].
+ */
+typedef struct mt_layer_norm_args {
+  const void *x, *residual, *weight, *bias;
+  void *normed, *new_residual;
+  uint8_t* residual_lo;
+  float* stat;
+  const void *dnormed, *dresidual_out;
+  void *dx, *dresidual, *dweight, *dbias;
+  int64_t x_t, residual_t, dnormed_t, dresidual_out_t, T, H;
+  float eps, block_scale, residual_scale;
+  int has_residual, dtype;
+} mt_layer_norm_args;
+
+int mt_layer_norm_forward(const mt_layer_norm_args* args, mt_stream_t stream);
+size_t mt_layer_norm_backward_workspace_bytes(int64_t T, int64_t H);
+int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size_t workspace_bytes,
+                           mt_stream_t stream);
 
 #ifdef __cplusplus
 }

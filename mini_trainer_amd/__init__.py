@@ -15,6 +15,7 @@ from .causal_lm import (
     patch_causal_lm,
     sample_loss_sums,
 )
+from .embedding import token_embedding
 from .flce import (
     backward_plan,
     path_of,
@@ -28,7 +29,7 @@ from .none_reduction_losses import (
     hf_fixed_cross_entropy_none_reduction,
     liger_fixed_fused_linear_cross_entropy_none_reduction,
 )
-from .norms import residual_rms_norm
+from .norms import layer_norm, residual_layer_norm, residual_rms_norm
 from .utils import patch_target_module
 
 __all__ = [
@@ -51,6 +52,9 @@ __all__ = [
     "packed_attention",
     "packed_attention_plan",
     "residual_rms_norm",
+    "layer_norm",
+    "residual_layer_norm",
+    "token_embedding",
     "clip_grad_norm_",
     "clip_gradients_",
 ]

@@ -15,7 +15,7 @@ import os
 # MT_FLCE_LIB: another build of the same library (the sanitized host-only
 # build of the CPU tests); unset in production.
 LIB_PATH = Path(os.environ.get("MT_FLCE_LIB") or Path(__file__).resolve().parent / "libmt_flce.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 MT_DTYPE_F32 = 0
 MT_DTYPE_BF16 = 1
@@ -51,6 +51,26 @@ class NormArgs(ctypes.Structure):
                 + [("gate_mode", c_int), ("dtype", c_int)])
 
 
+class EmbedArgs(ctypes.Structure):
+    """mt_embed_args of include/mt_flce.h."""
+    _fields_ = ([(n, c_void_p) for n in ("ids", "weight", "out", "dout", "dweight", "status")]
+                + [(n, c_int64) for n in ("weight_t", "dout_t", "dweight_t", "T", "V", "H",
+                                          "padding_idx")]
+                + [("scale", c_float)]
+                + [(n, c_int) for n in ("dtype", "ids_bytes", "accumulate")])
+
+
+class LayerNormArgs(ctypes.Structure):
+    """mt_layer_norm_args of include/mt_flce.h."""
+    _fields_ = ([(n, c_void_p) for n in ("x", "residual", "weight", "bias", "normed", "new_residual",
+                                         "residual_lo", "stat", "dnormed", "dresidual_out", "dx",
+                                         "dresidual", "dweight", "dbias")]
+                + [(n, c_int64) for n in ("x_t", "residual_t", "dnormed_t", "dresidual_out_t", "T",
+                                          "H")]
+                + [(n, c_float) for n in ("eps", "block_scale", "residual_scale")]
+                + [("has_residual", c_int), ("dtype", c_int)])
+
+
 def _packer(args) -> struct.Struct:
     """Writes a whole argument structure at once (its fields in order): 1 us where
     setting them one by one takes 5."""
@@ -60,6 +80,8 @@ def _packer(args) -> struct.Struct:
 
 pack_attn_args = _packer(AttnArgs).pack
 pack_norm_args = _packer(NormArgs).pack
+pack_embed_args = _packer(EmbedArgs).pack
+pack_layer_norm_args = _packer(LayerNormArgs).pack
 
 
 # name -> (restype, argtypes); mirrors include/mt_flce.h
@@ -157,6 +179,12 @@ SIGNATURES = {
     "mt_norm_forward": (c_int, [c_void_p, c_void_p]),
     "mt_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "mt_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mt_embed_forward": (c_int, [c_void_p, c_void_p]),
+    "mt_embed_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "mt_embed_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mt_layer_norm_forward": (c_int, [c_void_p, c_void_p]),
+    "mt_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "mt_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "mt_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int64]),
     "mt_grad_norm": (c_int, [POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64),
                              POINTER(c_int64), POINTER(ctypes.c_int32), c_int64, c_int,

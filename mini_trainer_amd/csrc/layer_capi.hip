@@ -1,0 +1,342 @@
+// C ABI of libmt_flce.so, the operators at the ends of a decoder's layers: token
+// embedding and layer norm.  Declarations and contracts: include/mt_flce.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mt_flce.h"
+#include "capi_common.h"
+#include "layer_embed.h"
+#include "layer_norm.h"
+#include "norm_pick.h"
+
+using namespace mtf;
+
+namespace {
+
+// --- token embedding -------------------------------------------------------------
+
+constexpr int64_t kEmbedMostH = (int64_t)1 << 24;
+constexpr int64_t kEmbedMostPitch = (int64_t)1 << 32;
+
+// 256 buckets, a workgroup for each CU, or as many more as keep a bucket's ids in LDS.
+int embed_log_buckets(int64_t V) {
+  int log = 8;
+  while (cdiv(V, (int64_t)1 << log) > kEmbedSlots) ++log;
+  return log;
+}
+
+struct EmbedLayout {
+  int log_buckets;
+  int64_t per, part_t;
+  size_t order, part, bytes;  // offsets of the parts behind starts, and the whole
+};
+EmbedLayout embed_layout(int64_t T, int64_t V, int64_t H) {
+  EmbedLayout l;
+  l.log_buckets = embed_log_buckets(V);
+  l.per = cdiv(V, (int64_t)1 << l.log_buckets);
+  l.part_t = cdiv(H, 4) * 4;
+  const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+  l.order = up(4 * (((size_t)l.per << l.log_buckets) + 1));
+  l.part = l.order + up(4 * (size_t)T);
+  // (up to kEmbedPiece tokens no row has pieces)
+  l.bytes = l.part + (T > kEmbedPiece ? 2 * (size_t)cdiv(T, kEmbedPiece) * (size_t)l.part_t * 4 : 0);
+  return l;
+}
+
+int embed_check(const mt_embed_args* p, bool backward) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_embed_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.ids_bytes != 4 && a.ids_bytes != 8)
+    return fail(MT_ERR_INVALID_ARGUMENT, "ids of %d bytes: 4 and 8 are supported", a.ids_bytes);
+  if (a.T < 0 || a.T > kMaxRows) return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld out of range", (long long)a.T);
+  if (a.V < 1 || a.V > kMaxRows) return fail(MT_ERR_INVALID_ARGUMENT, "V=%lld out of range", (long long)a.V);
+  if (a.H < 1) return fail(MT_ERR_INVALID_ARGUMENT, "H=%lld out of range", (long long)a.H);
+  if (a.H > kEmbedMostH)
+    return fail(MT_ERR_UNSUPPORTED, "H=%lld is above %lld", (long long)a.H, (long long)kEmbedMostH);
+  if (!std::isfinite(a.scale)) return fail(MT_ERR_INVALID_ARGUMENT, "scale must be finite");
+  if (a.padding_idx < -1 || a.padding_idx >= a.V)
+    return fail(MT_ERR_INVALID_ARGUMENT, "padding_idx=%lld out of range", (long long)a.padding_idx);
+  if ((!backward && a.weight_t < a.H) || (backward && ((a.T > 0 && a.dout_t < a.H) || a.dweight_t < a.H)))
+    return fail(MT_ERR_INVALID_ARGUMENT, "row pitches must be >= H");
+  if ((!backward && a.weight_t > kEmbedMostPitch) ||
+      (backward && ((a.T > 0 && a.dout_t > kEmbedMostPitch) || a.dweight_t > kEmbedMostPitch)))
+    return fail(MT_ERR_UNSUPPORTED, "rows more than 2^32 elements apart");
+  if ((a.T > 0 && !a.ids) || (!backward && a.T > 0 && (!a.weight || !a.out)) ||
+      (backward && ((a.T > 0 && !a.dout) || !a.dweight)))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  const int des = a.accumulate ? 4 : es;
+  if (reinterpret_cast<uintptr_t>(a.ids) % a.ids_bytes || reinterpret_cast<uintptr_t>(a.weight) % es ||
+      reinterpret_cast<uintptr_t>(a.out) % es || reinterpret_cast<uintptr_t>(a.dout) % es ||
+      reinterpret_cast<uintptr_t>(a.dweight) % des || reinterpret_cast<uintptr_t>(a.status) % 4)
+    return fail(MT_ERR_INVALID_ARGUMENT, "tensors must be aligned to their element size");
+  return MT_OK;
+}
+
+EmbedArgs embed_args(const mt_embed_args& a) {
+  EmbedArgs k{};
+  k.ids = a.ids;
+  k.w = static_cast<const char*>(a.weight);
+  k.dout = static_cast<const char*>(a.dout);
+  k.out = static_cast<char*>(a.out);
+  k.dw = static_cast<char*>(a.dweight);
+  k.status = a.status;
+  k.w_t = a.weight_t, k.dout_t = a.dout_t, k.dw_t = a.dweight_t;
+  k.padding = a.padding_idx;
+  k.T = (int32_t)a.T, k.V = (int32_t)a.V, k.H = (int32_t)a.H;
+  k.scale = a.scale;
+  return k;
+}
+
+// Calls f(V, K, log2 of the lanes of a row, workgroups) with the variant for `rows`
+// rows of H elements: most vectors in flight per lane (up to kmost) that a row fills.
+template <class T, int kMost, class F>
+int embed_pick(int64_t rows, int64_t H, bool vec, F f) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int64_t nv = vec ? H / W : H;
+  int log_lanes = 6;
+  while (log_lanes > 0 && nv <= (int64_t)1 << (log_lanes - 1)) --log_lanes;
+  const auto with = [&](auto V, auto K) {
+    const int64_t chunks = log_lanes == 6 ? cdiv(nv, 64 * decltype(K)::value) : 1;
+    const int64_t units = cdiv(rows, 64 >> log_lanes) * chunks;
+    if (cdiv(units, 4) * 256 >= (int64_t)1 << 32)  // threads of a launch
+      return fail(MT_ERR_UNSUPPORTED, "%lld rows of %lld exceed one launch", (long long)rows, (long long)H);
+    return f(V, K, log_lanes, (uint32_t)cdiv(units, 4));
+  };
+  const auto wide = [&](auto V) {
+    if constexpr (kMost >= 4) {
+      if (nv > 128) return with(V, std::integral_constant<int, 4>());
+    }
+    if (nv > 64) return with(V, std::integral_constant<int, 2>());
+    return with(V, std::integral_constant<int, 1>());
+  };
+  return vec ? wide(std::integral_constant<int, W>()) : wide(std::integral_constant<int, 1>());
+}
+
+template <class T, class I>
+int launch_embed_forward(const EmbedArgs& k, hipStream_t stream) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const bool vec = k.H % W == 0 && k.w_t % W == 0 && aligned16(k.w) && aligned16(k.out);
+  return embed_pick<T, 4>(k.T, k.H, vec, [&](auto V, auto K, int log_lanes, uint32_t groups) {
+    hipLaunchKernelGGL((embed_forward_kernel<T, I, decltype(V)::value, decltype(K)::value>), dim3(groups),
+                       dim3(256), 0, stream, k, log_lanes);
+    return check_launch("embed_forward_kernel");
+  });
+}
+
+template <class T, class I>
+int launch_embed_backward(const EmbedArgs& k, bool accumulate, hipStream_t stream) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const bool vec = k.H % W == 0 && k.dout_t % W == 0 && k.dw_t % (accumulate ? 4 : W) == 0 &&
+                   aligned16(k.dout) && aligned16(k.dw);
+  hipLaunchKernelGGL(embed_sort_kernel<I>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
+  MT_TRY(check_launch("embed_sort_kernel"));
+  if (k.T > kEmbedPiece)
+    MT_TRY((embed_pick<T, 2>(cdiv(k.T, kEmbedPiece), k.H, vec,
+                             [&](auto V, auto K, int log_lanes, uint32_t groups) {
+      hipLaunchKernelGGL((embed_pieces_kernel<T, I, decltype(V)::value, decltype(K)::value>), dim3(groups),
+                         dim3(256), 0, stream, k, log_lanes);
+      return check_launch("embed_pieces_kernel");
+    })));
+  if (accumulate && k.T == 0) return MT_OK;
+  return embed_pick<T, 2>(accumulate ? k.T : k.V, k.H, vec,
+                          [&](auto V, auto K, int log_lanes, uint32_t groups) {
+    constexpr int v = decltype(V)::value, n = decltype(K)::value;
+    if (accumulate)
+      hipLaunchKernelGGL((embed_rows_kernel<T, I, v, n, true>), dim3(groups), dim3(256), 0, stream, k, log_lanes);
+    else
+      hipLaunchKernelGGL((embed_rows_kernel<T, I, v, n, false>), dim3(groups), dim3(256), 0, stream, k, log_lanes);
+    return check_launch("embed_rows_kernel");
+  });
+}
+
+// --- layer norm --------------------------------------------------------------------
+
+int layer_norm_check(const mt_layer_norm_args* p, bool backward) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_layer_norm_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.T < 0 || a.T > kMaxRows) return fail(MT_ERR_INVALID_ARGUMENT, "T=%lld out of range", (long long)a.T);
+  if (a.H <= 0) return fail(MT_ERR_INVALID_ARGUMENT, "H=%lld out of range", (long long)a.H);
+  if (a.H > kNormMaxH)
+    return fail(MT_ERR_UNSUPPORTED, "H=%lld is above %lld", (long long)a.H, (long long)kNormMaxH);
+  if (!(a.eps >= 0.f) || !std::isfinite(a.eps) || !std::isfinite(a.block_scale) ||
+      !std::isfinite(a.residual_scale))
+    return fail(MT_ERR_INVALID_ARGUMENT, "eps must be >= 0 and the scales finite");
+  const bool res = a.has_residual != 0;
+  if ((!(backward && res) && a.x_t < a.H) || (!backward && res && a.residual_t < a.H) ||
+      (backward && (a.dnormed_t < a.H || (a.dresidual_out && a.dresidual_out_t < a.H))))
+    return fail(MT_ERR_INVALID_ARGUMENT, "row pitches must be >= H");
+  if (a.T == 0) return MT_OK;
+  if ((!backward && (!a.x || !a.normed || (res && (!a.residual || !a.new_residual)))) ||
+      (backward && (!a.dnormed || !a.stat || (res ? !a.new_residual : !a.x) ||
+                    (res && a.dtype == MT_DTYPE_BF16 && !a.residual_lo))))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (!res && (a.dresidual || a.dresidual_out))
+    return fail(MT_ERR_INVALID_ARGUMENT, "gradients of a residual that there is not");
+  const void* all[] = {a.x, a.residual, a.weight, a.bias, a.normed, a.new_residual,
+                       a.dnormed, a.dresidual_out, a.dx, a.dresidual, a.dweight, a.dbias};
+  for (const void* x : all)
+    if (reinterpret_cast<uintptr_t>(x) % es != 0)
+      return fail(MT_ERR_INVALID_ARGUMENT, "tensors must be aligned to their element size");
+  if (reinterpret_cast<uintptr_t>(a.stat) % 4)
+    return fail(MT_ERR_INVALID_ARGUMENT, "stat must be aligned to 4 bytes");
+  return MT_OK;
+}
+
+// Whether every row of every tensor is whole aligned 16-byte vectors.
+bool layer_norm_vectors(const mt_layer_norm_args& a, bool backward) {
+  const int64_t V = 16 / esize(a.dtype);
+  const bool res = a.has_residual != 0;
+  const void* all[] = {a.x, a.residual, a.weight, a.bias, a.normed, a.new_residual,
+                       a.dnormed, a.dresidual_out, a.dx, a.dresidual};
+  for (const void* x : all)
+    if (!aligned16(x)) return false;
+  if (reinterpret_cast<uintptr_t>(a.residual_lo) % 8) return false;
+  return a.H % V == 0 && ((backward && res) || a.x_t % V == 0) && (backward || !res || a.residual_t % V == 0) &&
+         (!backward || (a.dnormed_t % V == 0 && (!a.dresidual_out || a.dresidual_out_t % V == 0)));
+}
+
+LayerNormArgs layer_norm_args(const mt_layer_norm_args& a, bool backward) {
+  const bool res = a.has_residual != 0;
+  LayerNormArgs k{};
+  k.x = static_cast<const char*>(a.x);
+  k.residual = static_cast<const char*>(a.residual);
+  k.w = static_cast<const char*>(a.weight);
+  k.b = static_cast<const char*>(a.bias);
+  k.dy = static_cast<const char*>(a.dnormed);
+  k.dh = static_cast<const char*>(a.dresidual_out);
+  k.h = res ? static_cast<const char*>(a.new_residual) : k.x;
+  k.y = static_cast<char*>(a.normed);
+  k.h_out = backward ? nullptr : static_cast<char*>(a.new_residual);
+  k.dx = static_cast<char*>(a.dx);
+  k.dresidual = static_cast<char*>(a.dresidual);
+  k.lo = a.residual_lo;
+  k.stat = a.stat;
+  k.x_t = a.x_t, k.r_t = a.residual_t, k.dy_t = a.dnormed_t, k.dh_t = a.dresidual_out_t;
+  k.h_t = res ? a.H : a.x_t;
+  k.T = a.T;
+  k.H = (int32_t)a.H;
+  k.eps = a.eps;
+  k.block_scale = a.block_scale;
+  k.residual_scale = a.residual_scale;
+  return k;
+}
+
+template <class T>
+int launch_layer_norm_fwd(const LayerNormArgs& k, bool res, bool vec, hipStream_t stream) {
+  return norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+    constexpr int threads = norm_threads(decltype(TPR)::value);
+    constexpr int rows = threads / decltype(TPR)::value;
+    if (cdiv(k.T, rows) * threads >= (int64_t)1 << 32)  // threads of a launch
+      return fail(MT_ERR_UNSUPPORTED, "%lld rows of %d exceed one launch", (long long)k.T, k.H);
+    auto kern = res ? layer_norm_fwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, true>
+                    : layer_norm_fwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, false>;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)cdiv(k.T, rows)), dim3(threads), 0, stream, k);
+    return check_launch("layer_norm_fwd_kernel");
+  });
+}
+
+template <class T>
+int launch_layer_norm_bwd(LayerNormArgs k, const mt_layer_norm_args& a, bool res, bool vec,
+                          hipStream_t stream) {
+  MT_TRY(norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+    constexpr int threads = norm_threads(decltype(TPR)::value);
+    constexpr int rows = threads / decltype(TPR)::value;
+    const int64_t groups = std::min<int64_t>(cdiv(k.T, rows), kNormGroups);
+    k.parts = (int32_t)(groups * rows);
+    if (k.parts > norm_parts(k.T, k.H))  // (the workspace's partial rows)
+      return fail(MT_ERR_UNSUPPORTED, "%d partial rows", (int)k.parts);
+    auto kern = res ? layer_norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, true>
+                    : layer_norm_bwd_kernel<T, decltype(V)::value, decltype(K)::value, decltype(TPR)::value, false>;
+    hipLaunchKernelGGL(kern, dim3((uint32_t)groups), dim3(threads), 0, stream, k);
+    return check_launch("layer_norm_bwd_kernel");
+  }));
+  if (!a.dweight && !a.dbias) return MT_OK;
+  hipLaunchKernelGGL((norm_columns_kernel<T>), dim3((uint32_t)cdiv(k.H, 64), a.dbias ? 2 : 1), dim3(1024), 0,
+                     stream, k.part, k.parts, k.H, static_cast<T*>(a.dweight), static_cast<T*>(a.dbias),
+                     static_cast<T*>(nullptr));
+  return check_launch("norm_columns_kernel");
+}
+
+}  // namespace
+
+extern "C" {
+
+int mt_embed_forward(const mt_embed_args* args, mt_stream_t stream) {
+  MT_TRY(embed_check(args, false));
+  const mt_embed_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const EmbedArgs k = embed_args(a);
+  hipStream_t s = (hipStream_t)stream;
+  if (a.dtype == MT_DTYPE_BF16)
+    return a.ids_bytes == 8 ? launch_embed_forward<__bf16, int64_t>(k, s) : launch_embed_forward<__bf16, int32_t>(k, s);
+  return a.ids_bytes == 8 ? launch_embed_forward<float, int64_t>(k, s) : launch_embed_forward<float, int32_t>(k, s);
+}
+
+size_t mt_embed_backward_workspace_bytes(int64_t T, int64_t V, int64_t H) {
+  return T < 0 || T > kMaxRows || V < 1 || V > kMaxRows || H < 1 || H > kEmbedMostH ? 0
+                                                                                   : embed_layout(T, V, H).bytes;
+}
+
+int mt_embed_backward(const mt_embed_args* args, void* workspace, size_t workspace_bytes, mt_stream_t stream) {
+  MT_TRY(embed_check(args, true));
+  const mt_embed_args& a = *args;
+  if (!workspace || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
+  const EmbedLayout l = embed_layout(a.T, a.V, a.H);
+  if (workspace_bytes < l.bytes)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, l.bytes);
+  EmbedArgs k = embed_args(a);
+  char* ws = static_cast<char*>(workspace);
+  k.starts = reinterpret_cast<int32_t*>(ws);
+  k.order = reinterpret_cast<int32_t*>(ws + l.order);
+  k.part = reinterpret_cast<float*>(ws + l.part);
+  k.part_t = l.part_t;
+  k.log_buckets = l.log_buckets;
+  k.per = (int32_t)l.per;
+  hipStream_t s = (hipStream_t)stream;
+  const bool acc = a.accumulate != 0;
+  if (a.dtype == MT_DTYPE_BF16)
+    return a.ids_bytes == 8 ? launch_embed_backward<__bf16, int64_t>(k, acc, s)
+                            : launch_embed_backward<__bf16, int32_t>(k, acc, s);
+  return a.ids_bytes == 8 ? launch_embed_backward<float, int64_t>(k, acc, s)
+                          : launch_embed_backward<float, int32_t>(k, acc, s);
+}
+
+int mt_layer_norm_forward(const mt_layer_norm_args* args, mt_stream_t stream) {
+  MT_TRY(layer_norm_check(args, false));
+  const mt_layer_norm_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const LayerNormArgs k = layer_norm_args(a, false);
+  const bool res = a.has_residual != 0, vec = layer_norm_vectors(a, false);
+  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_fwd<__bf16>(k, res, vec, (hipStream_t)stream)
+                                  : launch_layer_norm_fwd<float>(k, res, vec, (hipStream_t)stream);
+}
+
+size_t mt_layer_norm_backward_workspace_bytes(int64_t T, int64_t H) {
+  return T <= 0 || T > kMaxRows || H <= 0 || H > kNormMaxH ? 0 : (size_t)2 * norm_parts(T, H) * (size_t)H * 4;
+}
+
+int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size_t workspace_bytes,
+                           mt_stream_t stream) {
+  MT_TRY(layer_norm_check(args, true));
+  const mt_layer_norm_args& a = *args;
+  if (a.T == 0) return MT_OK;
+  const size_t need = mt_layer_norm_backward_workspace_bytes(a.T, a.H);
+  if (!workspace || !aligned16(workspace))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
+  if (workspace_bytes < need)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
+  LayerNormArgs k = layer_norm_args(a, true);
+  k.part = static_cast<float*>(workspace);
+  const bool res = a.has_residual != 0, vec = layer_norm_vectors(a, true);
+  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_bwd<__bf16>(k, a, res, vec, (hipStream_t)stream)
+                                  : launch_layer_norm_bwd<float>(k, a, res, vec, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,10 +1,11 @@
-"""Residual and RMS norms between two blocks of a decoder, in one pass.
+"""Residual and norms between two blocks of a decoder, in one pass.
 
 A decoder layer of the models the reference trains adds a block's output to the
 residual and normalises the sum for the next block (the norm that
 setup_model_for_training.py:98-99 replaces); some normalise the block's output
-first, gate it, or scale it or the residual.  There is no CPU or eager-PyTorch
-fallback: non-device tensors or a missing library raise.
+first, gate it, or scale it or the residual.  Others have layer norms in the place of
+RMS norms.  There is no CPU or eager-PyTorch fallback: non-device tensors or a missing
+library raise.
 """
 from __future__ import annotations
 
@@ -13,10 +14,10 @@ from typing import Optional, Tuple
 
 import torch
 
-from ._lib import load, pack_norm_args
+from ._lib import load, pack_layer_norm_args, pack_norm_args
 from .flce import _backward_once, _dtype_code, _launch, _require_device
 
-__all__ = ["residual_rms_norm"]
+__all__ = ["layer_norm", "residual_layer_norm", "residual_rms_norm"]
 
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_ELEMENT = range(4)
 
@@ -161,3 +162,128 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
                              f"{tuple(x.shape)}, got {tuple(gate.shape)}")
     return _ResidualRmsNorm.apply(x, residual, weight, post_weight, gate, mode, float(eps),
                                   float(block_scale), float(residual_scale), float(weight_offset))
+
+
+class _LayerNorm(torch.autograd.Function):
+    """normed, or with a residual (normed, new_residual)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, block_scale, residual_scale, differentiable):
+        dev, shape = x.device, x.shape
+        H = shape[-1]
+        ctx.set_materialize_grads(False)
+        x2 = _rows(x)
+        r2 = None if residual is None else _rows(residual)
+        w = None if weight is None else weight.contiguous()
+        b = None if bias is None else bias.contiguous()
+        T = x2.shape[0]
+        normed = x.new_empty(shape)
+        h = None if r2 is None else x.new_empty(shape)
+        stat = low = None
+        if differentiable:  # (needs_input_grad does not say whether gradients are recorded)
+            stat = torch.empty((2, T), dtype=torch.float32, device=dev)
+            if h is not None and x.dtype == torch.bfloat16:
+                low = torch.empty((T, H), dtype=torch.uint8, device=dev)
+        tail = (eps, block_scale, residual_scale, int(h is not None), _dtype_code(x.dtype))
+        args = pack_layer_norm_args(x2.data_ptr(), _at(r2), _at(w), _at(b), normed.data_ptr(), _at(h),
+                                    _at(low), _at(stat), 0, 0, 0, 0, 0, 0, _pitch(x2),
+                                    0 if r2 is None else _pitch(r2), 0, 0, T, H, *tail)
+        _launch(dev, "mt_layer_norm_forward", load().mt_layer_norm_forward, args)
+        ctx.save_for_backward(x2 if h is None else h, w, low, stat)
+        ctx.meta = (T, H, shape, tail)
+        return normed if h is None else (normed, h)
+
+    @_backward_once
+    def backward(ctx, dnormed, dnew=None):
+        if dnormed is None and dnew is None:
+            return (None,) * 8
+        h, w, low, stat = ctx.saved_tensors
+        T, H, shape, tail = ctx.meta
+        _, block_scale, residual_scale, has_residual, _ = tail
+        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
+        dev = h.device
+        dn = _rows(torch.zeros(shape, dtype=h.dtype, device=dev) if dnormed is None else dnormed)
+        dh = None if dnew is None else _rows(dnew)
+        # where both are the same number the two inputs share one gradient, as an
+        # addition's do
+        same = need_x and need_r and block_scale == residual_scale
+        new = h.new_empty
+        dr = new(shape) if need_r else None
+        dx = new(shape) if need_x and not same else None
+        dw = new((H,)) if need_w else None
+        db = new((H,)) if need_b else None
+        args = pack_layer_norm_args(0 if has_residual else h.data_ptr(), 0, _at(w), 0, 0,
+                                    h.data_ptr() if has_residual else 0, _at(low), _at(stat),
+                                    dn.data_ptr(), _at(dh), _at(dx), _at(dr), _at(dw), _at(db),
+                                    H if has_residual else _pitch(h), 0, _pitch(dn),
+                                    H if dh is None else _pitch(dh), T, H, *tail)
+        lib = load()
+        nbytes = lib.mt_layer_norm_backward_workspace_bytes(T, H)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _launch(dev, "mt_layer_norm_backward", lib.mt_layer_norm_backward, args, ws.data_ptr(), nbytes)
+        if T == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+        return (dr if same else dx), dr, dw, db, None, None, None, None
+
+
+def _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale):
+    dtype, dev = x.dtype, x.device
+    grad = False
+    for name, t in (("x", x), ("residual", residual), ("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _require_device(name, t)
+        if t.dtype != dtype:
+            raise TypeError(f"{name} ({t.dtype}) and x ({dtype}) must have the same dtype")
+        if t.device != dev:
+            raise ValueError(f"{name} lies on {t.device}, x on {dev}")
+        grad = grad or t.requires_grad
+    _dtype_code(dtype)
+    if x.dim() < 1:
+        raise ValueError("x must be [..., H]")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"x {tuple(x.shape)} and residual {tuple(residual.shape)} must have one shape")
+    H = x.shape[-1]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.shape != (H,):
+            raise ValueError(f"{name} must be [{H}], got {tuple(t.shape)}")
+    if not 1 <= H <= 32768:
+        raise ValueError(f"hidden size {H}: 1 to 32768 are supported")
+    if not (eps >= 0 and math.isfinite(eps + block_scale + residual_scale)):
+        raise ValueError("eps must be >= 0, and it, block_scale and residual_scale finite")
+    return _LayerNorm.apply(x, residual, weight, bias, float(eps), float(block_scale),
+                            float(residual_scale), grad and torch.is_grad_enabled())
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """(x - mean(x)) / sqrt(var(x) + eps) * weight + bias over the last dimension of
+    x [..., H], differentiable in every tensor; weight and bias [H], or None for ones and
+    zeros.
+
+    All tensors are bf16, or all fp32; everything is computed in fp32 and rounded once,
+    var is the mean square of the centred row, and weight gradients are summed in fp32
+    in a fixed order.  H is at most 32768.
+    """
+    return _layer_norm(x, None, weight, bias, eps, 1.0, 1.0)
+
+
+def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor,
+                        weight: Optional[torch.Tensor] = None,
+                        bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                        block_scale: float = 1.0,
+                        residual_scale: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(normed, new_residual) of a block's output x [..., H] and the residual before it:
+
+        new_residual = residual_scale * residual + block_scale * x
+        normed       = layer_norm(new_residual, weight, bias, eps)
+
+    differentiable in every tensor, with layer_norm's types and rounding: normed comes
+    from the unrounded sum.  In bf16 a call whose gradients are recorded keeps 8 bits of
+    new_residual beyond its rounding (a byte per element) for them.
+    """
+    if residual is None:
+        raise ValueError("residual_layer_norm needs a residual")
+    return _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale)
