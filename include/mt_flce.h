@@ -774,6 +774,37 @@ size_t mt_layer_norm_backward_workspace_bytes(int64_t T, int64_t H);
 int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size_t workspace_bytes,
                            mt_stream_t stream);
 
+/*
+ * The orthogonalised update of weight matrices (of the momentum, between the clip at
+ * train.py:24 and the step; the reference's optimizer has none):
+ *   X = G / (|G| + eps),  steps times  X <- a X + (b A + c A^2) X,  A = X X^T
+ * for each of batch matrices G [m, n] (X its transpose where m > n), |G| the square root
+ * of the sum of squares.
+ *   in   rows of unit stride, in_row elements apart, matrices in_batch apart (0: the same
+ *        matrix again);  out [batch, m, n] contiguous;  both of one dtype
+ *   coefficients  a, b, c of each step (host, 3 steps doubles, read during the call);
+ *        such that singular values of at most 1 stay below 10^6 (MT_ERR_UNSUPPORTED)
+ *   eps >= 0;  steps 1 to 64
+ * bf16 matrices go through fp16 products, fp32 ones through three of split values (with
+ * the relative error of fp32 products); X is carried in fp32 and rounded once at the end.
+ * A matrix that holds NaN or infinities gives NaN; a zero matrix gives zeros (eps > 0).
+ * The workspace (256-byte aligned) must hold one matrix's part; the query's size, up to
+ * 2 GiB or one matrix, takes a stack together.  A matrix in fp16 must stay below 2 GiB
+ * (either side padded to whole 64).
+ */
+typedef struct mt_orthogonalize_args {
+  const void* in;
+  void* out;
+  const double* coefficients;
+  double eps;
+  int64_t batch, m, n, in_row, in_batch;
+  int steps, dtype;
+} mt_orthogonalize_args;
+
+size_t mt_orthogonalize_workspace_bytes(const mt_orthogonalize_args* args);
+int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

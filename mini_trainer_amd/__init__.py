@@ -30,6 +30,7 @@ from .none_reduction_losses import (
     liger_fixed_fused_linear_cross_entropy_none_reduction,
 )
 from .norms import layer_norm, residual_layer_norm, residual_rms_norm
+from .update import orthogonalize
 from .utils import patch_target_module
 
 __all__ = [
@@ -55,6 +56,7 @@ __all__ = [
     "layer_norm",
     "residual_layer_norm",
     "token_embedding",
+    "orthogonalize",
     "clip_grad_norm_",
     "clip_gradients_",
 ]

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import struct
-from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p, c_char_p, POINTER
+from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_void_p, c_char_p, POINTER
 from pathlib import Path
 
 import os
@@ -71,10 +71,17 @@ class LayerNormArgs(ctypes.Structure):
                 + [("has_residual", c_int), ("dtype", c_int)])
 
 
+class OrthogonalizeArgs(ctypes.Structure):
+    """mt_orthogonalize_args of include/mt_flce.h."""
+    _fields_ = ([(n, c_void_p) for n in ("input", "out", "coefficients")] + [("eps", c_double)]
+                + [(n, c_int64) for n in ("batch", "m", "n", "in_row", "in_batch")]
+                + [("steps", c_int), ("dtype", c_int)])
+
+
 def _packer(args) -> struct.Struct:
     """Writes a whole argument structure at once (its fields in order): 1 us where
     setting them one by one takes 5."""
-    kinds = {c_void_p: "P", c_int64: "q", c_float: "f", c_int: "i"}
+    kinds = {c_void_p: "P", c_int64: "q", c_float: "f", c_int: "i", c_double: "d"}
     return struct.Struct("@" + "".join(kinds[t] for _, t in args._fields_))
 
 
@@ -82,6 +89,7 @@ pack_attn_args = _packer(AttnArgs).pack
 pack_norm_args = _packer(NormArgs).pack
 pack_embed_args = _packer(EmbedArgs).pack
 pack_layer_norm_args = _packer(LayerNormArgs).pack
+pack_orthogonalize_args = _packer(OrthogonalizeArgs).pack
 
 
 # name -> (restype, argtypes); mirrors include/mt_flce.h
@@ -185,6 +193,8 @@ SIGNATURES = {
     "mt_layer_norm_forward": (c_int, [c_void_p, c_void_p]),
     "mt_layer_norm_backward_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "mt_layer_norm_backward": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mt_orthogonalize_workspace_bytes": (c_size_t, [c_void_p]),
+    "mt_orthogonalize": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "mt_grad_norm_workspace_bytes": (c_size_t, [POINTER(c_int64), c_int64]),
     "mt_grad_norm": (c_int, [POINTER(c_void_p), POINTER(c_int64), POINTER(c_int64),
                              POINTER(c_int64), POINTER(ctypes.c_int32), c_int64, c_int,

@@ -1,9 +1,9 @@
 """Build recipe for libmt_flce.so (gfx950 only).
 
-The library is four translation units (csrc/flce_capi.hip: the loss;
+The library is five translation units (csrc/flce_capi.hip: the loss;
 csrc/attn_capi.hip: attention; csrc/step_capi.hip: residual norms and clipping;
-csrc/layer_capi.hip: token embedding and layer norm; each includes its kernels'
-headers) compiled side by side with hipcc for gfx950 and linked into the package
+csrc/layer_capi.hip: token embedding and layer norm; csrc/update_capi.hip:
+orthogonalised updates; each includes its kernels' headers) compiled side by side with hipcc for gfx950 and linked into the package
 directory, so it travels with the source tree.  `python -m mini_trainer_amd.build` rebuilds it.
 """
 from __future__ import annotations
@@ -18,7 +18,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libmt_flce.so"
 SOURCES = [CSRC / "flce_capi.hip", CSRC / "attn_capi.hip", CSRC / "step_capi.hip",
-           CSRC / "layer_capi.hip"]
+           CSRC / "layer_capi.hip", CSRC / "update_capi.hip"]
 DEPENDS = sorted(CSRC.glob("*.h")) + SOURCES + [PKG_DIR.parent / "include" / "mt_flce.h"]
 
 ARCH = "gfx950"

@@ -1,0 +1,238 @@
+// C ABI of libmt_flce.so, the update behind a step's clipped gradients: its
+// orthogonalisation.  Declarations and contracts: include/mt_flce.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "../../include/mt_flce.h"
+#include "capi_common.h"
+#include "update_kernels.h"
+
+using namespace mtf;
+
+namespace {
+
+inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kUpdMost = (int64_t)1 << 31;  // bytes of an fp16 plane, an offset of 32 bits
+constexpr int64_t kUpdGroup = (int64_t)2 << 30; // bytes of the workspace that a stack of matrices asks for
+constexpr int kUpdMostSteps = 64;
+constexpr int kUpdCus = 256;
+
+struct UpdLayout {
+  int64_t r, c, ld_r, ld_c, ld_n;
+  int64_t l, s0, s1, e, d, carrier, partial, norm, state, bytes;  // of one matrix
+};
+bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
+  const auto up = [](int64_t v) { return cdiv(v, 64) * 64; };
+  if (m < 1 || n < 1 || m > (1 << 30) || n > (1 << 30)) return false;
+  x.r = std::min(m, n), x.c = std::max(m, n);
+  x.ld_r = up(x.r), x.ld_c = up(x.c), x.ld_n = up(n);
+  if (x.r * x.ld_c * 2 >= kUpdMost || x.c * x.ld_r * 2 >= kUpdMost || x.r * x.ld_r * 2 >= kUpdMost) return false;
+  const int64_t planes = dtype == MT_DTYPE_F32 ? 2 : 1;
+  int64_t at = 0;
+  const auto take = [&](int64_t& where, int64_t bytes) { where = at, at += cdiv(bytes, 256) * 256; };
+  take(x.l, x.r * x.ld_c * 2 * planes);
+  take(x.s0, x.c * x.ld_r * 2 * planes);
+  take(x.s1, x.c * x.ld_r * 2 * planes);
+  take(x.e, x.r * x.ld_r * 2 * planes);
+  take(x.d, x.r * x.ld_r * 2 * planes);
+  take(x.carrier, m * x.ld_n * 4);
+  take(x.partial, cdiv(m, 64) * cdiv(n, 64) * 4);  // (of the smallest tiles)
+  take(x.norm, kUpdParts * 8);
+  take(x.state, kUpdState * 4);
+  x.bytes = at;
+  return true;
+}
+
+int upd_check(const mt_orthogonalize_args* p, UpdLayout& l) {
+  if (!p) return fail(MT_ERR_INVALID_ARGUMENT, "null arguments");
+  const mt_orthogonalize_args& a = *p;
+  const int es = esize(a.dtype);
+  if (!es) return fail(MT_ERR_INVALID_ARGUMENT, "dtype %d is not MT_DTYPE_F32 or MT_DTYPE_BF16", a.dtype);
+  if (a.batch < 0 || a.m < 0 || a.n < 0)
+    return fail(MT_ERR_INVALID_ARGUMENT, "batch=%lld m=%lld n=%lld out of range", (long long)a.batch,
+                (long long)a.m, (long long)a.n);
+  if (a.steps < 1 || a.steps > kUpdMostSteps)
+    return fail(MT_ERR_INVALID_ARGUMENT, "steps=%d: 1 to %d are supported", a.steps, kUpdMostSteps);
+  if (!(a.eps >= 0.0) || !std::isfinite(a.eps)) return fail(MT_ERR_INVALID_ARGUMENT, "eps must be >= 0 and finite");
+  if (!a.coefficients) return fail(MT_ERR_INVALID_ARGUMENT, "null coefficients");
+  if (a.batch == 0 || a.m == 0 || a.n == 0) return MT_OK;
+  if (a.batch > (1 << 24) || !upd_layout(a.m, a.n, a.dtype, l))
+    return fail(MT_ERR_UNSUPPORTED, "%lld matrices of %lld x %lld: a matrix in fp16 must stay below 2 GiB",
+                (long long)a.batch, (long long)a.m, (long long)a.n);
+  const int64_t most = (int64_t)1 << 40;
+  if (a.in_row < a.n || a.in_row > most || a.in_batch < 0 || a.in_batch > most)
+    return fail(MT_ERR_INVALID_ARGUMENT, "rows %lld, matrices %lld elements apart", (long long)a.in_row,
+                (long long)a.in_batch);
+  if (!a.in || !a.out) return fail(MT_ERR_INVALID_ARGUMENT, "null tensor pointer");
+  if (reinterpret_cast<uintptr_t>(a.in) % es || reinterpret_cast<uintptr_t>(a.out) % es)
+    return fail(MT_ERR_INVALID_ARGUMENT, "tensors must be aligned to their element size");
+  return MT_OK;
+}
+
+// The scales of a step's fp16 copies: powers of two that keep what they hold below 2^14,
+// from what the coefficients can make of singular values in [0, most].
+struct UpdScales {
+  int x, e, d;
+  double next;  // the largest singular value after the step
+};
+bool upd_scales(const double* k, double most, UpdScales& s) {
+  const auto scale = [](double bound) {
+    return bound > 0.0 ? std::max(-100, std::min(14 - std::ilogb(bound) - 1, 60)) : 0;
+  };
+  double top = 0.0, lo = 0.0, hi = 0.0;
+  for (int i = 0; i <= 4096; ++i) {  // (the grid's gaps and the roundings below it: 1%)
+    const double v = most * i / 4096, t = v * v;
+    top = std::max(top, std::fabs(v * (k[0] + t * (k[1] + t * k[2]))));
+    const double p = t * (k[1] + t * k[2]);
+    lo = std::min(lo, p), hi = std::max(hi, p);
+  }
+  s.x = scale(most), s.e = scale(most * most * 1.01), s.d = scale((hi - lo) * 1.01);
+  s.next = top * 1.01;
+  return std::isfinite(top) && top < 1e6 && hi - lo < 1e12;
+}
+
+// The tile of a product of tiles(t) output tiles of t x t: the one whose rounds over the
+// CUs cost least.  A CU takes one workgroup of 256- or 192-tiles at a time, two of 128 and
+// four of 64.
+template <class Tiles>
+int upd_pick(Tiles tiles) {
+  static const struct { int F, slots; double rate; } kinds[] = {{8, 1, 1.0}, {6, 1, 0.9}, {4, 2, 0.7}, {2, 4, 0.35}};
+  int best = 2;
+  double least = INFINITY;
+  for (const auto& k : kinds) {
+    const int64_t load = cdiv(tiles(upd_tile(k.F)), kUpdCus);
+    const double alone = k.rate * (0.5 + 0.5 * std::min<double>(1.0, (double)load / k.slots));
+    const double cost = (double)load * k.F * k.F / alone;
+    if (cost < least) least = cost, best = k.F;
+  }
+  return best;
+}
+
+template <class F>
+int upd_with(int kind, F f) {
+  switch (kind) {
+    case 8: return f(std::integral_constant<int, 8>());
+    case 6: return f(std::integral_constant<int, 6>());
+    case 4: return f(std::integral_constant<int, 4>());
+    default: return f(std::integral_constant<int, 2>());
+  }
+}
+
+template <class T>
+int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t stream) {
+  constexpr int V = 16 / (int)sizeof(T), TERMS = sizeof(T) == 4 ? 3 : 1;
+  const int64_t runs = (int64_t)k.m * cdiv(k.n, 256 * (k.vec ? V : 1));
+  k.norm_parts = (int32_t)std::min<int64_t>(runs, kUpdParts);
+  const dim3 norm_grid((uint32_t)k.norm_parts, (uint32_t)k.batch);
+  if (k.vec) hipLaunchKernelGGL((upd_norm_kernel<T, V>), norm_grid, dim3(256), 0, stream, k);
+  else hipLaunchKernelGGL((upd_norm_kernel<T, 1>), norm_grid, dim3(256), 0, stream, k);
+  MT_TRY(check_launch("upd_norm_kernel"));
+  const dim3 convert_grid((uint32_t)(cdiv(k.m, 64) * cdiv(k.n, 64)), (uint32_t)k.batch);
+  if (k.vec) hipLaunchKernelGGL((upd_convert_kernel<T, V, TERMS>), convert_grid, dim3(256), 0, stream, k);
+  else hipLaunchKernelGGL((upd_convert_kernel<T, 1, TERMS>), convert_grid, dim3(256), 0, stream, k);
+  MT_TRY(check_launch("upd_convert_kernel"));
+
+  const auto triangle = [&](int64_t t) { return k.batch * (cdiv(k.r, t) * (cdiv(k.r, t) + 1) / 2); };
+  const auto all = [&](int64_t t) { return k.batch * cdiv(k.m, t) * cdiv(k.n, t); };
+  const int symmetric = upd_pick(triangle), apply = upd_pick(all);
+  double most = 1.0;
+  UpdScales now, next;
+  if (!upd_scales(p.coefficients, most, now)) return fail(MT_ERR_UNSUPPORTED, "these coefficients diverge");
+  for (int step = 0; step < p.steps; ++step, now = next) {
+    const double* q = p.coefficients + 3 * step;
+    next = now;
+    if (step + 1 < p.steps && !upd_scales(q + 3, now.next, next))
+      return fail(MT_ERR_UNSUPPORTED, "these coefficients diverge");
+    k.first = step == 0, k.last = step + 1 == p.steps;
+    k.a = (float)q[0], k.b = (float)q[1], k.cc = (float)q[2];
+    k.x_unscale = std::ldexp(1.f, -now.x), k.x_scale = std::ldexp(1.f, next.x);
+    k.e_scale = std::ldexp(1.f, now.e), k.e_unscale = std::ldexp(1.f, -now.e);
+    k.d_scale = std::ldexp(1.f, now.d), k.d_unscale = std::ldexp(1.f, -now.d);
+    MT_TRY(upd_with(symmetric, [&](auto F) {
+      constexpr int f = decltype(F)::value;
+      k.tiles_m = k.tiles_n = (int32_t)cdiv(k.r, upd_tile(f));
+      k.tiles = k.tiles_m * (k.tiles_m + 1) / 2;
+      const dim3 grid((uint32_t)(k.tiles * k.batch));
+      hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, false>), grid, dim3(256), 0, stream, k);
+      MT_TRY(check_launch("upd_symmetric_kernel"));
+      hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, true>), grid, dim3(256), 0, stream, k);
+      return check_launch("upd_symmetric_kernel");
+    }));
+    MT_TRY(upd_with(apply, [&](auto F) {
+      constexpr int f = decltype(F)::value;
+      k.tiles_m = (int32_t)cdiv(k.m, upd_tile(f)), k.tiles_n = (int32_t)cdiv(k.n, upd_tile(f));
+      k.tiles = k.partials = k.tiles_m * k.tiles_n;
+      hipLaunchKernelGGL((upd_apply_kernel<T, f, TERMS>), dim3((uint32_t)(k.tiles * k.batch)), dim3(256), 0, stream,
+                         k);
+      return check_launch("upd_apply_kernel");
+    }));
+    std::swap(k.s0, k.s1);
+  }
+  return MT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t mt_orthogonalize_workspace_bytes(const mt_orthogonalize_args* args) {
+  UpdLayout l;
+  if (!args || args->batch < 1 || args->batch > (1 << 24) || !esize(args->dtype) ||
+      !upd_layout(args->m, args->n, args->dtype, l))
+    return 0;
+  return (size_t)(l.bytes * std::max<int64_t>(1, std::min(args->batch, kUpdGroup / l.bytes)));
+}
+
+int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t workspace_bytes,
+                     mt_stream_t stream) {
+  UpdLayout l;
+  MT_TRY(upd_check(args, l));
+  const mt_orthogonalize_args& a = *args;
+  if (a.batch == 0 || a.m == 0 || a.n == 0) return MT_OK;
+  double most = 1.0;
+  for (int step = 0; step < a.steps; ++step) {  // before anything is launched
+    UpdScales s;
+    const double* q = a.coefficients + 3 * step;
+    if (!std::isfinite(q[0]) || !std::isfinite(q[1]) || !std::isfinite(q[2]))
+      return fail(MT_ERR_INVALID_ARGUMENT, "coefficients must be finite");
+    if (!upd_scales(q, most, s))
+      return fail(MT_ERR_UNSUPPORTED, "coefficients that carry singular values beyond 10^6");
+    most = s.next;
+  }
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(MT_ERR_INVALID_ARGUMENT, "null workspace, or one that is not aligned to 256 bytes");
+  if (workspace_bytes < (size_t)l.bytes)
+    return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, (size_t)l.bytes);
+  const int es = esize(a.dtype);
+  // matrices at a time: what the workspace holds, within one launch's workgroups
+  const int64_t tiles = cdiv(a.m, 64) * cdiv(a.n, 64);
+  const int64_t group = std::min<int64_t>({a.batch, (int64_t)(workspace_bytes / (size_t)l.bytes), 32768,
+                                           std::max<int64_t>(1, (1 << 23) / tiles)});
+  if (tiles > (1 << 23)) return fail(MT_ERR_UNSUPPORTED, "%lld x %lld exceeds one launch", (long long)a.m, (long long)a.n);
+  UpdArgs k{};
+  k.ws = static_cast<char*>(workspace);
+  k.ws_stride = l.bytes;
+  k.in_row = a.in_row, k.in_batch = a.in_batch;
+  k.l = l.l, k.s0 = l.s0, k.s1 = l.s1, k.e = l.e, k.d = l.d;
+  k.carrier = l.carrier, k.partial = l.partial, k.norm = l.norm, k.state = l.state;
+  k.eps = a.eps;
+  k.m = (int32_t)a.m, k.n = (int32_t)a.n, k.r = (int32_t)l.r, k.c = (int32_t)l.c;
+  k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c, k.ld_n = (int32_t)l.ld_n;
+  const int64_t V = 16 / es;
+  k.vec = aligned16(a.in) && aligned16(a.out) && a.n % V == 0 && (a.m == 1 || a.in_row % V == 0) &&
+          (a.batch == 1 || a.in_batch % V == 0);
+  for (int64_t at = 0; at < a.batch; at += group) {
+    k.batch = (int32_t)std::min(group, a.batch - at);
+    k.in = static_cast<const char*>(a.in) + at * a.in_batch * es;
+    k.out = static_cast<char*>(a.out) + at * a.m * a.n * es;
+    MT_TRY(a.dtype == MT_DTYPE_BF16 ? launch_orthogonalize<__bf16>(k, a, (hipStream_t)stream)
+                                    : launch_orthogonalize<float>(k, a, (hipStream_t)stream));
+  }
+  return MT_OK;
+}
+
+}  // extern "C"

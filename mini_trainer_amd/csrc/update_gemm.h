@@ -1,0 +1,190 @@
+// The matrix products of an orthogonalised update (gfx950): C = A B^T in fp16 with fp32
+// sums, both operands' rows contiguous along K.
+//
+// Workgroup = 4 waves, output tile 32 F x 32 F; wave (wm, wn) = (w >> 1, w & 1) owns a
+// block of 16 F x 16 F = F x F fragments of v_mfma_f32_16x16x32_f16.  F = 8 keeps 256
+// accumulators a lane (the AGPR file), reads the fewest LDS bytes per flop and leaves one
+// wave per SIMD; smaller F share a CU between workgroups.
+//
+// K advances in stages of 64 (128 bytes of each operand row), in two halves of 32, out of
+// a ring of LDS slots that LDS DMA fills: three for A, two for B, so that one operand's
+// DMA is issued beside each half.  With F0, F1 the fragments of the halves of stage g:
+//
+//   phase 1   F^2 MFMAs on F0(g)  | 2 F LDS reads of F1(g), F DMA: A of stage g + 2
+//   sync      own reads retired, own DMA of stage g + 1 landed, barrier
+//   phase 2   F^2 MFMAs on F1(g)  | 2 F LDS reads of F0(g + 1), F DMA: B of stage g + 2
+//
+// The barrier lies between two blocks of MFMAs whose operands are in registers.  Memory
+// instructions are spread thinly between the MFMAs by scheduling fences, as in
+// flce_gemm_bf16.h, whose tile layout (tile_off) and waits these loops use.
+//
+// Rows past the operand's end and K past its last stage need no masks: a buffer's bound
+// turns reads beyond its last row into zeros, and operands are stored with zeros up to
+// whole stages.
+#pragma once
+
+#include "flce_gemm_bf16.h"
+
+namespace mtf {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kUpdStage = 64;  // K elements of a stage
+
+constexpr int upd_tile(int F) { return 32 * F; }
+constexpr int upd_slot(int F) { return upd_tile(F) * 128; }   // bytes: one operand, one stage
+constexpr int upd_pitch(int F) { return upd_tile(F) * 2 + 16; }  // bytes of an image row, see below
+constexpr int upd_lds(int F) {
+  return 5 * upd_slot(F) > upd_tile(F) * upd_pitch(F) ? 5 * upd_slot(F) : upd_tile(F) * upd_pitch(F);
+}
+
+__device__ __forceinline__ f32x4_t upd_mma(u32x4_t a, u32x4_t b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b),
+                                                c, 0, 0, 0);
+}
+
+// An operand: `rows` rows of ld halves (whole stages).  fp32 updates keep two planes,
+// the rounded value and what the rounding left, plane bytes apart.
+struct UpdMatrix {
+  const char* at;
+  uint32_t bytes;  // of a plane: 2 rows ld, below 2^31
+  uint32_t ld;     // halves of a row
+  uint32_t rows;
+};
+
+template <int F>
+struct UpdOperand {
+  rsrc_t rsrc[2];
+  uint32_t off[F];
+  uint32_t frag[2];
+
+  __device__ __forceinline__ void init(const UpdMatrix& m, uint32_t row0, uint32_t wave_row0, bool two) {
+    rsrc[0] = make_rsrc(m.at, m.bytes);
+    rsrc[1] = make_rsrc(m.at + (two ? m.bytes : 0u), m.bytes);
+    const uint32_t l = lane_id();
+#pragma unroll
+    for (uint32_t i = 0; i < (uint32_t)F; ++i) {
+      // DMA instruction q fills 1 KiB: 8 rows of a 16-row group, in tile_off's order
+      const uint32_t q = wave_id() * F + i;
+      const uint32_t row = (q >> 1) * 16 + ((l >> 3) & 1u) * 8 + (q & 1u) * 4 + (l >> 4);
+      const uint32_t chunk = (l & 7u) ^ ((q & 1u) * 4 + (l >> 4));
+      off[i] = row0 + row < m.rows ? (row0 + row) * m.ld * 2u + chunk * 16u : 0xf0000000u;
+    }
+#pragma unroll
+    for (uint32_t kk = 0; kk < 2; ++kk) frag[kk] = tile_off(wave_row0 + (l & 15u), kk * 4 + (l >> 4));
+  }
+  __device__ __forceinline__ void issue(char* slot, int plane, int kt, int i) const {
+    dma16(plane ? rsrc[1] : rsrc[0], slot + (wave_id() * F + (uint32_t)i) * 1024u, off[i], (uint32_t)kt * 128u);
+  }
+  __device__ __forceinline__ u32x4_t read(const char* slot, int kk, int f) const {
+    return lds_read16(slot, frag[kk] + (uint32_t)f * 2048u);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void upd_wait_vm() {  // every DMA but the last N issued has landed
+  __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+// acc = sum over KT stages, and with TERMS = 3 over the planes (value, rest) x (rest,
+// value) and (value, value), of A B^T.
+template <int F, int TERMS>
+__device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, const UpdOperand<F>& b, int KT,
+                                             f32x4_t (&acc)[F][F]) {
+  constexpr int kSlot = upd_slot(F);
+  // MFMAs before each LDS read; the others follow the last one and hide its latency
+  constexpr int kPer = F >= 8 ? 3 : F >= 6 ? 2 : 1;
+  char* const two = lds;
+  char* const three = lds + 2 * kSlot;
+  const int stages = TERMS * KT;
+  // stage s of all: the planes and the stage within them
+  int term = 0, kt = 0;
+  auto advance = [&]() __attribute__((always_inline)) {  // past the end it stays at the last stage
+    if (kt + 1 < KT) {
+      ++kt;
+    } else if (term + 1 < TERMS) {
+      kt = 0;
+      ++term;
+    }
+  };
+  auto issue_a = [&](char* slot, int i) __attribute__((always_inline)) {
+    a.issue(slot, TERMS == 3 && term == 1, kt, i);
+  };
+  auto issue_b = [&](char* slot, int i) __attribute__((always_inline)) {
+    b.issue(slot, TERMS == 3 && term == 0, kt, i);
+  };
+#pragma unroll
+  for (int m = 0; m < F; ++m)
+#pragma unroll
+    for (int n = 0; n < F; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s) advance();
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      issue_a(three + s * kSlot, i);
+      issue_b(two + s * kSlot, i);
+    }
+  }
+  wait_vm0();
+  __builtin_amdgcn_s_barrier();
+  u32x4_t fa0[F], fb0[F], fa1[F], fb1[F];
+#pragma unroll
+  for (int f = 0; f < F; ++f) {
+    fa0[f] = a.read(three, 0, f);
+    fb0[f] = b.read(two, 0, f);
+  }
+  lgkm_wait0();
+  int g3 = 0;
+  for (int g = 0; g < stages; ++g, g3 = g3 == 2 ? 0 : g3 + 1) {
+    advance();
+    sched_fence();
+    const int g3n = g3 == 2 ? 0 : g3 + 1, g3p = g3 == 0 ? 2 : g3 - 1;
+    const char* ra = three + g3 * kSlot;
+    const char* rb = two + (g & 1) * kSlot;
+#pragma unroll
+    for (int i = 0; i < 2 * F; ++i) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = i * kPer + j;
+        acc[at / F][at % F] = upd_mma(fb0[at % F], fa0[at / F], acc[at / F][at % F]);
+      }
+      if (i & 1) fb1[i >> 1] = b.read(rb, 1, i >> 1);
+      else fa1[i >> 1] = a.read(ra, 1, i >> 1);
+      if (i & 1) issue_a(three + g3p * kSlot, i >> 1);
+      sched_fence();
+    }
+#pragma unroll
+    for (int at = 2 * F * kPer; at < F * F; ++at)
+      acc[at / F][at % F] = upd_mma(fb0[at % F], fa0[at / F], acc[at / F][at % F]);
+    sched_fence();
+    lgkm_wait0();
+    upd_wait_vm<F>();
+    __builtin_amdgcn_s_barrier();
+    sched_fence();
+    const char* ra1 = three + g3n * kSlot;
+    const char* rb1 = two + ((g & 1) ^ 1) * kSlot;
+#pragma unroll
+    for (int i = 0; i < 2 * F; ++i) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int at = i * kPer + j;
+        acc[at / F][at % F] = upd_mma(fb1[at % F], fa1[at / F], acc[at / F][at % F]);
+      }
+      if (i & 1) issue_b(two + (g & 1) * kSlot, i >> 1);
+      if (i & 1) fb0[i >> 1] = b.read(rb1, 0, i >> 1);
+      else fa0[i >> 1] = a.read(ra1, 0, i >> 1);
+      sched_fence();
+    }
+#pragma unroll
+    for (int at = 2 * F * kPer; at < F * F; ++at)
+      acc[at / F][at % F] = upd_mma(fb1[at % F], fa1[at / F], acc[at / F][at % F]);
+    sched_fence();
+    lgkm_wait0();
+  }
+  wait_vm0();
+  __syncthreads();  // the ring is free
+}
+
+}  // namespace mtf

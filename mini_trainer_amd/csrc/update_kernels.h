@@ -1,0 +1,479 @@
+// Orthogonalised updates by Newton-Schulz steps (gfx950).
+//
+//   X0 = G / (|G| + eps),   X <- a X + (b A + c A^2) X,   A = X X^T
+//
+// over the shorter side r of G [m, n] (X is G's transpose in the products where m > n).
+// Each step is three products: A and A^2 are symmetric, so that only the tiles on and
+// below the diagonal are computed and written twice.
+//
+// Number formats.  The products run on fp16 MFMA with fp32 sums; X itself is carried in
+// fp32 from step to step and enters a X unrounded, since that term alone lifts the small
+// singular values (by a^steps, 485 for the usual coefficients): a rounding there would be
+// lifted with them.  A is rounded as E = A - mu I with mu its mean eigenvalue tr(A) / r:
+//
+//   b A + c A^2 = p(mu) I + (b + 2 c mu) E + c E^2,   p(t) = b t + c t^2
+//   X <- (a + p(mu)) X + D X,   D = (b + 2 c mu) E + c E^2
+//
+// Around mu the terms no longer cancel (a + b + c = 0.7 out of 3.4, -4.8 and 2.0), and E
+// is small where A is near a multiple of one.  bf16 updates take one product for each
+// (off by 0.0005 to 0.0013 of their norm before the last rounding to bf16, which itself
+// is 0.0017; in bf16 operands 0.015, without mu up to 0.011), fp32 updates three, of the
+// values rounded to fp16 and of what that rounding left (1e-6, as fp32 products).  fp16
+// copies are scaled by powers of two that keep them below 2^15.
+//
+// Copies of X in fp16: L [r, c], whose rows are contiguous along the long side (A), and
+// S [c, r] (D X); a product writes both of the X it forms, out of one image in LDS.
+// All rows end in zeros up to whole stages of 64.
+#pragma once
+
+#include "step_norm.h"
+#include "update_gemm.h"
+
+namespace mtf {
+
+constexpr int kUpdParts = 256;  // partial sums of squares of G, at most
+
+// Per matrix, in fp32: the factor of X0 over its fp16 copy, 1 / (|G| + eps), mu.
+enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdState = 4 };
+
+struct UpdArgs {
+  const char* in;
+  char* out;
+  char* ws;               // of the first matrix; the others follow ws_stride bytes apart
+  int64_t ws_stride, in_row, in_batch;
+  int64_t l, s0, s1, e, d, carrier, partial, norm, state;  // byte offsets
+  double eps;
+  int32_t m, n, r, c, ld_r, ld_c, ld_n;  // ld_r, ld_c: r and c up to whole stages, ld_n: n
+  int32_t norm_parts, partials;          // partial sums of |G|^2, and of |X|^2
+  int32_t batch, tiles_m, tiles_n, tiles;
+  int32_t first, last;                   // of the steps
+  float a, b, cc;                        // the step's coefficients
+  float x_unscale, e_scale, e_unscale, d_scale, d_unscale, x_scale;
+  int32_t vec;                           // rows of G and of the result are whole 16-byte vectors
+};
+
+// Sums of squares of G, in 64 bits: workgroup p of norm_parts takes every
+// norm_parts-th run of 256 vectors.
+template <class T, int V>
+__global__ __launch_bounds__(256) void upd_norm_kernel(UpdArgs a) {
+  __shared__ double sums[4];
+  const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)blockIdx.y * a.in_batch;
+  const int32_t per_row = (a.n + 256 * V - 1) / (256 * V);
+  const int64_t runs = (int64_t)a.m * per_row;
+  double s = 0.0;
+  for (int64_t u = blockIdx.x; u < runs; u += a.norm_parts) {
+    const int64_t row = u / per_row;
+    const int32_t col = (int32_t)(u - row * per_row) * 256 * V + (int32_t)threadIdx.x * V;
+    if (col >= a.n) continue;
+    float x[V];
+    if constexpr (V > 1) NormVec<T, V>::load(in + row * a.in_row + col, x);
+    else x[0] = (float)in[row * a.in_row + col];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s = fma((double)x[i], (double)x[i], s);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
+  if (lane_id() == 0) sums[wave_id()] = s;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    reinterpret_cast<double*>(a.ws + (int64_t)blockIdx.y * a.ws_stride + a.norm)[blockIdx.x] =
+        sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+__device__ __forceinline__ uint16_t upd_half(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+__device__ __forceinline__ float upd_float(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+
+// G as fp16, scaled by the power of two that brings its norm to 2^13 .. 2^14: a 64 x 64
+// tile, as it lies and transposed, zeros up to whole stages.
+template <class T, int V, int TERMS>
+__global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
+  __shared__ uint16_t tile[TERMS == 3 ? 2 : 1][64][66];
+  __shared__ double sums[4];
+  char* ws = a.ws + (int64_t)blockIdx.y * a.ws_stride;
+  double s = 0.0;
+  if ((int)threadIdx.x < a.norm_parts) s = reinterpret_cast<const double*>(ws + a.norm)[threadIdx.x];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
+  if (lane_id() == 0) sums[wave_id()] = s;
+  __syncthreads();
+  const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
+  const double inverse = 1.0 / (norm + a.eps);
+  const int exponent = norm > 0.0 && norm < INFINITY ? 13 - ilogb(norm) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    float* state = reinterpret_cast<float*>(ws + a.state);
+    state[kUpdFactor] = (float)ldexp(inverse, -exponent);
+    state[kUpdInverse] = (float)inverse;
+    state[kUpdMu] = (float)(norm * inverse * (norm * inverse) / a.r);
+  }
+  const int32_t across = (a.n + 63) / 64;
+  const int32_t row0 = (int32_t)(blockIdx.x / across) * 64, col0 = (int32_t)(blockIdx.x % across) * 64;
+  const int32_t i = threadIdx.x >> 2, j = (threadIdx.x & 3) * 16;
+  const bool tall = a.m > a.n;
+  const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)blockIdx.y * a.in_batch;
+  uint16_t* natural = reinterpret_cast<uint16_t*>(ws + (tall ? a.s0 : a.l));
+  uint16_t* transposed = reinterpret_cast<uint16_t*>(ws + (tall ? a.l : a.s0));
+  const int64_t ld_nat = tall ? a.ld_r : a.ld_c, ld_tr = tall ? a.ld_c : a.ld_r;
+  const int64_t plane_nat = (int64_t)a.m * ld_nat, plane_tr = (int64_t)a.n * ld_tr;
+  uint16_t part[TERMS == 3 ? 2 : 1][16];
+#pragma unroll
+  for (int k = 0; k < 16; k += V) {
+    float x[V];
+    const int32_t left = row0 + i < a.m ? a.n - (col0 + j + k) : 0;
+    const T* p = in + (int64_t)(row0 + i) * a.in_row + col0 + j + k;
+    if constexpr (V > 1) {  // (whole vectors: left is 0 or less, or at least V)
+#pragma unroll
+      for (int q = 0; q < V; ++q) x[q] = 0.f;
+      if (left > 0) NormVec<T, V>::load(p, x);
+    } else {
+      x[0] = left > 0 ? (float)p[0] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+      const float v = ldexpf(x[q], exponent);
+      part[0][k + q] = upd_half(v);
+      if constexpr (TERMS == 3) part[1][k + q] = upd_half(v - upd_float(part[0][k + q]));
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) tile[t][i][j + k] = part[t][k];
+    if (row0 + i < a.m) {
+      u32x4_t* to = reinterpret_cast<u32x4_t*>(natural + t * plane_nat + (row0 + i) * ld_nat + col0 + j);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4_t v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[k] = (uint32_t)part[t][8 * h + 2 * k] | (uint32_t)part[t][8 * h + 2 * k + 1] << 16;
+        to[h] = v;
+      }
+    }
+  }
+  __syncthreads();
+  if (col0 + i >= a.n) return;
+#pragma unroll
+  for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
+    u32x4_t* to = reinterpret_cast<u32x4_t*>(transposed + t * plane_tr + (col0 + i) * ld_tr + row0 + j);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4_t v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        v[k] = (uint32_t)tile[t][j + 8 * h + 2 * k][i] | (uint32_t)tile[t][j + 8 * h + 2 * k + 1][i] << 16;
+      to[h] = v;
+    }
+  }
+}
+
+// --- tiles -----------------------------------------------------------------------
+
+// A lane's place in the tile: fragment (fm, fn) holds four columns of one row.
+template <int F>
+struct UpdPlace {
+  uint32_t row, col;
+  __device__ __forceinline__ UpdPlace() {
+    row = (wave_id() >> 1) * 16 * F + (lane_id() & 15u);
+    col = (wave_id() & 1u) * 16 * F + 4 * (lane_id() >> 4);
+  }
+};
+
+// Four values of the tile as fp16 into the image (plane 0), or what their rounding left.
+template <int F>
+__device__ __forceinline__ void upd_put(char* image, uint32_t row, uint32_t col, const float (&x)[4], bool rest) {
+  f16x4_t h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    h[i] = (_Float16)x[i];
+    if (rest) h[i] = (_Float16)(x[i] - (float)h[i]);
+  }
+  *reinterpret_cast<f16x4_t*>(image + row * upd_pitch(F) + col * 2) = h;
+}
+
+// The image's rows to rows row0.. (below `rows`) of a matrix, columns col0.. (below ld).
+template <int F>
+__device__ __forceinline__ void upd_write_rows(const char* image, char* to, int32_t row0, int32_t col0,
+                                               int32_t rows, int32_t ld) {
+  constexpr int kChunks = upd_tile(F) / 8;
+  for (int q = threadIdx.x; q < upd_tile(F) * kChunks; q += 256) {
+    const int32_t i = q / kChunks, j = (q % kChunks) * 8;
+    if (row0 + i < rows && col0 + j < ld)
+      *reinterpret_cast<u32x4_t*>(to + ((int64_t)(row0 + i) * ld + col0 + j) * 2) =
+          *reinterpret_cast<const u32x4_t*>(image + i * upd_pitch(F) + j * 2);
+  }
+}
+
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+
+// The image's columns to rows row0.. of a matrix: column i of the image is row row0 + i,
+// image row j column col0 + j.  A transposing read hands lane i of 16 the column c0 + i
+// of four rows (its lane 4 e + q reads columns c0 + 4 q .. of row e).
+template <int F>
+__device__ __forceinline__ void upd_write_columns(const char* image, char* to, int32_t row0, int32_t col0,
+                                                  int32_t rows, int32_t ld) {
+  constexpr int kTile = upd_tile(F);
+  const uint32_t l = lane_id(), in = l & 15u;
+  // a wave's unit: 16 columns of 32 rows, 8 rows to each 16 lanes
+  for (int u = wave_id(); u < (kTile / 16) * (kTile / 32); u += 4) {
+    const uint32_t c0 = (u % (kTile / 16)) * 16, j0 = (u / (kTile / 16)) * 32 + (l >> 4) * 8;
+    const char* from = image + (j0 + (in >> 2)) * upd_pitch(F) + (c0 + 4 * (in & 3u)) * 2;
+    typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+    const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)from);
+    const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(from + 4 * upd_pitch(F)));
+    const int32_t i = row0 + (int32_t)(c0 + in), j = col0 + (int32_t)j0;
+    if (i < rows && j < ld) {
+      struct { i16x4_t lo, hi; } both{lo, hi};
+      *reinterpret_cast<u32x4_t*>(to + ((int64_t)i * ld + j) * 2) = __builtin_bit_cast(u32x4_t, both);
+    }
+  }
+}
+
+// Tile `at` of the lower triangle, in bands of 8 tile rows walked column by column.
+__device__ __forceinline__ void upd_triangle(uint32_t at, uint32_t tiles, uint32_t& ti, uint32_t& tj) {
+  uint32_t first = 0, rows = tiles < 8 ? tiles : 8;
+  for (;;) {  // tiles of a band: the columns before it, full, and its own triangle
+    const uint32_t n = rows * first + rows * (rows + 1) / 2;
+    if (at < n) break;
+    at -= n;
+    first += rows;
+    rows = tiles - first < 8 ? tiles - first : 8;
+  }
+  if (at < rows * first) {
+    tj = at / rows;
+    ti = first + at % rows;
+  } else {
+    at -= rows * first;
+    uint32_t j = 0;
+    while (at >= rows - j) at -= rows - j, ++j;
+    tj = first + j;
+    ti = first + j + at;
+  }
+  ti = __builtin_amdgcn_readfirstlane(ti);
+  tj = __builtin_amdgcn_readfirstlane(tj);
+}
+
+// Both writes of a symmetric matrix's tile held in acc as values x(fm, fn, i).
+template <int F, int TERMS, class Value>
+__device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int64_t plane, int32_t row0, int32_t col0,
+                                                    int32_t r, int32_t ld, Value value) {
+  const UpdPlace<F> p;
+#pragma unroll
+  for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
+    if (t) __syncthreads();
+#pragma unroll
+    for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < F; ++fn) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = value(fm, fn, i);
+        upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, t);
+      }
+    __syncthreads();
+    upd_write_rows<F>(lds, to + t * plane, row0, col0, r, ld);
+    if (row0 != col0) upd_write_columns<F>(lds, to + t * plane, col0, row0, r, ld);
+  }
+}
+
+// E = A - mu I from L (SQUARE false), or D = (b + 2 c mu) E + c E^2 from E.
+template <int F, int TERMS, bool SQUARE>
+__global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[upd_lds(F)];
+  float* sums = reinterpret_cast<float*>(lds);  // (before and after the tile)
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t matrix = id / (uint32_t)a.tiles;
+  uint32_t ti, tj;
+  upd_triangle(id - matrix * (uint32_t)a.tiles, (uint32_t)a.tiles_m, ti, tj);
+  char* ws = a.ws + (int64_t)__builtin_amdgcn_readfirstlane(matrix) * a.ws_stride;
+  const int32_t row0 = (int32_t)ti * upd_tile(F), col0 = (int32_t)tj * upd_tile(F);
+  const UpdMatrix x = SQUARE ? UpdMatrix{ws + a.e, (uint32_t)a.r * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.r}
+                             : UpdMatrix{ws + a.l, (uint32_t)a.r * (uint32_t)a.ld_c * 2u, (uint32_t)a.ld_c, (uint32_t)a.r};
+  float* state = reinterpret_cast<float*>(ws + a.state);
+  float mu = 0.f;
+  if constexpr (!SQUARE) {
+    if (a.first) {
+      mu = state[kUpdMu];
+    } else {  // |X|^2 / r from the tiles of the product before: the same in every workgroup
+      const float* partial = reinterpret_cast<const float*>(ws + a.partial);
+      float s = 0.f;
+      for (int k = threadIdx.x; k < a.partials; k += 256) s += partial[k];
+      s = norm_wave_sum(s);
+      if (lane_id() == 0) sums[wave_id()] = s;
+      __syncthreads();
+      mu = (sums[0] + sums[1] + sums[2] + sums[3]) / (float)a.r;
+      __syncthreads();
+      if (ti == 0 && threadIdx.x == 0) state[kUpdMu] = mu;
+    }
+  } else {
+    mu = state[kUpdMu];
+  }
+  UpdOperand<F> oa, ob;
+  oa.init(x, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
+  ob.init(x, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
+  f32x4_t acc[F][F];
+  upd_mainloop<F, TERMS>(lds, oa, ob, (int)x.ld / kUpdStage, acc);
+  const UpdPlace<F> p;
+  const int64_t plane = (int64_t)a.r * a.ld_r * 2;
+  if constexpr (!SQUARE) {
+    const float f = a.first ? state[kUpdFactor] * state[kUpdFactor] : a.x_unscale * a.x_unscale;
+#pragma unroll
+    for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < F; ++fn)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn + i;
+          float v = acc[fm][fn][i] * f;
+          if (row == col && row < a.r) v -= mu;
+          acc[fm][fn][i] = v * a.e_scale;
+        }
+    upd_write_symmetric<F, TERMS>(lds, ws + a.e, plane, row0, col0, a.r, a.ld_r,
+                                  [&](int fm, int fn, int i) { return acc[fm][fn][i]; });
+  } else {
+    const float linear = (a.b + 2.f * a.cc * mu) * a.e_unscale * a.d_scale;
+    const float square = a.cc * a.e_unscale * a.e_unscale * a.d_scale;
+#pragma unroll
+    for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < F; ++fn) {
+        const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
+        float e[4] = {0.f, 0.f, 0.f, 0.f};
+        if (row < a.r && col < a.ld_r) {
+          const char* at = ws + a.e + ((int64_t)row * a.ld_r + col) * 2;
+          const f16x4_t hi = *reinterpret_cast<const f16x4_t*>(at);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[i] = (float)hi[i];
+          if constexpr (TERMS == 3) {
+            const f16x4_t lo = *reinterpret_cast<const f16x4_t*>(at + plane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] += (float)lo[i];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[fm][fn][i] = fmaf(linear, e[i], square * acc[fm][fn][i]);
+      }
+    upd_write_symmetric<F, TERMS>(lds, ws + a.d, plane, row0, col0, a.r, a.ld_r,
+                                  [&](int fm, int fn, int i) { return acc[fm][fn][i]; });
+  }
+}
+
+// X <- (a + p(mu)) X + D X, as it lies in memory [m, n]: D S^T, or S D where m > n.  Writes
+// the carried X, both fp16 copies and the tile's sum of squares, or at the last step the
+// result.
+template <class T, int F, int TERMS>
+__global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
+  __shared__ __attribute__((aligned(1024))) char lds[upd_lds(F)];
+  float* sums = reinterpret_cast<float*>(lds);  // (before and after the tile)
+  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t matrix = __builtin_amdgcn_readfirstlane(id / (uint32_t)a.tiles);
+  uint32_t tm, tn;
+  grouped_tile(id - matrix * (uint32_t)a.tiles, (uint32_t)a.tiles_m, (uint32_t)a.tiles_n, 8, tm, tn);
+  char* ws = a.ws + (int64_t)matrix * a.ws_stride;
+  const int32_t row0 = (int32_t)tm * upd_tile(F), col0 = (int32_t)tn * upd_tile(F);
+  const bool tall = a.m > a.n;
+  const UpdMatrix d{ws + a.d, (uint32_t)a.r * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.r};
+  const UpdMatrix s{ws + a.s0, (uint32_t)a.c * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.c};
+  UpdOperand<F> oa, ob;
+  oa.init(tall ? s : d, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
+  ob.init(tall ? d : s, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
+  f32x4_t acc[F][F];
+  upd_mainloop<F, TERMS>(lds, oa, ob, a.ld_r / kUpdStage, acc);
+  const float* state = reinterpret_cast<const float*>(ws + a.state);
+  const float mu = state[kUpdMu];
+  const float product = a.d_unscale * (a.first ? state[kUpdFactor] : a.x_unscale);
+  const float linear = (a.a + mu * (a.b + a.cc * mu)) * (a.first ? state[kUpdInverse] : 1.f);
+  const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)matrix * a.in_batch;
+  float* carrier = reinterpret_cast<float*>(ws + a.carrier);
+  T* out = reinterpret_cast<T*>(a.out) + (int64_t)matrix * a.m * a.n;
+  const UpdPlace<F> p;
+  float ss = 0.f;
+#pragma unroll
+  for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+    for (int fn = 0; fn < F; ++fn) {
+      const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
+      if (row < a.m && col < a.n) {
+        const int32_t left = a.n - col;
+        float x[4];
+        float* held = carrier + (int64_t)row * a.ld_n + col;
+        if (a.first) {
+          const T* from = in + (int64_t)row * a.in_row + col;
+          if (a.vec) {  // (n and the rows' distance are whole vectors: four aligned elements)
+            if constexpr (sizeof(T) == 4) {
+              const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[i] = v[i];
+            } else {
+              const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                x[i] = __uint_as_float((i & 1) ? (v[i / 2] & 0xffff0000u) : (v[i / 2] << 16));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = i < left ? (float)from[i] : 0.f;
+          }
+        } else {
+          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(held);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = i < left ? v[i] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = fmaf(linear, x[i], product * acc[fm][fn][i]);
+          if (i < left) ss = fmaf(x[i], x[i], ss);
+        }
+        if (a.last) {
+          T* to = out + (int64_t)row * a.n + col;
+          if (a.vec) {
+            if constexpr (sizeof(T) == 4)
+              *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
+            else
+              *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < left) to[i] = (T)x[i];
+          }
+        } else {
+          *reinterpret_cast<f32x4_t*>(held) = f32x4_t{x[0], x[1], x[2], x[3]};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[fm][fn][i] = x[i] * a.x_scale;
+      }
+    }
+  if (a.last) return;
+  // (columns and rows past the end are zero: D and S are there)
+  const int64_t plane_s = (int64_t)a.c * a.ld_r * 2, plane_l = (int64_t)a.r * a.ld_c * 2;
+#pragma unroll
+  for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
+    if (t) __syncthreads();
+#pragma unroll
+    for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+      for (int fn = 0; fn < F; ++fn) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = acc[fm][fn][i];
+        upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, t);
+      }
+    __syncthreads();
+    char* l = ws + a.l + t * plane_l;
+    char* next = ws + a.s1 + t * plane_s;
+    if (tall) {
+      upd_write_rows<F>(lds, next, row0, col0, a.c, a.ld_r);
+      upd_write_columns<F>(lds, l, col0, row0, a.r, a.ld_c);
+    } else {
+      upd_write_rows<F>(lds, l, row0, col0, a.r, a.ld_c);
+      upd_write_columns<F>(lds, next, col0, row0, a.c, a.ld_r);
+    }
+  }
+  ss = norm_wave_sum(ss);
+  __syncthreads();
+  if (lane_id() == 0) sums[wave_id()] = ss;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    reinterpret_cast<float*>(ws + a.partial)[id - matrix * (uint32_t)a.tiles] = sums[0] + sums[1] + sums[2] + sums[3];
+}
+
+}  // namespace mtf

@@ -1,0 +1,84 @@
+"""The orthogonalised update of weight matrices.
+
+An optimizer that orthogonalises the momentum of a weight matrix before its step takes
+it between the clipped gradients (grad_clip) and the weights.  Nothing here
+synchronises; there is no CPU or eager-PyTorch fallback: non-device tensors or a missing
+library raise.
+"""
+from __future__ import annotations
+
+import array
+import math
+from typing import Sequence, Tuple, Union
+
+import torch
+
+from ._lib import load, pack_orthogonalize_args
+from .flce import _dtype_code, _launch, _require_device
+
+__all__ = ["orthogonalize"]
+
+Triple = Tuple[float, float, float]
+
+
+def _coefficients(given, steps: int) -> array.array:
+    """a, b, c of every step in one run."""
+    rows = list(given)
+    if rows and all(isinstance(x, (int, float)) for x in rows):
+        rows = [rows] * steps
+    rows = [[float(x) for x in row] for row in rows]
+    if len(rows) != steps or any(len(row) != 3 for row in rows):
+        raise ValueError(f"coefficients must be (a, b, c), or such a triple for each of {steps} steps")
+    flat = array.array("d", [x for row in rows for x in row])
+    if not all(math.isfinite(x) for x in flat):
+        raise ValueError("coefficients must be finite")
+    return flat
+
+
+@torch.no_grad()
+def orthogonalize(update: torch.Tensor, steps: int = 5,
+                  coefficients: Union[Triple, Sequence[Triple]] = (3.4445, -4.7750, 2.0315),
+                  eps: float = 1e-7) -> torch.Tensor:
+    """The update [..., m, n] (bf16 or fp32: a momentum, or a stack of them) with its
+    singular values brought near 1, by Newton-Schulz steps over each matrix:
+
+        X = update / (norm(update) + eps)
+        steps times:  X = a X + (b A + c A^2) X,  A = X X^T
+
+    (over the shorter side: of the transpose where m > n), in the update's dtype and
+    contiguous.  coefficients: a, b, c of all steps, or such a triple for each (1 to 64
+    steps); those that would carry singular values in [0, 1] beyond 10^6 are refused.
+
+    X is carried in fp32 and rounded once.  bf16 updates go through fp16 matrix products,
+    whose error stays below that last rounding's; fp32 ones through products of split
+    values, with the error of fp32 products.  A matrix with NaN or infinities gives NaN, a
+    zero matrix zeros.  Matrices of one shape are cheapest as one stack.  Not
+    differentiable.  The workspace is some 14 bytes an element in bf16 (22 in fp32) of up
+    to 2 GiB of matrices at a time.
+    """
+    _require_device("update", update)
+    code = _dtype_code(update.dtype)
+    if update.dim() < 2:
+        raise ValueError(f"update must be [..., m, n], got {tuple(update.shape)}")
+    steps = int(steps)
+    if not 1 <= steps <= 64:
+        raise ValueError(f"steps {steps}: 1 to 64 are supported")
+    eps = float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError("eps must be >= 0 and finite")
+    flat = _coefficients(coefficients, steps)
+    m, n = update.shape[-2:]
+    out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
+    if out.numel() == 0:
+        return out
+    x = update if update.dim() == 3 else update.reshape(-1, m, n)
+    batch = x.shape[0]
+    if (n > 1 and x.stride(2) != 1) or (m > 1 and x.stride(1) < n):
+        x = x.clone(memory_format=torch.contiguous_format)
+    args = pack_orthogonalize_args(x.data_ptr(), out.data_ptr(), flat.buffer_info()[0], eps, batch, m, n,
+                                   x.stride(1) if m > 1 else n, x.stride(0) if batch > 1 else 0, steps, code)
+    lib = load()
+    nbytes = lib.mt_orthogonalize_workspace_bytes(args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=update.device)
+    _launch(update.device, "mt_orthogonalize", lib.mt_orthogonalize, args, ws.data_ptr(), nbytes)
+    return out
