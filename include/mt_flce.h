@@ -722,7 +722,8 @@ int mt_grad_scale(void* const* ptrs, const int64_t* numel, const int64_t* cols,
  * of scale dout[t] (row pitch dout_t) over the tokens of that id, rounded once, or with
  * accumulate != 0 adds these sums to an fp32 dweight, whose rows of ids that do not
  * occur it leaves as they are.  The row padding_idx (-1: none) gets no gradient.  Sums in
- * fp32 in a fixed order.  It reads ids and dout; H at most 2^24.
+ * fp32 in a fixed order.  It reads ids and dout; H at most 2^24.  Few tokens take no
+ * workspace (0 bytes, null).
  */
 typedef struct mt_embed_args {
   const void *ids, *weight;

@@ -33,15 +33,15 @@ struct EmbedLayout {
   size_t order, part, bytes;  // offsets of the parts behind starts, and the whole
 };
 EmbedLayout embed_layout(int64_t T, int64_t V, int64_t H) {
-  EmbedLayout l;
+  EmbedLayout l{};
+  if (T <= kEmbedDirect) return l;  // (nothing is sorted)
   l.log_buckets = embed_log_buckets(V);
   l.per = cdiv(V, (int64_t)1 << l.log_buckets);
   l.part_t = cdiv(H, 4) * 4;
-  const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+  const auto up = [](size_t n) { return (n + 63) / 64 * 64; };
   l.order = up(4 * (((size_t)l.per << l.log_buckets) + 1));
   l.part = l.order + up(4 * (size_t)T);
-  // (up to kEmbedPiece tokens no row has pieces)
-  l.bytes = l.part + (T > kEmbedPiece ? 2 * (size_t)cdiv(T, kEmbedPiece) * (size_t)l.part_t * 4 : 0);
+  l.bytes = l.part + 2 * (size_t)cdiv(T, kEmbedPiece) * (size_t)l.part_t * 4;
   return l;
 }
 
@@ -87,18 +87,28 @@ EmbedArgs embed_args(const mt_embed_args& a) {
   k.w_t = a.weight_t, k.dout_t = a.dout_t, k.dw_t = a.dweight_t;
   k.padding = a.padding_idx;
   k.T = (int32_t)a.T, k.V = (int32_t)a.V, k.H = (int32_t)a.H;
+  k.wide = a.ids_bytes == 8;
   k.scale = a.scale;
   return k;
 }
 
+// Elements of the widest vector (16, 8 or 4 bytes, or one element) that every row of the
+// tensors is whole aligned ones of: of their addresses in bytes, their pitches and H.
+template <class T>
+int embed_vector(int64_t H, uintptr_t at, int64_t pitches) {
+  for (int V = 16 / (int)sizeof(T); V > 1; V = V == 8 ? 2 : V / 2)
+    if (H % V == 0 && pitches % V == 0 && at % (V * sizeof(T)) == 0) return V;
+  return 1;
+}
+
 // Calls f(V, K, log2 of the lanes of a row, workgroups) with the variant for `rows`
-// rows of H elements: most vectors in flight per lane (up to kmost) that a row fills.
+// rows of H elements: vectors of V, most of them in flight per lane (up to kMost) that a
+// row fills; rows of few vectors share a wave unless share is false.
 template <class T, int kMost, class F>
-int embed_pick(int64_t rows, int64_t H, bool vec, F f) {
-  constexpr int W = 16 / (int)sizeof(T);
-  const int64_t nv = vec ? H / W : H;
+int embed_pick(int64_t rows, int64_t H, int vector, F f, bool share = true) {
+  const int64_t nv = H / vector;
   int log_lanes = 6;
-  while (log_lanes > 0 && nv <= (int64_t)1 << (log_lanes - 1)) --log_lanes;
+  while (share && log_lanes > 0 && nv <= (int64_t)1 << (log_lanes - 1)) --log_lanes;
   const auto with = [&](auto V, auto K) {
     const int64_t chunks = log_lanes == 6 ? cdiv(nv, 64 * decltype(K)::value) : 1;
     const int64_t units = cdiv(rows, 64 >> log_lanes) * chunks;
@@ -113,43 +123,49 @@ int embed_pick(int64_t rows, int64_t H, bool vec, F f) {
     if (nv > 64) return with(V, std::integral_constant<int, 2>());
     return with(V, std::integral_constant<int, 1>());
   };
-  return vec ? wide(std::integral_constant<int, W>()) : wide(std::integral_constant<int, 1>());
+  constexpr int W = 16 / (int)sizeof(T);
+  if (vector == W) return wide(std::integral_constant<int, W>());
+  if (vector == 2) return wide(std::integral_constant<int, 2>());
+  return wide(std::integral_constant<int, 1>());
 }
 
-template <class T, class I>
+template <class T>
 int launch_embed_forward(const EmbedArgs& k, hipStream_t stream) {
-  constexpr int W = 16 / (int)sizeof(T);
-  const bool vec = k.H % W == 0 && k.w_t % W == 0 && aligned16(k.w) && aligned16(k.out);
-  return embed_pick<T, 4>(k.T, k.H, vec, [&](auto V, auto K, int log_lanes, uint32_t groups) {
-    hipLaunchKernelGGL((embed_forward_kernel<T, I, decltype(V)::value, decltype(K)::value>), dim3(groups),
-                       dim3(256), 0, stream, k, log_lanes);
+  const int vector = embed_vector<T>(k.H, reinterpret_cast<uintptr_t>(k.w) | reinterpret_cast<uintptr_t>(k.out), k.w_t);
+  return embed_pick<T, 4>(k.T, k.H, vector, [&](auto V, auto K, int log_lanes, uint32_t groups) {
+    hipLaunchKernelGGL((embed_forward_kernel<T, decltype(V)::value, decltype(K)::value>), dim3(groups), dim3(256), 0,
+                       stream, k, log_lanes);
     return check_launch("embed_forward_kernel");
   });
 }
 
-template <class T, class I>
+template <class T>
 int launch_embed_backward(const EmbedArgs& k, bool accumulate, hipStream_t stream) {
-  constexpr int W = 16 / (int)sizeof(T);
-  const bool vec = k.H % W == 0 && k.dout_t % W == 0 && k.dw_t % (accumulate ? 4 : W) == 0 &&
-                   aligned16(k.dout) && aligned16(k.dw);
-  hipLaunchKernelGGL(embed_sort_kernel<I>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
-  MT_TRY(check_launch("embed_sort_kernel"));
-  if (k.T > kEmbedPiece)
-    MT_TRY((embed_pick<T, 2>(cdiv(k.T, kEmbedPiece), k.H, vec,
-                             [&](auto V, auto K, int log_lanes, uint32_t groups) {
-      hipLaunchKernelGGL((embed_pieces_kernel<T, I, decltype(V)::value, decltype(K)::value>), dim3(groups),
-                         dim3(256), 0, stream, k, log_lanes);
+  // (the accumulator's vectors are as many elements, but never more than 16 bytes)
+  int vector = embed_vector<T>(k.H, reinterpret_cast<uintptr_t>(k.dout), k.dout_t);
+  while (vector > 1 && (accumulate ? (k.dw_t % std::min(vector, 4) != 0 ||
+                                      reinterpret_cast<uintptr_t>(k.dw) % (4 * std::min(vector, 4)) != 0)
+                                   : (k.dw_t % vector != 0 || reinterpret_cast<uintptr_t>(k.dw) % (vector * sizeof(T)) != 0)))
+    vector = vector == 8 ? 2 : vector / 2;
+  const bool direct = k.T <= kEmbedDirect;
+  if (!direct) {
+    if (k.wide) hipLaunchKernelGGL(embed_sort_kernel<int64_t>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
+    else hipLaunchKernelGGL(embed_sort_kernel<int32_t>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
+    MT_TRY(check_launch("embed_sort_kernel"));
+    MT_TRY((embed_pick<T, 2>(cdiv(k.T, kEmbedPiece), k.H, vector, [&](auto V, auto K, int, uint32_t groups) {
+      hipLaunchKernelGGL((embed_pieces_kernel<T, decltype(V)::value, decltype(K)::value>), dim3(groups), dim3(256), 0,
+                         stream, k);
       return check_launch("embed_pieces_kernel");
-    })));
+    }, false)));
+  }
   if (accumulate && k.T == 0) return MT_OK;
-  return embed_pick<T, 2>(accumulate ? k.T : k.V, k.H, vec,
+  return embed_pick<T, 2>(accumulate ? k.T : k.V, k.H, vector,
                           [&](auto V, auto K, int log_lanes, uint32_t groups) {
     constexpr int v = decltype(V)::value, n = decltype(K)::value;
-    if (accumulate)
-      hipLaunchKernelGGL((embed_rows_kernel<T, I, v, n, true>), dim3(groups), dim3(256), 0, stream, k, log_lanes);
-    else
-      hipLaunchKernelGGL((embed_rows_kernel<T, I, v, n, false>), dim3(groups), dim3(256), 0, stream, k, log_lanes);
-    return check_launch("embed_rows_kernel");
+    auto kern = direct ? (accumulate ? embed_direct_kernel<T, v, n, true> : embed_direct_kernel<T, v, n, false>)
+                       : (accumulate ? embed_rows_kernel<T, v, n, true> : embed_rows_kernel<T, v, n, false>);
+    hipLaunchKernelGGL(kern, dim3(groups), dim3(256), 0, stream, k, log_lanes);
+    return check_launch(direct ? "embed_direct_kernel" : "embed_rows_kernel");
   });
 }
 
@@ -273,9 +289,7 @@ int mt_embed_forward(const mt_embed_args* args, mt_stream_t stream) {
   if (a.T == 0) return MT_OK;
   const EmbedArgs k = embed_args(a);
   hipStream_t s = (hipStream_t)stream;
-  if (a.dtype == MT_DTYPE_BF16)
-    return a.ids_bytes == 8 ? launch_embed_forward<__bf16, int64_t>(k, s) : launch_embed_forward<__bf16, int32_t>(k, s);
-  return a.ids_bytes == 8 ? launch_embed_forward<float, int64_t>(k, s) : launch_embed_forward<float, int32_t>(k, s);
+  return a.dtype == MT_DTYPE_BF16 ? launch_embed_forward<__bf16>(k, s) : launch_embed_forward<float>(k, s);
 }
 
 size_t mt_embed_backward_workspace_bytes(int64_t T, int64_t V, int64_t H) {
@@ -286,9 +300,9 @@ size_t mt_embed_backward_workspace_bytes(int64_t T, int64_t V, int64_t H) {
 int mt_embed_backward(const mt_embed_args* args, void* workspace, size_t workspace_bytes, mt_stream_t stream) {
   MT_TRY(embed_check(args, true));
   const mt_embed_args& a = *args;
-  if (!workspace || !aligned16(workspace))
-    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
   const EmbedLayout l = embed_layout(a.T, a.V, a.H);
+  if (l.bytes && (!workspace || !aligned16(workspace)))
+    return fail(MT_ERR_INVALID_ARGUMENT, "null or misaligned workspace");
   if (workspace_bytes < l.bytes)
     return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, l.bytes);
   EmbedArgs k = embed_args(a);
@@ -301,11 +315,8 @@ int mt_embed_backward(const mt_embed_args* args, void* workspace, size_t workspa
   k.per = (int32_t)l.per;
   hipStream_t s = (hipStream_t)stream;
   const bool acc = a.accumulate != 0;
-  if (a.dtype == MT_DTYPE_BF16)
-    return a.ids_bytes == 8 ? launch_embed_backward<__bf16, int64_t>(k, acc, s)
-                            : launch_embed_backward<__bf16, int32_t>(k, acc, s);
-  return a.ids_bytes == 8 ? launch_embed_backward<float, int64_t>(k, acc, s)
-                          : launch_embed_backward<float, int32_t>(k, acc, s);
+  return a.dtype == MT_DTYPE_BF16 ? launch_embed_backward<__bf16>(k, acc, s)
+                                  : launch_embed_backward<float>(k, acc, s);
 }
 
 int mt_layer_norm_forward(const mt_layer_norm_args* args, mt_stream_t stream) {

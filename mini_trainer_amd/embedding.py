@@ -7,6 +7,7 @@ is no CPU or eager-PyTorch fallback: non-device tensors or a missing library rai
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -17,6 +18,11 @@ from .flce import _backward_once, _dtype_code, _launch, _require_device
 from .norms import _pitch, _rows
 
 __all__ = ["token_embedding"]
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(T: int, V: int, H: int) -> int:
+    return load().mt_embed_backward_workspace_bytes(T, V, H)
 
 
 class _TokenEmbedding(torch.autograd.Function):
@@ -44,10 +50,10 @@ class _TokenEmbedding(torch.autograd.Function):
         dw = dout.new_empty((V, H)) if acc is None else acc
         args = pack_embed_args(ids.data_ptr(), 0, 0, d.data_ptr(), dw.data_ptr(), 0, 0, _pitch(d),
                                _pitch(dw), *ctx.tail, int(acc is not None))
-        lib = load()
-        nbytes = lib.mt_embed_backward_workspace_bytes(T, V, H)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device)
-        _launch(dout.device, "mt_embed_backward", lib.mt_embed_backward, args, ws.data_ptr(), nbytes)
+        nbytes = _workspace_bytes(T, V, H)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device) if nbytes else None
+        _launch(dout.device, "mt_embed_backward", load().mt_embed_backward, args,
+                0 if ws is None else ws.data_ptr(), nbytes)
         if acc is None:
             return None, dw, None, None, None, None
         torch.autograd.graph.increment_version([acc])

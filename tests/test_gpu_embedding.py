@@ -54,7 +54,7 @@ def test_matches_the_definition(gpu, T, V, H, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 1024, 1025, 5000])
+@pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 256, 257, 1024, 1025, 5000])
 def test_one_id_takes_all_tokens(gpu, T, dtype):
     """A row of many pieces, from the first sorted token on and behind another row's."""
     ids, w, d = make(T, 40, 136, dtype, seed=T)

@@ -73,14 +73,15 @@ def test_embedding_workspace():
     lib = _lib.load()
     need = lib.mt_embed_backward_workspace_bytes
     # 256 buckets of whole ids and one end, the tokens' order, two rows for each 32 tokens
-    assert need(65536, 128256, 4096) == 4 * (256 * 501 + 4) + 4 * 65536 + 2 * 2048 * 4096 * 4
-    assert need(32, 1000, 64) == 4 * (256 * 4 + 4) + 4 * 32
-    assert need(0, 1, 1) == 4 * (256 + 4)
-    assert need(5, 262145, 1) == 4 * (512 * 513 + 4) + 4 * 8
+    assert need(65536, 128256, 4096) == -(-4 * (256 * 501 + 1) // 64) * 64 + 4 * 65536 + 2 * 2048 * 4096 * 4
+    assert need(257, 1000, 64) == -(-4 * (256 * 4 + 1) // 64) * 64 + -(-4 * 257 // 64) * 64 + 2 * 9 * 64 * 4
+    assert need(300, 262145, 1) == -(-4 * (512 * 513 + 1) // 64) * 64 + -(-4 * 300 // 64) * 64 + 2 * 10 * 4 * 4
+    # few tokens are not sorted
+    assert need(256, 1000, 64) == need(0, 1, 1) == 0
     for bad in ((-1, 5, 5), (5, 0, 5), (5, 5, 0), (BIG, 5, 5), (5, BIG, 5), (5, 5, BIG)):
         assert need(*bad) == 0
-    a = embed()
-    n = need(10, 100, 64)
+    a = embed(T=300)
+    n = need(300, 100, 64)
     assert lib.mt_embed_backward(ctypes.byref(a), P, n - 1, None) == 2
     assert lib.mt_embed_backward(ctypes.byref(a), None, n, None) == 1
     assert lib.mt_embed_backward(ctypes.byref(a), P + 8, n, None) == 1
