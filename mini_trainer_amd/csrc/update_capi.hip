@@ -22,14 +22,14 @@ constexpr int kUpdMostSteps = 64;
 constexpr int kUpdCus = 256;
 
 struct UpdLayout {
-  int64_t r, c, ld_r, ld_c, ld_n;
-  int64_t l, s0, s1, e, d, carrier, partial, norm, state, bytes;  // of one matrix
+  int64_t r, c, ld_r, ld_c;
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, bytes;  // of one matrix
 };
 bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   const auto up = [](int64_t v) { return cdiv(v, 64) * 64; };
   if (m < 1 || n < 1 || m > (1 << 30) || n > (1 << 30)) return false;
   x.r = std::min(m, n), x.c = std::max(m, n);
-  x.ld_r = up(x.r), x.ld_c = up(x.c), x.ld_n = up(n);
+  x.ld_r = up(x.r), x.ld_c = up(x.c);
   if (x.r * x.ld_c * 2 >= kUpdMost || x.c * x.ld_r * 2 >= kUpdMost || x.r * x.ld_r * 2 >= kUpdMost) return false;
   const int64_t planes = dtype == MT_DTYPE_F32 ? 2 : 1;
   int64_t at = 0;
@@ -39,7 +39,8 @@ bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   take(x.s1, x.c * x.ld_r * 2 * planes);
   take(x.e, x.r * x.ld_r * 2 * planes);
   take(x.d, x.r * x.ld_r * 2 * planes);
-  take(x.carrier, m * x.ld_n * 4);
+  take(x.fragments, x.ld_r * x.ld_r * 2 * planes);
+  take(x.carrier, cdiv(m, 16) * cdiv(n, 16) * 1024);
   take(x.partial, cdiv(m, 64) * cdiv(n, 64) * 4);  // (of the smallest tiles)
   take(x.norm, kUpdParts * 8);
   take(x.state, kUpdState * 4);
@@ -99,11 +100,12 @@ bool upd_scales(const double* k, double most, UpdScales& s) {
 // CUs cost least.  A CU takes one workgroup of 256- or 192-tiles at a time, two of 128 and
 // four of 64.
 template <class Tiles>
-int upd_pick(Tiles tiles) {
+int upd_pick(Tiles tiles, bool split) {
   static const struct { int F, slots; double rate; } kinds[] = {{8, 1, 1.0}, {6, 1, 0.9}, {4, 2, 0.7}, {2, 4, 0.35}};
   int best = 2;
   double least = INFINITY;
   for (const auto& k : kinds) {
+    if (split && k.F == 8) continue;  // (its two writes of an image would spill)
     const int64_t load = cdiv(tiles(upd_tile(k.F)), kUpdCus);
     const double alone = k.rate * (0.5 + 0.5 * std::min<double>(1.0, (double)load / k.slots));
     const double cost = (double)load * k.F * k.F / alone;
@@ -112,10 +114,10 @@ int upd_pick(Tiles tiles) {
   return best;
 }
 
-template <class F>
+template <int MOST, class F>
 int upd_with(int kind, F f) {
   switch (kind) {
-    case 8: return f(std::integral_constant<int, 8>());
+    case 8: return f(std::integral_constant<int, MOST>());
     case 6: return f(std::integral_constant<int, 6>());
     case 4: return f(std::integral_constant<int, 4>());
     default: return f(std::integral_constant<int, 2>());
@@ -138,7 +140,8 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
 
   const auto triangle = [&](int64_t t) { return k.batch * (cdiv(k.r, t) * (cdiv(k.r, t) + 1) / 2); };
   const auto all = [&](int64_t t) { return k.batch * cdiv(k.m, t) * cdiv(k.n, t); };
-  const int symmetric = upd_pick(triangle), apply = upd_pick(all);
+  const int symmetric = upd_pick(triangle, TERMS == 3), apply = upd_pick(all, TERMS == 3);
+  constexpr int kMost = TERMS == 3 ? 6 : 8;
   double most = 1.0;
   UpdScales now, next;
   if (!upd_scales(p.coefficients, most, now)) return fail(MT_ERR_UNSUPPORTED, "these coefficients diverge");
@@ -152,7 +155,7 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
     k.x_unscale = std::ldexp(1.f, -now.x), k.x_scale = std::ldexp(1.f, next.x);
     k.e_scale = std::ldexp(1.f, now.e), k.e_unscale = std::ldexp(1.f, -now.e);
     k.d_scale = std::ldexp(1.f, now.d), k.d_unscale = std::ldexp(1.f, -now.d);
-    MT_TRY(upd_with(symmetric, [&](auto F) {
+    MT_TRY(upd_with<kMost>(symmetric, [&](auto F) {
       constexpr int f = decltype(F)::value;
       k.tiles_m = k.tiles_n = (int32_t)cdiv(k.r, upd_tile(f));
       k.tiles = k.tiles_m * (k.tiles_m + 1) / 2;
@@ -162,7 +165,7 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
       hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, true>), grid, dim3(256), 0, stream, k);
       return check_launch("upd_symmetric_kernel");
     }));
-    MT_TRY(upd_with(apply, [&](auto F) {
+    MT_TRY(upd_with<kMost>(apply, [&](auto F) {
       constexpr int f = decltype(F)::value;
       k.tiles_m = (int32_t)cdiv(k.m, upd_tile(f)), k.tiles_n = (int32_t)cdiv(k.n, upd_tile(f));
       k.tiles = k.partials = k.tiles_m * k.tiles_n;
@@ -218,10 +221,10 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   k.ws_stride = l.bytes;
   k.in_row = a.in_row, k.in_batch = a.in_batch;
   k.l = l.l, k.s0 = l.s0, k.s1 = l.s1, k.e = l.e, k.d = l.d;
-  k.carrier = l.carrier, k.partial = l.partial, k.norm = l.norm, k.state = l.state;
+  k.fragments = l.fragments, k.carrier = l.carrier, k.partial = l.partial, k.norm = l.norm, k.state = l.state;
   k.eps = a.eps;
   k.m = (int32_t)a.m, k.n = (int32_t)a.n, k.r = (int32_t)l.r, k.c = (int32_t)l.c;
-  k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c, k.ld_n = (int32_t)l.ld_n;
+  k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c;
   const int64_t V = 16 / es;
   k.vec = aligned16(a.in) && aligned16(a.out) && a.n % V == 0 && (a.m == 1 || a.in_row % V == 0) &&
           (a.batch == 1 || a.in_batch % V == 0);

@@ -7,12 +7,13 @@
 // wave per SIMD; smaller F share a CU between workgroups.
 //
 // K advances in stages of 64 (128 bytes of each operand row), in two halves of 32, out of
-// a ring of LDS slots that LDS DMA fills: three for A, two for B, so that one operand's
-// DMA is issued beside each half.  With F0, F1 the fragments of the halves of stage g:
+// a ring of LDS slots that LDS DMA fills: three for A, N = two (F = 8) or three for B, so
+// that one operand's DMA is issued beside each half.  With F0, F1 the fragments of the
+// halves of stage g:
 //
 //   phase 1   F^2 MFMAs on F0(g)  | 2 F LDS reads of F1(g), F DMA: A of stage g + 2
 //   sync      own reads retired, own DMA of stage g + 1 landed, barrier
-//   phase 2   F^2 MFMAs on F1(g)  | 2 F LDS reads of F0(g + 1), F DMA: B of stage g + 2
+//   phase 2   F^2 MFMAs on F1(g)  | 2 F LDS reads of F0(g + 1), F DMA: B of stage g + N
 //
 // The barrier lies between two blocks of MFMAs whose operands are in registers.  Memory
 // instructions are spread thinly between the MFMAs by scheduling fences, as in
@@ -35,9 +36,9 @@ constexpr int kUpdStage = 64;  // K elements of a stage
 constexpr int upd_tile(int F) { return 32 * F; }
 constexpr int upd_slot(int F) { return upd_tile(F) * 128; }   // bytes: one operand, one stage
 constexpr int upd_pitch(int F) { return upd_tile(F) * 2 + 16; }  // bytes of an image row, see below
-constexpr int upd_lds(int F) {
-  return 5 * upd_slot(F) > upd_tile(F) * upd_pitch(F) ? 5 * upd_slot(F) : upd_tile(F) * upd_pitch(F);
-}
+// Stages of B that the ring holds (A: 3).
+constexpr int upd_slots_b(int F) { return F == 8 ? 2 : 3; }
+constexpr int upd_lds(int F) { return (3 + upd_slots_b(F)) * upd_slot(F); }  // (an image of the tile fits in)
 
 __device__ __forceinline__ f32x4_t upd_mma(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b),
@@ -92,96 +93,101 @@ __device__ __forceinline__ void upd_wait_vm() {  // every DMA but the last N iss
 template <int F, int TERMS>
 __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, const UpdOperand<F>& b, int KT,
                                              f32x4_t (&acc)[F][F]) {
-  constexpr int kSlot = upd_slot(F);
+  constexpr int kSlot = upd_slot(F), NB = upd_slots_b(F);
+  static_assert(upd_lds(F) >= upd_tile(F) * upd_pitch(F), "an image of the tile");
   // MFMAs before each LDS read; the others follow the last one and hide its latency
   constexpr int kPer = F >= 8 ? 3 : F >= 6 ? 2 : 1;
-  char* const two = lds;
-  char* const three = lds + 2 * kSlot;
+  char* const slots_b = lds;
+  char* const slots_a = lds + NB * kSlot;
   const int stages = TERMS * KT;
-  // stage s of all: the planes and the stage within them
-  int term = 0, kt = 0;
-  auto advance = [&]() __attribute__((always_inline)) {  // past the end it stays at the last stage
-    if (kt + 1 < KT) {
-      ++kt;
-    } else if (term + 1 < TERMS) {
-      kt = 0;
-      ++term;
-    }
+  // The DMA of stage s of all.  Past the end it loads the last stage again, into slots that
+  // are not read any more, so that every stage issues as much.
+  auto at = [&](int s, int& term, int& kt) __attribute__((always_inline)) {
+    s = s < stages ? s : stages - 1;
+    term = TERMS == 1 ? 0 : s >= 2 * KT ? 2 : s >= KT ? 1 : 0;
+    kt = s - term * KT;
   };
-  auto issue_a = [&](char* slot, int i) __attribute__((always_inline)) {
+  auto issue_a = [&](char* slot, int term, int kt, int i) __attribute__((always_inline)) {
     a.issue(slot, TERMS == 3 && term == 1, kt, i);
   };
-  auto issue_b = [&](char* slot, int i) __attribute__((always_inline)) {
+  auto issue_b = [&](char* slot, int term, int kt, int i) __attribute__((always_inline)) {
     b.issue(slot, TERMS == 3 && term == 0, kt, i);
   };
 #pragma unroll
   for (int m = 0; m < F; ++m)
 #pragma unroll
     for (int n = 0; n < F; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // stages 0 and 1, and B of those that phases 2 are ahead
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (s) advance();
+  for (int s = 0; s < NB; ++s) {
+    int term, kt;
+    at(s, term, kt);
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      issue_a(three + s * kSlot, i);
-      issue_b(two + s * kSlot, i);
+      if (s < 2) issue_a(slots_a + s * kSlot, term, kt, i);
+      issue_b(slots_b + s * kSlot, term, kt, i);
     }
   }
-  wait_vm0();
+  upd_wait_vm<F * (2 * NB - 3 - (NB - 2))>();  // stage 0
   __builtin_amdgcn_s_barrier();
   u32x4_t fa0[F], fb0[F], fa1[F], fb1[F];
 #pragma unroll
   for (int f = 0; f < F; ++f) {
-    fa0[f] = a.read(three, 0, f);
-    fb0[f] = b.read(two, 0, f);
+    fa0[f] = a.read(slots_a, 0, f);
+    fb0[f] = b.read(slots_b, 0, f);
   }
   lgkm_wait0();
-  int g3 = 0;
-  for (int g = 0; g < stages; ++g, g3 = g3 == 2 ? 0 : g3 + 1) {
-    advance();
+  int ga = 0, gb = 0;  // slots of stage g
+  for (int g = 0; g < stages; ++g) {
     sched_fence();
-    const int g3n = g3 == 2 ? 0 : g3 + 1, g3p = g3 == 0 ? 2 : g3 - 1;
-    const char* ra = three + g3 * kSlot;
-    const char* rb = two + (g & 1) * kSlot;
+    const int ga1 = ga == 2 ? 0 : ga + 1, ga2 = ga == 0 ? 2 : ga - 1;  // of stages g + 1 and g + 2
+    const int gb1 = gb == NB - 1 ? 0 : gb + 1;
+    const char* ra = slots_a + ga * kSlot;
+    const char* rb = slots_b + gb * kSlot;
+    int term, kt;
+    at(g + 2, term, kt);
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int at = i * kPer + j;
-        acc[at / F][at % F] = upd_mma(fb0[at % F], fa0[at / F], acc[at / F][at % F]);
+        const int k = i * kPer + j;
+        acc[k / F][k % F] = upd_mma(fb0[k % F], fa0[k / F], acc[k / F][k % F]);
       }
       if (i & 1) fb1[i >> 1] = b.read(rb, 1, i >> 1);
       else fa1[i >> 1] = a.read(ra, 1, i >> 1);
-      if (i & 1) issue_a(three + g3p * kSlot, i >> 1);
+      if (i & 1) issue_a(slots_a + ga2 * kSlot, term, kt, i >> 1);
       sched_fence();
     }
 #pragma unroll
-    for (int at = 2 * F * kPer; at < F * F; ++at)
-      acc[at / F][at % F] = upd_mma(fb0[at % F], fa0[at / F], acc[at / F][at % F]);
+    for (int k = 2 * F * kPer; k < F * F; ++k)
+      acc[k / F][k % F] = upd_mma(fb0[k % F], fa0[k / F], acc[k / F][k % F]);
     sched_fence();
+    // stage g + 1 has landed: A of g + 2 was issued since, and B of g + 2 with three slots
     lgkm_wait0();
-    upd_wait_vm<F>();
+    upd_wait_vm<F * (NB - 1)>();
     __builtin_amdgcn_s_barrier();
     sched_fence();
-    const char* ra1 = three + g3n * kSlot;
-    const char* rb1 = two + ((g & 1) ^ 1) * kSlot;
+    const char* ra1 = slots_a + ga1 * kSlot;
+    const char* rb1 = slots_b + gb1 * kSlot;
+    at(g + NB, term, kt);
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int at = i * kPer + j;
-        acc[at / F][at % F] = upd_mma(fb1[at % F], fa1[at / F], acc[at / F][at % F]);
+        const int k = i * kPer + j;
+        acc[k / F][k % F] = upd_mma(fb1[k % F], fa1[k / F], acc[k / F][k % F]);
       }
-      if (i & 1) issue_b(two + (g & 1) * kSlot, i >> 1);
+      if (i & 1) issue_b(slots_b + gb * kSlot, term, kt, i >> 1);
       if (i & 1) fb0[i >> 1] = b.read(rb1, 0, i >> 1);
       else fa0[i >> 1] = a.read(ra1, 0, i >> 1);
       sched_fence();
     }
 #pragma unroll
-    for (int at = 2 * F * kPer; at < F * F; ++at)
-      acc[at / F][at % F] = upd_mma(fb1[at % F], fa1[at / F], acc[at / F][at % F]);
+    for (int k = 2 * F * kPer; k < F * F; ++k)
+      acc[k / F][k % F] = upd_mma(fb1[k % F], fa1[k / F], acc[k / F][k % F]);
     sched_fence();
     lgkm_wait0();
+    ga = ga1, gb = gb1;
   }
   wait_vm0();
   __syncthreads();  // the ring is free

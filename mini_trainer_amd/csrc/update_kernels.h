@@ -41,9 +41,9 @@ struct UpdArgs {
   char* out;
   char* ws;               // of the first matrix; the others follow ws_stride bytes apart
   int64_t ws_stride, in_row, in_batch;
-  int64_t l, s0, s1, e, d, carrier, partial, norm, state;  // byte offsets
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state;  // byte offsets
   double eps;
-  int32_t m, n, r, c, ld_r, ld_c, ld_n;  // ld_r, ld_c: r and c up to whole stages, ld_n: n
+  int32_t m, n, r, c, ld_r, ld_c;        // ld_r, ld_c: r and c up to whole stages
   int32_t norm_parts, partials;          // partial sums of |G|^2, and of |X|^2
   int32_t batch, tiles_m, tiles_n, tiles;
   int32_t first, last;                   // of the steps
@@ -252,7 +252,7 @@ __device__ __forceinline__ void upd_triangle(uint32_t at, uint32_t tiles, uint32
   tj = __builtin_amdgcn_readfirstlane(tj);
 }
 
-// Both writes of a symmetric matrix's tile held in acc as values x(fm, fn, i).
+// Both writes of a symmetric matrix's tile, whose fragment (fm, fn) value(fm, fn, x) gives.
 template <int F, int TERMS, class Value>
 __device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int64_t plane, int32_t row0, int32_t col0,
                                                     int32_t r, int32_t ld, Value value) {
@@ -261,18 +261,25 @@ __device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int64_t
   for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
     if (t) __syncthreads();
 #pragma unroll
-    for (int fm = 0; fm < F; ++fm)
+    for (int fm = 0; fm < F; ++fm) {
 #pragma unroll
       for (int fn = 0; fn < F; ++fn) {
         float x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = value(fm, fn, i);
+        value(fm, fn, t, x);
         upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, t);
       }
+      sched_fence();  // (a row of fragments at a time: all at once would spill)
+    }
     __syncthreads();
     upd_write_rows<F>(lds, to + t * plane, row0, col0, r, ld);
     if (row0 != col0) upd_write_columns<F>(lds, to + t * plane, col0, row0, r, ld);
   }
+}
+
+// Where a lane's four values of a 16 x 16 fragment lie in a matrix kept by fragments, in
+// elements: 64 lanes side by side.
+__device__ __forceinline__ int64_t upd_fragment(int32_t row, int32_t col, int32_t across) {
+  return ((int64_t)(row >> 4) * across + (col >> 4)) * 256 + 4 * (int32_t)lane_id();
 }
 
 // E = A - mu I from L (SQUARE false), or D = (b + 2 c mu) E + c E^2 from E.
@@ -314,46 +321,63 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
   upd_mainloop<F, TERMS>(lds, oa, ob, (int)x.ld / kUpdStage, acc);
   const UpdPlace<F> p;
   const int64_t plane = (int64_t)a.r * a.ld_r * 2;
+  // E is also kept by fragments, for the product that squares it: the same lanes of the
+  // same tile read it there
+  const int32_t across = a.ld_r / 16;
+  f16x4_t* kept = reinterpret_cast<f16x4_t*>(ws + a.fragments);
+  const int64_t kept_plane = (int64_t)a.ld_r * a.ld_r / 4;
+  // a wave's fragment that lies within whole stages of the matrix
+  auto within = [&](int fm, int fn) {
+    return row0 + (int32_t)(wave_id() >> 1) * 16 * F + 16 * fm < a.ld_r &&
+           col0 + (int32_t)(wave_id() & 1u) * 16 * F + 16 * fn < a.ld_r;
+  };
   if constexpr (!SQUARE) {
-    const float f = a.first ? state[kUpdFactor] * state[kUpdFactor] : a.x_unscale * a.x_unscale;
+    const float f = (a.first ? state[kUpdFactor] * state[kUpdFactor] : a.x_unscale * a.x_unscale) * a.e_scale;
+    const float centre = mu * a.e_scale;
+    upd_write_symmetric<F, TERMS>(
+        lds, ws + a.e, plane, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
+          const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
+          f16x4_t h;
 #pragma unroll
-    for (int fm = 0; fm < F; ++fm)
-#pragma unroll
-      for (int fn = 0; fn < F; ++fn)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn + i;
-          float v = acc[fm][fn][i] * f;
-          if (row == col && row < a.r) v -= mu;
-          acc[fm][fn][i] = v * a.e_scale;
-        }
-    upd_write_symmetric<F, TERMS>(lds, ws + a.e, plane, row0, col0, a.r, a.ld_r,
-                                  [&](int fm, int fn, int i) { return acc[fm][fn][i]; });
+          for (int i = 0; i < 4; ++i) {
+            x[i] = acc[fm][fn][i] * f;
+            if (row == col + i && row < a.r) x[i] -= centre;
+            h[i] = (_Float16)x[i];
+            if (t) h[i] = (_Float16)(x[i] - (float)h[i]);
+          }
+          if (within(fm, fn)) kept[t * kept_plane + upd_fragment(row, col, across) / 4] = h;
+        });
   } else {
     const float linear = (a.b + 2.f * a.cc * mu) * a.e_unscale * a.d_scale;
     const float square = a.cc * a.e_unscale * a.e_unscale * a.d_scale;
+    f16x4_t held[TERMS == 3 ? 2 : 1][F][F];  // (in the registers of the loop's fragments)
 #pragma unroll
     for (int fm = 0; fm < F; ++fm)
 #pragma unroll
       for (int fn = 0; fn < F; ++fn) {
         const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
-        float e[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row < a.r && col < a.ld_r) {
-          const char* at = ws + a.e + ((int64_t)row * a.ld_r + col) * 2;
-          const f16x4_t hi = *reinterpret_cast<const f16x4_t*>(at);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[i] = (float)hi[i];
-          if constexpr (TERMS == 3) {
-            const f16x4_t lo = *reinterpret_cast<const f16x4_t*>(at + plane);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] += (float)lo[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[fm][fn][i] = fmaf(linear, e[i], square * acc[fm][fn][i]);
+        const f16x4_t* at = kept + upd_fragment(row, col, across) / 4;
+        held[0][fm][fn] = f16x4_t{0, 0, 0, 0};
+        if constexpr (TERMS == 3) held[1][fm][fn] = f16x4_t{0, 0, 0, 0};
+        if (!within(fm, fn)) continue;
+        held[0][fm][fn] = at[0];
+        if constexpr (TERMS == 3) held[1][fm][fn] = at[kept_plane];
       }
-    upd_write_symmetric<F, TERMS>(lds, ws + a.d, plane, row0, col0, a.r, a.ld_r,
-                                  [&](int fm, int fn, int i) { return acc[fm][fn][i]; });
+    upd_write_symmetric<F, TERMS>(
+        lds, ws + a.d, plane, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
+          if (TERMS == 1 || t == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float e = (float)held[0][fm][fn][i];
+              if constexpr (TERMS == 3) e += (float)held[1][fm][fn][i];
+              x[i] = fmaf(linear, e, square * acc[fm][fn][i]);
+            }
+            if constexpr (TERMS == 3) acc[fm][fn] = f32x4_t{x[0], x[1], x[2], x[3]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = acc[fm][fn][i];
+          }
+        });
   }
 }
 
@@ -386,77 +410,105 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   float* carrier = reinterpret_cast<float*>(ws + a.carrier);
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)matrix * a.m * a.n;
   const UpdPlace<F> p;
-  float ss = 0.f;
+  const int32_t across = (a.n + 15) / 16;
+  // a wave's fragment that lies at least partly within the matrix
+  auto within = [&](int fm, int fn) {
+    return row0 + (int32_t)(wave_id() >> 1) * 16 * F + 16 * fm < a.m &&
+           col0 + (int32_t)(wave_id() & 1u) * 16 * F + 16 * fn < a.n;
+  };
+  // X before the step: G, or what the last step left, which is zero past the matrix's ends
+  auto fetch = [&](int fm, f32x4_t (&x)[F]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int fm = 0; fm < F; ++fm)
+    for (int fn = 0; fn < F; ++fn) {
+      x[fn] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (!within(fm, fn)) continue;
+      const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
+      if (!a.first) {
+        x[fn] = *reinterpret_cast<const f32x4_t*>(carrier + upd_fragment(row, col, across));
+        continue;
+      }
+      const T* from = in + (int64_t)row * a.in_row + col;
+      if (row >= a.m) continue;
+      if (!a.vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (col + i < a.n) x[fn][i] = (float)from[i];
+      } else if (col < a.n) {  // (n and the rows' distance are whole vectors: four aligned elements)
+        if constexpr (sizeof(T) == 4) {
+          x[fn] = *reinterpret_cast<const f32x4_t*>(from);
+        } else {
+          const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            x[fn][i] = __uint_as_float((i & 1) ? (v[i / 2] & 0xffff0000u) : (v[i / 2] << 16));
+        }
+      }
+    }
+  };
+  // bf16 results of whole vectors leave through the image, the fp16 copies always
+  const bool by_image = sizeof(T) == 2 && a.vec;
+  float ss = 0.f;
+  f32x4_t held[3][F];  // this row of fragments, and two on their way
+  fetch(0, held[0]);
+  if (F > 1) fetch(1, held[1]);
+#pragma unroll
+  for (int fm = 0; fm < F; ++fm) {
+    if (fm + 2 < F) fetch(fm + 2, held[(fm + 2) % 3]);
 #pragma unroll
     for (int fn = 0; fn < F; ++fn) {
       const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
-      if (row < a.m && col < a.n) {
-        const int32_t left = a.n - col;
-        float x[4];
-        float* held = carrier + (int64_t)row * a.ld_n + col;
-        if (a.first) {
-          const T* from = in + (int64_t)row * a.in_row + col;
-          if (a.vec) {  // (n and the rows' distance are whole vectors: four aligned elements)
-            if constexpr (sizeof(T) == 4) {
-              const f32x4_t v = *reinterpret_cast<const f32x4_t*>(from);
+      float x[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[i] = v[i];
-            } else {
-              const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from);
+      for (int i = 0; i < 4; ++i) {
+        x[i] = fmaf(linear, held[fm % 3][fn][i], product * acc[fm][fn][i]);
+        ss = fmaf(x[i], x[i], ss);
+      }
+      if (!a.last) {
+        if (within(fm, fn))
+          *reinterpret_cast<f32x4_t*>(carrier + upd_fragment(row, col, across)) = f32x4_t{x[0], x[1], x[2], x[3]};
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                x[i] = __uint_as_float((i & 1) ? (v[i / 2] & 0xffff0000u) : (v[i / 2] << 16));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = i < left ? (float)from[i] : 0.f;
-          }
+        for (int i = 0; i < 4; ++i) x[i] *= a.x_scale;
+        upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, false);
+        if constexpr (TERMS == 3) acc[fm][fn] = f32x4_t{x[0], x[1], x[2], x[3]};
+      } else if (by_image) {
+        *reinterpret_cast<u32x2_t*>(lds + (p.row + 16 * fm) * upd_pitch(F) + (p.col + 16 * fn) * 2) =
+            u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+      } else if (row < a.m) {
+        T* to = out + (int64_t)row * a.n + col;
+        if (sizeof(T) == 4 && a.vec) {
+          if (col < a.n) *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
         } else {
-          const f32x4_t v = *reinterpret_cast<const f32x4_t*>(held);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = i < left ? v[i] : 0.f;
+          for (int i = 0; i < 4; ++i)
+            if (col + i < a.n) to[i] = (T)x[i];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = fmaf(linear, x[i], product * acc[fm][fn][i]);
-          if (i < left) ss = fmaf(x[i], x[i], ss);
-        }
-        if (a.last) {
-          T* to = out + (int64_t)row * a.n + col;
-          if (a.vec) {
-            if constexpr (sizeof(T) == 4)
-              *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
-            else
-              *reinterpret_cast<u32x2_t*>(to) = u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (i < left) to[i] = (T)x[i];
-          }
-        } else {
-          *reinterpret_cast<f32x4_t*>(held) = f32x4_t{x[0], x[1], x[2], x[3]};
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[fm][fn][i] = x[i] * a.x_scale;
       }
     }
-  if (a.last) return;
-  // (columns and rows past the end are zero: D and S are there)
+    sched_fence();
+  }
+  if (a.last) {
+    if (!by_image) return;
+    __syncthreads();
+    upd_write_rows<F>(lds, reinterpret_cast<char*>(out), row0, col0, a.m, a.n);
+    return;
+  }
   const int64_t plane_s = (int64_t)a.c * a.ld_r * 2, plane_l = (int64_t)a.r * a.ld_c * 2;
 #pragma unroll
   for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
-    if (t) __syncthreads();
+    if (t) {
+      __syncthreads();
 #pragma unroll
-    for (int fm = 0; fm < F; ++fm)
+      for (int fm = 0; fm < F; ++fm) {
 #pragma unroll
-      for (int fn = 0; fn < F; ++fn) {
-        float x[4];
+        for (int fn = 0; fn < F; ++fn) {
+          float x[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = acc[fm][fn][i];
-        upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, t);
+          for (int i = 0; i < 4; ++i) x[i] = acc[fm][fn][i];
+          upd_put<F>(lds, p.row + 16 * fm, p.col + 16 * fn, x, true);
+        }
+        sched_fence();
       }
+    }
     __syncthreads();
     char* l = ws + a.l + t * plane_l;
     char* next = ws + a.s1 + t * plane_s;
