@@ -96,19 +96,29 @@ bool upd_scales(const double* k, double most, UpdScales& s) {
   return std::isfinite(top) && top < 1e6 && hi - lo < 1e12;
 }
 
-// The tile of a product of tiles(t) output tiles of t x t: the one whose rounds over the
-// CUs cost least.  A CU takes one workgroup of 256- or 192-tiles at a time, two of 128 and
-// four of 64.
+// The tile of a product of tiles(t) output tiles of t x t, `stages` stages of K each, that
+// move `bytes` an element beside it: the one that costs least, in us.  A CU takes `load`
+// of them one after the other; tiles of 64 share it and hide most of what they move behind
+// each other's products, the larger ones do not.  A lone tile is as slow as its
+// stages' latency.  The constants are fitted to 24 sizes from 128 x 352 to 14336 x 4096 and
+// 1 to 200 matrices, timed with every tile: the choice is within 7% of the best at each
+// (4096 x 4096, all of its symmetric products in tiles of 64, 128, 192 and 256: 2022, 1831,
+// 1567 and 1807 us; 28 of 256 x 1536: 305, 324, 401, 482).
 template <class Tiles>
-int upd_pick(Tiles tiles, bool split) {
-  static const struct { int F, slots; double rate; } kinds[] = {{8, 1, 1.0}, {6, 1, 0.9}, {4, 2, 0.7}, {2, 4, 0.35}};
+int upd_pick(Tiles tiles, double stages, double bytes, bool split) {
+  static const struct { int F; double stage, alone, exposed; } kinds[] = {
+      {8, 1.6, 0.75, 1.0}, {6, 1.07, 0.72, 1.0}, {4, 0.54, 0.3, 1.0}, {2, 0.25, 0.22, 0.36}};
+  constexpr double kRate = 21e3;  // bytes a us of a CU, when all of them ask
   int best = 2;
   double least = INFINITY;
   for (const auto& k : kinds) {
     if (split && k.F == 8) continue;  // (its two writes of an image would spill)
-    const int64_t load = cdiv(tiles(upd_tile(k.F)), kUpdCus);
-    const double alone = k.rate * (0.5 + 0.5 * std::min<double>(1.0, (double)load / k.slots));
-    const double cost = (double)load * k.F * k.F / alone;
+    const int64_t n = tiles(upd_tile(k.F));
+    const double busy = std::min(1.0, std::max((double)n / kUpdCus, 0.15));
+    const double moved = bytes * upd_tile(k.F) * upd_tile(k.F) / kRate * busy, product = stages * k.stage;
+    const double many = (double)cdiv(n, kUpdCus) *
+                        (std::max(moved, product) + k.exposed * std::min(moved, product));
+    const double cost = std::max(many, 2.0 + 0.145 * k.F * k.F + stages * k.alone + moved);
     if (cost < least) least = cost, best = k.F;
   }
   return best;
@@ -140,7 +150,10 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
 
   const auto triangle = [&](int64_t t) { return k.batch * (cdiv(k.r, t) * (cdiv(k.r, t) + 1) / 2); };
   const auto all = [&](int64_t t) { return k.batch * cdiv(k.m, t) * cdiv(k.n, t); };
-  const int symmetric = upd_pick(triangle, TERMS == 3), apply = upd_pick(all, TERMS == 3);
+  // both symmetric products go by one tile (fragments of E pass between them): by their mean
+  constexpr int planes = TERMS == 3 ? 2 : 1;
+  const int symmetric = upd_pick(triangle, TERMS * (cdiv(k.c, 64) + cdiv(k.r, 64)) / 2.0, 6.0 * planes, TERMS == 3);
+  const int apply = upd_pick(all, (double)TERMS * cdiv(k.r, 64), 8.0 + 4.0 * planes, TERMS == 3);
   constexpr int kMost = TERMS == 3 ? 6 : 8;
   double most = 1.0;
   UpdScales now, next;
