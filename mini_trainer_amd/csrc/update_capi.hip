@@ -9,6 +9,7 @@
 #include "../../include/mt_flce.h"
 #include "capi_common.h"
 #include "update_kernels.h"
+#include "update_small.h"
 
 using namespace mtf;
 
@@ -134,6 +135,30 @@ int upd_with(int kind, F f) {
   }
 }
 
+// The fragment rows of the small matrices' kernel that a matrix goes to, or 0.
+int upd_small_rows(const UpdLayout& l, int steps, int terms) {
+  if (steps > kUpdSmallSteps) return 0;
+  for (int R = 1; R <= (terms == 3 ? 4 : 8); R *= 2)
+    if (l.r <= 16 * R)
+      return l.c <= 128 * upd_small_columns(R, terms) && upd_small_lds(R, l.c, terms) <= kUpdSmallLds ? R : 0;
+  return 0;
+}
+
+template <class T>
+int launch_small(int R, const UpdSmallArgs& k, int64_t batch, hipStream_t stream) {
+  constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
+  const auto with = [&](auto rows) {
+    hipLaunchKernelGGL((upd_small_kernel<T, decltype(rows)::value, TERMS>), dim3((uint32_t)batch), dim3(512), 0, stream,
+                       k);
+    return check_launch("upd_small_kernel");
+  };
+  if (R == 1) return with(std::integral_constant<int, 1>());
+  if (R == 2) return with(std::integral_constant<int, 2>());
+  if (TERMS == 3 || R == 4) return with(std::integral_constant<int, 4>());
+  if constexpr (TERMS == 1) return with(std::integral_constant<int, 8>());
+  return MT_OK;
+}
+
 template <class T>
 int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t stream) {
   constexpr int V = 16 / (int)sizeof(T), TERMS = sizeof(T) == 4 ? 3 : 1;
@@ -198,7 +223,8 @@ extern "C" {
 size_t mt_orthogonalize_workspace_bytes(const mt_orthogonalize_args* args) {
   UpdLayout l;
   if (!args || args->batch < 1 || args->batch > (1 << 24) || !esize(args->dtype) ||
-      !upd_layout(args->m, args->n, args->dtype, l))
+      !upd_layout(args->m, args->n, args->dtype, l) ||
+      upd_small_rows(l, args->steps, args->dtype == MT_DTYPE_F32 ? 3 : 1))
     return 0;
   return (size_t)(l.bytes * std::max<int64_t>(1, std::min(args->batch, kUpdGroup / l.bytes)));
 }
@@ -209,6 +235,12 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   MT_TRY(upd_check(args, l));
   const mt_orthogonalize_args& a = *args;
   if (a.batch == 0 || a.m == 0 || a.n == 0) return MT_OK;
+  const int es = esize(a.dtype);
+  const int64_t V = 16 / es;
+  const bool vec = aligned16(a.in) && aligned16(a.out) && a.n % V == 0 && (a.m == 1 || a.in_row % V == 0) &&
+                   (a.batch == 1 || a.in_batch % V == 0);
+  const int small = upd_small_rows(l, a.steps, a.dtype == MT_DTYPE_F32 ? 3 : 1);
+  UpdSmallArgs sm{};
   double most = 1.0;
   for (int step = 0; step < a.steps; ++step) {  // before anything is launched
     UpdScales s;
@@ -218,12 +250,31 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
     if (!upd_scales(q, most, s))
       return fail(MT_ERR_UNSUPPORTED, "coefficients that carry singular values beyond 10^6");
     most = s.next;
+    if (small) {
+      if (step) sm.step[step - 1].x_scale = std::ldexp(1.f, s.x);
+      sm.step[step] = {(float)q[0], (float)q[1], (float)q[2], std::ldexp(1.f, -s.x), std::ldexp(1.f, s.e),
+                       std::ldexp(1.f, -s.e), std::ldexp(1.f, s.d), std::ldexp(1.f, -s.d), 1.f};
+    }
+  }
+  if (small) {
+    sm.in_row = a.in_row, sm.in_batch = a.in_batch;
+    sm.eps = a.eps;
+    sm.m = (int32_t)a.m, sm.n = (int32_t)a.n, sm.r = (int32_t)l.r, sm.c = (int32_t)l.c;
+    sm.steps = a.steps, sm.vec = vec;
+    constexpr int64_t most_at_once = (int64_t)1 << 22;  // workgroups of a launch
+    for (int64_t at = 0; at < a.batch; at += most_at_once) {
+      const int64_t n = std::min(most_at_once, a.batch - at);
+      sm.in = static_cast<const char*>(a.in) + at * a.in_batch * es;
+      sm.out = static_cast<char*>(a.out) + at * a.m * a.n * es;
+      MT_TRY(a.dtype == MT_DTYPE_BF16 ? launch_small<__bf16>(small, sm, n, (hipStream_t)stream)
+                                      : launch_small<float>(small, sm, n, (hipStream_t)stream));
+    }
+    return MT_OK;
   }
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(MT_ERR_INVALID_ARGUMENT, "null workspace, or one that is not aligned to 256 bytes");
   if (workspace_bytes < (size_t)l.bytes)
     return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, (size_t)l.bytes);
-  const int es = esize(a.dtype);
   // matrices at a time: what the workspace holds, within one launch's workgroups
   const int64_t tiles = cdiv(a.m, 64) * cdiv(a.n, 64);
   const int64_t group = std::min<int64_t>({a.batch, (int64_t)(workspace_bytes / (size_t)l.bytes), 32768,
@@ -238,9 +289,7 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   k.eps = a.eps;
   k.m = (int32_t)a.m, k.n = (int32_t)a.n, k.r = (int32_t)l.r, k.c = (int32_t)l.c;
   k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c;
-  const int64_t V = 16 / es;
-  k.vec = aligned16(a.in) && aligned16(a.out) && a.n % V == 0 && (a.m == 1 || a.in_row % V == 0) &&
-          (a.batch == 1 || a.in_batch % V == 0);
+  k.vec = vec;
   for (int64_t at = 0; at < a.batch; at += group) {
     k.batch = (int32_t)std::min(group, a.batch - at);
     k.in = static_cast<const char*>(a.in) + at * a.in_batch * es;

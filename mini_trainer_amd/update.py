@@ -79,6 +79,7 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
                                    x.stride(1) if m > 1 else n, x.stride(0) if batch > 1 else 0, steps, code)
     lib = load()
     nbytes = lib.mt_orthogonalize_workspace_bytes(args)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=update.device)
-    _launch(update.device, "mt_orthogonalize", lib.mt_orthogonalize, args, ws.data_ptr(), nbytes)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=update.device) if nbytes else None
+    _launch(update.device, "mt_orthogonalize", lib.mt_orthogonalize, args, 0 if ws is None else ws.data_ptr(),
+            nbytes)
     return out

@@ -30,8 +30,9 @@ def make(*shape, dtype=torch.bfloat16, seed=0, rank=0, scale=1.0):
 
 @BOTH
 @pytest.mark.parametrize("m,n", [(1, 1), (1, 100), (100, 1), (2, 3), (8, 24), (63, 65), (64, 64), (65, 200),
-                                 (128, 352), (352, 128), (130, 127), (257, 300), (300, 257), (96, 1000),
-                                 (1000, 1030)])
+                                 (128, 352), (352, 128), (128, 353), (130, 127), (257, 300), (300, 257),
+                                 (96, 1000), (16, 4096), (17, 2048), (2049, 32), (33, 1000), (1000, 64), (64, 460),
+                                 (4100, 16), (1000, 1030)])
 def test_matches_the_definition(gpu, m, n, dtype):
     x = make(m, n, dtype=dtype, seed=m + n)
     out = orthogonalize(x)
@@ -51,8 +52,9 @@ def test_stacks(gpu, shape, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("batch,m,n", [(1, 2048, 2048), (1, 4100, 1990), (3, 1400, 2000), (40, 500, 700),
-                                       (2, 2300, 2300), (1, 1536, 5000)])
+@pytest.mark.parametrize("batch,m,n", [(1, 962, 2144), (15, 327, 338), (3, 1106, 1515), (43, 351, 336),
+                                       (11, 716, 1483), (7, 849, 721), (53, 197, 459), (40, 814, 515),
+                                       (31, 519, 560), (30, 705, 870), (1, 4100, 1990), (2, 2300, 2300)])
 def test_every_tile(gpu, batch, m, n, dtype):
     """Sizes that take each tile of the symmetric products and of the last one."""
     x = make(batch, m, n, dtype=dtype, seed=m)
@@ -110,7 +112,7 @@ def test_special_spectra(gpu, dtype):
 @BOTH
 def test_steps_and_coefficients(gpu, dtype):
     x = make(40, 60, dtype=dtype, seed=9)
-    for steps in (1, 2, 6, 10):
+    for steps in (1, 2, 6, 10, 16, 17):
         ref.assert_within(orthogonalize(x, steps=steps), x, steps=steps)
     each = [(4.0, -7.0, 3.5), (3.0, -3.5, 1.4), (1.5, -0.5, 0.0)]
     ref.assert_within(orthogonalize(x, steps=3, coefficients=each), x, steps=3, coefficients=each)
@@ -143,12 +145,12 @@ def test_nothing_to_do(gpu):
 
 def test_a_workspace_of_one_matrix(gpu):
     """The stack in parts, each through the same memory."""
-    x = make(5, 70, 130, seed=13)
+    x = make(5, 170, 130, seed=13)
     want = orthogonalize(x)
     out = torch.empty_like(x)
     k = (ctypes.c_double * 15)(*ref.COEFFICIENTS * 5)
     a = _lib.OrthogonalizeArgs(input=x.data_ptr(), out=out.data_ptr(), coefficients=ctypes.addressof(k), eps=1e-7,
-                               batch=1, m=70, n=130, in_row=130, in_batch=70 * 130, steps=5, dtype=1)
+                               batch=1, m=170, n=130, in_row=130, in_batch=170 * 130, steps=5, dtype=1)
     lib = _lib.load()
     nbytes = lib.mt_orthogonalize_workspace_bytes(ctypes.byref(a))
     a.batch = 5

@@ -21,7 +21,7 @@ FIVE = (ctypes.c_double * 15)(*ref.COEFFICIENTS * 5)
 def args(coefficients=FIVE, **kw):
     a = _lib.OrthogonalizeArgs()
     base = dict(input=P, out=P, coefficients=ctypes.addressof(coefficients) if coefficients else None, eps=1e-7,
-                batch=2, m=40, n=72, in_row=72, in_batch=40 * 72, steps=5, dtype=1)
+                batch=2, m=140, n=172, in_row=172, in_batch=140 * 172, steps=5, dtype=1)
     for name, value in {**base, **kw}.items():
         setattr(a, name, value)
     return a
@@ -32,7 +32,7 @@ def args(coefficients=FIVE, **kw):
     (dict(steps=65), 1), (dict(eps=-1.0), 1), (dict(eps=math.nan), 1), (dict(eps=math.inf), 1),
     (dict(coefficients=None), 1), (dict(batch=BIG), 3), (dict(m=BIG), 3), (dict(n=BIG), 3),
     (dict(m=32768, n=32768, in_row=32768), 3), (dict(m=1, n=1 << 24, in_row=1 << 24), 3),
-    (dict(in_row=71), 1), (dict(in_row=BIG), 1), (dict(in_batch=-1), 1), (dict(in_batch=BIG), 1),
+    (dict(in_row=171), 1), (dict(in_row=BIG), 1), (dict(in_batch=-1), 1), (dict(in_batch=BIG), 1),
     (dict(input=None), 1), (dict(out=None), 1), (dict(input=P + 1), 1), (dict(out=P + 1), 1),
     (dict(coefficients=(ctypes.c_double * 15)(*[40.0, 0.0, 0.0] * 5)), 3),
     (dict(coefficients=(ctypes.c_double * 15)(*[3.0, math.nan, 0.0] * 5)), 1),
@@ -47,7 +47,7 @@ def test_host_checks(kw, code):
 def test_workspace():
     lib = _lib.load()
     need = lib.mt_orthogonalize_workspace_bytes(ctypes.byref(args()))
-    assert need % 512 == 0 and need >= 2 * (40 * 128 * 2 + 2 * 72 * 64 * 2 + 2 * 40 * 64 * 2 + 40 * 128 * 4)
+    assert need % 512 == 0 and need >= 2 * (140 * 192 * 2 + 2 * 172 * 192 * 2 + 3 * 140 * 192 * 2 + 140 * 172 * 4)
     one = lib.mt_orthogonalize_workspace_bytes(ctypes.byref(args(batch=1)))
     assert need == 2 * one
     assert lib.mt_orthogonalize(ctypes.byref(args()), P, one - 1, None) == 2
@@ -60,6 +60,14 @@ def test_workspace():
     assert lib.mt_orthogonalize_workspace_bytes(ctypes.byref(big)) == (2 << 30) // single * single
     for kw in (dict(batch=0), dict(m=0), dict(m=BIG), dict(batch=BIG), dict(dtype=9), dict(batch=-BIG)):
         assert lib.mt_orthogonalize_workspace_bytes(ctypes.byref(args(**kw))) == 0
+    # small matrices take none
+    for m, n, dtype, none in ((128, 352, 1, True), (352, 128, 1, True), (128, 353, 1, False), (16, 4096, 1, True),
+                              (16, 4097, 1, False), (17, 2048, 1, True), (64, 992, 1, True), (64, 993, 1, False), (129, 129, 1, False),
+                              (64, 416, 0, True), (64, 417, 0, False), (65, 65, 0, False), (16, 2400, 0, True)):
+        a = args(batch=1, m=m, n=n, in_row=n, dtype=dtype)
+        assert (lib.mt_orthogonalize_workspace_bytes(ctypes.byref(a)) == 0) == none, (m, n, dtype)
+        a = args(batch=1, m=m, n=n, in_row=n, dtype=dtype, steps=17)
+        assert lib.mt_orthogonalize_workspace_bytes(ctypes.byref(a)) > 0
     # nothing to do: no launch
     for kw in (dict(batch=0), dict(m=0), dict(n=0)):
         assert lib.mt_orthogonalize(ctypes.byref(args(**kw, input=None, out=None)), None, 0, None) == 0
