@@ -22,9 +22,19 @@ constexpr int64_t kUpdGroup = (int64_t)2 << 30; // bytes of the workspace that a
 constexpr int kUpdMostSteps = 64;
 constexpr int kUpdCus = 256;
 
+// Workgroups that share the long axis, `stages` of K, of each of `tiles` tiles of 64 of A: as
+// many as fill the CUs twice, at most 16, where that saves more than the launch that adds
+// their parts costs (a stage of a lone tile 0.22 us, the launch 6).  One 256 x 16384 (10
+// tiles of 256 stages): 424 -> 190 us.
+int64_t upd_split(int64_t tiles, int64_t stages) {
+  if (tiles >= kUpdCus) return 1;
+  const int64_t n = std::min<int64_t>({16, 2 * kUpdCus / tiles, stages / 4});
+  return n > 1 && 0.22 * (double)(stages - cdiv(stages, n)) > 6.0 ? n : 1;
+}
+
 struct UpdLayout {
   int64_t r, c, ld_r, ld_c;
-  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, bytes;  // of one matrix
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, parts, bytes;  // of one matrix
 };
 bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   const auto up = [](int64_t v) { return cdiv(v, 64) * 64; };
@@ -45,6 +55,8 @@ bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   take(x.partial, cdiv(m, 64) * cdiv(n, 64) * 4);  // (of the smallest tiles)
   take(x.norm, kUpdParts * 8);
   take(x.state, kUpdState * 4);
+  const int64_t tiles = cdiv(x.r, 64) * (cdiv(x.r, 64) + 1) / 2, split = upd_split(tiles, x.ld_c / 64);  // (a stack splits less)
+  take(x.parts, split > 1 ? tiles * split * 64 * 64 * 4 : 0);
   x.bytes = at;
   return true;
 }
@@ -162,8 +174,10 @@ int launch_small(int R, const UpdSmallArgs& k, int64_t batch, hipStream_t stream
 template <class T>
 int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t stream) {
   constexpr int V = 16 / (int)sizeof(T), TERMS = sizeof(T) == 4 ? 3 : 1;
+  const int64_t small_tiles = cdiv(k.r, 64) * (cdiv(k.r, 64) + 1) / 2;
+  k.split = (int32_t)upd_split(k.batch * small_tiles, k.ld_c / 64);
   const int64_t runs = (int64_t)k.m * cdiv(k.n, 256 * (k.vec ? V : 1));
-  k.norm_parts = (int32_t)std::min<int64_t>(runs, kUpdParts);
+  k.norm_parts = (int32_t)std::min<int64_t>(cdiv(runs, 4), kUpdParts);
   const dim3 norm_grid((uint32_t)k.norm_parts, (uint32_t)k.batch);
   if (k.vec) hipLaunchKernelGGL((upd_norm_kernel<T, V>), norm_grid, dim3(256), 0, stream, k);
   else hipLaunchKernelGGL((upd_norm_kernel<T, 1>), norm_grid, dim3(256), 0, stream, k);
@@ -198,9 +212,16 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
       k.tiles_m = k.tiles_n = (int32_t)cdiv(k.r, upd_tile(f));
       k.tiles = k.tiles_m * (k.tiles_m + 1) / 2;
       const dim3 grid((uint32_t)(k.tiles * k.batch));
-      hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, false>), grid, dim3(256), 0, stream, k);
+      if (f == 2 && k.split > 1) {
+        hipLaunchKernelGGL((upd_symmetric_kernel<2, TERMS, kUpdPart>), dim3(grid.x * (uint32_t)k.split), dim3(256), 0,
+                           stream, k);
+        MT_TRY(check_launch("upd_symmetric_kernel"));
+        hipLaunchKernelGGL((upd_symmetric_kernel<2, TERMS, kUpdJoin>), grid, dim3(256), 0, stream, k);
+      } else {
+        hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, kUpdWhole>), grid, dim3(256), 0, stream, k);
+      }
       MT_TRY(check_launch("upd_symmetric_kernel"));
-      hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, true>), grid, dim3(256), 0, stream, k);
+      hipLaunchKernelGGL((upd_symmetric_kernel<f, TERMS, kUpdSquare>), grid, dim3(256), 0, stream, k);
       return check_launch("upd_symmetric_kernel");
     }));
     MT_TRY(upd_with<kMost>(apply, [&](auto F) {
@@ -286,6 +307,7 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   k.in_row = a.in_row, k.in_batch = a.in_batch;
   k.l = l.l, k.s0 = l.s0, k.s1 = l.s1, k.e = l.e, k.d = l.d;
   k.fragments = l.fragments, k.carrier = l.carrier, k.partial = l.partial, k.norm = l.norm, k.state = l.state;
+  k.parts = l.parts;
   k.eps = a.eps;
   k.m = (int32_t)a.m, k.n = (int32_t)a.n, k.r = (int32_t)l.r, k.c = (int32_t)l.c;
   k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c;

@@ -36,9 +36,12 @@ constexpr int kUpdStage = 64;  // K elements of a stage
 constexpr int upd_tile(int F) { return 32 * F; }
 constexpr int upd_slot(int F) { return upd_tile(F) * 128; }   // bytes: one operand, one stage
 constexpr int upd_pitch(int F) { return upd_tile(F) * 2 + 16; }  // bytes of an image row, see below
-// Stages of B that the ring holds (A: 3).
+// Stages of A and of B that the ring holds.  More would cost tiles of 64 their neighbours on
+// the CU (4 instead of 3: one 256 x 16384 370 instead of 424 us, 28 of 256 x 1536 289 instead
+// of 261).
+constexpr int upd_slots_a(int) { return 3; }
 constexpr int upd_slots_b(int F) { return F == 8 ? 2 : 3; }
-constexpr int upd_lds(int F) { return (3 + upd_slots_b(F)) * upd_slot(F); }  // (an image of the tile fits in)
+constexpr int upd_lds(int F) { return (upd_slots_a(F) + upd_slots_b(F)) * upd_slot(F); }
 
 __device__ __forceinline__ f32x4_t upd_mma(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b),
@@ -88,12 +91,13 @@ __device__ __forceinline__ void upd_wait_vm() {  // every DMA but the last N iss
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
-// acc = sum over KT stages, and with TERMS = 3 over the planes (value, rest) x (rest,
+// acc = sum over the KT stages from `first` on, and with TERMS = 3 over the planes (value, rest) x (rest,
 // value) and (value, value), of A B^T.
 template <int F, int TERMS>
-__device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, const UpdOperand<F>& b, int KT,
-                                             f32x4_t (&acc)[F][F]) {
-  constexpr int kSlot = upd_slot(F), NB = upd_slots_b(F);
+__device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, const UpdOperand<F>& b, int first,
+                                             int KT, f32x4_t (&acc)[F][F]) {
+  constexpr int kSlot = upd_slot(F), NA = upd_slots_a(F), NB = upd_slots_b(F);
+  static_assert(NA == NB || NA == NB + 1, "what the waits count on");
   static_assert(upd_lds(F) >= upd_tile(F) * upd_pitch(F), "an image of the tile");
   // MFMAs before each LDS read; the others follow the last one and hide its latency
   constexpr int kPer = F >= 8 ? 3 : F >= 6 ? 2 : 1;
@@ -105,7 +109,7 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   auto at = [&](int s, int& term, int& kt) __attribute__((always_inline)) {
     s = s < stages ? s : stages - 1;
     term = TERMS == 1 ? 0 : s >= 2 * KT ? 2 : s >= KT ? 1 : 0;
-    kt = s - term * KT;
+    kt = first + s - term * KT;
   };
   auto issue_a = [&](char* slot, int term, int kt, int i) __attribute__((always_inline)) {
     a.issue(slot, TERMS == 3 && term == 1, kt, i);
@@ -117,18 +121,18 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   for (int m = 0; m < F; ++m)
 #pragma unroll
     for (int n = 0; n < F; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // stages 0 and 1, and B of those that phases 2 are ahead
+  // the stages that the phases are ahead
 #pragma unroll
-  for (int s = 0; s < NB; ++s) {
+  for (int s = 0; s < (NA - 1 > NB ? NA - 1 : NB); ++s) {
     int term, kt;
     at(s, term, kt);
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      if (s < 2) issue_a(slots_a + s * kSlot, term, kt, i);
-      issue_b(slots_b + s * kSlot, term, kt, i);
+      if (s < NA - 1) issue_a(slots_a + s * kSlot, term, kt, i);
+      if (s < NB) issue_b(slots_b + s * kSlot, term, kt, i);
     }
   }
-  upd_wait_vm<F * (2 * NB - 3 - (NB - 2))>();  // stage 0
+  upd_wait_vm<F * (NA + NB - 3)>();  // stage 0: of A NA - 2 stages follow it, of B NB - 1
   __builtin_amdgcn_s_barrier();
   u32x4_t fa0[F], fb0[F], fa1[F], fb1[F];
 #pragma unroll
@@ -140,12 +144,12 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   int ga = 0, gb = 0;  // slots of stage g
   for (int g = 0; g < stages; ++g) {
     sched_fence();
-    const int ga1 = ga == 2 ? 0 : ga + 1, ga2 = ga == 0 ? 2 : ga - 1;  // of stages g + 1 and g + 2
+    const int ga1 = ga == NA - 1 ? 0 : ga + 1, gap = ga == 0 ? NA - 1 : ga - 1;  // of stages g + 1 and g - 1
     const int gb1 = gb == NB - 1 ? 0 : gb + 1;
     const char* ra = slots_a + ga * kSlot;
     const char* rb = slots_b + gb * kSlot;
     int term, kt;
-    at(g + 2, term, kt);
+    at(g + NA - 1, term, kt);
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
 #pragma unroll
@@ -155,16 +159,16 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
       }
       if (i & 1) fb1[i >> 1] = b.read(rb, 1, i >> 1);
       else fa1[i >> 1] = a.read(ra, 1, i >> 1);
-      if (i & 1) issue_a(slots_a + ga2 * kSlot, term, kt, i >> 1);
+      if (i & 1) issue_a(slots_a + gap * kSlot, term, kt, i >> 1);
       sched_fence();
     }
 #pragma unroll
     for (int k = 2 * F * kPer; k < F * F; ++k)
       acc[k / F][k % F] = upd_mma(fb0[k % F], fa0[k / F], acc[k / F][k % F]);
     sched_fence();
-    // stage g + 1 has landed: A of g + 2 was issued since, and B of g + 2 with three slots
+    // stage g + 1 has landed: the stages g + 2 .. g + NA - 1 of A and .. g + NB - 1 of B follow it
     lgkm_wait0();
-    upd_wait_vm<F * (NB - 1)>();
+    upd_wait_vm<F * (NA + NB - 4)>();
     __builtin_amdgcn_s_barrier();
     sched_fence();
     const char* ra1 = slots_a + ga1 * kSlot;

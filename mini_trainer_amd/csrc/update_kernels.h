@@ -31,7 +31,7 @@
 
 namespace mtf {
 
-constexpr int kUpdParts = 256;  // partial sums of squares of G, at most
+constexpr int kUpdParts = 1024;  // partial sums of squares of G, at most
 
 // Per matrix, in fp32: the factor of X0 over its fp16 copy, 1 / (|G| + eps), mu.
 enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdState = 4 };
@@ -41,11 +41,12 @@ struct UpdArgs {
   char* out;
   char* ws;               // of the first matrix; the others follow ws_stride bytes apart
   int64_t ws_stride, in_row, in_batch;
-  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state;  // byte offsets
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, parts;  // byte offsets
   double eps;
   int32_t m, n, r, c, ld_r, ld_c;        // ld_r, ld_c: r and c up to whole stages
   int32_t norm_parts, partials;          // partial sums of |G|^2, and of |X|^2
   int32_t batch, tiles_m, tiles_n, tiles;
+  int32_t split;                         // workgroups of a tile of A
   int32_t first, last;                   // of the steps
   float a, b, cc;                        // the step's coefficients
   float x_unscale, e_scale, e_unscale, d_scale, d_unscale, x_scale;
@@ -61,15 +62,28 @@ __global__ __launch_bounds__(256) void upd_norm_kernel(UpdArgs a) {
   const int32_t per_row = (a.n + 256 * V - 1) / (256 * V);
   const int64_t runs = (int64_t)a.m * per_row;
   double s = 0.0;
-  for (int64_t u = blockIdx.x; u < runs; u += a.norm_parts) {
-    const int64_t row = u / per_row;
-    const int32_t col = (int32_t)(u - row * per_row) * 256 * V + (int32_t)threadIdx.x * V;
-    if (col >= a.n) continue;
-    float x[V];
-    if constexpr (V > 1) NormVec<T, V>::load(in + row * a.in_row + col, x);
-    else x[0] = (float)in[row * a.in_row + col];
+  constexpr int U = 4;  // runs in flight
+  for (int64_t u0 = blockIdx.x; u0 < runs; u0 += (int64_t)U * a.norm_parts) {
+    T raw[U][V];
+    bool there[U];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s = fma((double)x[i], (double)x[i], s);
+    for (int k = 0; k < U; ++k) {
+      const int64_t u = u0 + (int64_t)k * a.norm_parts;
+      const uint32_t row = (uint32_t)(u < runs ? u : 0) / (uint32_t)per_row;  // (runs: below 2^31)
+      const int32_t col = (int32_t)((uint32_t)(u < runs ? u : 0) - row * per_row) * 256 * V + (int32_t)threadIdx.x * V;
+      there[k] = u < runs && col < a.n;
+      typedef T vec_t __attribute__((ext_vector_type(V)));
+      const vec_t v = *reinterpret_cast<const vec_t*>(in + (there[k] ? row * a.in_row + col : 0));
+#pragma unroll
+      for (int i = 0; i < V; ++i) raw[k][i] = v[i];
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const double x = there[k] ? (double)(float)raw[k][i] : 0.0;
+        s = fma(x, x, s);
+      }
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
@@ -91,7 +105,7 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
   __shared__ double sums[4];
   char* ws = a.ws + (int64_t)blockIdx.y * a.ws_stride;
   double s = 0.0;
-  if ((int)threadIdx.x < a.norm_parts) s = reinterpret_cast<const double*>(ws + a.norm)[threadIdx.x];
+  for (int i = threadIdx.x; i < a.norm_parts; i += 256) s += reinterpret_cast<const double*>(ws + a.norm)[i];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
   if (lane_id() == 0) sums[wave_id()] = s;
@@ -282,22 +296,29 @@ __device__ __forceinline__ int64_t upd_fragment(int32_t row, int32_t col, int32_
   return ((int64_t)(row >> 4) * across + (col >> 4)) * 256 + 4 * (int32_t)lane_id();
 }
 
-// E = A - mu I from L (SQUARE false), or D = (b + 2 c mu) E + c E^2 from E.
-template <int F, int TERMS, bool SQUARE>
+// What upd_symmetric_kernel computes: E = A - mu I from L, whole tiles of it, its parts where
+// a.split workgroups share a tile's long axis (few tiles), or the sum of these parts, in
+// their order; or D = (b + 2 c mu) E + c E^2 from E.
+enum { kUpdWhole, kUpdPart, kUpdJoin, kUpdSquare };
+
+template <int F, int TERMS, int WHAT>
 __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[upd_lds(F)];
   float* sums = reinterpret_cast<float*>(lds);  // (before and after the tile)
-  const uint32_t id = xcd_remap(blockIdx.x, gridDim.x);
-  const uint32_t matrix = id / (uint32_t)a.tiles;
+  constexpr bool SQUARE = WHAT == kUpdSquare;
+  const uint32_t group = xcd_remap(blockIdx.x, gridDim.x);
+  const uint32_t id = WHAT == kUpdPart ? group / (uint32_t)a.split : group;
+  const uint32_t matrix = id / (uint32_t)a.tiles, tile = id - matrix * (uint32_t)a.tiles;
   uint32_t ti, tj;
-  upd_triangle(id - matrix * (uint32_t)a.tiles, (uint32_t)a.tiles_m, ti, tj);
+  upd_triangle(tile, (uint32_t)a.tiles_m, ti, tj);
   char* ws = a.ws + (int64_t)__builtin_amdgcn_readfirstlane(matrix) * a.ws_stride;
   const int32_t row0 = (int32_t)ti * upd_tile(F), col0 = (int32_t)tj * upd_tile(F);
   const UpdMatrix x = SQUARE ? UpdMatrix{ws + a.e, (uint32_t)a.r * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.r}
                              : UpdMatrix{ws + a.l, (uint32_t)a.r * (uint32_t)a.ld_c * 2u, (uint32_t)a.ld_c, (uint32_t)a.r};
   float* state = reinterpret_cast<float*>(ws + a.state);
   float mu = 0.f;
-  if constexpr (!SQUARE) {
+  if constexpr (WHAT == kUpdPart) {
+  } else if constexpr (!SQUARE) {
     if (a.first) {
       mu = state[kUpdMu];
     } else {  // |X|^2 / r from the tiles of the product before: the same in every workgroup
@@ -314,11 +335,38 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
   } else {
     mu = state[kUpdMu];
   }
-  UpdOperand<F> oa, ob;
-  oa.init(x, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
-  ob.init(x, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
   f32x4_t acc[F][F];
-  upd_mainloop<F, TERMS>(lds, oa, ob, (int)x.ld / kUpdStage, acc);
+  // the parts of this tile, by fragments
+  f32x4_t* parts = reinterpret_cast<f32x4_t*>(ws + a.parts) + (int64_t)tile * a.split * F * F * 256 + threadIdx.x;
+  if constexpr (WHAT == kUpdJoin) {
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+      for (int n = 0; n < F; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int q = 0; q < a.split; ++q)
+#pragma unroll
+      for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n) acc[m][n] += parts[(q * F * F + m * F + n) * 256];
+  } else {
+    UpdOperand<F> oa, ob;
+    oa.init(x, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
+    ob.init(x, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
+    const int stages = (int)x.ld / kUpdStage;
+    if constexpr (WHAT == kUpdPart) {
+      const int part = (int)(group - id * (uint32_t)a.split);
+      const int begin = stages * part / a.split, end = stages * (part + 1) / a.split;
+      upd_mainloop<F, TERMS>(lds, oa, ob, begin, end - begin, acc);
+#pragma unroll
+      for (int m = 0; m < F; ++m)
+#pragma unroll
+        for (int n = 0; n < F; ++n) parts[(part * F * F + m * F + n) * 256] = acc[m][n];
+      return;
+    } else {
+      upd_mainloop<F, TERMS>(lds, oa, ob, 0, stages, acc);
+    }
+  }
   const UpdPlace<F> p;
   const int64_t plane = (int64_t)a.r * a.ld_r * 2;
   // E is also kept by fragments, for the product that squares it: the same lanes of the
@@ -401,7 +449,7 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   oa.init(tall ? s : d, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
   ob.init(tall ? d : s, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
   f32x4_t acc[F][F];
-  upd_mainloop<F, TERMS>(lds, oa, ob, a.ld_r / kUpdStage, acc);
+  upd_mainloop<F, TERMS>(lds, oa, ob, 0, a.ld_r / kUpdStage, acc);
   const float* state = reinterpret_cast<const float*>(ws + a.state);
   const float mu = state[kUpdMu];
   const float product = a.d_unscale * (a.first ? state[kUpdFactor] : a.x_unscale);

@@ -32,7 +32,7 @@ def make(*shape, dtype=torch.bfloat16, seed=0, rank=0, scale=1.0):
 @pytest.mark.parametrize("m,n", [(1, 1), (1, 100), (100, 1), (2, 3), (8, 24), (63, 65), (64, 64), (65, 200),
                                  (128, 352), (352, 128), (128, 353), (130, 127), (257, 300), (300, 257),
                                  (96, 1000), (16, 4096), (17, 2048), (2049, 32), (33, 1000), (1000, 64), (64, 460),
-                                 (4100, 16), (1000, 1030)])
+                                 (4100, 16), (100, 5000), (3000, 200), (1000, 1030)])
 def test_matches_the_definition(gpu, m, n, dtype):
     x = make(m, n, dtype=dtype, seed=m + n)
     out = orthogonalize(x)
@@ -41,7 +41,7 @@ def test_matches_the_definition(gpu, m, n, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("shape", [(1, 40, 72), (5, 72, 40), (2, 3, 33, 129), (28, 64, 200), (70, 9, 9)])
+@pytest.mark.parametrize("shape", [(1, 40, 72), (5, 72, 40), (2, 3, 33, 129), (28, 64, 200), (70, 9, 9), (3, 130, 2500)])
 def test_stacks(gpu, shape, dtype):
     x = make(*shape, dtype=dtype, seed=3)
     out = orthogonalize(x)
