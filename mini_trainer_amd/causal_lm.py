@@ -81,7 +81,8 @@ def _output_cls():
 
 
 def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tensor] = None,
-                    packed_layers: bool = False) -> torch.nn.Module:
+                    packed_layers: bool = False, embedding_and_norms: bool = False,
+                    accumulate_embedding: bool = False) -> torch.nn.Module:
     """Give a transformers *ForCausalLM model a forward that, when labels (or
     shift_labels) are passed, runs the decoder, hands its last hidden states
     and the output-embedding weight to causal_lm_loss and returns a
@@ -118,6 +119,14 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
     minibatch is then zero, and `attention_status` of the output (int32 [1] on
     the device) is 1.
     Without labels the model's own attention runs as before.
+
+    With embedding_and_norms (and packed_layers) the labelled forward also runs the
+    decoder's token embedding as token_embedding (torch's own, or transformers' scaled one)
+    and torch's layer norms, where its layers have those, as layer_norm, the one behind the
+    attention of a plain layer as residual_layer_norm.  A token id out of range then gives
+    NaN in place of a device assertion.  accumulate_embedding adds the embedding's gradient
+    to dw_accumulator in fp32, beside the head's, instead of returning it to autograd: for
+    a head that shares the embedding's weight.
     """
     decoder = model.get_decoder()
     head = model.get_output_embeddings()
@@ -125,8 +134,15 @@ def patch_causal_lm(model: torch.nn.Module, dw_accumulator: Optional[torch.Tenso
         raise ValueError("patch_causal_lm needs an output embedding without bias")
     original = model.forward
     softcap = getattr(model.config, "final_logit_softcapping", None)
+    if embedding_and_norms and not packed_layers:
+        raise ValueError("embedding_and_norms is for packed_layers")
+    if accumulate_embedding:
+        if not embedding_and_norms or dw_accumulator is None:
+            raise ValueError("accumulate_embedding needs embedding_and_norms and a dw_accumulator")
+        if decoder.get_input_embeddings().weight is not head.weight:
+            raise ValueError("accumulate_embedding needs a head that shares the embedding's weight")
     if packed_layers:
-        patch_decoder_layers(decoder)
+        patch_decoder_layers(decoder, embedding_and_norms, dw_accumulator if accumulate_embedding else None)
 
     def forward(input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
                 inputs_embeds=None, labels=None, use_cache=None, logits_to_keep=0,

@@ -17,7 +17,8 @@ from typing import Optional
 import torch
 
 from .attention import AttentionPlan, packed_attention, packed_attention_plan
-from .norms import residual_rms_norm
+from .embedding import token_embedding
+from .norms import layer_norm, residual_layer_norm, residual_rms_norm
 
 __all__ = ["AttentionPlans", "patch_decoder_layers", "unlabelled_forward"]
 
@@ -27,6 +28,8 @@ PLANS_KWARG = "mt_attention_plans"
 # and the norms that are rms_norm(x) * weight.
 PLAIN_LAYERS = ("LlamaDecoderLayer", "Qwen2DecoderLayer")
 PLAIN_NORMS = ("LlamaRMSNorm", "Qwen2RMSNorm")
+# The same with layer norms, where those are asked for.
+LAYER_NORM_LAYERS = ("Starcoder2DecoderLayer",)
 # Layer types whose mask is packed_attention's, without and with a window.
 FULL, SLIDING = "full_attention", "sliding_attention"
 # What a layer may hand to its attention beside what _attention reads: none of it
@@ -39,6 +42,10 @@ HARMLESS = ("position_ids", "cache_position", "use_cache", "position_embeddings"
 # attention, and whether the unlabelled forward of a patched model is running.
 _packed = contextvars.ContextVar("mt_packed", default=False)
 _unlabelled = contextvars.ContextVar("mt_unlabelled", default=False)
+# Whether embeddings and layer norms that were patched are the package's: within a
+# decoder's labelled forward, but in a layer only where it is handed the plans, so that a
+# checkpoint's recomputation of the layer does what its first run did.
+_own_ops = contextvars.ContextVar("mt_own_ops", default=False)
 
 
 @contextlib.contextmanager
@@ -54,7 +61,7 @@ def _set(var, value=True):
 def unlabelled_forward():
     """A context in which a patched decoder runs as it was, within another's labelled
     forward too."""
-    with _set(_packed, False), _set(_unlabelled):
+    with _set(_packed, False), _set(_own_ops, False), _set(_unlabelled):
         yield
 
 
@@ -168,10 +175,81 @@ def _has_hooks(module: torch.nn.Module) -> bool:
                 or every._global_backward_pre_hooks)
 
 
+def _own_tensor(t) -> bool:
+    """Whether the package's operators take a module's parameter: a tensor of its own, not a
+    shard or another wrapper."""
+    return type(t) in (torch.Tensor, torch.nn.Parameter) and t.dtype in (torch.bfloat16, torch.float32)
+
+
+def _takes_layer_norm(norm: torch.nn.Module, *tensors) -> bool:
+    """Whether a module is torch's layer norm over one dimension as it is written there, with
+    nothing that wants to see it called, for tensors of its parameters' type."""
+    if type(norm) is not torch.nn.LayerNorm or len(norm.normalized_shape) != 1 or _has_hooks(norm) or \
+            torch.is_autocast_enabled():
+        return False
+    parameters = [p for p in (norm.weight, norm.bias) if p is not None]
+    return all(_own_tensor(p) for p in parameters) and \
+        all(t.dtype in (torch.bfloat16, torch.float32) and t.dtype == tensors[0].dtype
+            for t in (*tensors, *parameters))
+
+
+def _norm_forward(self, input):
+    """torch.nn.LayerNorm's forward: the package's where a labelled forward runs."""
+    if _own_ops.get() and _takes_layer_norm(self, input):
+        return layer_norm(input, self.weight, self.bias, self.eps)
+    return type(self).forward(self, input)
+
+
+def _patch_embedding(module: torch.nn.Module, accumulator: Optional[torch.Tensor]) -> None:
+    """Give a decoder's token embedding a forward that is the package's where a labelled
+    forward runs: torch's own, or transformers' that multiplies by scalar_embed_scale, rounded
+    to the weight's type.  Others, and those with options token_embedding has not (max_norm,
+    sparse, gradients scaled by frequency), keep theirs."""
+    cls = type(module)
+    scaled = cls.__name__.endswith("ScaledWordEmbedding") and _is_plain(module, (cls.__name__,)) and \
+        isinstance(getattr(module, "scalar_embed_scale", None), (int, float))
+    if "forward" in module.__dict__ or (cls is not torch.nn.Embedding and not scaled) or \
+            module.max_norm is not None or module.sparse or module.scale_grad_by_freq:
+        if accumulator is not None:
+            raise ValueError(f"the gradient of {cls.__name__} cannot go to dw_accumulator")
+        return
+
+    @functools.wraps(cls.forward)
+    def forward(self, input):
+        if _own_ops.get():
+            if _own_tensor(self.weight) and not _has_hooks(self):
+                scale = 1.0
+                if scaled:
+                    scale = float(torch.tensor(self.scalar_embed_scale, dtype=self.weight.dtype))
+                return token_embedding(input, self.weight, scale=scale, padding_idx=self.padding_idx,
+                                       dw_accumulator=accumulator, validate=False)
+            if accumulator is not None:
+                raise RuntimeError("the token embedding's gradient cannot go to dw_accumulator: its "
+                                   f"weight ({type(self.weight).__name__}, {self.weight.dtype}) or hooks "
+                                   "forbid it")
+        return cls.forward(self, input)
+
+    module.forward = types.MethodType(forward, module)
+
+
+def _patch_norms(module: torch.nn.Module) -> None:
+    """Give a module's own layer norms the package's forward."""
+    for child in module.children():
+        if type(child) is torch.nn.LayerNorm and "forward" not in child.__dict__:
+            child.forward = types.MethodType(_norm_forward, child)
+
+
 def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
                    past_key_values=None, use_cache=False, position_embeddings=None, **kwargs):
     """A PLAIN_LAYERS forward with the addition after attention and the norm
     behind it in one pass."""
+    with _set(_own_ops, kwargs.get(PLANS_KWARG) is not None):
+        return _run_layer(self, hidden_states, attention_mask, position_ids, past_key_values, use_cache,
+                          position_embeddings, kwargs)
+
+
+def _run_layer(self, hidden_states, attention_mask, position_ids, past_key_values, use_cache,
+               position_embeddings, kwargs):
     residual = hidden_states
     hidden_states, _ = self.self_attn(
         hidden_states=self.input_layernorm(hidden_states), attention_mask=attention_mask,
@@ -182,6 +260,10 @@ def _layer_forward(self, hidden_states, attention_mask=None, position_ids=None,
             hidden_states.dtype == residual.dtype == norm.weight.dtype:
         hidden_states, residual = residual_rms_norm(hidden_states, residual, norm.weight,
                                                     eps=norm.variance_epsilon)
+    elif PLANS_KWARG in kwargs and getattr(norm.forward, "__func__", None) is _norm_forward and \
+            _takes_layer_norm(norm, hidden_states, residual):
+        hidden_states, residual = residual_layer_norm(hidden_states, residual, norm.weight, norm.bias,
+                                                      eps=norm.eps)
     else:
         residual = residual + hidden_states
         hidden_states = norm(residual)
@@ -239,37 +321,54 @@ def _packed_forward(own, is_decoder: bool):
     def forward(self, *args, **kwargs):
         run = self.__dict__.get(OWN_FORWARD) or functools.partial(own, self)
         if kwargs.get(PLANS_KWARG) is not None:
-            with _set(_packed):
+            with _set(_packed), _set(_own_ops):
                 return run(*args, **kwargs)
         if is_decoder and not _unlabelled.get():
             raise RuntimeError("the decoder of a model patched with patch_causal_lm(packed_layers=True) "
                                "runs in the model's own forward only: the labelled forward for packed "
                                "attention")
-        return run(*args, **kwargs)
+        with _set(_own_ops, False):
+            return run(*args, **kwargs)
 
     return forward
 
 
-def patch_decoder_layers(decoder: torch.nn.Module) -> None:
+def patch_decoder_layers(decoder: torch.nn.Module, embedding_and_norms: bool = False,
+                         embedding_accumulator: Optional[torch.Tensor] = None) -> None:
     """Give the decoder's modules, where they run with plans among their keywords, a
     configuration that names packed attention, and its plain layers the fused
-    forward.  Without plans the modules run as before."""
+    forward.  With embedding_and_norms the token embedding (its gradient added to
+    embedding_accumulator, where that is given) and the layer norms of the decoder and of
+    the modules that are handed the plans are the package's there too.  Without plans the
+    modules run as before."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
 
     _refuse_other_mixers(decoder)
     ALL_ATTENTION_FUNCTIONS.register(ATTENTION_NAME, _attention)
+    layers = PLAIN_LAYERS + (LAYER_NORM_LAYERS if embedding_and_norms else ())
+    if embedding_and_norms:
+        _patch_embedding(decoder.get_input_embeddings(), embedding_accumulator)
     for module in decoder.modules():
-        if _is_plain(module, PLAIN_LAYERS):
+        if _is_plain(module, layers):
             module.forward = types.MethodType(_layer_forward, module)
+            if embedding_and_norms:
+                _patch_norms(module)
             continue
         config = module.__dict__.get("config")
-        if config is None or getattr(type(config), "mt_view", False) or \
-                not hasattr(type(config), "_attn_implementation"):
+        configured = config is not None and not getattr(type(config), "mt_view", False) and \
+            hasattr(type(config), "_attn_implementation")
+        # (a checkpointed layer runs again outside the decoder's forward: its norms are
+        # patched only where the plans it is handed tell them so then, too)
+        normed = embedding_and_norms and any(type(c) is torch.nn.LayerNorm for c in module.children())
+        if not configured and not normed:
             continue
         parameters = inspect.signature(module.forward).parameters.values()
         if module is not decoder and all(p.kind is not p.VAR_KEYWORD for p in parameters):
             continue  # (no plans reach it)
-        module.config = _config_view(config)
+        if normed:
+            _patch_norms(module)
+        if configured:
+            module.config = _config_view(config)
         if "forward" in module.__dict__:
             module.__dict__[OWN_FORWARD] = module.forward
         module.forward = types.MethodType(_packed_forward(type(module).forward, module is decoder), module)
