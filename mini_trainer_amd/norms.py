@@ -9,6 +9,7 @@ library raise.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -164,6 +165,11 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
                                   float(block_scale), float(residual_scale), float(weight_offset))
 
 
+@functools.lru_cache(maxsize=256)
+def _layer_norm_workspace(T: int, H: int) -> int:
+    return load().mt_layer_norm_backward_workspace_bytes(T, H)
+
+
 class _LayerNorm(torch.autograd.Function):
     """normed, or with a residual (normed, new_residual)."""
 
@@ -179,26 +185,29 @@ class _LayerNorm(torch.autograd.Function):
         T = x2.shape[0]
         normed = x.new_empty(shape)
         h = None if r2 is None else x.new_empty(shape)
-        stat = low = None
+        # one buffer: 8 bytes a row, and behind them (whole 16 bytes) the low byte of each
+        # element of a bf16 sum
+        kept, low = None, 0
         if differentiable:  # (needs_input_grad does not say whether gradients are recorded)
-            stat = torch.empty((2, T), dtype=torch.float32, device=dev)
+            words = -(-T // 2) * 4
             if h is not None and x.dtype == torch.bfloat16:
-                low = torch.empty((T, H), dtype=torch.uint8, device=dev)
+                low, words = 4 * words, words + -(-T * H // 4)
+            kept = torch.empty(words, dtype=torch.float32, device=dev)
         tail = (eps, block_scale, residual_scale, int(h is not None), _dtype_code(x.dtype))
         args = pack_layer_norm_args(x2.data_ptr(), _at(r2), _at(w), _at(b), normed.data_ptr(), _at(h),
-                                    _at(low), _at(stat), 0, 0, 0, 0, 0, 0, _pitch(x2),
+                                    _at(kept) + low if low else 0, _at(kept), 0, 0, 0, 0, 0, 0, _pitch(x2),
                                     0 if r2 is None else _pitch(r2), 0, 0, T, H, *tail)
         _launch(dev, "mt_layer_norm_forward", load().mt_layer_norm_forward, args)
-        ctx.save_for_backward(x2 if h is None else h, w, low, stat)
-        ctx.meta = (T, H, shape, tail)
+        ctx.save_for_backward(x2 if h is None else h, w, kept)
+        ctx.meta = (T, H, shape, low, tail)
         return normed if h is None else (normed, h)
 
     @_backward_once
     def backward(ctx, dnormed, dnew=None):
         if dnormed is None and dnew is None:
             return (None,) * 8
-        h, w, low, stat = ctx.saved_tensors
-        T, H, shape, tail = ctx.meta
+        h, w, kept = ctx.saved_tensors
+        T, H, shape, low, tail = ctx.meta
         _, block_scale, residual_scale, has_residual, _ = tail
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         dev = h.device
@@ -213,14 +222,14 @@ class _LayerNorm(torch.autograd.Function):
         dw = new((H,)) if need_w else None
         db = new((H,)) if need_b else None
         args = pack_layer_norm_args(0 if has_residual else h.data_ptr(), 0, _at(w), 0, 0,
-                                    h.data_ptr() if has_residual else 0, _at(low), _at(stat),
+                                    h.data_ptr() if has_residual else 0,
+                                    _at(kept) + low if low else 0, _at(kept),
                                     dn.data_ptr(), _at(dh), _at(dx), _at(dr), _at(dw), _at(db),
                                     H if has_residual else _pitch(h), 0, _pitch(dn),
                                     H if dh is None else _pitch(dh), T, H, *tail)
-        lib = load()
-        nbytes = lib.mt_layer_norm_backward_workspace_bytes(T, H)
+        nbytes = _layer_norm_workspace(T, H)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _launch(dev, "mt_layer_norm_backward", lib.mt_layer_norm_backward, args, ws.data_ptr(), nbytes)
+        _launch(dev, "mt_layer_norm_backward", load().mt_layer_norm_backward, args, ws.data_ptr(), nbytes)
         if T == 0:
             for t in (dw, db):
                 if t is not None:

@@ -8,6 +8,7 @@ library raise.
 from __future__ import annotations
 
 import array
+import functools
 import math
 from typing import Sequence, Tuple, Union
 
@@ -23,6 +24,14 @@ Triple = Tuple[float, float, float]
 
 def _coefficients(given, steps: int) -> array.array:
     """a, b, c of every step in one run."""
+    try:
+        return _flat_coefficients(tuple(x if isinstance(x, (int, float)) else tuple(x) for x in given), steps)
+    except TypeError:
+        raise ValueError("coefficients must be numbers") from None
+
+
+@functools.lru_cache(maxsize=64)  # (an optimizer's are the same at every step)
+def _flat_coefficients(given: tuple, steps: int) -> array.array:
     rows = list(given)
     if rows and all(isinstance(x, (int, float)) for x in rows):
         rows = [rows] * steps
