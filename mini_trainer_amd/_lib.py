@@ -6,6 +6,7 @@ version, every entry point raises.  Nothing here touches the GPU at import.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import struct
 from ctypes import c_double, c_float, c_int, c_int64, c_size_t, c_void_p, c_char_p, POINTER
 from pathlib import Path
@@ -87,9 +88,6 @@ def _packer(args) -> struct.Struct:
 
 pack_attn_args = _packer(AttnArgs).pack
 pack_norm_args = _packer(NormArgs).pack
-pack_embed_args = _packer(EmbedArgs).pack
-pack_layer_norm_args = _packer(LayerNormArgs).pack
-pack_orthogonalize_args = _packer(OrthogonalizeArgs).pack
 
 
 # name -> (restype, argtypes); mirrors include/mt_flce.h
@@ -231,6 +229,29 @@ def load() -> ctypes.CDLL:
         raise FlceError(f"{LIB_PATH} ABI version {v} != expected {ABI_VERSION}")
     _lib = lib
     return lib
+
+
+# The functions that csrc/torch_ops.cpp calls, in the order of its bind().
+_BOUND = ("mt_flce_last_error", "mt_embed_forward", "mt_embed_backward_workspace_bytes",
+          "mt_embed_backward", "mt_layer_norm_forward", "mt_layer_norm_backward_workspace_bytes",
+          "mt_layer_norm_backward", "mt_orthogonalize_workspace_bytes", "mt_orthogonalize",
+          "hipStreamIsCapturing")  # (the last is found in the library's own dependency)
+_torch_ops = None
+
+
+def torch_ops():
+    """The C++ autograd nodes (once), bound to load()'s library; raise if they are missing."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            ops = importlib.import_module("._mt_torch", __package__)
+        except ImportError as e:
+            raise FlceError("_mt_torch is not built for this torch: build it with "
+                            f"`python -m mini_trainer_amd.build` ({e})") from e
+        ops.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND], FlceError)
+        _torch_ops = ops
+    return _torch_ops
 
 
 def check(status: int, what: str) -> None:

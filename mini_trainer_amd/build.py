@@ -21,6 +21,11 @@ SOURCES = [CSRC / "flce_capi.hip", CSRC / "attn_capi.hip", CSRC / "step_capi.hip
            CSRC / "layer_capi.hip", CSRC / "update_capi.hip"]
 DEPENDS = sorted(CSRC.glob("*.h")) + SOURCES + [PKG_DIR.parent / "include" / "mt_flce.h"]
 
+# The autograd nodes in C++ (csrc/torch_ops.cpp): a Python module built against this
+# torch, which is handed the library's functions when both are loaded.
+TORCH_SOURCE = CSRC / "torch_ops.cpp"
+TORCH_PATH = PKG_DIR / "_mt_torch.so"
+
 ARCH = "gfx950"
 HIPCC_FLAGS = [
     f"--offload-arch={ARCH}",
@@ -117,6 +122,29 @@ def build_library(verbose: bool = False) -> Path:
     return LIB_PATH
 
 
+def build_torch_ops(verbose: bool = False) -> Path:
+    """Compile _mt_torch.so with the host compiler.  Always recompiles."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include",
+               sysconfig.get_paths()["include"]]
+    tmp = TORCH_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-fvisibility=hidden",
+           str(TORCH_SOURCE), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stderr}")
+    os.replace(tmp, TORCH_PATH)
+    return TORCH_PATH
+
+
 def is_stale() -> bool:
     if not LIB_PATH.exists():
         return True
@@ -126,3 +154,4 @@ def is_stale() -> bool:
 
 if __name__ == "__main__":
     print(build_library(verbose=True))
+    print(build_torch_ops(verbose=True))

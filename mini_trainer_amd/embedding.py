@@ -7,57 +7,15 @@ is no CPU or eager-PyTorch fallback: non-device tensors or a missing library rai
 """
 from __future__ import annotations
 
-import functools
 import math
 from typing import Optional
 
 import torch
 
-from ._lib import load, pack_embed_args
-from .flce import _backward_once, _dtype_code, _launch, _require_device
-from .norms import _pitch, _rows
+from ._lib import torch_ops
+from .flce import _dtype_code, _require_device
 
 __all__ = ["token_embedding"]
-
-
-@functools.lru_cache(maxsize=256)
-def _workspace_bytes(T: int, V: int, H: int) -> int:
-    return load().mt_embed_backward_workspace_bytes(T, V, H)
-
-
-class _TokenEmbedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, weight, scale, padding, accumulator, status):
-        w, flat = _rows(weight), ids.reshape(-1).contiguous()
-        V, H = w.shape
-        T = flat.numel()
-        out = weight.new_empty(ids.shape + (H,))
-        tail = (T, V, H, padding, scale, _dtype_code(weight.dtype), flat.element_size())
-        args = pack_embed_args(flat.data_ptr(), w.data_ptr(), out.data_ptr(), 0, 0,
-                               0 if status is None else status.data_ptr(), _pitch(w), 0, 0, *tail, 0)
-        _launch(w.device, "mt_embed_forward", load().mt_embed_forward, args)
-        ctx.save_for_backward(flat)
-        ctx.tail, ctx.accumulator = tail, accumulator
-        return out
-
-    @_backward_once
-    def backward(ctx, dout):
-        if not ctx.needs_input_grad[1]:
-            return (None,) * 6
-        (ids,) = ctx.saved_tensors
-        T, V, H = ctx.tail[:3]
-        d, acc = _rows(dout), ctx.accumulator
-        dw = dout.new_empty((V, H)) if acc is None else acc
-        args = pack_embed_args(ids.data_ptr(), 0, 0, d.data_ptr(), dw.data_ptr(), 0, 0, _pitch(d),
-                               _pitch(dw), *ctx.tail, int(acc is not None))
-        nbytes = _workspace_bytes(T, V, H)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device) if nbytes else None
-        _launch(dout.device, "mt_embed_backward", load().mt_embed_backward, args,
-                0 if ws is None else ws.data_ptr(), nbytes)
-        if acc is None:
-            return None, dw, None, None, None, None
-        torch.autograd.graph.increment_version([acc])
-        return (None,) * 6
 
 
 def token_embedding(input_ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
@@ -108,7 +66,8 @@ def token_embedding(input_ids: torch.Tensor, weight: torch.Tensor, scale: float 
         if acc.requires_grad:
             raise ValueError("dw_accumulator must not require a gradient")
     status = torch.zeros(1, dtype=torch.int32, device=weight.device) if validate else None
-    out = _TokenEmbedding.apply(input_ids, weight, scale, padding, acc, status)
+    out = torch_ops().embedding(input_ids, weight, scale, padding, acc, status,
+                                torch._C._cuda_getCurrentRawStream(weight.device.index))
     if validate and int(status.item()):
         raise IndexError(f"input_ids must lie in [0, {V})")
     return out

@@ -9,13 +9,12 @@ library raise.
 """
 from __future__ import annotations
 
-import functools
 import math
 from typing import Optional, Tuple
 
 import torch
 
-from ._lib import load, pack_layer_norm_args, pack_norm_args
+from ._lib import load, pack_norm_args, torch_ops
 from .flce import _backward_once, _dtype_code, _launch, _require_device
 
 __all__ = ["layer_norm", "residual_layer_norm", "residual_rms_norm"]
@@ -165,78 +164,6 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
                                   float(block_scale), float(residual_scale), float(weight_offset))
 
 
-@functools.lru_cache(maxsize=256)
-def _layer_norm_workspace(T: int, H: int) -> int:
-    return load().mt_layer_norm_backward_workspace_bytes(T, H)
-
-
-class _LayerNorm(torch.autograd.Function):
-    """normed, or with a residual (normed, new_residual)."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, block_scale, residual_scale, differentiable):
-        dev, shape = x.device, x.shape
-        H = shape[-1]
-        ctx.set_materialize_grads(False)
-        x2 = _rows(x)
-        r2 = None if residual is None else _rows(residual)
-        w = None if weight is None else weight.contiguous()
-        b = None if bias is None else bias.contiguous()
-        T = x2.shape[0]
-        normed = x.new_empty(shape)
-        h = None if r2 is None else x.new_empty(shape)
-        # one buffer: 8 bytes a row, and behind them (whole 16 bytes) the low byte of each
-        # element of a bf16 sum
-        kept, low = None, 0
-        if differentiable:  # (needs_input_grad does not say whether gradients are recorded)
-            words = -(-T // 2) * 4
-            if h is not None and x.dtype == torch.bfloat16:
-                low, words = 4 * words, words + -(-T * H // 4)
-            kept = torch.empty(words, dtype=torch.float32, device=dev)
-        tail = (eps, block_scale, residual_scale, int(h is not None), _dtype_code(x.dtype))
-        args = pack_layer_norm_args(x2.data_ptr(), _at(r2), _at(w), _at(b), normed.data_ptr(), _at(h),
-                                    _at(kept) + low if low else 0, _at(kept), 0, 0, 0, 0, 0, 0, _pitch(x2),
-                                    0 if r2 is None else _pitch(r2), 0, 0, T, H, *tail)
-        _launch(dev, "mt_layer_norm_forward", load().mt_layer_norm_forward, args)
-        ctx.save_for_backward(x2 if h is None else h, w, kept)
-        ctx.meta = (T, H, shape, low, tail)
-        return normed if h is None else (normed, h)
-
-    @_backward_once
-    def backward(ctx, dnormed, dnew=None):
-        if dnormed is None and dnew is None:
-            return (None,) * 8
-        h, w, kept = ctx.saved_tensors
-        T, H, shape, low, tail = ctx.meta
-        _, block_scale, residual_scale, has_residual, _ = tail
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
-        dev = h.device
-        dn = _rows(torch.zeros(shape, dtype=h.dtype, device=dev) if dnormed is None else dnormed)
-        dh = None if dnew is None else _rows(dnew)
-        # where both are the same number the two inputs share one gradient, as an
-        # addition's do
-        same = need_x and need_r and block_scale == residual_scale
-        new = h.new_empty
-        dr = new(shape) if need_r else None
-        dx = new(shape) if need_x and not same else None
-        dw = new((H,)) if need_w else None
-        db = new((H,)) if need_b else None
-        args = pack_layer_norm_args(0 if has_residual else h.data_ptr(), 0, _at(w), 0, 0,
-                                    h.data_ptr() if has_residual else 0,
-                                    _at(kept) + low if low else 0, _at(kept),
-                                    dn.data_ptr(), _at(dh), _at(dx), _at(dr), _at(dw), _at(db),
-                                    H if has_residual else _pitch(h), 0, _pitch(dn),
-                                    H if dh is None else _pitch(dh), T, H, *tail)
-        nbytes = _layer_norm_workspace(T, H)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _launch(dev, "mt_layer_norm_backward", load().mt_layer_norm_backward, args, ws.data_ptr(), nbytes)
-        if T == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        return (dr if same else dx), dr, dw, db, None, None, None, None
-
-
 def _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale):
     dtype, dev = x.dtype, x.device
     grad = False
@@ -262,8 +189,9 @@ def _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale):
         raise ValueError(f"hidden size {H}: 1 to 32768 are supported")
     if not (eps >= 0 and math.isfinite(eps + block_scale + residual_scale)):
         raise ValueError("eps must be >= 0, and it, block_scale and residual_scale finite")
-    return _LayerNorm.apply(x, residual, weight, bias, float(eps), float(block_scale),
-                            float(residual_scale), grad and torch.is_grad_enabled())
+    return torch_ops().layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale,
+                                  grad and torch.is_grad_enabled(),
+                                  torch._C._cuda_getCurrentRawStream(dev.index))
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -276,7 +204,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     var is the mean square of the centred row, and weight gradients are summed in fp32
     in a fixed order.  H is at most 32768.
     """
-    return _layer_norm(x, None, weight, bias, eps, 1.0, 1.0)
+    return _layer_norm(x, None, weight, bias, eps, 1.0, 1.0)[0]
 
 
 def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor,
@@ -295,4 +223,4 @@ def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor,
     """
     if residual is None:
         raise ValueError("residual_layer_norm needs a residual")
-    return _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale)
+    return tuple(_layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale))

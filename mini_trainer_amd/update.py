@@ -14,8 +14,8 @@ from typing import Sequence, Tuple, Union
 
 import torch
 
-from ._lib import load, pack_orthogonalize_args
-from .flce import _dtype_code, _launch, _require_device
+from ._lib import torch_ops
+from .flce import _dtype_code, _require_device
 
 __all__ = ["orthogonalize"]
 
@@ -44,7 +44,6 @@ def _flat_coefficients(given: tuple, steps: int) -> array.array:
     return flat
 
 
-@torch.no_grad()
 def orthogonalize(update: torch.Tensor, steps: int = 5,
                   coefficients: Union[Triple, Sequence[Triple]] = (3.4445, -4.7750, 2.0315),
                   eps: float = 1e-7) -> torch.Tensor:
@@ -76,19 +75,5 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be >= 0 and finite")
     flat = _coefficients(coefficients, steps)
-    m, n = update.shape[-2:]
-    out = torch.empty(update.shape, dtype=update.dtype, device=update.device)
-    if out.numel() == 0:
-        return out
-    x = update if update.dim() == 3 else update.reshape(-1, m, n)
-    batch = x.shape[0]
-    if (n > 1 and x.stride(2) != 1) or (m > 1 and x.stride(1) < n):
-        x = x.clone(memory_format=torch.contiguous_format)
-    args = pack_orthogonalize_args(x.data_ptr(), out.data_ptr(), flat.buffer_info()[0], eps, batch, m, n,
-                                   x.stride(1) if m > 1 else n, x.stride(0) if batch > 1 else 0, steps, code)
-    lib = load()
-    nbytes = lib.mt_orthogonalize_workspace_bytes(args)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=update.device) if nbytes else None
-    _launch(update.device, "mt_orthogonalize", lib.mt_orthogonalize, args, 0 if ws is None else ws.data_ptr(),
-            nbytes)
-    return out
+    return torch_ops().orthogonalize(update, flat.buffer_info()[0], steps, eps,
+                                     torch._C._cuda_getCurrentRawStream(update.device.index))

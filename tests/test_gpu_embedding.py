@@ -203,3 +203,37 @@ def test_gradient_against_differences(gpu):
     size = (1.7 * (w.abs() + step.abs())[ids] * d.abs()).sum()
     assert abs(float(ends[0] - ends[1]) - 2 * float((grad.double() * step.double()).sum())) <= \
         8 * 2.0 ** -23 * float(size)
+
+
+def test_captured_beside_an_eager_graph_of_the_leaf(gpu):
+    """Refused where the leaf's gradient node belongs to the eager graph's stream; without
+    that graph the same capture runs."""
+    ids, w, d = make(400, 50, 64, torch.bfloat16)
+    leaf = w.detach().requires_grad_(True)
+    want, = torch.autograd.grad(token_embedding(ids, leaf), leaf, d)
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (grad,) = torch.autograd.grad(token_embedding(ids, leaf, validate=False), leaf, d)
+        return graph, grad
+
+    alive = token_embedding(ids, leaf, validate=False)
+    with pytest.raises(RuntimeError, match="another stream"):
+        capture()
+    del alive
+    graph, grad = capture()
+    for _ in range(3):
+        grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+
+
+def test_not_differentiable_twice(gpu):
+    ids, w, d = make(40, 50, 64, torch.float32)
+    leaf = w.detach().requires_grad_(True)
+    d.requires_grad_(True)
+    (grad,) = torch.autograd.grad(token_embedding(ids, leaf), leaf, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        grad.sum().backward()

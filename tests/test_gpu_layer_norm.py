@@ -219,3 +219,29 @@ def test_gradient_against_differences(gpu):
     # are of the order of 1), and roundings of 2^-23 of each of 2 x 576 outputs of
     # magnitude up to 10
     assert abs((value(1) - value(-1)) / 2 - slope) <= 576 * 10 * 2.0 ** -30 + 1152 * 10 * 2.0 ** -23
+
+
+def test_captured_beside_an_eager_graph_of_the_leaf(gpu):
+    x, w = (torch.randn(*s, device=gpu, requires_grad=True) for s in ((9, 64), (64,)))
+    alive = layer_norm(x, w)
+    with pytest.raises(RuntimeError, match="another stream"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.autograd.grad(layer_norm(x, w).sum(), w)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dw,) = torch.autograd.grad(layer_norm(x, w), w, x.detach())
+    (want,) = torch.autograd.grad(layer_norm(x, w), w, x.detach())
+    for _ in range(3):
+        dw.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dw, want)
+
+
+def test_not_differentiable_twice(gpu):
+    x, r = (torch.randn(5, 64, device=gpu, requires_grad=True) for _ in range(2))
+    normed, _ = residual_layer_norm(x, r)
+    dx, dr = torch.autograd.grad((normed * normed).sum(), (x, r), create_graph=True)
+    assert torch.equal(dx, dr)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        dx.sum().backward()

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
 
 import pytest
 import torch
@@ -143,6 +144,32 @@ def test_layer_norm_workspace():
     assert lib.mt_layer_norm_backward(None, P, n, None) == lib.mt_layer_norm_forward(None, None) == 1
     assert lib.mt_layer_norm_forward(ctypes.byref(norm(T=0, x=None)), None) == 0
     assert lib.mt_layer_norm_backward(ctypes.byref(norm(T=0, dnormed=None)), None, 0, None) == 0
+
+
+def test_the_nodes_are_there_and_fail_loudly(monkeypatch):
+    ops = _lib.torch_ops()
+    assert ops is _lib.torch_ops()
+    with pytest.raises(_lib.FlceError, match="null coefficients"):
+        ops.orthogonalize(torch.zeros(4, 4), 0, 5, 1e-7, 0)
+    monkeypatch.setattr(_lib, "_torch_ops", None)
+    monkeypatch.setitem(sys.modules, "mini_trainer_amd._mt_torch", None)  # (as if it were not there)
+    with pytest.raises(_lib.FlceError, match="not built"):
+        _lib.torch_ops()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True), (True, True)])
+def test_gradients_go_to_the_tensors_that_are_there(residual, weight, bias):
+    """No rows: nothing is launched, so that the nodes' edges can be looked at here."""
+    leaf = lambda there, *shape: torch.zeros(*shape, requires_grad=True) if there else None  # noqa: E731
+    given = leaf(True, 0, 8), leaf(residual, 0, 8), leaf(weight, 8), leaf(bias, 8)
+    outs = _lib.torch_ops().layer_norm(*given, 1e-5, 1.0, 0.5, True, 0)
+    assert len(outs) == 1 + residual
+    leaves = [t for t in given if t is not None]
+    both = torch.autograd.grad(outs, leaves, [torch.zeros_like(t) for t in outs], retain_graph=True)
+    alone = [torch.autograd.grad(outs[0], t, outs[0], retain_graph=True)[0] for t in leaves]
+    for t, a, b in zip(leaves, both, alone):
+        assert a.shape == b.shape == t.shape and not a.any() and not b.any()
 
 
 def test_the_references_agree_with_torch():
