@@ -33,8 +33,15 @@ namespace mtf {
 
 constexpr int kUpdParts = 1024;  // partial sums of squares of G, at most
 
-// Per matrix, in fp32: the factor of X0 over its fp16 copy, 1 / (|G| + eps), mu.
-enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdState = 4 };
+// Per matrix, in fp32: the factor of X0 over its fp16 copy, mu, and the two factors of X0
+// over G, 2^k and 1 / (|G| + eps) / 2^k (their product leaves fp32's range where |G| does).
+enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdShift = 3, kUpdState = 4 };
+
+// 1 / (|G| + eps) in 64 bits; for a zero matrix, where it matters to nothing, one that fp32
+// holds, so that X0 is zero and not its product with infinity.
+__device__ __forceinline__ double upd_inverse(double norm, double eps) {
+  return norm == 0.0 && eps > 0.0 ? 1.0 : 1.0 / (norm + eps);
+}
 
 struct UpdArgs {
   const char* in;
@@ -111,12 +118,13 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
   if (lane_id() == 0) sums[wave_id()] = s;
   __syncthreads();
   const double norm = sqrt(sums[0] + sums[1] + sums[2] + sums[3]);
-  const double inverse = 1.0 / (norm + a.eps);
+  const double inverse = upd_inverse(norm, a.eps);
   const int exponent = norm > 0.0 && norm < INFINITY ? 13 - ilogb(norm) : 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     float* state = reinterpret_cast<float*>(ws + a.state);
     state[kUpdFactor] = (float)ldexp(inverse, -exponent);
-    state[kUpdInverse] = (float)inverse;
+    state[kUpdShift] = (float)ldexp(1.0, exponent / 2);
+    state[kUpdInverse] = (float)ldexp(inverse, -(exponent / 2));
     state[kUpdMu] = (float)(norm * inverse * (norm * inverse) / a.r);
   }
   const int32_t across = (a.n + 63) / 64;
@@ -454,6 +462,7 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   const float mu = state[kUpdMu];
   const float product = a.d_unscale * (a.first ? state[kUpdFactor] : a.x_unscale);
   const float linear = (a.a + mu * (a.b + a.cc * mu)) * (a.first ? state[kUpdInverse] : 1.f);
+  const float shift = a.first ? state[kUpdShift] : 1.f;
   const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)matrix * a.in_batch;
   float* carrier = reinterpret_cast<float*>(ws + a.carrier);
   T* out = reinterpret_cast<T*>(a.out) + (int64_t)matrix * a.m * a.n;
@@ -508,7 +517,7 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
       float x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = fmaf(linear, held[fm % 3][fn][i], product * acc[fm][fn][i]);
+        x[i] = fmaf(linear, held[fm % 3][fn][i] * shift, product * acc[fm][fn][i]);
         ss = fmaf(x[i], x[i], ss);
       }
       if (!a.last) {

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
   __syncthreads();
   square = 0.0;
   for (int i = 0; i < 8; ++i) square += sums[i];
-  const double norm = sqrt(square), inverse = 1.0 / (norm + a.eps);
+  const double norm = sqrt(square), inverse = upd_inverse(norm, a.eps);
   const int exponent = norm > 0.0 && norm < INFINITY ? 13 - ilogb(norm) : 0;
   float unscale = (float)ldexp(inverse, -exponent);
   float mu = (float)(norm * inverse * (norm * inverse) / a.r);
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         v[i] = ldexpf(x[j][f][i], exponent);
-        x[j][f][i] *= (float)inverse;
+        x[j][f][i] = v[i] * unscale;
       }
       put(L, plane_l, PL, 16 * f + l16, at + 4 * g, v);
     }

@@ -99,6 +99,26 @@ def test_scales(gpu, scale, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("m,n", [(12, 20), (40, 12), (200, 300), (300, 200)])
+def test_scales_at_the_ends_of_the_range(gpu, m, n, dtype):
+    """A power of two changes nothing without eps, also where 1 / norm is beyond fp32 or one
+    of its subnormal numbers."""
+    few = torch.zeros(m, n, dtype=dtype, device=gpu)
+    for i in range(8):
+        few[i, i + 2] = 1 - 2 * (i % 3 == 0)
+    g = torch.Generator().manual_seed(m)
+    many = torch.randint(-100, 101, (m, n), generator=g).to(dtype).cuda()
+    for x, exponent in ((few, -133), (many, 120)):
+        scaled = x * 2.0 ** (exponent / 2 // 1) * 2.0 ** (exponent - exponent / 2 // 1)
+        norm = scaled.double().norm()
+        assert 0 < norm < 2.0 ** -128 or norm > 2.0 ** 128
+        got = orthogonalize(scaled, eps=0.0)
+        assert got.isfinite().all() and torch.equal(got, orthogonalize(x, eps=0.0))
+    for eps in (1e-300, 1e-45, 1.0):
+        assert not orthogonalize(torch.zeros_like(few), eps=eps).any()
+
+
+@BOTH
 def test_special_spectra(gpu, dtype):
     for rank in (1, 4):
         x = make(48, 80, dtype=dtype, rank=rank, seed=rank)
