@@ -790,8 +790,9 @@ int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size
  * the relative error of fp32 products); X is carried in fp32 and rounded once at the end.
  * A matrix that holds NaN or infinities gives NaN; a zero matrix gives zeros (eps > 0).
  * The workspace (256-byte aligned) must hold one matrix's part; the query's size, up to
- * 2 GiB or one matrix, takes a stack together.  Small matrices take none (0 bytes, null).  A matrix in fp16 must stay below 2 GiB
- * (either side padded to whole 64).
+ * 2 GiB or one matrix, takes a stack together.  Small matrices take none (0 bytes, null).
+ * A matrix in fp16 must stay below 2 GiB, of fp32 ones below 1.875 (either side padded to
+ * whole 64).
  */
 typedef struct mt_orthogonalize_args {
   const void* in;

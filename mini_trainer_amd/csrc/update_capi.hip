@@ -17,7 +17,8 @@ namespace {
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int64_t kUpdMost = (int64_t)1 << 31;  // bytes of an fp16 plane, an offset of 32 bits
+constexpr int64_t kUpdMost = (int64_t)1 << 31;  // bytes of a copy in fp16
+constexpr int64_t kUpdReach = 0xf0000000;      // and of both its terms: offsets of 32 bits
 constexpr int64_t kUpdGroup = (int64_t)2 << 30; // bytes of the workspace that a stack of matrices asks for
 constexpr int kUpdMostSteps = 64;
 constexpr int kUpdCus = 256;
@@ -41,8 +42,9 @@ bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   if (m < 1 || n < 1 || m > (1 << 30) || n > (1 << 30)) return false;
   x.r = std::min(m, n), x.c = std::max(m, n);
   x.ld_r = up(x.r), x.ld_c = up(x.c);
-  if (x.r * x.ld_c * 2 >= kUpdMost || x.c * x.ld_r * 2 >= kUpdMost || x.r * x.ld_r * 2 >= kUpdMost) return false;
   const int64_t planes = dtype == MT_DTYPE_F32 ? 2 : 1;
+  for (int64_t one : {x.r * x.ld_c * 2, x.c * x.ld_r * 2, x.r * x.ld_r * 2})
+    if (one >= kUpdMost || planes * one > kUpdReach) return false;
   int64_t at = 0;
   const auto take = [&](int64_t& where, int64_t bytes) { where = at, at += cdiv(bytes, 256) * 256; };
   take(x.l, x.r * x.ld_c * 2 * planes);
@@ -75,7 +77,7 @@ int upd_check(const mt_orthogonalize_args* p, UpdLayout& l) {
   if (!a.coefficients) return fail(MT_ERR_INVALID_ARGUMENT, "null coefficients");
   if (a.batch == 0 || a.m == 0 || a.n == 0) return MT_OK;
   if (a.batch > (1 << 24) || !upd_layout(a.m, a.n, a.dtype, l))
-    return fail(MT_ERR_UNSUPPORTED, "%lld matrices of %lld x %lld: a matrix in fp16 must stay below 2 GiB",
+    return fail(MT_ERR_UNSUPPORTED, "%lld matrices of %lld x %lld: a matrix in fp16 must stay below 2 GiB (of fp32 ones below 1.875)",
                 (long long)a.batch, (long long)a.m, (long long)a.n);
   const int64_t most = (int64_t)1 << 40;
   if (a.in_row < a.n || a.in_row > most || a.in_batch < 0 || a.in_batch > most)
@@ -113,19 +115,24 @@ bool upd_scales(const double* k, double most, UpdScales& s) {
 // move `bytes` an element beside it: the one that costs least, in us.  A CU takes `load`
 // of them one after the other; tiles of 64 share it and hide most of what they move behind
 // each other's products, the larger ones do not.  A lone tile is as slow as its
-// stages' latency.  The constants are fitted to 24 sizes from 128 x 352 to 14336 x 4096 and
-// 1 to 200 matrices, timed with every tile: the choice is within 7% of the best at each
-// (4096 x 4096, all of its symmetric products in tiles of 64, 128, 192 and 256: 2022, 1831,
-// 1567 and 1807 us; 28 of 256 x 1536: 305, 324, 401, 482).
+// stages' latency.  The constants are fitted to 24 sizes in bf16 and 12 in fp32 (three terms
+// to a stage) from 128 x 352 to 14336 x 4096 and 1 to 200 matrices, timed with every tile: the
+// choice is within 7% of the best at each (4096 x 4096, all of its symmetric products in
+// tiles of 64, 128, 192 and 256: 2022, 1831, 1567 and 1807 us; 28 of 256 x 1536: 305, 324,
+// 401, 482; 3 of 1001 x 1537 in fp32, all products: 455, 680, 981).
 template <class Tiles>
 int upd_pick(Tiles tiles, double stages, double bytes, bool split) {
-  static const struct { int F; double stage, alone, exposed; } kinds[] = {
-      {8, 1.6, 0.75, 1.0}, {6, 1.07, 0.72, 1.0}, {4, 0.54, 0.3, 1.0}, {2, 0.25, 0.22, 0.36}};
+  struct Kind { int F; double stage, alone, exposed; };
+  static const Kind one[] = {{8, 1.6, 0.75, 1.0}, {6, 1.07, 0.72, 1.0}, {4, 0.54, 0.3, 1.0}, {2, 0.25, 0.22, 0.36}};
+  // (F = 8 would spill in its two writes of an image)
+  static const Kind three[] = {{6, 2.2, 1.6, 1.0}, {4, 1.1, 0.75, 1.0}, {2, 0.5, 0.5, 0.36}};
+  const Kind* kinds = split ? three : one;
+  const int count = split ? 3 : 4;
   constexpr double kRate = 21e3;  // bytes a us of a CU, when all of them ask
   int best = 2;
   double least = INFINITY;
-  for (const auto& k : kinds) {
-    if (split && k.F == 8) continue;  // (its two writes of an image would spill)
+  for (int i = 0; i < count; ++i) {
+    const Kind& k = kinds[i];
     const int64_t n = tiles(upd_tile(k.F));
     const double busy = std::min(1.0, std::max((double)n / kUpdCus, 0.15));
     const double moved = bytes * upd_tile(k.F) * upd_tile(k.F) / kRate * busy, product = stages * k.stage;
@@ -191,8 +198,8 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
   const auto all = [&](int64_t t) { return k.batch * cdiv(k.m, t) * cdiv(k.n, t); };
   // both symmetric products go by one tile (fragments of E pass between them): by their mean
   constexpr int planes = TERMS == 3 ? 2 : 1;
-  const int symmetric = upd_pick(triangle, TERMS * (cdiv(k.c, 64) + cdiv(k.r, 64)) / 2.0, 6.0 * planes, TERMS == 3);
-  const int apply = upd_pick(all, (double)TERMS * cdiv(k.r, 64), 8.0 + 4.0 * planes, TERMS == 3);
+  const int symmetric = upd_pick(triangle, (cdiv(k.c, 64) + cdiv(k.r, 64)) / 2.0, 6.0 * planes, TERMS == 3);
+  const int apply = upd_pick(all, (double)cdiv(k.r, 64), 8.0 + 4.0 * planes, TERMS == 3);
   constexpr int kMost = TERMS == 3 ? 6 : 8;
   double most = 1.0;
   UpdScales now, next;

@@ -48,24 +48,30 @@ __device__ __forceinline__ f32x4_t upd_mma(u32x4_t a, u32x4_t b, f32x4_t c) {
                                                 c, 0, 0, 0);
 }
 
-// An operand: `rows` rows of ld halves (whole stages).  fp32 updates keep two planes,
-// the rounded value and what the rounding left, plane bytes apart.
+// An operand: `rows` rows of ld halves (whole stages).  fp32 updates keep the value rounded
+// to fp16 and what the rounding left (hi, lo), 32 of each in turn: a stage is 32 columns of
+// the matrix, hi in its first half and lo in its second.
 struct UpdMatrix {
   const char* at;
-  uint32_t bytes;  // of a plane: 2 rows ld, below 2^31
+  uint32_t bytes;  // 2 rows ld, below 0xf0000000
   uint32_t ld;     // halves of a row
   uint32_t rows;
 };
+// Place in a row of 2 ld halves of column `col`, t = 1 for lo; with one term a row is the
+// matrix's.
+template <int TERMS>
+__device__ __forceinline__ int32_t upd_column(int32_t col, int t) {
+  return TERMS == 1 ? col : (col & ~31) * 2 + 32 * t + (col & 31);
+}
 
 template <int F>
 struct UpdOperand {
-  rsrc_t rsrc[2];
+  rsrc_t rsrc;
   uint32_t off[F];
   uint32_t frag[2];
 
-  __device__ __forceinline__ void init(const UpdMatrix& m, uint32_t row0, uint32_t wave_row0, bool two) {
-    rsrc[0] = make_rsrc(m.at, m.bytes);
-    rsrc[1] = make_rsrc(m.at + (two ? m.bytes : 0u), m.bytes);
+  __device__ __forceinline__ void init(const UpdMatrix& m, uint32_t row0, uint32_t wave_row0) {
+    rsrc = make_rsrc(m.at, m.bytes);
     const uint32_t l = lane_id();
 #pragma unroll
     for (uint32_t i = 0; i < (uint32_t)F; ++i) {
@@ -78,8 +84,8 @@ struct UpdOperand {
 #pragma unroll
     for (uint32_t kk = 0; kk < 2; ++kk) frag[kk] = tile_off(wave_row0 + (l & 15u), kk * 4 + (l >> 4));
   }
-  __device__ __forceinline__ void issue(char* slot, int plane, int kt, int i) const {
-    dma16(plane ? rsrc[1] : rsrc[0], slot + (wave_id() * F + (uint32_t)i) * 1024u, off[i], (uint32_t)kt * 128u);
+  __device__ __forceinline__ void issue(char* slot, int kt, int i) const {
+    dma16(rsrc, slot + (wave_id() * F + (uint32_t)i) * 1024u, off[i], (uint32_t)kt * 128u);
   }
   __device__ __forceinline__ u32x4_t read(const char* slot, int kk, int f) const {
     return lds_read16(slot, frag[kk] + (uint32_t)f * 2048u);
@@ -91,8 +97,7 @@ __device__ __forceinline__ void upd_wait_vm() {  // every DMA but the last N iss
   __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
-// acc = sum over the KT stages from `first` on, and with TERMS = 3 over the planes (value, rest) x (rest,
-// value) and (value, value), of A B^T.
+// acc = sum over the KT stages from `first` on of A B^T; with TERMS = 3 of hi hi, hi lo and lo hi.
 template <int F, int TERMS>
 __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, const UpdOperand<F>& b, int first,
                                              int KT, f32x4_t (&acc)[F][F]) {
@@ -103,20 +108,9 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   constexpr int kPer = F >= 8 ? 3 : F >= 6 ? 2 : 1;
   char* const slots_b = lds;
   char* const slots_a = lds + NB * kSlot;
-  const int stages = TERMS * KT;
-  // The DMA of stage s of all.  Past the end it loads the last stage again, into slots that
-  // are not read any more, so that every stage issues as much.
-  auto at = [&](int s, int& term, int& kt) __attribute__((always_inline)) {
-    s = s < stages ? s : stages - 1;
-    term = TERMS == 1 ? 0 : s >= 2 * KT ? 2 : s >= KT ? 1 : 0;
-    kt = first + s - term * KT;
-  };
-  auto issue_a = [&](char* slot, int term, int kt, int i) __attribute__((always_inline)) {
-    a.issue(slot, TERMS == 3 && term == 1, kt, i);
-  };
-  auto issue_b = [&](char* slot, int term, int kt, int i) __attribute__((always_inline)) {
-    b.issue(slot, TERMS == 3 && term == 0, kt, i);
-  };
+  // Past the end the DMA loads the last stage again, into slots that are not read any more,
+  // so that every stage issues as much.
+  auto at = [&](int s) __attribute__((always_inline)) { return first + (s < KT ? s : KT - 1); };
 #pragma unroll
   for (int m = 0; m < F; ++m)
 #pragma unroll
@@ -124,12 +118,11 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   // the stages that the phases are ahead
 #pragma unroll
   for (int s = 0; s < (NA - 1 > NB ? NA - 1 : NB); ++s) {
-    int term, kt;
-    at(s, term, kt);
+    const int kt = at(s);
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      if (s < NA - 1) issue_a(slots_a + s * kSlot, term, kt, i);
-      if (s < NB) issue_b(slots_b + s * kSlot, term, kt, i);
+      if (s < NA - 1) a.issue(slots_a + s * kSlot, kt, i);
+      if (s < NB) b.issue(slots_b + s * kSlot, kt, i);
     }
   }
   upd_wait_vm<F * (NA + NB - 3)>();  // stage 0: of A NA - 2 stages follow it, of B NB - 1
@@ -142,14 +135,50 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
   }
   lgkm_wait0();
   int ga = 0, gb = 0;  // slots of stage g
-  for (int g = 0; g < stages; ++g) {
+  for (int g = 0; g < KT; ++g) {
     sched_fence();
     const int ga1 = ga == NA - 1 ? 0 : ga + 1, gap = ga == 0 ? NA - 1 : ga - 1;  // of stages g + 1 and g - 1
     const int gb1 = gb == NB - 1 ? 0 : gb + 1;
     const char* ra = slots_a + ga * kSlot;
     const char* rb = slots_b + gb * kSlot;
-    int term, kt;
-    at(g + NA - 1, term, kt);
+    int kt = at(g + NA - 1);
+    if constexpr (TERMS == 3) {
+      // hi hi beside the reads of lo, hi lo beside the DMA of A, and behind the barrier lo hi
+      // beside the next stage's reads of hi, each of B into the registers that its column of
+      // products has just left (a third fewer LDS reads and DMA than three products of one
+      // term)
+#pragma unroll
+      for (int n = 0; n < F; ++n) {
+#pragma unroll
+        for (int m = 0; m < F; ++m) acc[m][n] = upd_mma(fb0[n], fa0[m], acc[m][n]);
+        fa1[n] = a.read(ra, 1, n);
+        fb1[n] = b.read(rb, 1, n);
+        sched_fence();
+      }
+#pragma unroll
+      for (int n = 0; n < F; ++n) {
+#pragma unroll
+        for (int m = 0; m < F; ++m) acc[m][n] = upd_mma(fb1[n], fa0[m], acc[m][n]);
+        a.issue(slots_a + gap * kSlot, kt, n);
+        sched_fence();
+      }
+      lgkm_wait0();
+      upd_wait_vm<F * (NA + NB - 4)>();  // as below
+      __builtin_amdgcn_s_barrier();
+      sched_fence();
+      kt = at(g + NB);
+#pragma unroll
+      for (int n = 0; n < F; ++n) {
+        fa0[n] = a.read(slots_a + ga1 * kSlot, 0, n);
+#pragma unroll
+        for (int m = 0; m < F; ++m) acc[m][n] = upd_mma(fb0[n], fa1[m], acc[m][n]);
+        b.issue(slots_b + gb * kSlot, kt, n);
+        fb0[n] = b.read(slots_b + gb1 * kSlot, 0, n);
+        sched_fence();
+      }
+      ga = ga1, gb = gb1;
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
 #pragma unroll
@@ -159,7 +188,7 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
       }
       if (i & 1) fb1[i >> 1] = b.read(rb, 1, i >> 1);
       else fa1[i >> 1] = a.read(ra, 1, i >> 1);
-      if (i & 1) issue_a(slots_a + gap * kSlot, term, kt, i >> 1);
+      if (i & 1) a.issue(slots_a + gap * kSlot, kt, i >> 1);
       sched_fence();
     }
 #pragma unroll
@@ -173,7 +202,7 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
     sched_fence();
     const char* ra1 = slots_a + ga1 * kSlot;
     const char* rb1 = slots_b + gb1 * kSlot;
-    at(g + NB, term, kt);
+    kt = at(g + NB);
 #pragma unroll
     for (int i = 0; i < 2 * F; ++i) {
 #pragma unroll
@@ -181,7 +210,7 @@ __device__ __forceinline__ void upd_mainloop(char* lds, const UpdOperand<F>& a, 
         const int k = i * kPer + j;
         acc[k / F][k % F] = upd_mma(fb1[k % F], fa1[k / F], acc[k / F][k % F]);
       }
-      if (i & 1) issue_b(slots_b + gb * kSlot, term, kt, i >> 1);
+      if (i & 1) b.issue(slots_b + gb * kSlot, kt, i >> 1);
       if (i & 1) fb0[i >> 1] = b.read(rb1, 0, i >> 1);
       else fa0[i >> 1] = a.read(ra1, 0, i >> 1);
       sched_fence();

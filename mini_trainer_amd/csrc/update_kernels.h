@@ -134,34 +134,51 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
   const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)blockIdx.y * a.in_batch;
   uint16_t* natural = reinterpret_cast<uint16_t*>(ws + (tall ? a.s0 : a.l));
   uint16_t* transposed = reinterpret_cast<uint16_t*>(ws + (tall ? a.l : a.s0));
-  const int64_t ld_nat = tall ? a.ld_r : a.ld_c, ld_tr = tall ? a.ld_c : a.ld_r;
-  const int64_t plane_nat = (int64_t)a.m * ld_nat, plane_tr = (int64_t)a.n * ld_tr;
+  constexpr int64_t P = TERMS == 3 ? 2 : 1;
+  const int64_t ld_nat = P * (tall ? a.ld_r : a.ld_c), ld_tr = P * (tall ? a.ld_c : a.ld_r);
   uint16_t part[TERMS == 3 ? 2 : 1][16];
+  if constexpr (V == 1) {  // a wave reads 64 columns of 16 rows, and each thread its part out of LDS
+    const int32_t col = col0 + (int32_t)lane_id(), w = (int32_t)wave_id() * 16;
+    const T* from = in + (col < a.n ? col : a.n - 1);
+    T x[16];
 #pragma unroll
-  for (int k = 0; k < 16; k += V) {
-    float x[V];
-    const int32_t left = row0 + i < a.m ? a.n - (col0 + j + k) : 0;
-    const T* p = in + (int64_t)(row0 + i) * a.in_row + col0 + j + k;
-    if constexpr (V > 1) {  // (whole vectors: left is 0 or less, or at least V)
+    for (int k = 0; k < 16; ++k) x[k] = from[(int64_t)(row0 + w + k < a.m ? row0 + w + k : a.m - 1) * a.in_row];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float v = col < a.n && row0 + w + k < a.m ? ldexpf((float)x[k], exponent) : 0.f;
+      const uint16_t h = upd_half(v);
+      tile[0][w + k][lane_id()] = h;
+      if constexpr (TERMS == 3) tile[1][w + k][lane_id()] = upd_half(v - upd_float(h));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) part[t][k] = tile[t][i][j + k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; k += V) {
+      float x[V];
 #pragma unroll
       for (int q = 0; q < V; ++q) x[q] = 0.f;
-      if (left > 0) NormVec<T, V>::load(p, x);
-    } else {
-      x[0] = left > 0 ? (float)p[0] : 0.f;
+      if (row0 + i < a.m && col0 + j + k < a.n)  // (whole vectors)
+        NormVec<T, V>::load(in + (int64_t)(row0 + i) * a.in_row + col0 + j + k, x);
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const float v = ldexpf(x[q], exponent);
+        part[0][k + q] = upd_half(v);
+        if constexpr (TERMS == 3) part[1][k + q] = upd_half(v - upd_float(part[0][k + q]));
+      }
     }
 #pragma unroll
-    for (int q = 0; q < V; ++q) {
-      const float v = ldexpf(x[q], exponent);
-      part[0][k + q] = upd_half(v);
-      if constexpr (TERMS == 3) part[1][k + q] = upd_half(v - upd_float(part[0][k + q]));
-    }
+    for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t)
+#pragma unroll
+      for (int k = 0; k < 16; ++k) tile[t][i][j + k] = part[t][k];
   }
+  if (row0 + i < a.m) {
 #pragma unroll
-  for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) tile[t][i][j + k] = part[t][k];
-    if (row0 + i < a.m) {
-      u32x4_t* to = reinterpret_cast<u32x4_t*>(natural + t * plane_nat + (row0 + i) * ld_nat + col0 + j);
+    for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
+      u32x4_t* to = reinterpret_cast<u32x4_t*>(natural + (row0 + i) * ld_nat + upd_column<TERMS>(col0 + j, t));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         u32x4_t v;
@@ -176,7 +193,7 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
   if (col0 + i >= a.n) return;
 #pragma unroll
   for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
-    u32x4_t* to = reinterpret_cast<u32x4_t*>(transposed + t * plane_tr + (col0 + i) * ld_tr + row0 + j);
+    u32x4_t* to = reinterpret_cast<u32x4_t*>(transposed + (col0 + i) * ld_tr + upd_column<TERMS>(row0 + j, t));
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       u32x4_t v;
@@ -189,6 +206,12 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
 }
 
 // --- tiles -----------------------------------------------------------------------
+
+template <int TERMS>
+__device__ __forceinline__ UpdMatrix upd_matrix(const char* at, int32_t rows, int32_t ld) {
+  const uint32_t wide = (uint32_t)ld * (TERMS == 3 ? 2u : 1u);
+  return {at, (uint32_t)rows * wide * 2u, wide, (uint32_t)rows};
+}
 
 // A lane's place in the tile: fragment (fm, fn) holds four columns of one row.
 template <int F>
@@ -212,15 +235,17 @@ __device__ __forceinline__ void upd_put(char* image, uint32_t row, uint32_t col,
   *reinterpret_cast<f16x4_t*>(image + row * upd_pitch(F) + col * 2) = h;
 }
 
-// The image's rows to rows row0.. (below `rows`) of a matrix, columns col0.. (below ld).
-template <int F>
-__device__ __forceinline__ void upd_write_rows(const char* image, char* to, int32_t row0, int32_t col0,
+// The image's rows to rows row0.. (below `rows`) of a matrix, columns col0.. (below ld); t: to
+// which of its terms.
+template <int F, int TERMS>
+__device__ __forceinline__ void upd_write_rows(const char* image, char* to, int t, int32_t row0, int32_t col0,
                                                int32_t rows, int32_t ld) {
+  constexpr int64_t P = TERMS == 3 ? 2 : 1;
   constexpr int kChunks = upd_tile(F) / 8;
   for (int q = threadIdx.x; q < upd_tile(F) * kChunks; q += 256) {
     const int32_t i = q / kChunks, j = (q % kChunks) * 8;
     if (row0 + i < rows && col0 + j < ld)
-      *reinterpret_cast<u32x4_t*>(to + ((int64_t)(row0 + i) * ld + col0 + j) * 2) =
+      *reinterpret_cast<u32x4_t*>(to + ((row0 + i) * (P * ld) + upd_column<TERMS>(col0 + j, t)) * 2) =
           *reinterpret_cast<const u32x4_t*>(image + i * upd_pitch(F) + j * 2);
   }
 }
@@ -230,9 +255,10 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 // The image's columns to rows row0.. of a matrix: column i of the image is row row0 + i,
 // image row j column col0 + j.  A transposing read hands lane i of 16 the column c0 + i
 // of four rows (its lane 4 e + q reads columns c0 + 4 q .. of row e).
-template <int F>
-__device__ __forceinline__ void upd_write_columns(const char* image, char* to, int32_t row0, int32_t col0,
+template <int F, int TERMS>
+__device__ __forceinline__ void upd_write_columns(const char* image, char* to, int t, int32_t row0, int32_t col0,
                                                   int32_t rows, int32_t ld) {
+  constexpr int64_t P = TERMS == 3 ? 2 : 1;
   constexpr int kTile = upd_tile(F);
   const uint32_t l = lane_id(), in = l & 15u;
   // a wave's unit: 16 columns of 32 rows, 8 rows to each 16 lanes
@@ -245,7 +271,7 @@ __device__ __forceinline__ void upd_write_columns(const char* image, char* to, i
     const int32_t i = row0 + (int32_t)(c0 + in), j = col0 + (int32_t)j0;
     if (i < rows && j < ld) {
       struct { i16x4_t lo, hi; } both{lo, hi};
-      *reinterpret_cast<u32x4_t*>(to + ((int64_t)i * ld + j) * 2) = __builtin_bit_cast(u32x4_t, both);
+      *reinterpret_cast<u32x4_t*>(to + (i * (P * ld) + upd_column<TERMS>(j, t)) * 2) = __builtin_bit_cast(u32x4_t, both);
     }
   }
 }
@@ -276,8 +302,8 @@ __device__ __forceinline__ void upd_triangle(uint32_t at, uint32_t tiles, uint32
 
 // Both writes of a symmetric matrix's tile, whose fragment (fm, fn) value(fm, fn, x) gives.
 template <int F, int TERMS, class Value>
-__device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int64_t plane, int32_t row0, int32_t col0,
-                                                    int32_t r, int32_t ld, Value value) {
+__device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int32_t row0, int32_t col0, int32_t r,
+                                                    int32_t ld, Value value) {
   const UpdPlace<F> p;
 #pragma unroll
   for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
@@ -293,8 +319,8 @@ __device__ __forceinline__ void upd_write_symmetric(char* lds, char* to, int64_t
       sched_fence();  // (a row of fragments at a time: all at once would spill)
     }
     __syncthreads();
-    upd_write_rows<F>(lds, to + t * plane, row0, col0, r, ld);
-    if (row0 != col0) upd_write_columns<F>(lds, to + t * plane, col0, row0, r, ld);
+    upd_write_rows<F, TERMS>(lds, to, t, row0, col0, r, ld);
+    if (row0 != col0) upd_write_columns<F, TERMS>(lds, to, t, col0, row0, r, ld);
   }
 }
 
@@ -321,8 +347,7 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
   upd_triangle(tile, (uint32_t)a.tiles_m, ti, tj);
   char* ws = a.ws + (int64_t)__builtin_amdgcn_readfirstlane(matrix) * a.ws_stride;
   const int32_t row0 = (int32_t)ti * upd_tile(F), col0 = (int32_t)tj * upd_tile(F);
-  const UpdMatrix x = SQUARE ? UpdMatrix{ws + a.e, (uint32_t)a.r * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.r}
-                             : UpdMatrix{ws + a.l, (uint32_t)a.r * (uint32_t)a.ld_c * 2u, (uint32_t)a.ld_c, (uint32_t)a.r};
+  const UpdMatrix x = SQUARE ? upd_matrix<TERMS>(ws + a.e, a.r, a.ld_r) : upd_matrix<TERMS>(ws + a.l, a.r, a.ld_c);
   float* state = reinterpret_cast<float*>(ws + a.state);
   float mu = 0.f;
   if constexpr (WHAT == kUpdPart) {
@@ -359,8 +384,8 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
         for (int n = 0; n < F; ++n) acc[m][n] += parts[(q * F * F + m * F + n) * 256];
   } else {
     UpdOperand<F> oa, ob;
-    oa.init(x, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
-    ob.init(x, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
+    oa.init(x, (uint32_t)row0, (wave_id() >> 1) * 16 * F);
+    ob.init(x, (uint32_t)col0, (wave_id() & 1u) * 16 * F);
     const int stages = (int)x.ld / kUpdStage;
     if constexpr (WHAT == kUpdPart) {
       const int part = (int)(group - id * (uint32_t)a.split);
@@ -376,7 +401,6 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
     }
   }
   const UpdPlace<F> p;
-  const int64_t plane = (int64_t)a.r * a.ld_r * 2;
   // E is also kept by fragments, for the product that squares it: the same lanes of the
   // same tile read it there
   const int32_t across = a.ld_r / 16;
@@ -391,7 +415,7 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
     const float f = (a.first ? state[kUpdFactor] * state[kUpdFactor] : a.x_unscale * a.x_unscale) * a.e_scale;
     const float centre = mu * a.e_scale;
     upd_write_symmetric<F, TERMS>(
-        lds, ws + a.e, plane, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
+        lds, ws + a.e, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
           const int32_t row = row0 + (int32_t)p.row + 16 * fm, col = col0 + (int32_t)p.col + 16 * fn;
           f16x4_t h;
 #pragma unroll
@@ -420,7 +444,7 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
         if constexpr (TERMS == 3) held[1][fm][fn] = at[kept_plane];
       }
     upd_write_symmetric<F, TERMS>(
-        lds, ws + a.d, plane, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
+        lds, ws + a.d, row0, col0, a.r, a.ld_r, [&](int fm, int fn, int t, float (&x)[4]) {
           if (TERMS == 1 || t == 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -451,13 +475,12 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   char* ws = a.ws + (int64_t)matrix * a.ws_stride;
   const int32_t row0 = (int32_t)tm * upd_tile(F), col0 = (int32_t)tn * upd_tile(F);
   const bool tall = a.m > a.n;
-  const UpdMatrix d{ws + a.d, (uint32_t)a.r * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.r};
-  const UpdMatrix s{ws + a.s0, (uint32_t)a.c * (uint32_t)a.ld_r * 2u, (uint32_t)a.ld_r, (uint32_t)a.c};
+  const UpdMatrix d = upd_matrix<TERMS>(ws + a.d, a.r, a.ld_r), s = upd_matrix<TERMS>(ws + a.s0, a.c, a.ld_r);
   UpdOperand<F> oa, ob;
-  oa.init(tall ? s : d, (uint32_t)row0, (wave_id() >> 1) * 16 * F, TERMS == 3);
-  ob.init(tall ? d : s, (uint32_t)col0, (wave_id() & 1u) * 16 * F, TERMS == 3);
+  oa.init(tall ? s : d, (uint32_t)row0, (wave_id() >> 1) * 16 * F);
+  ob.init(tall ? d : s, (uint32_t)col0, (wave_id() & 1u) * 16 * F);
   f32x4_t acc[F][F];
-  upd_mainloop<F, TERMS>(lds, oa, ob, 0, a.ld_r / kUpdStage, acc);
+  upd_mainloop<F, TERMS>(lds, oa, ob, 0, (int)d.ld / kUpdStage, acc);
   const float* state = reinterpret_cast<const float*>(ws + a.state);
   const float mu = state[kUpdMu];
   const float product = a.d_unscale * (a.first ? state[kUpdFactor] : a.x_unscale);
@@ -546,10 +569,9 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   if (a.last) {
     if (!by_image) return;
     __syncthreads();
-    upd_write_rows<F>(lds, reinterpret_cast<char*>(out), row0, col0, a.m, a.n);
+    upd_write_rows<F, 1>(lds, reinterpret_cast<char*>(out), 0, row0, col0, a.m, a.n);
     return;
   }
-  const int64_t plane_s = (int64_t)a.c * a.ld_r * 2, plane_l = (int64_t)a.r * a.ld_c * 2;
 #pragma unroll
   for (int t = 0; t < (TERMS == 3 ? 2 : 1); ++t) {
     if (t) {
@@ -567,14 +589,13 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
       }
     }
     __syncthreads();
-    char* l = ws + a.l + t * plane_l;
-    char* next = ws + a.s1 + t * plane_s;
+    char *l = ws + a.l, *next = ws + a.s1;
     if (tall) {
-      upd_write_rows<F>(lds, next, row0, col0, a.c, a.ld_r);
-      upd_write_columns<F>(lds, l, col0, row0, a.r, a.ld_c);
+      upd_write_rows<F, TERMS>(lds, next, t, row0, col0, a.c, a.ld_r);
+      upd_write_columns<F, TERMS>(lds, l, t, col0, row0, a.r, a.ld_c);
     } else {
-      upd_write_rows<F>(lds, l, row0, col0, a.r, a.ld_c);
-      upd_write_columns<F>(lds, next, col0, row0, a.c, a.ld_r);
+      upd_write_rows<F, TERMS>(lds, l, t, row0, col0, a.r, a.ld_c);
+      upd_write_columns<F, TERMS>(lds, next, t, col0, row0, a.c, a.ld_r);
     }
   }
   ss = norm_wave_sum(ss);
