@@ -92,21 +92,14 @@ EmbedArgs embed_args(const mt_embed_args& a) {
   return k;
 }
 
-// Elements of the widest vector (16, 8 or 4 bytes, or one element) that every row of the
-// tensors is whole aligned ones of: of their addresses in bytes, their pitches and H.
-template <class T>
-int embed_vector(int64_t H, uintptr_t at, int64_t pitches) {
-  for (int V = 16 / (int)sizeof(T); V > 1; V = V == 8 ? 2 : V / 2)
-    if (H % V == 0 && pitches % V == 0 && at % (V * sizeof(T)) == 0) return V;
-  return 1;
-}
-
 // Calls f(V, K, log2 of the lanes of a row, workgroups) with the variant for `rows`
-// rows of H elements: vectors of V, most of them in flight per lane (up to kMost) that a
-// row fills; rows of few vectors share a wave unless share is false.
+// rows of H elements: 16-byte vectors (one element where a row is shorter), as many of them in
+// flight per lane (up to kMost) as a row fills; rows of few vectors share a wave unless share
+// is false.
 template <class T, int kMost, class F>
-int embed_pick(int64_t rows, int64_t H, int vector, F f, bool share = true) {
-  const int64_t nv = H / vector;
+int embed_pick(int64_t rows, int64_t H, F f, bool share = true) {
+  constexpr int W = 16 / (int)sizeof(T);
+  const int64_t nv = H < W ? H : cdiv(H, W);
   int log_lanes = 6;
   while (share && log_lanes > 0 && nv <= (int64_t)1 << (log_lanes - 1)) --log_lanes;
   const auto with = [&](auto V, auto K) {
@@ -116,23 +109,18 @@ int embed_pick(int64_t rows, int64_t H, int vector, F f, bool share = true) {
       return fail(MT_ERR_UNSUPPORTED, "%lld rows of %lld exceed one launch", (long long)rows, (long long)H);
     return f(V, K, log_lanes, (uint32_t)cdiv(units, 4));
   };
-  const auto wide = [&](auto V) {
-    if constexpr (kMost >= 4) {
-      if (nv > 128) return with(V, std::integral_constant<int, 4>());
-    }
-    if (nv > 64) return with(V, std::integral_constant<int, 2>());
-    return with(V, std::integral_constant<int, 1>());
-  };
-  constexpr int W = 16 / (int)sizeof(T);
-  if (vector == W) return wide(std::integral_constant<int, W>());
-  if (vector == 2) return wide(std::integral_constant<int, 2>());
-  return wide(std::integral_constant<int, 1>());
+  constexpr std::integral_constant<int, W> whole{};
+  if (H < W) return with(std::integral_constant<int, 1>(), std::integral_constant<int, 1>());
+  if constexpr (kMost >= 4) {
+    if (nv > 128) return with(whole, std::integral_constant<int, 4>());
+  }
+  if (nv > 64) return with(whole, std::integral_constant<int, 2>());
+  return with(whole, std::integral_constant<int, 1>());
 }
 
 template <class T>
 int launch_embed_forward(const EmbedArgs& k, hipStream_t stream) {
-  const int vector = embed_vector<T>(k.H, reinterpret_cast<uintptr_t>(k.w) | reinterpret_cast<uintptr_t>(k.out), k.w_t);
-  return embed_pick<T, 4>(k.T, k.H, vector, [&](auto V, auto K, int log_lanes, uint32_t groups) {
+  return embed_pick<T, 4>(k.T, k.H, [&](auto V, auto K, int log_lanes, uint32_t groups) {
     hipLaunchKernelGGL((embed_forward_kernel<T, decltype(V)::value, decltype(K)::value>), dim3(groups), dim3(256), 0,
                        stream, k, log_lanes);
     return check_launch("embed_forward_kernel");
@@ -141,26 +129,19 @@ int launch_embed_forward(const EmbedArgs& k, hipStream_t stream) {
 
 template <class T>
 int launch_embed_backward(const EmbedArgs& k, bool accumulate, hipStream_t stream) {
-  // (the accumulator's vectors are as many elements, but never more than 16 bytes)
-  int vector = embed_vector<T>(k.H, reinterpret_cast<uintptr_t>(k.dout), k.dout_t);
-  while (vector > 1 && (accumulate ? (k.dw_t % std::min(vector, 4) != 0 ||
-                                      reinterpret_cast<uintptr_t>(k.dw) % (4 * std::min(vector, 4)) != 0)
-                                   : (k.dw_t % vector != 0 || reinterpret_cast<uintptr_t>(k.dw) % (vector * sizeof(T)) != 0)))
-    vector = vector == 8 ? 2 : vector / 2;
   const bool direct = k.T <= kEmbedDirect;
   if (!direct) {
     if (k.wide) hipLaunchKernelGGL(embed_sort_kernel<int64_t>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
     else hipLaunchKernelGGL(embed_sort_kernel<int32_t>, dim3(1u << k.log_buckets), dim3(1024), 0, stream, k);
     MT_TRY(check_launch("embed_sort_kernel"));
-    MT_TRY((embed_pick<T, 2>(cdiv(k.T, kEmbedPiece), k.H, vector, [&](auto V, auto K, int, uint32_t groups) {
+    MT_TRY((embed_pick<T, 2>(cdiv(k.T, kEmbedPiece), k.H, [&](auto V, auto K, int, uint32_t groups) {
       hipLaunchKernelGGL((embed_pieces_kernel<T, decltype(V)::value, decltype(K)::value>), dim3(groups), dim3(256), 0,
                          stream, k);
       return check_launch("embed_pieces_kernel");
     }, false)));
   }
   if (accumulate && k.T == 0) return MT_OK;
-  return embed_pick<T, 2>(accumulate ? k.T : k.V, k.H, vector,
-                          [&](auto V, auto K, int log_lanes, uint32_t groups) {
+  return embed_pick<T, 2>(accumulate ? k.T : k.V, k.H, [&](auto V, auto K, int log_lanes, uint32_t groups) {
     constexpr int v = decltype(V)::value, n = decltype(K)::value;
     auto kern = direct ? (accumulate ? embed_direct_kernel<T, v, n, true> : embed_direct_kernel<T, v, n, false>)
                        : (accumulate ? embed_rows_kernel<T, v, n, true> : embed_rows_kernel<T, v, n, false>);

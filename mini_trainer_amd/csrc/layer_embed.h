@@ -34,17 +34,21 @@ constexpr int kEmbedFlight = 2;       // rows of dout, or partial rows, that a r
 constexpr int32_t kEmbedList = 512;  // tokens of a bucket and wave that are kept between its passes
 constexpr int32_t kEmbedDirect = 256;  // tokens that are not sorted, at most
 
-// V elements of T: 16, 8 or 4 bytes, or one element.
+// V elements of T, 16 bytes or one element, aligned as one: rows of an odd width begin
+// anywhere, and the memory instructions take any address of an element (gradient of 447
+// tokens into 67988 x 4415 in bf16 by single elements 317 us, so 147; of 65536 into 32000 x
+// 4095 314 and 215, the lookup 427 and 192).
 template <class T, int V>
 struct EmbedVec {
-  typedef T Raw __attribute__((ext_vector_type(V)));
+  typedef T Whole __attribute__((ext_vector_type(V)));
+  typedef Whole Raw __attribute__((aligned(sizeof(T))));
   __device__ __forceinline__ static Raw raw(const T* p) { return *reinterpret_cast<const Raw*>(p); }
   __device__ __forceinline__ static void open(const Raw& v, float (&x)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = (float)v[i];
   }
   __device__ __forceinline__ static void store(T* p, const float (&x)[V]) {
-    Raw v;
+    Whole v;
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = (T)x[i];
     *reinterpret_cast<Raw*>(p) = v;
@@ -75,15 +79,21 @@ __device__ __forceinline__ int32_t embed_place(const EmbedArgs& a, int32_t id) {
 
 // A row is read by 2^log_lanes lanes of a wave, K vectors of V elements each; rows
 // wider than a wave's 64 K vectors are cut into column chunks, narrower ones share a
-// wave.  Returns this lane's row, its first vector, and the number of vectors.
+// wave.  The last vector ends with the row: where V does not divide H it begins within
+// the one before, with equal values (H is at least V).
 struct EmbedSpan {
-  int64_t row;
-  int32_t first, step, nv;
+  int64_t row;                 // this lane's
+  int32_t first, step, nv, H;  // its first vector, the distance to its next, a row's vectors
+  template <int V>
+  __device__ __forceinline__ int32_t at(int32_t v) const {  // the first element of vector v
+    return v * V < H - V ? v * V : H - V;
+  }
 };
 template <int V, int K>
 __device__ __forceinline__ EmbedSpan embed_span(int32_t H, int32_t log_lanes) {
   EmbedSpan s;
-  s.nv = H / V;
+  s.H = H;
+  s.nv = (H + V - 1) / V;
   s.step = 1 << log_lanes;
   const uint32_t unit = blockIdx.x * 4u + wave_id();  // (below 2^26: 2^32 threads)
   const uint32_t lane = lane_id() & (uint32_t)(s.step - 1);
@@ -109,7 +119,7 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(EmbedArgs a, int32_t
   typename Vec::Raw raw[K];
 #pragma unroll
   for (int k = 0; k < K; ++k)
-    if (s.first + k * s.step < s.nv) raw[k] = Vec::raw(w + (int64_t)(s.first + k * s.step) * V);
+    if (s.first + k * s.step < s.nv) raw[k] = Vec::raw(w + s.template at<V>(s.first + k * s.step));
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int32_t v = s.first + k * s.step;
@@ -118,7 +128,7 @@ __global__ __launch_bounds__(256) void embed_forward_kernel(EmbedArgs a, int32_t
     Vec::open(raw[k], x);
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] *= scale;
-    Vec::store(out + (int64_t)v * V, x);
+    Vec::store(out + s.template at<V>(v), x);
   }
 }
 
@@ -265,7 +275,7 @@ __device__ __forceinline__ void embed_add(const EmbedArgs& a, const EmbedSpan& s
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int32_t v = s.first + k * s.step;
-      raw[u][k] = Vec::raw(row + (int64_t)(v < s.nv ? v : s.nv - 1) * V);
+      raw[u][k] = Vec::raw(row + s.template at<V>(v));
     }
   }
 #pragma unroll
@@ -332,7 +342,7 @@ __global__ __launch_bounds__(256) void embed_pieces_kernel(EmbedArgs a) {
     for (int k = 0; k < K; ++k)
       if (s.first + k * s.step < s.nv)
 #pragma unroll
-        for (int i = 0; i < V; ++i) to[(int64_t)(s.first + k * s.step) * V + i] = sum[k][i];
+        for (int i = 0; i < V; ++i) to[s.template at<V>(s.first + k * s.step) + i] = sum[k][i];
   }
 }
 
@@ -347,11 +357,20 @@ __device__ __forceinline__ void embed_put_row(const EmbedArgs& a, const EmbedSpa
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[k][i] *= a.scale;
     if constexpr (ADD) {
-      float* to = reinterpret_cast<float*>(a.dw) + id * a.dw_t + (int64_t)v * V;
+      float* to = reinterpret_cast<float*>(a.dw) + id * a.dw_t + s.template at<V>(v);
+      const int32_t twice = v * V - s.template at<V>(v);  // elements that are the vector's before
+      if (twice == 0) {
+        const typename EmbedVec<float, V>::Raw old = EmbedVec<float, V>::raw(to);
 #pragma unroll
-      for (int i = 0; i < V; ++i) to[i] += sum[k][i];
+        for (int i = 0; i < V; ++i) sum[k][i] += old[i];
+        EmbedVec<float, V>::store(to, sum[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i >= twice) to[i] += sum[k][i];
+      }
     } else {
-      EmbedVec<T, V>::store(reinterpret_cast<T*>(a.dw) + id * a.dw_t + (int64_t)v * V, sum[k]);
+      EmbedVec<T, V>::store(reinterpret_cast<T*>(a.dw) + id * a.dw_t + s.template at<V>(v), sum[k]);
     }
   }
 }
@@ -374,7 +393,7 @@ __device__ __forceinline__ void embed_add_parts(const EmbedArgs& a, const EmbedS
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int32_t v = s.first + k * s.step;
-      raw[u][k] = Vec::raw(a.part + (at + 2 * u) * a.part_t + (int64_t)(v < s.nv ? v : s.nv - 1) * V);
+      raw[u][k] = Vec::raw(a.part + (at + 2 * u) * a.part_t + s.template at<V>(v));
     }
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -481,8 +500,8 @@ __global__ __launch_bounds__(256) void embed_direct_kernel(EmbedArgs a, int32_t 
       for (int k = 0; k < K; ++k) {
         const int32_t v = s.first + k * s.step;
         if (v >= s.nv) continue;
-        const typename EmbedVec<T, V>::Raw r0 = EmbedVec<T, V>::raw(row + (int64_t)v * V);
-        const typename EmbedVec<T, V>::Raw r1 = EmbedVec<T, V>::raw(next + (int64_t)v * V);
+        const typename EmbedVec<T, V>::Raw r0 = EmbedVec<T, V>::raw(row + s.template at<V>(v));
+        const typename EmbedVec<T, V>::Raw r1 = EmbedVec<T, V>::raw(next + s.template at<V>(v));
         float x[V], y[V];
         EmbedVec<T, V>::open(r0, x);
         EmbedVec<T, V>::open(r1, y);

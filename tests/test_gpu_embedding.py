@@ -54,6 +54,15 @@ def test_matches_the_definition(gpu, T, V, H, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("H", [2, 3, 4, 5, 7, 9, 15, 17, 31, 33, 511, 513, 1023, 1025, 2047, 4095])
+def test_widths_of_no_whole_vectors(gpu, H, dtype):
+    """The last vector of a row begins within the one before: twice summed, once added."""
+    for T, V in ((200, 30), (700, 90)):
+        ids, w, d = make(T, V, H, dtype, seed=H)
+        check(ids, w, d, scale=1.7, accumulate=True)
+
+
+@BOTH
 @pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 256, 257, 1024, 1025, 5000])
 def test_one_id_takes_all_tokens(gpu, T, dtype):
     """A row of many pieces, from the first sorted token on and behind another row's."""
