@@ -723,7 +723,7 @@ int mt_grad_scale(void* const* ptrs, const int64_t* numel, const int64_t* cols,
  * accumulate != 0 adds these sums to an fp32 dweight, whose rows of ids that do not
  * occur it leaves as they are.  The row padding_idx (-1: none) gets no gradient.  Sums in
  * fp32 in a fixed order.  It reads ids and dout; H at most 2^24.  Few tokens take no
- * workspace (0 bytes, null).
+ * workspace (0 bytes, null).  No output may overlap another tensor.
  */
 typedef struct mt_embed_args {
   const void *ids, *weight;
@@ -749,14 +749,14 @@ int mt_embed_backward(const mt_embed_args* args, void* workspace, size_t workspa
  * computed in fp32 and rounded once; var is the mean square of the centred row.
  *   x, residual [T, H] with row pitches x_t, residual_t (elements); weight (null:
  *     ones), bias (null: zeros) [H]; normed, new_residual [T, H] contiguous
- *   residual_lo  [T, H] bytes (bf16 with a residual; 8-byte aligned for the fastest
- *     kernels): what new_residual's rounding took from it, from the forward to the
- *     backward (null in a forward without a backward)
+ *   residual_lo  [T, H] bytes (bf16 with a residual): what new_residual's rounding took
+ *     from it, from the forward to the backward (null in a forward without a backward)
  *   stat fp32 [2, T]: 1 / sqrt(var + eps) and the mean, from the forward to the
  *     backward (null as above);  H at most 32768;  all tensors of one dtype
  * The backward takes dnormed and (null: zeros) dresidual_out with row pitches, reads
  * new_residual, or x without a residual, stat and weight, and writes what is not null of
- * dx, dresidual [T, H] (contiguous), dweight, dbias [H].
+ * dx, dresidual [T, H] (contiguous), dweight, dbias [H].  No output may overlap another
+ * tensor.
  */
 typedef struct mt_layer_norm_args {
   const void *x, *residual, *weight, *bias;
@@ -782,7 +782,7 @@ int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size
  * for each of batch matrices G [m, n] (X its transpose where m > n), |G| the square root
  * of the sum of squares.
  *   in   rows of unit stride, in_row elements apart, matrices in_batch apart (0: the same
- *        matrix again);  out [batch, m, n] contiguous;  both of one dtype
+ *        matrix again);  out [batch, m, n] contiguous, not overlapping in;  both of one dtype
  *   coefficients  a, b, c of each step (host, 3 steps doubles, read during the call);
  *        such that singular values of at most 1 stay below 10^6 (MT_ERR_UNSUPPORTED)
  *   eps >= 0;  steps 1 to 64

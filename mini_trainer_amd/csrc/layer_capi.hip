@@ -185,19 +185,6 @@ int layer_norm_check(const mt_layer_norm_args* p, bool backward) {
   return MT_OK;
 }
 
-// Whether every row of every tensor is whole aligned 16-byte vectors.
-bool layer_norm_vectors(const mt_layer_norm_args& a, bool backward) {
-  const int64_t V = 16 / esize(a.dtype);
-  const bool res = a.has_residual != 0;
-  const void* all[] = {a.x, a.residual, a.weight, a.bias, a.normed, a.new_residual,
-                       a.dnormed, a.dresidual_out, a.dx, a.dresidual};
-  for (const void* x : all)
-    if (!aligned16(x)) return false;
-  if (reinterpret_cast<uintptr_t>(a.residual_lo) % 8) return false;
-  return a.H % V == 0 && ((backward && res) || a.x_t % V == 0) && (backward || !res || a.residual_t % V == 0) &&
-         (!backward || (a.dnormed_t % V == 0 && (!a.dresidual_out || a.dresidual_out_t % V == 0)));
-}
-
 LayerNormArgs layer_norm_args(const mt_layer_norm_args& a, bool backward) {
   const bool res = a.has_residual != 0;
   LayerNormArgs k{};
@@ -224,9 +211,32 @@ LayerNormArgs layer_norm_args(const mt_layer_norm_args& a, bool backward) {
   return k;
 }
 
+// Calls f with the kernels' template arguments for a row of H elements: the fewest threads and
+// registers that hold it (norm_pick's, but for rows of any width and alignment).
+template <class T, class F>
+int layer_norm_pick(int64_t H, F f) {
+  constexpr int W = 16 / (int)sizeof(T);
+  constexpr std::integral_constant<int, W> V{};
+  const auto with = [&](auto K, auto TPR) { return f(V, K, TPR); };
+  constexpr std::integral_constant<int, 1> k1{};
+  constexpr std::integral_constant<int, 2> k2{};
+  constexpr std::integral_constant<int, 4> k4{};
+  constexpr std::integral_constant<int, 64> wave{};
+  constexpr std::integral_constant<int, 256> four{};
+  constexpr std::integral_constant<int, 1024> all{};
+  if (H < W) return f(k1, k1, wave);
+  if (H <= 64 * 2 * W) return with(k2, wave);
+  if (H <= 256 * 1 * W) return with(k1, four);
+  if (H <= 256 * 2 * W) return with(k2, four);
+  if (H <= 256 * 4 * W) return with(k4, four);
+  if (H <= 1024 * 2 * W) return with(k2, all);
+  if constexpr (W == 8) return with(k4, all);
+  else return H <= 1024 * 4 * W ? with(k4, all) : with(std::integral_constant<int, 8>(), all);
+}
+
 template <class T>
-int launch_layer_norm_fwd(const LayerNormArgs& k, bool res, bool vec, hipStream_t stream) {
-  return norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+int launch_layer_norm_fwd(const LayerNormArgs& k, bool res, hipStream_t stream) {
+  return layer_norm_pick<T>(k.H, [&](auto V, auto K, auto TPR) {
     constexpr int threads = norm_threads(decltype(TPR)::value);
     constexpr int rows = threads / decltype(TPR)::value;
     if (cdiv(k.T, rows) * threads >= (int64_t)1 << 32)  // threads of a launch
@@ -239,9 +249,8 @@ int launch_layer_norm_fwd(const LayerNormArgs& k, bool res, bool vec, hipStream_
 }
 
 template <class T>
-int launch_layer_norm_bwd(LayerNormArgs k, const mt_layer_norm_args& a, bool res, bool vec,
-                          hipStream_t stream) {
-  MT_TRY(norm_pick<T>(k.H, vec, [&](auto V, auto K, auto TPR) {
+int launch_layer_norm_bwd(LayerNormArgs k, const mt_layer_norm_args& a, bool res, hipStream_t stream) {
+  MT_TRY(layer_norm_pick<T>(k.H, [&](auto V, auto K, auto TPR) {
     constexpr int threads = norm_threads(decltype(TPR)::value);
     constexpr int rows = threads / decltype(TPR)::value;
     const int64_t groups = std::min<int64_t>(cdiv(k.T, rows), kNormGroups);
@@ -305,9 +314,9 @@ int mt_layer_norm_forward(const mt_layer_norm_args* args, mt_stream_t stream) {
   const mt_layer_norm_args& a = *args;
   if (a.T == 0) return MT_OK;
   const LayerNormArgs k = layer_norm_args(a, false);
-  const bool res = a.has_residual != 0, vec = layer_norm_vectors(a, false);
-  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_fwd<__bf16>(k, res, vec, (hipStream_t)stream)
-                                  : launch_layer_norm_fwd<float>(k, res, vec, (hipStream_t)stream);
+  const bool res = a.has_residual != 0;
+  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_fwd<__bf16>(k, res, (hipStream_t)stream)
+                                  : launch_layer_norm_fwd<float>(k, res, (hipStream_t)stream);
 }
 
 size_t mt_layer_norm_backward_workspace_bytes(int64_t T, int64_t H) {
@@ -326,9 +335,9 @@ int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size
     return fail(MT_ERR_WORKSPACE_TOO_SMALL, "workspace: %zu bytes, %zu needed", workspace_bytes, need);
   LayerNormArgs k = layer_norm_args(a, true);
   k.part = static_cast<float*>(workspace);
-  const bool res = a.has_residual != 0, vec = layer_norm_vectors(a, true);
-  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_bwd<__bf16>(k, a, res, vec, (hipStream_t)stream)
-                                  : launch_layer_norm_bwd<float>(k, a, res, vec, (hipStream_t)stream);
+  const bool res = a.has_residual != 0;
+  return a.dtype == MT_DTYPE_BF16 ? launch_layer_norm_bwd<__bf16>(k, a, res, (hipStream_t)stream)
+                                  : launch_layer_norm_bwd<float>(k, a, res, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -18,8 +18,10 @@
 // norm, its own rounding by 0.0017, and rows with a large mean lose more.
 //
 // Bound by HBM: 32768 x 4096 in bf16 with a residual, forward 206 us (5.9 TB/s of 1.21 GB),
-// backward 235 us (5.2 TB/s of 1.23 GB).  Rows that are no whole vectors go by single
-// elements (2999 x 1601 in fp32: 13 and 24 us, 2.9 and 2.4 TB/s).
+// backward 235 us (5.2 TB/s of 1.23 GB).  Rows of any width go by 16-byte vectors at the
+// address of any element, the last one ending with the row: where it begins within the one
+// before, both hold equal values, and the sums over a row take them once (16384 x 4095 in bf16 by
+// single elements 259 and 426 us, so 136 and 174; 4096 wide 111 and 124).
 #pragma once
 
 #include "step_norm.h"
@@ -49,20 +51,44 @@ __device__ __forceinline__ float with_low_byte(float hi, uint32_t byte) {
   return __uint_as_float(__float_as_uint(hi) + (uint32_t)((int32_t)(int8_t)byte * 256));
 }
 
-// V bytes of a row from element v V on.
+// NormVec's vectors at the address of any element.
+template <class T, int V>
+struct LayerVec : NormVec<T, V> {
+  typedef typename NormVec<T, V>::Raw Whole;
+  typedef Whole Raw __attribute__((aligned(sizeof(T))));
+  __device__ __forceinline__ static Raw raw(const T* p) { return *reinterpret_cast<const Raw*>(p); }
+  __device__ __forceinline__ static void load(const T* p, float (&out)[V]) {
+    const Whole v = *reinterpret_cast<const Raw*>(p);
+    NormVec<T, V>::open(v, out);
+  }
+  __device__ __forceinline__ static void store(T* p, const float (&in)[V]) {
+    Whole v;
+    NormVec<T, V>::store(reinterpret_cast<T*>(&v), in);
+    *reinterpret_cast<Raw*>(p) = v;
+  }
+};
+
+// The first element of vector v of a row of H, and how many of it are the vector's before.
+template <int V>
+__device__ __forceinline__ int32_t layer_at(int32_t v, int32_t H) { return v * V < H - V ? v * V : H - V; }
+template <int V>
+__device__ __forceinline__ int32_t layer_twice(int32_t v, int32_t H) { return v * V - layer_at<V>(v, H); }
+
+// V bytes of a row.
 template <int V>
 struct LowBytes {
-  typedef typename std::conditional<V == 1, uint8_t, u32x2_t>::type Raw;
-  __device__ __forceinline__ static uint32_t at(const Raw& r, int i) {
+  typedef typename std::conditional<V == 1, uint8_t, u32x2_t>::type Whole;
+  typedef Whole Raw __attribute__((aligned(1)));
+  __device__ __forceinline__ static uint32_t at(const Whole& r, int i) {
     if constexpr (V == 1) return r;
     else return (r[i / 4] >> (8 * (i % 4))) & 0xffu;
   }
   __device__ __forceinline__ static void store(uint8_t* p, const float (&h)[V]) {
-    Raw r;
+    Whole r;
     if constexpr (V == 1) {
       r = (uint8_t)low_byte(h[0], (float)(__bf16)h[0]);
     } else {
-      r = Raw{0u, 0u};
+      r = Whole{0u, 0u};
 #pragma unroll
       for (int i = 0; i < V; i += 2) {
         float lo = h[i], hi = h[i + 1];
@@ -77,12 +103,12 @@ struct LowBytes {
 template <class T, int V, int K, int TPR, bool RES>
 __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_fwd_kernel(LayerNormArgs a) {
   constexpr int kRows = norm_threads(TPR) / TPR;
-  typedef NormVec<T, V> Vec;
+  typedef LayerVec<T, V> Vec;
   __shared__ float scratch[32];
   uint32_t turn = 0;
   const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
   if (row >= a.T) return;  // (whole waves; with TPR > 64 the workgroup)
-  const int32_t lane = threadIdx.x % TPR, nv = a.H / V;
+  const int32_t lane = threadIdx.x % TPR, nv = (a.H + V - 1) / V;
   const T* x = reinterpret_cast<const T*>(a.x) + row * a.x_t;
   const float inv_h = 1.0f / (float)a.H;
   float h[K][V];
@@ -93,15 +119,22 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_fwd_kernel(Layer
 #pragma unroll
     for (int i = 0; i < V; ++i) h[k][i] = 0.f;
     if (v < nv) {
-      Vec::load(x + (int64_t)v * V, h[k]);
+      const int32_t at = layer_at<V>(v, a.H);
+      Vec::load(x + at, h[k]);
       if constexpr (RES) {
         float r[V];
-        Vec::load(reinterpret_cast<const T*>(a.residual) + row * a.r_t + (int64_t)v * V, r);
+        Vec::load(reinterpret_cast<const T*>(a.residual) + row * a.r_t + at, r);
 #pragma unroll
         for (int i = 0; i < V; ++i) h[k][i] = fmaf(a.block_scale, h[k][i], a.residual_scale * r[i]);
       }
+      const int32_t twice = v * V - at;
+      if (twice == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) s += h[k][i];
+        for (int i = 0; i < V; ++i) s += h[k][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) s += i < twice ? 0.f : h[k][i];
+      }
     }
   }
   if constexpr (RES) {
@@ -109,9 +142,10 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_fwd_kernel(Layer
     for (int k = 0; k < K; ++k) {
       const int32_t v = lane + k * TPR;
       if (v >= nv) continue;
-      Vec::store(reinterpret_cast<T*>(a.h_out) + row * a.H + (int64_t)v * V, h[k]);
+      const int64_t at = row * a.H + layer_at<V>(v, a.H);
+      Vec::store(reinterpret_cast<T*>(a.h_out) + at, h[k]);
       if constexpr (sizeof(T) == 2) {
-        if (a.lo) LowBytes<V>::store(a.lo + row * a.H + (int64_t)v * V, h[k]);
+        if (a.lo) LowBytes<V>::store(a.lo + at, h[k]);
       }
     }
   }
@@ -119,11 +153,17 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_fwd_kernel(Layer
   float ss = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (lane + k * TPR >= nv) continue;
+    const int32_t v = lane + k * TPR;
+    if (v >= nv) continue;
+    const int32_t twice = layer_twice<V>(v, a.H);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      h[k][i] -= mean;
-      ss = fmaf(h[k][i], h[k][i], ss);
+    for (int i = 0; i < V; ++i) h[k][i] -= mean;
+    if (twice == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) ss = fmaf(h[k][i], h[k][i], ss);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) ss = i < twice ? ss : fmaf(h[k][i], h[k][i], ss);
     }
   }
   const float rstd = 1.0f / sqrtf(norm_row_sum<TPR>(ss, scratch, turn) * inv_h + a.eps);
@@ -138,11 +178,12 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_fwd_kernel(Layer
     float w[V], b[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i] = 1.f, b[i] = 0.f;
-    if (a.w) Vec::load(reinterpret_cast<const T*>(a.w) + (int64_t)v * V, w);
-    if (a.b) Vec::load(reinterpret_cast<const T*>(a.b) + (int64_t)v * V, b);
+    const int32_t at = layer_at<V>(v, a.H);
+    if (a.w) Vec::load(reinterpret_cast<const T*>(a.w) + at, w);
+    if (a.b) Vec::load(reinterpret_cast<const T*>(a.b) + at, b);
 #pragma unroll
     for (int i = 0; i < V; ++i) h[k][i] = fmaf(h[k][i] * rstd, w[i], b[i]);
-    Vec::store(reinterpret_cast<T*>(a.y) + row * a.H + (int64_t)v * V, h[k]);
+    Vec::store(reinterpret_cast<T*>(a.y) + row * a.H + at, h[k]);
   }
 }
 
@@ -150,11 +191,11 @@ template <class T, int V, int K, int TPR, bool RES>
 __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(LayerNormArgs a) {
   constexpr int kRows = norm_threads(TPR) / TPR;
   constexpr bool kLow = RES && sizeof(T) == 2;
-  typedef NormVec<T, V> Vec;
+  typedef LayerVec<T, V> Vec;
   typedef LowBytes<V == 1 ? 1 : 8> Low;
   __shared__ float scratch[32];
   uint32_t turn = 0;
-  const int32_t lane = threadIdx.x % TPR, nv = a.H / V;
+  const int32_t lane = threadIdx.x % TPR, nv = (a.H + V - 1) / V;
   const int32_t part = (int32_t)blockIdx.x * kRows + (int32_t)(threadIdx.x / TPR);
   const float inv_h = 1.0f / (float)a.H;
   float dw[K][V], db[K][V];
@@ -163,8 +204,9 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.f;
   // the weight stays in registers over the rows, and the next row's tensors are on
-  // their way while this one is worked on (single elements are read as they are used)
-  constexpr bool kHold = V > 1;
+  // their way while this one is worked on (wider rows leave no registers for it:
+  // 16384 x 12288 in bf16 391 us, held 1555)
+  constexpr bool kHold = K * V * TPR <= 8192;
   typename Vec::Raw w_raw[kHold ? K : 1];
   typename Vec::Raw r_h[kHold ? K : 1], r_dy[kHold ? K : 1], r_dh[kHold && RES ? K : 1];
   typename Low::Raw r_lo[kHold && kLow ? K : 1];
@@ -172,20 +214,21 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
 #pragma unroll
     for (int k = 0; k < (kHold ? K : 0); ++k)
       if (lane + k * TPR < nv)
-        w_raw[k] = Vec::raw(reinterpret_cast<const T*>(a.w) + (int64_t)(lane + k * TPR) * V);
+        w_raw[k] = Vec::raw(reinterpret_cast<const T*>(a.w) + layer_at<V>(lane + k * TPR, a.H));
   }
   auto fetch = [&](int64_t row) {
 #pragma unroll
     for (int k = 0; k < (kHold ? K : 0); ++k) {
       const int32_t v = lane + k * TPR;
       if (v >= nv) continue;
-      r_h[k] = Vec::raw(reinterpret_cast<const T*>(a.h) + row * a.h_t + (int64_t)v * V);
-      r_dy[k] = Vec::raw(reinterpret_cast<const T*>(a.dy) + row * a.dy_t + (int64_t)v * V);
+      const int32_t at = layer_at<V>(v, a.H);
+      r_h[k] = Vec::raw(reinterpret_cast<const T*>(a.h) + row * a.h_t + at);
+      r_dy[k] = Vec::raw(reinterpret_cast<const T*>(a.dy) + row * a.dy_t + at);
       if constexpr (RES) {
-        if (a.dh) r_dh[k] = Vec::raw(reinterpret_cast<const T*>(a.dh) + row * a.dh_t + (int64_t)v * V);
+        if (a.dh) r_dh[k] = Vec::raw(reinterpret_cast<const T*>(a.dh) + row * a.dh_t + at);
       }
       if constexpr (kLow)
-        r_lo[k] = *reinterpret_cast<const typename Low::Raw*>(a.lo + row * a.H + (int64_t)v * V);
+        r_lo[k] = *reinterpret_cast<const typename Low::Raw*>(a.lo + row * a.H + at);
     }
   };
   if (part < a.T) fetch(part);
@@ -217,13 +260,18 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
           for (int i = 0; i < V; ++i) hn[k][i] = with_low_byte(hn[k][i], Low::at(r_lo[k], i));
         }
       } else {
-        if (a.w) Vec::load(reinterpret_cast<const T*>(a.w) + v, w);
-        Vec::load(reinterpret_cast<const T*>(a.h) + row * a.h_t + v, hn[k]);
-        Vec::load(reinterpret_cast<const T*>(a.dy) + row * a.dy_t + v, g[k]);
+        const int32_t at = layer_at<V>(v, a.H);
+        if (a.w) Vec::load(reinterpret_cast<const T*>(a.w) + at, w);
+        Vec::load(reinterpret_cast<const T*>(a.h) + row * a.h_t + at, hn[k]);
+        Vec::load(reinterpret_cast<const T*>(a.dy) + row * a.dy_t + at, g[k]);
         if constexpr (RES) {
-          if (a.dh) Vec::load(reinterpret_cast<const T*>(a.dh) + row * a.dh_t + v, d[k]);
+          if (a.dh) Vec::load(reinterpret_cast<const T*>(a.dh) + row * a.dh_t + at, d[k]);
         }
-        if constexpr (kLow) hn[k][0] = with_low_byte(hn[k][0], a.lo[row * a.H + v]);
+        if constexpr (kLow) {
+          const typename Low::Whole lo = *reinterpret_cast<const typename Low::Raw*>(a.lo + row * a.H + at);
+#pragma unroll
+          for (int i = 0; i < V; ++i) hn[k][i] = with_low_byte(hn[k][i], Low::at(lo, i));
+        }
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
@@ -231,8 +279,20 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
         dw[k][i] = fmaf(g[k][i], hn[k][i], dw[k][i]);
         db[k][i] += g[k][i];
         g[k][i] *= w[i];
-        s0 += g[k][i];
-        s1 = fmaf(g[k][i], hn[k][i], s1);
+      }
+      const int32_t twice = layer_twice<V>(v, a.H);
+      if (twice == 0) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          s0 += g[k][i];
+          s1 = fmaf(g[k][i], hn[k][i], s1);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          s0 += i < twice ? 0.f : g[k][i];
+          s1 = i < twice ? s1 : fmaf(g[k][i], hn[k][i], s1);
+        }
       }
     }
     if (kHold && row + a.parts < a.T) fetch(row + a.parts);
@@ -251,11 +311,11 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
           g[k][i] *= a.block_scale;
         }
       }
+      const int64_t at = row * a.H + layer_at<V>(v, a.H);
       if constexpr (RES) {
-        if (a.dresidual)
-          Vec::store(reinterpret_cast<T*>(a.dresidual) + row * a.H + (int64_t)v * V, d[k]);
+        if (a.dresidual) Vec::store(reinterpret_cast<T*>(a.dresidual) + at, d[k]);
       }
-      if (a.dx) Vec::store(reinterpret_cast<T*>(a.dx) + row * a.H + (int64_t)v * V, g[k]);
+      if (a.dx) Vec::store(reinterpret_cast<T*>(a.dx) + at, g[k]);
     }
   }
   if (part < a.parts) {
@@ -265,7 +325,7 @@ __global__ __launch_bounds__(norm_threads(TPR)) void layer_norm_bwd_kernel(Layer
       if (v >= nv) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int64_t c = (int64_t)part * a.H + (int64_t)v * V + i;
+        const int64_t c = (int64_t)part * a.H + layer_at<V>(v, a.H) + i;
         a.part[c] = dw[k][i];
         a.part[(int64_t)a.parts * a.H + c] = db[k][i];
       }

@@ -71,6 +71,16 @@ def test_widths(gpu, H, dtype):
     check(*make(6, H, dtype, False, seed=H))
 
 
+@BOTH
+@pytest.mark.parametrize("T,H", [(2100, 3), (2100, 5), (9, 7), (2100, 9), (9, 15), (2100, 17), (9, 511), (2100, 513),
+                                 (600, 1025), (9, 2047), (600, 2051), (9, 4095), (9, 4097), (520, 8193),
+                                 (9, 12289), (9, 16385), (9, 20001), (9, 24577)])
+def test_the_last_vector_begins_within_the_one_before(gpu, T, H, dtype):
+    t, ups = make(T, H, dtype, seed=H)
+    check(t, ups, **SCALES)
+    check(*make(T, H, dtype, False, seed=H))
+
+
 def test_more_rows_than_workgroups(gpu):
     for T, H, residual in ((5000, 64, False), (3000, 520, True), (1100, 2056, True), (1100, 2056, False)):
         check(*make(T, H, torch.bfloat16, residual, seed=T))
