@@ -466,6 +466,8 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
   }
 }
 
+typedef f32x4_t any_f32x4_t __attribute__((aligned(4)));
+
 // X <- (a + p(mu)) X + D X, as it lies in memory [m, n]: D S^T, or S D where m > n.  Writes
 // the carried X, both fp16 copies and the tile's sum of squares, or at the last step the
 // result.
@@ -501,6 +503,11 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
     return row0 + (int32_t)(wave_id() >> 1) * 16 * F + 16 * fm < a.m &&
            col0 + (int32_t)(wave_id() & 1u) * 16 * F + 16 * fn < a.n;
   };
+  // Whether four elements of G and of the result from `col` on go one by one: in fp32 where
+  // the row ends within them (vectors lie at any element's address: 3 of 1001 x 1537 479 -> 470
+  // us), in bf16 where not all rows are whole vectors (asked per fragment it costs the 256 x
+  // 256 tiles of 14336 x 4096 2%)
+  auto singly = [&](int32_t col) { return sizeof(T) == 4 ? col + 4 > a.n : !a.vec; };
   // X before the step: G, or what the last step left, which is zero past the matrix's ends
   auto fetch = [&](int fm, f32x4_t (&x)[F]) __attribute__((always_inline)) {
 #pragma unroll
@@ -514,13 +521,13 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
       }
       const T* from = in + (int64_t)row * a.in_row + col;
       if (row >= a.m) continue;
-      if (!a.vec) {
+      if (singly(col)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (col + i < a.n) x[fn][i] = (float)from[i];
-      } else if (col < a.n) {  // (n and the rows' distance are whole vectors: four aligned elements)
+      } else if (col < a.n) {
         if constexpr (sizeof(T) == 4) {
-          x[fn] = *reinterpret_cast<const f32x4_t*>(from);
+          x[fn] = *reinterpret_cast<const any_f32x4_t*>(from);
         } else {
           const u32x2_t v = *reinterpret_cast<const u32x2_t*>(from);
 #pragma unroll
@@ -560,12 +567,12 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
             u32x2_t{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
       } else if (row < a.m) {
         T* to = out + (int64_t)row * a.n + col;
-        if (sizeof(T) == 4 && a.vec) {
-          if (col < a.n) *reinterpret_cast<f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
-        } else {
+        if (sizeof(T) == 2 || singly(col)) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (col + i < a.n) to[i] = (T)x[i];
+        } else if (col < a.n) {
+          *reinterpret_cast<any_f32x4_t*>(to) = f32x4_t{x[0], x[1], x[2], x[3]};
         }
       }
     }
