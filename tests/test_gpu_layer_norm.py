@@ -86,6 +86,21 @@ def test_more_rows_than_workgroups(gpu):
         check(*make(T, H, torch.bfloat16, residual, seed=T))
 
 
+def test_offsets_beyond_32_bits(gpu):
+    """The last rows of tensors of more than 2^31 elements as those rows alone."""
+    T, H = 270000, 8193
+    x = torch.empty(T, H, dtype=torch.bfloat16, device=gpu).normal_(generator=torch.Generator("cuda").manual_seed(1))
+    w = torch.linspace(-2, 2, H, device=gpu).bfloat16()
+    x.requires_grad_(True)
+    normed, h = residual_layer_norm(x, x.detach(), w, w)
+    (dx,) = torch.autograd.grad([normed, h], x, [x.detach(), x.detach()])
+    last = x.detach()[-5:].clone().requires_grad_(True)
+    n5, h5 = residual_layer_norm(last, last.detach(), w, w)
+    (d5,) = torch.autograd.grad([n5, h5], last, [last.detach(), last.detach()])
+    for got, want in ((normed, n5), (h, h5), (dx, d5)):
+        assert torch.equal(got[-5:], want)
+
+
 @BOTH
 def test_large_means(gpu, dtype):
     """Rows whose mean is 50 times their deviation."""

@@ -207,3 +207,15 @@ def test_captured(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, orthogonalize(x)) and torch.equal(little, orthogonalize(small))
+
+
+def test_stacks_of_more_than_32_bits(gpu):
+    """The ends of a stack of more than 2^31 elements: small matrices of one launch, and larger
+    ones that the workspace takes in groups."""
+    for batch, m, n in ((70000, 128, 256), (4300, 500, 1001)):
+        x = torch.empty(batch, m, n, dtype=torch.bfloat16, device=gpu)
+        for i, part in enumerate(x.split(1 << 12)):
+            part.normal_(generator=torch.Generator("cuda").manual_seed(i))
+        got = orthogonalize(x)
+        for at in (0, batch // 2, batch - 1):
+            ref.assert_within(got[at], x[at])
