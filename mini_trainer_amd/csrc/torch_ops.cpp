@@ -125,7 +125,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list none(7);
     if (!ctx->needs_input_grad(1) || !grads[0].defined()) return none;
-    const Tensor ids = ctx->get_saved_variables()[0], d = rows(grads[0]);
+    const Tensor ids = ctx->get_saved_variables()[0].contiguous(), d = rows(grads[0]);  // (as below)
     const auto found = ctx->saved_data.find("accumulator");
     const bool add = found != ctx->saved_data.end();
     const int64_t V = ctx->saved_data["V"].toInt(), T = ids.numel(), H = d.size(1);
@@ -209,13 +209,15 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const bool second = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !second) return none;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &kept = saved[2];
     auto& data = ctx->saved_data;
     const auto shape = data["shape"].toIntVector();
     const bool residual = data["residual"].toBool();
     const double block_scale = data["block_scale"].toDouble(), residual_scale = data["residual_scale"].toDouble();
     const int64_t low = data["low"].toInt();
-    const c10::DeviceGuard guard(h.device());
+    const c10::DeviceGuard guard(saved[0].device());
+    // (a hook on saved tensors may hand them back in another layout)
+    const Tensor h = residual ? saved[0].contiguous() : rows(saved[0]);
+    const Tensor w = saved[1].defined() ? saved[1].contiguous() : Tensor(), kept = saved[2].contiguous();
     refuse_foreign_leaves(h.device(), data["stream"].toInt());
     const Tensor dn = rows(grads[0].defined() ? grads[0] : at::zeros(shape, h.options()));
     const Tensor dh = second ? rows(grads[1]) : Tensor();
@@ -243,7 +245,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     a.dresidual = at_or_null(dr);
     a.dweight = at_or_null(dw);
     a.dbias = at_or_null(db);
-    a.x_t = residual ? H : pitch(rows(h));
+    a.x_t = residual ? H : pitch(h);
     a.dnormed_t = pitch(dn), a.dresidual_out_t = dh.defined() ? pitch(dh) : H;
     a.T = T, a.H = H;
     a.eps = (float)data["eps"].toDouble();
