@@ -20,6 +20,7 @@ from .flce import _backward_once, _dtype_code, _launch, _require_device
 __all__ = ["layer_norm", "residual_layer_norm", "residual_rms_norm"]
 
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_ELEMENT = range(4)
+ROWS_SAVED = (0, 3)  # of _ResidualRmsNorm's saved tensors: x and the gate, read by rows
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -69,16 +70,22 @@ class _ResidualRmsNorm(torch.autograd.Function):
         # x is read again only for the gradients of a gate or of a norm on it
         extra = pw is not None or g is not None
         ctx.save_for_backward(x2 if extra else None, w, pw, g, new_residual, rstd)
-        ctx.meta = (T, H, x_t, gate_t, tail, None if gate is None else gate.shape)
+        ctx.meta = (T, H, tail, None if gate is None else gate.shape)
         return normed, new_residual
 
     @_backward_once
     def backward(ctx, dnormed, dnew):
         if dnormed is None and dnew is None:
             return (None,) * 10
-        x2, w, pw, g, new_residual, rstd = ctx.saved_tensors
-        T, H, x_t, gate_t, tail, gate_shape = ctx.meta
-        _, block_scale, residual_scale, _, _, _ = tail
+        # a hook on saved tensors may hand them back in another layout (save_on_cpu: rows of
+        # a wider tensor as rows of their own)
+        x2, w, pw, g, new_residual, rstd = (
+            t if t is None or t.is_contiguous() else _rows(t) if k in ROWS_SAVED else t.contiguous()
+            for k, t in enumerate(ctx.saved_tensors))
+        T, H, tail, gate_shape = ctx.meta
+        _, block_scale, residual_scale, _, gate_mode, _ = tail
+        x_t = H if x2 is None else _pitch(x2)
+        gate_t = _pitch(g) if gate_mode in (GATE_TOKEN, GATE_ELEMENT) else 0
         need_x, need_r, need_w, need_pw, need_g = ctx.needs_input_grad[:5]
         dev = new_residual.device
         dn = _rows(torch.zeros_like(new_residual) if dnormed is None else dnormed)

@@ -1,5 +1,5 @@
-"""The C++ autograd nodes without a GPU: what they hand to the C ABI, whose backward entries
-are replaced by functions of this file that look at it."""
+"""Autograd nodes without a GPU: what they hand to the C ABI, whose entries are replaced by
+functions of this file that look at it."""
 from __future__ import annotations
 
 import ctypes
@@ -8,8 +8,8 @@ from ctypes import POINTER, c_int, c_int64, c_size_t, c_void_p
 import pytest
 import torch
 
-from mini_trainer_amd import _lib
-from mini_trainer_amd._lib import EmbedArgs, LayerNormArgs
+from mini_trainer_amd import _lib, norms
+from mini_trainer_amd._lib import EmbedArgs, LayerNormArgs, NormArgs
 
 OK = ctypes.CFUNCTYPE(c_int, c_void_p, c_void_p)
 BYTES = ctypes.CFUNCTYPE(c_size_t, c_int64, c_int64)
@@ -93,3 +93,37 @@ def test_saved_ids_may_come_back_in_another_layout(nodes):
         out = ops.embedding(ids, w, 1.0, -1, None, None, 0)
         torch.autograd.grad(out, w, torch.zeros(7, 4))
     assert torch.equal(seen[0][0], ids)
+
+
+@pytest.mark.parametrize("back", [shuffled, torch.Tensor.contiguous])
+@pytest.mark.parametrize("gated", [norms.GATE_CHANNEL, norms.GATE_TOKEN, norms.GATE_ELEMENT])
+def test_residual_rms_norm_reads_what_a_hook_hands_back(monkeypatch, back, gated):
+    """contiguous: as torch.autograd.graph.save_on_cpu does it with rows of a wider tensor."""
+    T, H = 6, 8
+    shape = {norms.GATE_CHANNEL: (H,), norms.GATE_TOKEN: (T, 1), norms.GATE_ELEMENT: (T, H)}[gated]
+    wide = torch.arange(T * 24, dtype=torch.float32).view(T, 24)
+    x, w = wide[:, 3:3 + H].requires_grad_(True), torch.arange(H, dtype=torch.float32)
+    gate = wide[:, 12:12 + shape[-1]] if len(shape) == 2 else torch.arange(H) + 0.5
+    r, seen = torch.ones(T, H), []
+
+    def launch(dev, what, entry, args, *rest):
+        a = NormArgs.from_buffer_copy(args)
+        if what == "mt_norm_forward":
+            ctypes.memmove(a.new_residual, r.data_ptr(), 4 * T * H)
+            for i in range(2 * T):
+                (ctypes.c_float * (2 * T)).from_address(a.rstd)[i] = i
+            return
+        seen.append((a.x_t, a.gate_t))
+        assert a.x_t <= H and a.gate_t <= H  # (what came back has no more)
+        pitch, rows_ = (a.gate_t, T) if gated != norms.GATE_CHANNEL else (H, 1)
+        seen.append((matrix(a.x, a.x_t, T, H), matrix(a.gate, pitch, rows_, shape[-1]),
+                     matrix(a.weight, H, 1, H)[0], matrix(a.new_residual, H, T, H),
+                     matrix(a.rstd, 2 * T, 1, 2 * T)[0]))
+
+    monkeypatch.setattr(norms, "_launch", launch)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), back):
+        y, _ = norms._ResidualRmsNorm.apply(x, r, w, None, gate, gated, 1e-6, 1.0, 1.0, 0.0)
+        torch.autograd.grad(y, x, torch.zeros(T, H))
+    got_x, got_gate, got_w, got_r, got_rstd = seen[1]
+    assert torch.equal(got_x, x) and torch.equal(got_gate.reshape(shape), gate) and torch.equal(got_w, w)
+    assert torch.equal(got_r, r) and torch.equal(got_rstd, torch.arange(2.0 * T))
