@@ -8,6 +8,7 @@
 // on the stream of its forward, which the engine makes the current one and waits for.
 #include <torch/extension.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -38,6 +39,22 @@ struct Api {
 struct Error : std::runtime_error {
   using std::runtime_error::runtime_error;
 };
+PyObject* error_class = nullptr;  // what it is in Python
+
+// f(), an Error as the exception that it is in Python: what a node's backward throws gets
+// there by way of the engine, where the module's translation does not reach.
+template <class F>
+variable_list in_engine(F f) {
+  try {
+    return f();
+  } catch (const Error& e) {
+    const py::gil_scoped_acquire gil;
+    PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
+    python_error raised;
+    raised.persist();
+    throw raised;
+  }
+}
 
 void check(int status, const char* what) {
   if (status == MT_OK) return;
@@ -123,6 +140,10 @@ struct Embedding : torch::autograd::Function<Embedding> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return in_engine([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     variable_list none(7);
     if (!ctx->needs_input_grad(1) || !grads[0].defined()) return none;
     const Tensor ids = ctx->get_saved_variables()[0].contiguous(), d = rows(grads[0]);  // (as below)
@@ -205,6 +226,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return in_engine([&] { return gradients(ctx, grads); });
+  }
+
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     variable_list none(9);
     const bool second = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !second) return none;
@@ -299,8 +324,6 @@ Tensor orthogonalize(const Tensor& update, int64_t coefficients, int64_t steps, 
   check(api.orthogonalize(&a, at_or_null(ws), bytes, stream_of(stream)), "mt_orthogonalize");
   return out;
 }
-
-PyObject* error_class = nullptr;
 
 // The addresses of the functions, in Api's order, and the class that Error becomes.
 void bind(const std::vector<int64_t>& at, const py::object& error) {

@@ -127,3 +127,16 @@ def test_residual_rms_norm_reads_what_a_hook_hands_back(monkeypatch, back, gated
     got_x, got_gate, got_w, got_r, got_rstd = seen[1]
     assert torch.equal(got_x, x) and torch.equal(got_gate.reshape(shape), gate) and torch.equal(got_w, w)
     assert torch.equal(got_r, r) and torch.equal(got_rstd, torch.arange(2.0 * T))
+
+
+def test_errors_of_a_backward_are_the_packages(nodes):
+    """They come to Python out of the engine, not through a call of the module."""
+    refuse = lambda *a: 3  # noqa: E731
+    ops = nodes(mt_layer_norm_forward=OK(lambda a, stream: 0), mt_embed_forward=OK(lambda a, stream: 0),
+                mt_layer_norm_backward=ctypes.CFUNCTYPE(c_int, c_void_p, c_void_p, c_size_t, c_void_p)(refuse),
+                mt_embed_backward=ctypes.CFUNCTYPE(c_int, c_void_p, c_void_p, c_size_t, c_void_p)(refuse))
+    x, w = torch.zeros(3, 8, requires_grad=True), torch.zeros(9, 4, requires_grad=True)
+    for out, leaf in ((ops.layer_norm(x, None, None, None, 1e-5, 1.0, 1.0, True, 0)[0], x),
+                      (ops.embedding(torch.arange(7), w, 1.0, -1, None, None, 0), w)):
+        with pytest.raises(_lib.FlceError, match="_backward: MT_ERR_UNSUPPORTED"):
+            torch.autograd.grad(out, leaf, torch.zeros_like(out))
