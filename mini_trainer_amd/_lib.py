@@ -240,15 +240,24 @@ _torch_ops = None
 
 
 def torch_ops():
-    """The C++ autograd nodes (once), bound to load()'s library; raise if they are missing."""
+    """The C++ autograd nodes (once), bound to load()'s library; raise if they are missing or
+    built for another version of it or of torch."""
     global _torch_ops
     if _torch_ops is None:
+        import torch
+
         lib = load()
         try:
             ops = importlib.import_module("._mt_torch", __package__)
         except ImportError as e:
             raise FlceError("_mt_torch is not built for this torch: build it with "
                             f"`python -m mini_trainer_amd.build` ({e})") from e
+        # (it is compiled apart from the library, with argument structures of its own)
+        built = getattr(ops, "abi_version", None), getattr(ops, "torch_version", None)
+        if built != (ABI_VERSION, str(torch.__version__)):
+            raise FlceError(f"_mt_torch is built for ABI version {built[0]} and torch {built[1]}, expected "
+                            f"{ABI_VERSION} and {torch.__version__}: build it with "
+                            "`python -m mini_trainer_amd.build`")
         ops.bind([ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND], FlceError)
         _torch_ops = ops
     return _torch_ops

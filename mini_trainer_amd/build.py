@@ -25,6 +25,7 @@ DEPENDS = sorted(CSRC.glob("*.h")) + SOURCES + [PKG_DIR.parent / "include" / "mt
 # torch, which is handed the library's functions when both are loaded.
 TORCH_SOURCE = CSRC / "torch_ops.cpp"
 TORCH_PATH = PKG_DIR / "_mt_torch.so"
+TORCH_DEPENDS = [TORCH_SOURCE, PKG_DIR.parent / "include" / "mt_flce.h"]
 
 ARCH = "gfx950"
 HIPCC_FLAGS = [
@@ -60,11 +61,16 @@ SAN_FLAGS = [
 ]
 
 
-def san_is_stale() -> bool:
-    if not SAN_LIB_PATH.exists():
+def _older(built: Path, sources: list) -> bool:
+    """Whether a build is missing, or older than one of its sources."""
+    if not built.exists():
         return True
-    t = SAN_LIB_PATH.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in DEPENDS if p.exists())
+    t = built.stat().st_mtime
+    return any(p.stat().st_mtime > t for p in sources if p.exists())
+
+
+def san_is_stale() -> bool:
+    return _older(SAN_LIB_PATH, DEPENDS)
 
 
 def _compile(out: Path, flags: list, verbose: bool) -> str:
@@ -134,6 +140,7 @@ def build_torch_ops(verbose: bool = False) -> Path:
     tmp = TORCH_PATH.with_suffix(".so.tmp")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include),
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-fvisibility=hidden",
+           f'-DMT_TORCH_VERSION="{torch.__version__}"',
            str(TORCH_SOURCE), "-o", str(tmp), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-lc10"]
     if verbose:
@@ -146,10 +153,8 @@ def build_torch_ops(verbose: bool = False) -> Path:
 
 
 def is_stale() -> bool:
-    if not LIB_PATH.exists():
-        return True
-    t = LIB_PATH.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in DEPENDS if p.exists())
+    """Of the library and the autograd nodes."""
+    return _older(LIB_PATH, DEPENDS) or _older(TORCH_PATH, TORCH_DEPENDS)
 
 
 if __name__ == "__main__":

@@ -4,8 +4,9 @@
 // an empty Python function's backward alone takes 30).
 //
 // The module links no library of this package: bind() is handed the addresses that
-// _lib.py has loaded.  Checks of arguments stay in Python.  Streams: a node's backward runs
-// on the stream of its forward, which the engine makes the current one and waits for.
+// _lib.py has loaded, once the versions of both agree.  Checks of arguments stay in
+// Python.  Streams: a node's backward runs on the stream of its forward, which the engine
+// makes the current one and waits for.
 #include <torch/extension.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
@@ -345,6 +346,9 @@ PYBIND11_MODULE(_mt_torch, m) {
       PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
     }
   });
+  // what _lib.py compares before it binds
+  m.attr("abi_version") = MT_FLCE_ABI_VERSION;
+  m.attr("torch_version") = MT_TORCH_VERSION;
   m.def("bind", &bind);
   m.def("embedding", &embedding);
   m.def("layer_norm", &layer_norm);

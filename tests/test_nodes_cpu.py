@@ -3,12 +3,15 @@ functions of this file that look at it."""
 from __future__ import annotations
 
 import ctypes
+import os
+import sys
+import types
 from ctypes import POINTER, c_int, c_int64, c_size_t, c_void_p
 
 import pytest
 import torch
 
-from mini_trainer_amd import _lib, norms
+from mini_trainer_amd import _lib, build, norms
 from mini_trainer_amd._lib import EmbedArgs, LayerNormArgs, NormArgs
 
 OK = ctypes.CFUNCTYPE(c_int, c_void_p, c_void_p)
@@ -140,3 +143,40 @@ def test_errors_of_a_backward_are_the_packages(nodes):
                       (ops.embedding(torch.arange(7), w, 1.0, -1, None, None, 0), w)):
         with pytest.raises(_lib.FlceError, match="_backward: MT_ERR_UNSUPPORTED"):
             torch.autograd.grad(out, leaf, torch.zeros_like(out))
+
+
+@pytest.mark.parametrize("change,what", [(dict(abi_version=_lib.ABI_VERSION - 1), "ABI version"),
+                                         (dict(abi_version=None), "ABI version"),
+                                         (dict(torch_version="1.13.0"), "torch 1.13.0")])
+def test_nodes_of_another_build_are_refused(monkeypatch, change, what):
+    """Before they are handed the library's functions: a struct of theirs may differ."""
+    have = dict(abi_version=_lib.ABI_VERSION, torch_version=torch.__version__,
+                bind=lambda *a: pytest.fail("bound"))
+    have = {k: v for k, v in {**have, **change}.items() if v is not None}
+    monkeypatch.setattr(_lib, "_torch_ops", None)
+    monkeypatch.setitem(sys.modules, "mini_trainer_amd._mt_torch", types.SimpleNamespace(**have))
+    with pytest.raises(_lib.FlceError, match=what):
+        _lib.torch_ops()
+    assert _lib._torch_ops is None
+
+
+def test_nodes_are_stale_with_their_source(tmp_path, monkeypatch):
+    """The module counts as the library does: missing, or older than what it is built from."""
+    lib, module, source, header = (tmp_path / n for n in ("lib.so", "module.so", "ops.cpp", "abi.h"))
+    for p in (source, header, lib, module):
+        p.write_text("")
+    for name, value in (("LIB_PATH", lib), ("TORCH_PATH", module), ("DEPENDS", [header]),
+                        ("TORCH_DEPENDS", [source, header])):
+        monkeypatch.setattr(build, name, value, raising=False)
+
+    def at(**times):
+        for p in (source, header, lib, module):
+            os.utime(p, (times.get(p.stem, 100),) * 2)
+        return build.is_stale()
+
+    assert not at(lib=200, module=200)
+    assert at(lib=200, module=50) and at(lib=50, module=200)
+    assert at(lib=200, module=200, ops=300) and at(lib=400, module=200, abi=300)
+    assert not at(lib=200, module=400, ops=300)
+    module.unlink()
+    assert build.is_stale()
