@@ -18,7 +18,7 @@ import torch
 
 from .attention import AttentionPlan, packed_attention, packed_attention_plan
 from .embedding import token_embedding
-from .norms import layer_norm, residual_layer_norm, residual_rms_norm
+from .norms import MAX_WIDTH, layer_norm, residual_layer_norm, residual_rms_norm
 
 __all__ = ["AttentionPlans", "patch_decoder_layers", "unlabelled_forward"]
 
@@ -183,9 +183,13 @@ def _own_tensor(t) -> bool:
 
 def _takes_layer_norm(norm: torch.nn.Module, *tensors) -> bool:
     """Whether a module is torch's layer norm over one dimension as it is written there, with
-    nothing that wants to see it called, for tensors of its parameters' type."""
+    nothing that wants to see it called, for tensors of its parameters' type and of its
+    width."""
     if type(norm) is not torch.nn.LayerNorm or len(norm.normalized_shape) != 1 or _has_hooks(norm) or \
             torch.is_autocast_enabled():
+        return False
+    H = norm.normalized_shape[0]
+    if H > MAX_WIDTH or any(t.shape[-1:] != (H,) for t in tensors):
         return False
     parameters = [p for p in (norm.weight, norm.bias) if p is not None]
     return all(_own_tensor(p) for p in parameters) and \

@@ -19,6 +19,7 @@ from .flce import _backward_once, _dtype_code, _launch, _require_device
 
 __all__ = ["layer_norm", "residual_layer_norm", "residual_rms_norm"]
 
+MAX_WIDTH = 32768  # elements of a row
 GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_ELEMENT = range(4)
 ROWS_SAVED = (0, 3)  # of _ResidualRmsNorm's saved tensors: x and the gate, read by rows
 
@@ -151,8 +152,8 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Ten
     for name, t in (("weight", weight), ("post_weight", post_weight)):
         if t is not None and t.shape != (H,):
             raise ValueError(f"{name} must be [{H}], got {tuple(t.shape)}")
-    if not 1 <= H <= 32768:
-        raise ValueError(f"hidden size {H}: 1 to 32768 are supported")
+    if not 1 <= H <= MAX_WIDTH:
+        raise ValueError(f"hidden size {H}: 1 to {MAX_WIDTH} are supported")
     if not (eps >= 0 and math.isfinite(eps + block_scale + residual_scale + weight_offset)):
         raise ValueError("eps must be >= 0, and it, block_scale, residual_scale and weight_offset "
                          "finite")
@@ -192,8 +193,8 @@ def _layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.shape != (H,):
             raise ValueError(f"{name} must be [{H}], got {tuple(t.shape)}")
-    if not 1 <= H <= 32768:
-        raise ValueError(f"hidden size {H}: 1 to 32768 are supported")
+    if not 1 <= H <= MAX_WIDTH:
+        raise ValueError(f"hidden size {H}: 1 to {MAX_WIDTH} are supported")
     if not (eps >= 0 and math.isfinite(eps + block_scale + residual_scale)):
         raise ValueError("eps must be >= 0, and it, block_scale and residual_scale finite")
     return torch_ops().layer_norm(x, residual, weight, bias, eps, block_scale, residual_scale,
