@@ -112,8 +112,8 @@ bool upd_scales(const double* k, double most, UpdScales& s) {
 }
 
 // The tile of a product of tiles(t) output tiles of t x t, `stages` stages of K each, that
-// move `bytes` an element beside it: the one that costs least, in us.  A CU takes `load`
-// of them one after the other; tiles of 64 share it and hide most of what they move behind
+// move `bytes` an element beside it: the one that costs least, in us.  A CU takes one
+// after the other its share of them; tiles of 64 share it and hide most of what they move behind
 // each other's products, the larger ones do not.  A lone tile is as slow as its
 // stages' latency.  The constants are fitted to 24 sizes in bf16 and 12 in fp32 (three terms
 // to a stage) from 128 x 352 to 14336 x 4096 and 1 to 200 matrices, timed with every tile: the

@@ -15,9 +15,14 @@
 //   X <- (a + p(mu)) X + D X,   D = (b + 2 c mu) E + c E^2
 //
 // Around mu the terms no longer cancel (a + b + c = 0.7 out of 3.4, -4.8 and 2.0), and E
-// is small where A is near a multiple of one.  bf16 updates take one product for each
-// (off by 0.0005 to 0.0013 of their norm before the last rounding to bf16, which itself
-// is 0.0017; in bf16 operands 0.015, without mu up to 0.011), fp32 updates three, of the
+// is small where A is near a multiple of one.  bf16 updates take one product for each: five
+// steps of the usual coefficients are off by 0.0005 to 0.0013 of their norm at the measured
+// sizes before the last rounding to bf16, which itself is 0.0017 (in bf16 operands 0.015, without mu
+// up to 0.011).  Over twelve kinds of spectra, emulated in 64 bits, it is 0.00003 to 0.0015,
+// most where singular values spread over decades (10^(-3 i / r): 0.0013) or are an eighth
+// strong ones over noise (0.0015): the result is then off by 0.0022 where fp32 products
+// give 0.0017.  Those coefficients do not settle, so that more steps carry errors on (8:
+// up to 0.0026, 64: 0.006); ones that do stay below 0.0016.  fp32 updates take three, of the
 // values rounded to fp16 and of what that rounding left (1.1e-6; fp32 products 2.9e-6).  fp16
 // copies are scaled by powers of two that keep them below 2^15.
 //
