@@ -227,7 +227,9 @@ def residual_layer_norm(x: torch.Tensor, residual: torch.Tensor,
 
     differentiable in every tensor, with layer_norm's types and rounding: normed comes
     from the unrounded sum.  In bf16 a call whose gradients are recorded keeps 8 bits of
-    new_residual beyond its rounding (a byte per element) for them.
+    new_residual beyond its rounding (a byte per element) for them; rows whose mean is more
+    than some 200 times their deviation lose bits of the weight's gradient with that (off by
+    0.005 of its norm at 1000 times, 0.0016 otherwise).
     """
     if residual is None:
         raise ValueError("residual_layer_norm needs a residual")
