@@ -154,28 +154,49 @@ int upd_with(int kind, F f) {
   }
 }
 
-// The fragment rows of the small matrices' kernel that a matrix goes to, or 0.
-int upd_small_rows(const UpdLayout& l, int steps, int terms) {
-  if (steps > kUpdSmallSteps) return 0;
-  for (int R = 1; R <= (terms == 3 ? 4 : 8); R *= 2)
-    if (l.r <= 16 * R)
-      return l.c <= 128 * upd_small_columns(R, terms) && upd_small_lds(R, l.c, terms) <= kUpdSmallLds ? R : 0;
-  return 0;
+// The fragment rows of the small matrices' kernel that a matrix goes to (0: none), and the
+// products to a term there.  bf16 matrices of at most 32 rows take three as fp32 ones do,
+// where LDS holds them: a rounding of one of their few elements reaches the whole result
+// (4 x 4 off by up to 0.015 of the norm, 16 x 64 of rank 1 by 0.008, so by 1e-6 before the
+// last rounding).
+struct UpdSmall {
+  int rows, terms;
+};
+UpdSmall upd_small(const UpdLayout& l, int steps, int dtype) {
+  if (steps > kUpdSmallSteps) return {0, 0};
+  const auto rows = [&](int terms, int most) {
+    for (int R = 1; R <= most; R *= 2)
+      if (l.r <= 16 * R)
+        return l.c <= 128 * upd_small_columns(R, terms) && upd_small_lds(R, l.c, terms) <= kUpdSmallLds ? R : 0;
+    return 0;
+  };
+  const int split = rows(3, dtype == MT_DTYPE_F32 ? 4 : 2);
+  if (split || dtype == MT_DTYPE_F32) return {split, 3};
+  return {rows(1, 8), 1};
 }
 
 template <class T>
-int launch_small(int R, const UpdSmallArgs& k, int64_t batch, hipStream_t stream) {
-  constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
-  const auto with = [&](auto rows) {
-    hipLaunchKernelGGL((upd_small_kernel<T, decltype(rows)::value, TERMS>), dim3((uint32_t)batch), dim3(512), 0, stream,
-                       k);
+int launch_small(UpdSmall way, const UpdSmallArgs& k, int64_t batch, hipStream_t stream) {
+  const auto with = [&](auto rows, auto terms) {
+    hipLaunchKernelGGL((upd_small_kernel<T, decltype(rows)::value, decltype(terms)::value>), dim3((uint32_t)batch),
+                       dim3(512), 0, stream, k);
     return check_launch("upd_small_kernel");
   };
-  if (R == 1) return with(std::integral_constant<int, 1>());
-  if (R == 2) return with(std::integral_constant<int, 2>());
-  if (TERMS == 3 || R == 4) return with(std::integral_constant<int, 4>());
-  if constexpr (TERMS == 1) return with(std::integral_constant<int, 8>());
-  return MT_OK;
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 3> three{};
+  constexpr std::integral_constant<int, 4> four{};
+  if (way.terms == 3) {
+    if (way.rows == 1) return with(one, three);
+    if (way.rows == 2) return with(two, three);
+    if constexpr (sizeof(T) == 4) return with(four, three);
+  } else if constexpr (sizeof(T) == 2) {
+    if (way.rows == 1) return with(one, one);
+    if (way.rows == 2) return with(two, one);
+    if (way.rows == 4) return with(four, one);
+    return with(std::integral_constant<int, 8>(), one);
+  }
+  return fail(MT_ERR_UNSUPPORTED, "%d rows of fragments, %d terms", way.rows, way.terms);
 }
 
 template <class T>
@@ -251,8 +272,7 @@ extern "C" {
 size_t mt_orthogonalize_workspace_bytes(const mt_orthogonalize_args* args) {
   UpdLayout l;
   if (!args || args->batch < 1 || args->batch > (1 << 24) || !esize(args->dtype) ||
-      !upd_layout(args->m, args->n, args->dtype, l) ||
-      upd_small_rows(l, args->steps, args->dtype == MT_DTYPE_F32 ? 3 : 1))
+      !upd_layout(args->m, args->n, args->dtype, l) || upd_small(l, args->steps, args->dtype).rows)
     return 0;
   return (size_t)(l.bytes * std::max<int64_t>(1, std::min(args->batch, kUpdGroup / l.bytes)));
 }
@@ -267,7 +287,7 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   const int64_t V = 16 / es;
   const bool vec = aligned16(a.in) && aligned16(a.out) && a.n % V == 0 && (a.m == 1 || a.in_row % V == 0) &&
                    (a.batch == 1 || a.in_batch % V == 0);
-  const int small = upd_small_rows(l, a.steps, a.dtype == MT_DTYPE_F32 ? 3 : 1);
+  const UpdSmall small = upd_small(l, a.steps, a.dtype);
   UpdSmallArgs sm{};
   double most = 1.0;
   for (int step = 0; step < a.steps; ++step) {  // before anything is launched
@@ -278,13 +298,13 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
     if (!upd_scales(q, most, s))
       return fail(MT_ERR_UNSUPPORTED, "coefficients that carry singular values beyond 10^6");
     most = s.next;
-    if (small) {
+    if (small.rows) {
       if (step) sm.step[step - 1].x_scale = std::ldexp(1.f, s.x);
       sm.step[step] = {(float)q[0], (float)q[1], (float)q[2], std::ldexp(1.f, -s.x), std::ldexp(1.f, s.e),
                        std::ldexp(1.f, -s.e), std::ldexp(1.f, s.d), std::ldexp(1.f, -s.d), 1.f};
     }
   }
-  if (small) {
+  if (small.rows) {
     sm.in_row = a.in_row, sm.in_batch = a.in_batch;
     sm.eps = a.eps;
     sm.m = (int32_t)a.m, sm.n = (int32_t)a.n, sm.r = (int32_t)l.r, sm.c = (int32_t)l.c;

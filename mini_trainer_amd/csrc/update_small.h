@@ -2,8 +2,9 @@
 // workgroup and one launch, where the tiles of update_kernels.h would take three launches a
 // step that mostly wait (128 x 352: 106 us in 17 launches, 53 here).
 //
-// The mathematics and the number formats are those of update_kernels.h.  X [r, c] (r at
-// most 128) lies in LDS in fp16, as do E and D; X in fp32 stays in the registers of the
+// The mathematics and the number formats are those of update_kernels.h; bf16 matrices of at
+// most 32 rows take three products to a term, too, where LDS holds both terms of X.  X [r, c]
+// (r at most 128) lies in LDS in fp16, as do E and D; X in fp32 stays in the registers of the
 // wave that owns its columns (16 at a time: fragment columns w, w + 8, ...).  Of the
 // 8 waves each forms a block of up to 2 x 4 fragments of X X^T; where there are fewer blocks
 // than waves the long axis is split between them and their parts are added in LDS one wave
