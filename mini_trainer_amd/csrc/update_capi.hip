@@ -35,7 +35,7 @@ int64_t upd_split(int64_t tiles, int64_t stages) {
 
 struct UpdLayout {
   int64_t r, c, ld_r, ld_c;
-  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, parts, bytes;  // of one matrix
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, spread, norm, state, parts, bytes;  // of one matrix
 };
 bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   const auto up = [](int64_t v) { return cdiv(v, 64) * 64; };
@@ -55,6 +55,7 @@ bool upd_layout(int64_t m, int64_t n, int dtype, UpdLayout& x) {
   take(x.fragments, x.ld_r * x.ld_r * 2 * planes);
   take(x.carrier, cdiv(m, 16) * cdiv(n, 16) * 1024);
   take(x.partial, cdiv(m, 64) * cdiv(n, 64) * 4);  // (of the smallest tiles)
+  take(x.spread, cdiv(x.r, 64) * 4);
   take(x.norm, kUpdParts * 8);
   take(x.state, kUpdState * 4);
   const int64_t tiles = cdiv(x.r, 64) * (cdiv(x.r, 64) + 1) / 2, split = upd_split(tiles, x.ld_c / 64);  // (a stack splits less)
@@ -230,7 +231,8 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
     next = now;
     if (step + 1 < p.steps && !upd_scales(q + 3, now.next, next))
       return fail(MT_ERR_UNSUPPORTED, "these coefficients diverge");
-    k.first = step == 0, k.last = step + 1 == p.steps;
+    k.first = step == 0, k.last = step + 1 == p.steps, k.lifted = step + 2 < p.steps;
+    k.x_exponent = now.x;
     k.a = (float)q[0], k.b = (float)q[1], k.cc = (float)q[2];
     k.x_unscale = std::ldexp(1.f, -now.x), k.x_scale = std::ldexp(1.f, next.x);
     k.e_scale = std::ldexp(1.f, now.e), k.e_unscale = std::ldexp(1.f, -now.e);
@@ -238,7 +240,7 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
     MT_TRY(upd_with<kMost>(symmetric, [&](auto F) {
       constexpr int f = decltype(F)::value;
       k.tiles_m = k.tiles_n = (int32_t)cdiv(k.r, upd_tile(f));
-      k.tiles = k.tiles_m * (k.tiles_m + 1) / 2;
+      k.tiles = k.tiles_m * (k.tiles_m + 1) / 2, k.spreads = k.tiles_m;
       const dim3 grid((uint32_t)(k.tiles * k.batch));
       if (f == 2 && k.split > 1) {
         hipLaunchKernelGGL((upd_symmetric_kernel<2, TERMS, kUpdPart>), dim3(grid.x * (uint32_t)k.split), dim3(256), 0,
@@ -256,8 +258,9 @@ int launch_orthogonalize(UpdArgs k, const mt_orthogonalize_args& p, hipStream_t 
       constexpr int f = decltype(F)::value;
       k.tiles_m = (int32_t)cdiv(k.m, upd_tile(f)), k.tiles_n = (int32_t)cdiv(k.n, upd_tile(f));
       k.tiles = k.partials = k.tiles_m * k.tiles_n;
-      hipLaunchKernelGGL((upd_apply_kernel<T, f, TERMS>), dim3((uint32_t)(k.tiles * k.batch)), dim3(256), 0, stream,
-                         k);
+      const auto kern = TERMS == 1 && k.lifted ? upd_apply_kernel<T, f, TERMS, TERMS == 1>
+                                               : upd_apply_kernel<T, f, TERMS, false>;
+      hipLaunchKernelGGL(kern, dim3((uint32_t)(k.tiles * k.batch)), dim3(256), 0, stream, k);
       return check_launch("upd_apply_kernel");
     }));
     std::swap(k.s0, k.s1);
@@ -333,8 +336,8 @@ int mt_orthogonalize(const mt_orthogonalize_args* args, void* workspace, size_t 
   k.ws_stride = l.bytes;
   k.in_row = a.in_row, k.in_batch = a.in_batch;
   k.l = l.l, k.s0 = l.s0, k.s1 = l.s1, k.e = l.e, k.d = l.d;
-  k.fragments = l.fragments, k.carrier = l.carrier, k.partial = l.partial, k.norm = l.norm, k.state = l.state;
-  k.parts = l.parts;
+  k.fragments = l.fragments, k.carrier = l.carrier, k.partial = l.partial, k.spread = l.spread;
+  k.norm = l.norm, k.state = l.state, k.parts = l.parts;
   k.eps = a.eps;
   k.m = (int32_t)a.m, k.n = (int32_t)a.n, k.r = (int32_t)l.r, k.c = (int32_t)l.c;
   k.ld_r = (int32_t)l.ld_r, k.ld_c = (int32_t)l.ld_c;

@@ -15,16 +15,25 @@
 //   X <- (a + p(mu)) X + D X,   D = (b + 2 c mu) E + c E^2
 //
 // Around mu the terms no longer cancel (a + b + c = 0.7 out of 3.4, -4.8 and 2.0), and E
-// is small where A is near a multiple of one.  bf16 updates take one product for each: five
-// steps of the usual coefficients are off by 0.0005 to 0.0013 of their norm at the measured
-// sizes before the last rounding to bf16, which itself is 0.0017 (in bf16 operands 0.015, without mu
-// up to 0.011).  Over twelve kinds of spectra, emulated in 64 bits, it is 0.00003 to 0.0015,
-// most where singular values spread over decades (10^(-3 i / r): 0.0013) or are an eighth
-// strong ones over noise (0.0015): the result is then off by 0.0022 where fp32 products
-// give 0.0017.  Those coefficients do not settle, so that more steps carry errors on (8:
-// up to 0.0026, 64: 0.006); ones that do stay below 0.0016.  fp32 updates take three, of the
-// values rounded to fp16 and of what that rounding left (1.1e-6; fp32 products 2.9e-6).  fp16
-// copies are scaled by powers of two that keep them below 2^15.
+// is small where A is near a multiple of one.  fp32 updates take three products for each, of
+// the values rounded to fp16 and of what that rounding left (1.1e-6 of the norm; fp32 products
+// 2.9e-6).  bf16 updates take one, whose operand X~ is X rounded: D (X~ - X) is small where all
+// eigenvalues of A lie near mu, but D is -p(mu) along singular vectors of small singular
+// values, and what gets in there is lifted by the later steps as those are (half of the singular
+// values strong, the others 0.05 of them: 0.004 of the norm after 5 steps, 0.04 after 12).  So
+//
+//   X <- (a + f p(mu)) X + (1 - f) p(mu) X~ + D X~,   f = max(0, 1 - |E|^2 / (r mu^2))
+//
+// with the error (M - f p(mu) I) (X~ - X), M = b A + c A^2.  Its sum over the eigenvalues, each
+// lifted to about 1 in the end, is least where f mu is their harmonic mean: that ratio to mu is
+// 1 - variance / mu^2 for large random matrices, and 0 where the eigenvalues spread further.  The
+// last two steps, after which little is lifted, take f = 1.  |E|^2 is the trace of E^2, from
+// the diagonal tiles of that product.  Five steps of the usual coefficients are then off by
+// 0.0003 to 0.0016 of their norm before the last rounding to bf16, which itself is 0.0017, over
+// nine kinds of spectra of 33 rows and more (products of bf16 operands: 0.018 at 4096 x 4096).
+// Those coefficients do not settle, so that more steps carry errors on (12: 0.001 to 0.003,
+// more where a singular value comes to lie where their map is steep); with ones that do it
+// stays below the rounding.  fp16 copies are scaled by powers of two that keep them below 2^15.
 //
 // Copies of X in fp16: L [r, c], whose rows are contiguous along the long side (A), and
 // S [c, r] (D X); a product writes both of the X it forms, out of one image in LDS.
@@ -43,9 +52,16 @@ namespace mtf {
 
 constexpr int kUpdParts = 1024;  // partial sums of squares of G, at most
 
-// Per matrix, in fp32: the factor of X0 over its fp16 copy, mu, and the two factors of X0
-// over G, 2^k and 1 / (|G| + eps) / 2^k (their product leaves fp32's range where |G| does).
-enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdShift = 3, kUpdState = 4 };
+// Per matrix, in fp32: the factor of X0 over its fp16 copy, mu, the two factors of X0
+// over G, 2^k and 1 / (|G| + eps) / 2^k (their product leaves fp32's range where |G| does), and
+// the power of two of G's fp16 copy.
+enum { kUpdFactor = 0, kUpdInverse = 1, kUpdMu = 2, kUpdShift = 3, kUpdExponent = 4, kUpdState = 5 };
+
+// f of a matrix with the trace `square` of E^2.  (Any f is right: where these numbers leave
+// fp32's range it is one of 0 .. 1.)
+__device__ __forceinline__ float upd_share(float square, float mu, int32_t r) {
+  return fminf(fmaxf(1.f - square / ((float)r * mu * mu), 0.f), 1.f);
+}
 
 // 1 / (|G| + eps) in 64 bits; for a zero matrix, where it matters to nothing, one that fp32
 // holds, so that X0 is zero and not its product with infinity.
@@ -58,13 +74,15 @@ struct UpdArgs {
   char* out;
   char* ws;               // of the first matrix; the others follow ws_stride bytes apart
   int64_t ws_stride, in_row, in_batch;
-  int64_t l, s0, s1, e, d, fragments, carrier, partial, norm, state, parts;  // byte offsets
+  int64_t l, s0, s1, e, d, fragments, carrier, partial, spread, norm, state, parts;  // byte offsets
   double eps;
   int32_t m, n, r, c, ld_r, ld_c;        // ld_r, ld_c: r and c up to whole stages
-  int32_t norm_parts, partials;          // partial sums of |G|^2, and of |X|^2
+  int32_t norm_parts, partials, spreads; // partial sums of |G|^2, of |X|^2, and of E^2's trace
   int32_t batch, tiles_m, tiles_n, tiles;
   int32_t split;                         // workgroups of a tile of A
   int32_t first, last;                   // of the steps
+  int32_t lifted;                        // not of the last two steps: f counts (above)
+  int32_t x_exponent;                    // X's fp16 copy is X 2^x_exponent, but for the first step's
   float a, b, cc;                        // the step's coefficients
   float x_unscale, e_scale, e_unscale, d_scale, d_unscale, x_scale;
   int32_t vec;                           // rows of G and of the result are whole 16-byte vectors
@@ -136,6 +154,7 @@ __global__ __launch_bounds__(256) void upd_convert_kernel(UpdArgs a) {
     state[kUpdShift] = (float)ldexp(1.0, exponent / 2);
     state[kUpdInverse] = (float)ldexp(inverse, -(exponent / 2));
     state[kUpdMu] = (float)(norm * inverse * (norm * inverse) / a.r);
+    state[kUpdExponent] = (float)exponent;
   }
   const int32_t across = (a.n + 63) / 64;
   const int32_t row0 = (int32_t)(blockIdx.x / across) * 64, col0 = (int32_t)(blockIdx.x % across) * 64;
@@ -438,6 +457,25 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
           if (within(fm, fn)) kept[t * kept_plane + upd_fragment(row, col, across) / 4] = h;
         });
   } else {
+    if constexpr (TERMS == 1) {
+      if (a.lifted && ti == tj) {  // this tile's part of the trace of E^2
+        float s = 0.f;
+#pragma unroll
+        for (int fm = 0; fm < F; ++fm)
+#pragma unroll
+          for (int fn = 0; fn < F; ++fn)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s += p.row + 16 * fm == p.col + 16 * fn + i ? acc[fm][fn][i] : 0.f;
+        s = norm_wave_sum(s);
+        if (lane_id() == 0) sums[wave_id()] = s;
+        __syncthreads();
+        if (threadIdx.x == 0)
+          reinterpret_cast<float*>(ws + a.spread)[ti] =
+              (sums[0] + sums[1] + sums[2] + sums[3]) * a.e_unscale * a.e_unscale;
+        __syncthreads();
+      }
+    }
     const float linear = (a.b + 2.f * a.cc * mu) * a.e_unscale * a.d_scale;
     const float square = a.cc * a.e_unscale * a.e_unscale * a.d_scale;
     f16x4_t held[TERMS == 3 ? 2 : 1][F][F];  // (in the registers of the loop's fragments)
@@ -473,10 +511,11 @@ __global__ __launch_bounds__(256) void upd_symmetric_kernel(UpdArgs a) {
 
 typedef f32x4_t any_f32x4_t __attribute__((aligned(4)));
 
-// X <- (a + p(mu)) X + D X, as it lies in memory [m, n]: D S^T, or S D where m > n.  Writes
-// the carried X, both fp16 copies and the tile's sum of squares, or at the last step the
-// result.
-template <class T, int F, int TERMS>
+// X <- (a + f p(mu)) X + (1 - f) p(mu) X~ + D X~, as it lies in memory [m, n]: D S^T, or S D
+// where m > n.  Writes the carried X, both fp16 copies and the tile's sum of squares, or at
+// the last step the result.
+// LIFTED: f counts (one kernel with a branch for it would spill).
+template <class T, int F, int TERMS, bool LIFTED>
 __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   __shared__ __attribute__((aligned(1024))) char lds[upd_lds(F)];
   float* sums = reinterpret_cast<float*>(lds);  // (before and after the tile)
@@ -496,7 +535,17 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
   const float* state = reinterpret_cast<const float*>(ws + a.state);
   const float mu = state[kUpdMu];
   const float product = a.d_unscale * (a.first ? state[kUpdFactor] : a.x_unscale);
-  const float linear = (a.a + mu * (a.b + a.cc * mu)) * (a.first ? state[kUpdInverse] : 1.f);
+  const float around = mu * (a.b + a.cc * mu);
+  float share = 1.f;
+  if constexpr (LIFTED) {
+    const float* spread = reinterpret_cast<const float*>(ws + a.spread);
+    float s = 0.f;
+    for (int32_t k = (int32_t)lane_id(); k < a.spreads; k += 64) s += spread[k];
+    share = upd_share(norm_wave_sum(s), mu, a.r);
+  }
+  const float copied = (1.f - share) * around * (a.first ? state[kUpdFactor] : a.x_unscale);
+  const int exponent = a.first ? (int)state[kUpdExponent] : a.x_exponent;
+  const float linear = (a.a + share * around) * (a.first ? state[kUpdInverse] : 1.f);
   const float shift = a.first ? state[kUpdShift] : 1.f;
   const T* in = reinterpret_cast<const T*>(a.in) + (int64_t)matrix * a.in_batch;
   float* carrier = reinterpret_cast<float*>(ws + a.carrier);
@@ -558,6 +607,8 @@ __global__ __launch_bounds__(256) void upd_apply_kernel(UpdArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         x[i] = fmaf(linear, held[fm % 3][fn][i] * shift, product * acc[fm][fn][i]);
+        if constexpr (LIFTED)
+          x[i] = fmaf(copied, upd_float(upd_half(ldexpf(held[fm % 3][fn][i], exponent))), x[i]);
         ss = fmaf(x[i], x[i], ss);
       }
       if (!a.last) {

@@ -68,6 +68,7 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
   char* const D = E + P * plane_e;
   float* const sum = reinterpret_cast<float*>(D + P * plane_e);  // [16 R][16 R] where SPLIT > 1
   double* const sums = reinterpret_cast<double*>(reinterpret_cast<char*>(sum) + (SPLIT > 1 ? 16 * R * 16 * R * 4 : 0));
+  float* const spread = reinterpret_cast<float*>(sums + 8);  // [BLOCKS]
   const uint32_t l = lane_id(), w = wave_id(), l16 = l & 15u, g = l >> 4;
   const bool tall = a.m > a.n;
   const int64_t matrix = blockIdx.x;
@@ -278,10 +279,31 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
           for (int e = 0; e < 4; ++e) v[e] = fmaf(linear, v[e], squared * acc[i][j][e]);
           put(D, plane_e, PE, row, col, v);
         }
+      if (TERMS == 1 && step + 2 < a.steps) {  // this block's part of the trace of E^2
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < BR; ++i)
+#pragma unroll
+          for (int j = 0; j < BC; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s += 16 * (fr + i) + (int32_t)l16 == 16 * (fc + j) + 4 * (int32_t)g + e ? acc[i][j][e] : 0.f;
+        s = norm_wave_sum(s);
+        if (l == 0) spread[w] = s;
+      }
     }
     __syncthreads();
-    // X <- (a + p(mu)) X + D X, each wave its columns
-    const float product = k.d_unscale * unscale, linear = k.a + mu * (k.b + k.c * mu);
+    // X <- (a + f p(mu)) X + (1 - f) p(mu) X~ + D X~, each wave its columns
+    const float around = mu * (k.b + k.c * mu);
+    const bool lifted = TERMS == 1 && step + 2 < a.steps;
+    float share = 1.f;
+    if (lifted) {
+      float s = 0.f;
+      for (int i = 0; i < BLOCKS; ++i) s += spread[i];
+      share = upd_share(s * k.e_unscale * k.e_unscale, mu, a.r);
+    }
+    const float product = k.d_unscale * unscale, linear = k.a + share * around;
+    const float copied = (1.f - share) * around * unscale;
     float ss = 0.f;
 #pragma unroll
     for (int j0 = 0; j0 < COLS; j0 += GROUP) {
@@ -291,6 +313,18 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
       for (int j = 0; j < GROUP; ++j)
 #pragma unroll
         for (int f = 0; f < R; ++f) y[j][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      // X~ of the group, on its way beside the products (where each element waited for its own,
+      // 128 x 352 took 59 us)
+      f16x4_t h[GROUP][TERMS == 1 ? R : 1];
+      if constexpr (TERMS == 1) {
+#pragma unroll
+        for (int j = 0; j < GROUP; ++j) {
+          const int32_t at = 16 * (int32_t)(w + 8 * (j0 + j));
+#pragma unroll
+          for (int f = 0; f < R; ++f)
+            h[j][f] = *reinterpret_cast<const f16x4_t*>(L + (16 * f + l16) * PL + ((at < ld ? at : 0) + 4 * g) * 2);
+        }
+      }
 #pragma unroll
       for (int kk = 0; kk < K / 32; ++kk) {
         // rows 32 kk + 8 g .. of a column's halves; a single fragment row has no more than 16
@@ -329,6 +363,7 @@ __global__ __launch_bounds__(512) void upd_small_kernel(UpdSmallArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             v[i] = fmaf(linear, x[j0 + j][f][i], product * y[j][f][i]);
+            if constexpr (TERMS == 1) v[i] = fmaf(copied, (float)h[j][f][i], v[i]);
             x[j0 + j][f][i] = v[i];
             ss = fmaf(v[i], v[i], ss);
             v[i] *= k.x_scale;  // (the last step's go nowhere)

@@ -1,12 +1,41 @@
-"""bf16 matrices whose singular values are far apart, and their orthogonalised updates in 64
-bits."""
+"""Orthogonalised updates of bf16 matrices whose singular values are far apart, and how
+their fp16 products may be rounded.
+
+A step maps X to a X + M X, M = b A + c A^2.  The product's operand is X rounded to fp16, X~,
+and its error M (X~ - X).  Taken around mu, as D X~ + p(mu) X with D = M - p(mu) I, the
+error is D (X~ - X) instead: smaller where all eigenvalues of A lie near mu, but D is -p(mu)
+and not 0 along singular vectors of small singular values, and what gets in there is lifted by
+the steps that follow as those are.  With p(mu) (f X + (1 - f) X~) the error is (M - f p(mu) I)
+(X~ - X).  Its sum over the eigenvalues, each lifted to about 1 in the end, is least where
+f mu is their harmonic mean; f = 1 - var / mu^2, at least 0, is that mean's ratio to mu for
+the eigenvalues of large random matrices, and 0 where they spread further.  The last two steps
+take f = 1: little is lifted after them.
+"""
 from __future__ import annotations
 
 import math
 
 import torch
 
-from update_reference import COEFFICIENTS, iterate, triples
+from update_reference import COEFFICIENTS, _product, _split, iterate, triples
+
+
+def rounded(x, coefficients, norm, eps, around=False):
+    """The last state of a wide matrix with one fp16 product a term: f as above, or f = 1 in
+    every step (around)."""
+    x = x / (norm + eps)
+    scale, mid, r = 2.0 ** 13, 2.0 ** 12, x.shape[0]
+    for i, (a, b, c) in enumerate(coefficients):
+        mu = float(x.square().sum()) / r
+        e = _product(x, x, 1, scale) - mu * torch.eye(r, dtype=x.dtype)
+        linear = _split(e, mid, 1)[0]
+        square = _product(e, e, 1, mid)
+        var = float(square.trace()) / r
+        f = 1.0 if around or i + 2 >= len(coefficients) else max(0.0, 1.0 - var / mu ** 2)
+        p = mu * (b + c * mu)
+        d = (b + 2 * c * mu) * linear + c * square
+        x = (a + f * p) * x + (1 - f) * p * _split(x, scale, 1)[0] + _product(d, x.T.contiguous(), 1, mid)
+    return x
 
 
 def matrices(r, c, seed=0):

@@ -1,5 +1,6 @@
-"""Orthogonalised updates of bf16 matrices whose singular values are far apart, on the GPU,
-against the rounded exact value's error (spectra_reference.py)."""
+"""Orthogonalised updates of bf16 matrices whose singular values are far apart, on the GPU:
+the error before the last rounding stays below that rounding's, so that the whole is less than
+1.45 times what the rounded exact value is off by (spectra_reference.py)."""
 from __future__ import annotations
 
 import pytest
@@ -29,6 +30,20 @@ def test_small_matrices_are_as_exact_as_their_rounding(gpu, r, c):
         for tall in (False, True):
             got = ratios(r, c, gpu, tall, seed)
             assert max(got.values()) < 1.01, got
+
+
+@pytest.mark.parametrize("r,c", [(16, 2900), (24, 1600), (33, 300), (48, 200), (64, 256), (64, 992), (100, 101), (128, 128),
+                                 (128, 352), (128, 353), (256, 1024), (300, 301), (500, 900)])
+@pytest.mark.parametrize("tall", [False, True])
+def test_five_steps(gpu, r, c, tall):
+    got = ratios(r, c, gpu, tall)
+    assert max(got.values()) < 1.45, got
+
+
+@pytest.mark.parametrize("r,c", [(96, 256), (200, 600)])
+def test_more_steps_of_coefficients_that_settle(gpu, r, c):
+    got = ratios(r, c, gpu, steps=12, coefficients=(1.875, -1.25, 0.375))
+    assert max(got.values()) < 1.45, got
 
 
 def test_stacks_take_each_matrix_spectrum(gpu):
