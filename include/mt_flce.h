@@ -786,8 +786,9 @@ int mt_layer_norm_backward(const mt_layer_norm_args* args, void* workspace, size
  *   coefficients  a, b, c of each step (host, 3 steps doubles, read during the call);
  *        such that singular values of at most 1 stay below 10^6 (MT_ERR_UNSUPPORTED)
  *   eps >= 0;  steps 1 to 64
- * bf16 matrices go through fp16 products, fp32 ones through three of split values (with
- * the relative error of fp32 products); X is carried in fp32 and rounded once at the end.
+ * bf16 matrices go through fp16 products, fp32 ones, and bf16 ones of up to 32 rows or
+ * columns that one workgroup holds, through three of split values (with the relative error
+ * of fp32 products); X is carried in fp32 and rounded once at the end.
  * A matrix that holds NaN or infinities gives NaN; a zero matrix gives zeros (eps > 0).
  * The workspace (256-byte aligned) must hold one matrix's part; the query's size, up to
  * 2 GiB or one matrix, takes a stack together.  Small matrices take none (0 bytes, null).

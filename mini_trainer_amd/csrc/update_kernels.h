@@ -30,7 +30,8 @@
 // last two steps, after which little is lifted, take f = 1.  |E|^2 is the trace of E^2, from
 // the diagonal tiles of that product.  Five steps of the usual coefficients are then off by
 // 0.0003 to 0.0016 of their norm before the last rounding to bf16, which itself is 0.0017, over
-// nine kinds of spectra of 33 rows and more (products of bf16 operands: 0.018 at 4096 x 4096).
+// nine kinds of spectra of 33 rows and more (products of bf16 operands: 0.018 at 4096 x 4096),
+// by 0.002 where a few eigenvalues, which the variance does not show, lie far below many equal ones.
 // Those coefficients do not settle, so that more steps carry errors on (12: 0.001 to 0.003,
 // more where a singular value comes to lie where their map is steep); with ones that do it
 // stays below the rounding.  fp16 copies are scaled by powers of two that keep them below 2^15.
@@ -39,10 +40,11 @@
 // S [c, r] (D X); a product writes both of the X it forms, out of one image in LDS.
 // All rows end in zeros up to whole stages of 64.
 //
-// 4096 x 4096 in bf16: A 79 us, D 78 (1740 TFLOP/s if they were whole), D X 146, of which
-// some 45 move X (4 bytes read, 8 written an element) with no product beside them: one tile of
-// 256 x 256 fills a CU.  The products are bound by LDS (192 x 192 tiles) and the power limit
-// (1.9 to 2.0 GHz).  28 of 256 x 1536: D X 29 us, 4.9 TB/s.
+// 4096 x 4096 in bf16: A 76 us, D 75 (1810 TFLOP/s if they were whole), D X 148 (141 in the
+// last two steps), of which some 45 move X (4 bytes read, 8 written an element) with no product
+// beside them: one tile of 256 x 256 fills a CU.  The products are bound by LDS (192 x 192 tiles) and the power limit
+// (1.9 to 2.2 GHz).  28 of 256 x 1536: D X 31 us, 4.9 TB/s (much of it out of the cache behind L2):
+// with four stages of K a tile's product, its reads of X and its writes follow one another.
 #pragma once
 
 #include "step_norm.h"

@@ -1,6 +1,6 @@
 // Orthogonalised updates of small matrices (gfx950): all steps of one matrix in one
 // workgroup and one launch, where the tiles of update_kernels.h would take three launches a
-// step that mostly wait (128 x 352: 106 us in 17 launches, 53 here).
+// step that mostly wait (128 x 352: 56 us here; 128 x 360 in 17 launches there 89).
 //
 // The mathematics and the number formats are those of update_kernels.h; bf16 matrices of at
 // most 32 rows take three products to a term, too, where LDS holds both terms of X.  X [r, c]
@@ -11,9 +11,9 @@
 // after the other, in a fixed order.  D X reads X's columns as operands through
 // transposing LDS reads, and the wave that owns them writes them back.
 // It is bound by LDS and by the barriers between its products: 128 x 352 in bf16 keeps the
-// LDS of its CU busy for 60% of the 53 us (half of that conflicts), each SIMD's matrix
-// instructions for 25%.  Its largest matrices are the last that profit: 128 x 360 by the tiles
-// takes 85 us, 64 x 416 in fp32 58 here and 64 x 424 93 there.
+// LDS of its CU busy for 58% of the 56 us (half of that conflicts), each SIMD's matrix
+// instructions for 24%.  Its largest matrices are the last that profit: 64 x 416 in fp32 takes 58
+// us here, 64 x 424 94 by the tiles.
 #pragma once
 
 #include "update_kernels.h"

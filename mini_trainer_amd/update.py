@@ -58,10 +58,10 @@ def orthogonalize(update: torch.Tensor, steps: int = 5,
     steps); those that would carry singular values in [0, 1] beyond 10^6 are refused.
 
     X is carried in fp32 and rounded once.  bf16 updates go through fp16 matrix products: the
-    default five steps are off by less than that last rounding, which is 0.0017 of the norm,
-    whatever the singular values (bf16 products: 0.02), and so are more steps of coefficients
-    that settle; more of the default ones, which do not, carry errors on (12: mostly up to
-    0.003).  fp32 updates, and bf16 ones of up to 32 rows or columns where one workgroup holds
+    default five steps are off by about that last rounding, which is 0.0017 of the norm, or
+    less, whatever the singular values (bf16 products: 0.02), and so are more steps of
+    coefficients that settle; more of the default ones, which do not, carry errors on (12:
+    mostly up to 0.003).  fp32 updates, and bf16 ones of up to 32 rows or columns where one workgroup holds
     them, go through products of split values, with the error of fp32 products or less.  A matrix with NaN or infinities gives NaN, a zero
     matrix zeros (with eps > 0).  Matrices of one shape are cheapest as one stack.  Not
     differentiable.
