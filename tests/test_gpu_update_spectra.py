@@ -53,3 +53,17 @@ def test_stacks_take_each_matrix_spectrum(gpu):
         got = orthogonalize(stack)
         for one, x in zip(got, stack):
             assert torch.equal(one, orthogonalize(x))
+
+
+@pytest.mark.parametrize("r,c", [(4, 20), (16, 300), (32, 64)])
+def test_split_small_matrices_that_are_zero_or_not_finite(gpu, r, c):
+    x = torch.stack(list(ref.matrices(r, c).values())[:5]).to(gpu)
+    want = orthogonalize(x)
+    bad = x.clone()
+    bad[0] = 0
+    bad[2, r - 1, c - 1] = float("nan")
+    bad[4, 0, 0] = float("-inf")
+    got = orthogonalize(bad)
+    assert not got[0].any() and got[2].isnan().all() and got[4].isnan().all()
+    assert torch.equal(got[1], want[1]) and torch.equal(got[3], want[3])
+    assert torch.equal(orthogonalize(x.transpose(1, 2).contiguous()), want.transpose(1, 2))
